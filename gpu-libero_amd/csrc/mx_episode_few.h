@@ -1,0 +1,349 @@
+// Attention of few rows: the four waves of a workgroup each take 32 keys at a time of one world's key
+// head, for up to 16 * kBlocks rows (new tokens times the query heads that share the key head).
+//
+// One pass over the keys with a running maximum m, sum l and output O per row (in 32 bits):
+//   S^T = K Q^T (scores of 32 keys in two products' results, a row of the chunk per lane column),
+//   m' = max(m, S), p = 2^(S - m'), l' = l 2^(m - m') + sum p, O^T = O^T 2^(m - m') + V^T P^T.
+// With the scores transposed, a lane holds eight keys of its own row, which is the operand that the
+// second product wants if its keys are numbered 4 q + (0..3), 16 + 4 q + (0..3) for lane quarter q; V's
+// columns come in that order out of LDS by transposing reads, so probabilities never cross lanes.
+// They enter the product as two 16-bit parts, value and remainder, which costs matrix instructions
+// that a kernel bound by reading K and V has to spare, and keeps 16 bits of them.
+#pragma once
+#include "mx_episode_types.h"
+
+namespace mxe {
+
+template <int kType, bool kFp8, int D, int kBlocks>
+__global__ __launch_bounds__(256) void attend_few(const Attend a) {
+  typedef Elem<kType> E;
+  typedef typename E::T T;
+  typedef typename E::V8 V8;
+  constexpr int kRows = 16 * kBlocks, kC = D / 32;            // products along head_dim
+  constexpr int kStride = D + 16;                             // V's row in LDS: transposing reads of 16 rows hit all banks once
+  constexpr int kVPer = kFp8 ? 16 : 8, kVLoads = 32 * D / kVPer / 64;
+  constexpr int kPairs = kFp8 ? D / 64 : 0;                   // 8-bit keys: 16 bytes are the operands of two products
+  constexpr int kOStride = D + 4;
+  __shared__ __attribute__((aligned(16))) union Shared {
+    T v[4][32 * kStride];
+    float o[4][16 * kOStride];
+  } sh;
+  __shared__ float sh_m[4][kRows], sh_l[4][kRows];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n16 = lane & 15, quarter = lane >> 4;
+  unsigned block = blockIdx.x;
+  const int split = block % a.splits;
+  block /= a.splits;
+  const int head = block % a.kv_heads, tile = block / a.kv_heads;
+  Tile t;
+  if (!find_tile(a, tile, kRows, t)) return;
+
+  // keys that any row of the tile sees, and keys that all its rows see
+  const int last_row = min(t.row + kRows, t.rows) - 1;
+  int first_low, first_high, last_low, last_high;
+  limits(a, t, t.row / a.group, first_low, first_high);
+  limits(a, t, last_row / a.group, last_low, last_high);
+  const int all_low = last_low, all_high = first_high, high = last_high;
+  const int base = first_low & ~31;
+  const int begin = base + split * a.split_keys;
+  const int end = a.splits > 1 ? (int)min((long long)high, (long long)begin + a.split_keys) : high;
+
+  // this lane's rows
+  int low_r[kBlocks], high_r[kBlocks];
+  V8 q[kBlocks][kC];
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    const int r = t.row + 16 * b + n16;
+    const bool is = r < t.rows;
+    const int i = (is ? r : t.row) / a.group, h = (is ? r : t.row) - i * a.group;
+    limits(a, t, i, low_r[b], high_r[b]);
+    if (!is) high_r[b] = 0;
+    const T* from = (const T*)a.q + (int64_t)(t.token + i) * a.q_token + (int64_t)(head * a.group + h) * a.q_head;
+#pragma unroll
+    for (int c = 0; c < kC; c++) {
+      const int d = c < 2 * kPairs ? 64 * (c / 2) + 16 * quarter + 8 * (c & 1) : 32 * c + 8 * quarter;
+      if (a.q_vector) {
+        q[b][c] = *(const V8*)(from + d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) q[b][c][j] = from[d + j];
+      }
+    }
+  }
+
+  f4 o[kBlocks][D / 16];
+  float m[kBlocks], l[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 16; c++) o[b][c] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t* table = a.table + (int64_t)t.world * a.width;
+  const int page_mask = (1 << a.page_shift) - 1;
+
+  // The 16 keys from `key` on lie in one page: its number, or 0 with the keys marked absent
+  struct Keys {
+    int64_t at;           // first key's element / D
+    int left;             // keys up to `end`, less one (lanes beyond repeat the last)
+    bool is;
+  };
+  auto locate = [&](int key) {
+    Keys s;
+    const int from = min(key, (end - 1) & ~15);
+    const int page = table[from >> a.page_shift];
+    s.is = (unsigned)page < (unsigned)a.npage;
+    s.at = (((int64_t)(s.is ? page : 0) * a.kv_heads + head) << a.page_shift) + (from & page_mask);
+    s.left = end - 1 - from;
+    return s;
+  };
+
+  u4 kreg[2][kFp8 ? kPairs + 1 : kC];
+  u2 kodd[2];
+  unsigned kbyte[2][kFp8 ? kPairs + 1 : 1];
+  u4 vreg[kVLoads];
+  unsigned vbyte[kFp8 ? kVLoads : 1];
+  Keys keys[2];
+
+  auto load = [&](int key) {
+    keys[0] = locate(key);
+    keys[1] = locate(key + 16);
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const int64_t at = keys[s].at + min(n16, keys[s].left);
+      if constexpr (kFp8) {
+        const uint8_t* from = a.k + at * D;
+        const uint8_t* scale = a.k_scale + at * kC;
+#pragma unroll
+        for (int c = 0; c < kPairs; c++) {
+          kreg[s][c] = *(const u4*)(from + 64 * c + 16 * quarter);
+          kbyte[s][c] = scale[2 * c + (quarter >> 1)];
+        }
+        if constexpr (kC & 1) {
+          kodd[s] = *(const u2*)(from + 32 * (kC - 1) + 8 * quarter);
+          kbyte[s][kPairs] = scale[kC - 1];
+        }
+      } else {
+        const T* from = (const T*)a.k + at * D;
+#pragma unroll
+        for (int c = 0; c < kC; c++) kreg[s][c] = *(const u4*)(from + 32 * c + 8 * quarter);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kVLoads; j++) {
+      const int x = j * 64 + lane, key_in = x / (D / kVPer), d = (x - key_in * (D / kVPer)) * kVPer;
+      const Keys& s = keys[key_in >> 4];
+      const int64_t at = s.at + min(key_in & 15, s.left);
+      if constexpr (kFp8) {
+        vreg[j] = *(const u4*)(a.v + at * D + d);
+        vbyte[j] = a.v_scale[at * kC + d / 32];
+      } else {
+        vreg[j] = *(const u4*)((const T*)a.v + at * D + d);
+      }
+    }
+  };
+
+  T* vs = sh.v[wave];
+  typedef __attribute__((address_space(3))) s4* TrPtr;
+  int key = begin + 32 * wave;
+  if (key < end) load(key);
+  for (; key < end; key += 128) {
+    // scores
+    f4 s[kBlocks][2];
+    const bool is0 = keys[0].is, is1 = keys[1].is;
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) s[b][0] = s[b][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int c = 0; c < kC; c++) {
+        V8 x;
+        if constexpr (kFp8) {
+          if (c < 2 * kPairs) {
+            const u4 w = kreg[u][c / 2];
+            x = from_fp8<E>(c & 1 ? u2{w.z, w.w} : u2{w.x, w.y}, kbyte[u][c / 2]);
+          } else {
+            x = from_fp8<E>(kodd[u], kbyte[u][kPairs]);
+          }
+        } else {
+          x = __builtin_bit_cast(V8, kreg[u][c]);
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) s[b][u] = E::mfma16(x, q[b][c], s[b][u]);
+      }
+    }
+    // values into LDS, those of keys that do not exist as zeros
+    const bool edge = key < all_low || key + 32 > all_high || key + 32 > end || !is0 || !is1;
+    // an infinity or NaN among the values: added apart below, to the rows that see it (a remainder of a
+    // probability times an infinity is no remainder).  8-bit values have no infinity, and a NaN need not be
+    // kept from rows that all see it.
+    unsigned wild = 0;
+    V8 vx[kVLoads][kVPer / 8];
+#pragma unroll
+    for (int j = 0; j < kVLoads; j++) {
+      const int x = j * 64 + lane, key_in = x / (D / kVPer);
+      if constexpr (kFp8) {
+        vx[j][0] = from_fp8<E>(u2{vreg[j].x, vreg[j].y}, vbyte[j]);
+        vx[j][1] = from_fp8<E>(u2{vreg[j].z, vreg[j].w}, vbyte[j]);
+      } else {
+        vx[j][0] = __builtin_bit_cast(V8, vreg[j]);
+      }
+      const bool none = edge && (key + key_in >= end || !(key_in < 16 ? is0 : is1));
+#pragma unroll
+      for (int e = 0; e < kVPer / 8; e++) {
+        u4 words = __builtin_bit_cast(u4, vx[j][e]);
+        if (edge && none) words = u4{0, 0, 0, 0};
+        if (!kFp8 || edge)
+#pragma unroll
+          for (int y = 0; y < 4; y++) wild |= not_finite<E>(words[y]);
+        vx[j][e] = __builtin_bit_cast(V8, words);
+      }
+    }
+    const bool repair = __ballot((wild & 0x80008000u) != 0);
+    auto store = [&](bool clean) {
+#pragma unroll
+      for (int j = 0; j < kVLoads; j++) {
+        const int x = j * 64 + lane, key_in = x / (D / kVPer), d = (x - key_in * (D / kVPer)) * kVPer;
+#pragma unroll
+        for (int e = 0; e < kVPer / 8; e++) {
+          s8 bits = __builtin_bit_cast(s8, vx[j][e]);
+          if (clean) {
+#pragma unroll
+            for (int y = 0; y < 8; y++)
+              if ((bits[y] & E::kExponent) == E::kExponent) bits[y] = 0;
+          }
+          *(s8*)(vs + key_in * kStride + d + 8 * e) = bits;
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
+    store(repair);
+    // the next keys are on their way while these are weighed
+    const int now = key;
+    if (key + 128 < end) load(key + 128);
+
+    V8 p_high[kBlocks], p_low[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) {
+      float x[8], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float y = s[b][u][i] * a.scale2;
+          if (edge) {
+            const int at = now + 16 * u + 4 * quarter + i;
+            if (!(at >= low_r[b] && at < high_r[b] && at < end && (u ? is1 : is0))) y = -INFINITY;
+          }
+          x[4 * u + i] = y;
+          top = fmaxf(top, y);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float next = fmaxf(m[b], top), zero = next == -INFINITY ? 0.f : next;
+      const float shrink = __builtin_amdgcn_exp2f(m[b] - zero);
+      m[b] = next;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float p = __builtin_amdgcn_exp2f(x[j] - zero);
+        sum += p;
+        const T h = (T)p;
+        p_high[b][j] = h;
+        p_low[b][j] = (T)(p - (float)h);
+      }
+      l[b] = l[b] * shrink + sum;
+      if (__ballot(shrink != 1.f)) {
+#pragma unroll
+        for (int c = 0; c < D / 16; c++) o[b][c] *= shrink;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < D / 16; c++) {
+      const T* at = vs + (4 * quarter + (n16 >> 2)) * kStride + 16 * c + 4 * (n16 & 3);
+      const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TrPtr)at);
+      const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TrPtr)(at + 16 * kStride));
+      const V8 vt = __builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) {
+        o[b][c] = E::mfma16(vt, p_high[b], o[b][c]);
+        o[b][c] = E::mfma16(vt, p_low[b], o[b][c]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (repair) {
+      // rows that see a value that is not finite get it added; the others' products had a zero for it
+      store(false);
+      for (int k = 0; k < 32; k++) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+          const bool sees = now + k >= low_r[b] && now + k < high_r[b];
+#pragma unroll
+          for (int c = 0; c < D / 16; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float value = (float)vs[k * kStride + 16 * c + 4 * quarter + i];
+              if (sees && !(fabsf(value) < INFINITY)) o[b][c][i] += value;
+            }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+
+  // join the four waves, 16 rows at a time
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    l[b] += __shfl_xor(l[b], 16);
+    l[b] += __shfl_xor(l[b], 32);
+    if (quarter == 0) {
+      sh_m[wave][16 * b + n16] = m[b];
+      sh_l[wave][16 * b + n16] = l[b];
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    __syncthreads();
+    float top = fmaxf(fmaxf(sh_m[0][16 * b + n16], sh_m[1][16 * b + n16]),
+                      fmaxf(sh_m[2][16 * b + n16], sh_m[3][16 * b + n16]));
+    if (top == -INFINITY) top = 0.f;
+    const float shrink = __builtin_amdgcn_exp2f(m[b] - top);
+#pragma unroll
+    for (int c = 0; c < D / 16; c++) *(f4*)&sh.o[wave][n16 * kOStride + 16 * c + 4 * quarter] = o[b][c] * shrink;
+    __syncthreads();
+    for (int x = threadIdx.x; x < 16 * (D / 4); x += 256) {
+      const int row = x / (D / 4), d = (x - row * (D / 4)) * 4, r = t.row + 16 * b + row;
+      if (r >= t.rows) continue;
+      f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+      float most = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) most = fmaxf(most, sh_m[w][16 * b + row]);
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        sum += *(const f4*)&sh.o[w][row * kOStride + d];
+        total += sh_l[w][16 * b + row] * __builtin_amdgcn_exp2f(sh_m[w][16 * b + row] - (most == -INFINITY ? 0.f : most));
+      }
+      const int i = r / a.group, h = head * a.group + (r - i * a.group);
+      const int64_t row_at = (int64_t)(t.token + i) * a.heads + h;
+      if (a.splits > 1) {
+        const int64_t at = (int64_t)split * a.tokens * a.heads + row_at;
+        if (total != 0.f) *(f4*)(a.part + at * D + d) = sum;
+        if (d == 0) *(f2*)(a.part_ml + 2 * at) = f2{most, total};
+      } else {
+        const float inverse = 1.f / total;
+        T* to = (T*)a.out + (int64_t)(t.token + i) * a.o_token + (int64_t)h * a.o_head + d;
+#pragma unroll
+        for (int e = 0; e < 4; e++) to[e] = (T)(total == 0.f ? 0.f : sum[e] * inverse);
+        if (a.lse && d == 0) a.lse[row_at] = total == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(total)) * kLn2;
+      }
+    }
+  }
+}
+
+}  // namespace mxe

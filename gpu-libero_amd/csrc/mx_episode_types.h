@@ -1,0 +1,155 @@
+// Element types, matrix instructions and 8-bit conversions of the episode memory's kernels (gfx950),
+// and what the kernels share: arguments, chunk lookup, row limits.
+//
+// Lane layouts used below (l = lane; checked by running them against plain products):
+//   16x16x32: A row l % 16, k = 8 (l / 16) + j; B column l % 16, same k; C column l % 16, rows 4 (l / 16) + i.
+//   32x32x16: A row l % 32, k = 8 (l / 32) + j; B column l % 32, same k; C column l % 32,
+//             rows 8 (i / 4) + 4 (l / 32) + i % 4.
+//   ds_read_tr16_b64: the 16 lanes of a group each address 8 bytes, four lanes to a row of 16 values;
+//             lane i of the group receives column i of the four rows.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include "../../include/mx_physics.h"
+#include "../../include/mx_episode.h"
+
+namespace mxe {
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 hf4 __attribute__((ext_vector_type(4)));
+typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int kType> struct Elem;
+template <> struct Elem<MX_TYPE_BF16> {
+  typedef __bf16 T;
+  typedef bf8 V8;
+  typedef bf2 V2;
+  static constexpr unsigned kExponent = 0x7f80;   // all ones in an infinity or NaN
+  static __device__ f4 mfma16(V8 a, V8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ f16v mfma32(V8 a, V8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  // two e4m3 codes (low or high half of w) times a power of two; exact: three fraction bits
+  template <bool kHigh> static __device__ V2 from_fp8(unsigned w, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHigh);
+  }
+};
+template <> struct Elem<MX_TYPE_F16> {
+  typedef _Float16 T;
+  typedef hf8 V8;
+  typedef hf2 V2;
+  static constexpr unsigned kExponent = 0x7c00;
+  static __device__ f4 mfma16(V8 a, V8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ f16v mfma32(V8 a, V8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  // exact from 2^-24 up to 65504, as any value of the queries' type
+  template <bool kHigh> static __device__ V2 from_fp8(unsigned w, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, kHigh);
+  }
+};
+
+// Two 16-bit values in a word: the top bit of each half is set if it is an infinity or NaN (an exponent of
+// all ones carries into the sign's place when its last bit is added; other bits mean nothing)
+template <class E> __device__ inline unsigned not_finite(unsigned w) {
+  constexpr unsigned e = E::kExponent | E::kExponent << 16, last = E::kExponent & -E::kExponent;
+  return (w & e) + (last | last << 16);
+}
+
+// E8M0: byte b stands for 2^(b - 127); 255 for NaN, which the codes then carry (nan_codes)
+__device__ inline float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
+__device__ inline unsigned nan_codes(unsigned w, unsigned byte) { return byte == 255 ? 0x7f7f7f7fu : w; }
+
+template <class E> __device__ inline typename E::V8 from_fp8(u2 w, unsigned byte) {
+  typedef typename E::V8 V8;
+  const float s = scale_of(byte == 255 ? 127 : byte);
+  w.x = nan_codes(w.x, byte);
+  w.y = nan_codes(w.y, byte);
+  const auto a = E::template from_fp8<false>(w.x, s), b = E::template from_fp8<true>(w.x, s);
+  const auto c = E::template from_fp8<false>(w.y, s), d = E::template from_fp8<true>(w.y, s);
+  V8 r;
+  r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1];
+  r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+  return r;
+}
+
+// The kernels' arguments, by value.  `rows` are (token, head of the group) pairs of one key head, in
+// the order token * group + head, in tiles of a kernel's own number of rows.
+struct Attend {
+  const uint8_t *k, *v, *k_scale, *v_scale;
+  const int32_t *table, *length, *start;
+  const void* q;
+  void* out;
+  float *lse, *part, *part_ml;       // part: [split][token][head][D]; part_ml: [split][token][head][2]
+  int64_t q_token, q_head, o_token, o_head;
+  int nworld, npage, width, kv_heads, page_shift, tokens, count, max_count, heads, group;
+  int causal, window, tiles, splits, split_keys;
+  float scale2;                      // scale * log2(e): probabilities are powers of two
+  bool q_vector;                     // q's rows are 16-byte aligned
+};
+
+// The world of a tile.  Ragged chunks: world w has the tile numbers from start[w] group / rows + w on,
+// at least as many as its rows need, so that the tile of a block follows from `start` by a search,
+// 64 probes at a time, and the number of tiles from sizes that the host knows.
+struct Tile {
+  int world, row, rows, token, length, position;   // first row, rows in all, first packed token, tokens
+                                                   // in reach, position of the chunk's first token
+};
+
+__device__ inline long long tile_base(const Attend& a, int w, int rows_per_tile) {
+  return (long long)a.start[w] * a.group / rows_per_tile + w;
+}
+
+__device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, Tile& t) {
+  int count, token;
+  if (!a.start) {
+    const int per = (a.max_count * a.group + rows_per_tile - 1) / rows_per_tile;
+    t.world = tile / per;
+    t.row = (tile - t.world * per) * rows_per_tile;
+    token = t.world * a.count;
+    count = a.count;
+  } else {
+    const int lane = threadIdx.x & 63;
+    int low = 0, high = a.nworld;
+    while (high - low > 1) {
+      const int step = (high - low + 63) >> 6, probe = low + lane * step;
+      const bool below = probe < high && tile_base(a, probe, rows_per_tile) <= tile;
+      const int passed = max(1, (int)__popcll(__ballot(below)));
+      low += (passed - 1) * step;
+      high = min(high, low + step);
+    }
+    low = __builtin_amdgcn_readfirstlane(low);
+    t.world = low;
+    const long long row = (tile - tile_base(a, low, rows_per_tile)) * rows_per_tile;
+    token = a.start[low];
+    const int end = min(a.start[low + 1], a.tokens);
+    if (token < 0 || end <= token || row < 0 || row >= (long long)(end - token) * a.group) return false;
+    t.row = (int)row;
+    count = a.start[low + 1] - token;
+    t.rows = (int)min((long long)min(end - token, a.max_count) * a.group, (long long)INT32_MAX);
+  }
+  if (!a.start) t.rows = a.max_count * a.group;
+  if (t.row >= t.rows) return false;
+  t.token = token;
+  const int length = max(a.length[t.world], 0);
+  t.position = length - count;
+  t.length = (int)min((long long)length, (long long)a.width << a.page_shift);
+  return true;
+}
+
+// The keys [low, high) that the chunk's token i sees
+__device__ inline void limits(const Attend& a, const Tile& t, int i, int& low, int& high) {
+  const int position = t.position + i;
+  high = position < 0 ? 0 : a.causal ? min(position + 1, t.length) : t.length;
+  low = a.window > 0 ? max(0, position - a.window + 1) : 0;
+}
+
+}  // namespace mxe

@@ -19,6 +19,7 @@
 #include <cmath>
 #include <mutex>
 #include "../../include/mx_physics.h"
+#include "../../include/mx_episode.h"
 #include "mx_math.h"
 #include "mx_image.h"
 #include "mx_collide.h"
@@ -5700,6 +5701,7 @@ const char* mx_error_string(int code) {
     case MX_ERR_DOMAIN: return "model outside the admitted domain";
     case MX_ERR_LDS: return "per-world working set exceeds the LDS budget and no (or too small a) workspace is given";
     case MX_ERR_SCRATCH: return "the batch's workspace slabs exceed the library's fixed device scratch (MX_SCRATCH_BYTES per device)";
+    case MX_ERR_WORKSPACE: return "workspace missing, misaligned or smaller than mx_episode_workspace";
     default: return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown error";
   }
 }

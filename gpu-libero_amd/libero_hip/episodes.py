@@ -1,0 +1,249 @@
+"""Episode memory: the keys and values of every world's running episode, and attention over them.
+
+A policy that steps a batch of worlds keeps, per attention layer, the keys and values of the tokens that
+each world's episode has brought so far (instruction, observations, actions).  The worlds of a batch share
+pages of that memory: worlds differ in how far their episodes are, and a reset gives one world's pages back.
+
+Operators (``include/mx_episode.h``, on the current stream or ``stream``; they can be captured into a HIP
+graph, and read ``table``, ``length`` and ``start`` on the device):
+
+* :func:`write` stores a chunk's keys and values in the pages, in 16 bits or quantised to 8;
+* :func:`read` returns them as the pages stand for them;
+* :func:`attend` attends from the chunk's queries to all tokens of their worlds.
+
+A chunk is the last tokens of each world's ``length``: ``(nworld, n, heads, head_dim)``, the same number
+for every world, or packed rows ``(tokens, heads, head_dim)`` with ``start`` (int32, ``nworld + 1``): world
+w has the rows ``start[w]:start[w + 1]``.
+
+:class:`Pages` holds the tensors of one layer; :class:`EpisodeCache` keeps the pages of several layers, the
+worlds' tables and lengths, and hands out pages.  The reference has no counterpart: its policies
+(``libero/lifelong/``) recompute their history at every step.
+"""
+from __future__ import annotations
+
+import ctypes as ct
+import math
+
+import numpy as np
+import torch
+
+from . import native
+
+SCALE_BLOCK = 32                      # values along head_dim that share a scale in 8-bit pages
+HEAD_DIMS = (32, 64, 96, 128, 256)
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+_SIZES = {0: 4, 1: 2, 2: 2, 3: 1}
+STORAGE = {'bf16': torch.bfloat16, 'f16': torch.float16, 'fp8': torch.float8_e4m3fn}
+
+EXPORTS = ['mx_pages_bytes', 'mx_chunk_bytes', 'mx_rows_bytes', 'mx_attention_bytes', 'mx_episode_write',
+           'mx_episode_read', 'mx_episode_attend', 'mx_episode_workspace']
+
+
+class MxPages(ct.Structure):
+    _fields_ = ([(n, ct.c_void_p) for n in ('k', 'v', 'k_scale', 'v_scale', 'table', 'length')]
+                + [(n, ct.c_int32) for n in ('nworld', 'npage', 'width', 'kv_heads', 'head_dim', 'page_tokens', 'type')])
+
+
+class MxChunk(ct.Structure):
+    _fields_ = [('start', ct.c_void_p), ('tokens', ct.c_int32), ('count', ct.c_int32)]
+
+
+class MxRows(ct.Structure):
+    _fields_ = [('data', ct.c_void_p), ('token_stride', ct.c_int64), ('head_stride', ct.c_int64),
+                ('heads', ct.c_int32), ('type', ct.c_int32)]
+
+
+class MxAttention(ct.Structure):
+    _fields_ = [('q', MxRows), ('out', MxRows), ('lse', ct.c_void_p), ('workspace', ct.c_void_p),
+                ('workspace_bytes', ct.c_size_t), ('max_count', ct.c_int32), ('causal', ct.c_int32),
+                ('window', ct.c_int32), ('scale', ct.c_float)]
+
+
+_LIB = None
+
+
+def load():
+    """The library, with the episode memory's entry points bound and their structs' sizes checked."""
+    global _LIB
+    if _LIB is None:
+        lib = native.load()
+        for name, struct in (('pages', MxPages), ('chunk', MxChunk), ('rows', MxRows), ('attention', MxAttention)):
+            f = getattr(lib, 'mx_%s_bytes' % name)
+            f.restype = ct.c_size_t
+            if f() != ct.sizeof(struct):
+                raise ImportError('libmx_physics struct sizes differ from the Python mirror')
+        lib.mx_episode_write.argtypes = lib.mx_episode_read.argtypes = [ct.c_void_p] * 5
+        lib.mx_episode_attend.argtypes = [ct.c_void_p] * 4
+        lib.mx_episode_workspace.argtypes = [ct.c_void_p] * 3
+        lib.mx_episode_workspace.restype = ct.c_size_t
+        _LIB = lib
+    return _LIB
+
+
+def _require(ok, message, *args):
+    if not ok:
+        raise ValueError(message % args)
+
+
+class Pages:
+    """One layer's pages and the worlds' tables into them.
+
+    ``k``, ``v``: (npage, kv_heads, page_tokens, head_dim), bfloat16, float16, or float8_e4m3fn with
+    ``k_scale``, ``v_scale``: (npage, kv_heads, page_tokens, head_dim / 32) uint8, the exponent of each
+    block's scale (2^(byte - 127); 255: the block is NaN).  ``table``: (nworld, pages of a world) int32, token t of world w is in
+    page ``table[w, t // page_tokens]``; ``length``: (nworld,) int32, the worlds' tokens.  page_tokens is a power
+    of two from 16 to 4096, head_dim one of 32, 64, 96, 128, 256.  The tensors stay the caller's, and are
+    held here."""
+
+    __slots__ = ('k', 'v', 'table', 'length', 'k_scale', 'v_scale', 'struct', 'device')
+
+    def __init__(self, k, v, table, length, k_scale=None, v_scale=None):
+        _require(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype,
+                 'k and v pages must have one shape (npage, kv_heads, page_tokens, head_dim) and type')
+        kind = _TYPES.get(k.dtype, 0)
+        _require(kind > 0, 'pages must be bfloat16, float16 or float8_e4m3fn, got %s', k.dtype)
+        npage, kv, tokens, dim = k.shape
+        _require(dim in HEAD_DIMS, 'head_dim must be one of %s, got %d', HEAD_DIMS, dim)
+        _require(16 <= tokens <= 4096 and not tokens & (tokens - 1),
+                 'page_tokens must be a power of two from 16 to 4096, got %d', tokens)
+        _require(npage > 0 and 0 < kv <= 1024, 'pages need at least one page and 1 to 1024 heads')
+        device = k.device
+        _require(device.type == 'cuda', 'pages must be on the GPU')
+        _require(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.numel() > 0,
+                 'table must be contiguous int32 of shape (nworld, pages of a world)')
+        _require(length.dtype == torch.int32 and length.shape == table.shape[:1] and length.is_contiguous(),
+                 'length must be contiguous int32 of shape (nworld,)')
+        _require(npage * tokens < 2 ** 31 and table.shape[1] * tokens < 2 ** 31,
+                 'npage * page_tokens and the tokens of a table row must be below 2^31')
+        _require(k.is_contiguous() and v.is_contiguous() and not (k.data_ptr() | v.data_ptr()) & 15,
+                 'pages must be contiguous and 16-byte aligned')
+        if kind == 3:
+            shape = (npage, kv, tokens, dim // SCALE_BLOCK)
+            for s in (k_scale, v_scale):
+                _require(s is not None and s.dtype == torch.uint8 and s.shape == shape and s.is_contiguous(),
+                         '8-bit pages need contiguous uint8 scales of shape %s', shape)
+        else:
+            _require(k_scale is None and v_scale is None, 'only 8-bit pages have scales')
+        for t in (v, table, length, k_scale, v_scale):
+            _require(t is None or t.device == device, 'pages, scales, table and length must be on one device')
+        self.k, self.v, self.table, self.length, self.k_scale, self.v_scale = k, v, table, length, k_scale, v_scale
+        self.device = device
+        self.struct = MxPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if kind == 3 else None,
+                              v_scale.data_ptr() if kind == 3 else None, table.data_ptr(), length.data_ptr(),
+                              table.shape[0], npage, table.shape[1], kv, dim, tokens, kind)
+
+
+def _chunk(pages, shape, start):
+    """MxChunk of rows of this shape (without heads and head_dim)."""
+    nworld = pages.struct.nworld
+    if start is None:
+        _require(len(shape) == 2 and shape[0] == nworld,
+                 'rows must be (nworld, n, heads, head_dim), or packed (tokens, heads, head_dim) with start')
+        return MxChunk(None, shape[0] * shape[1], shape[1])
+    _require(len(shape) == 1, 'rows with start must be packed: (tokens, heads, head_dim)')
+    _require(start.dtype == torch.int32 and start.shape == (nworld + 1,) and start.is_contiguous()
+             and start.device == pages.device, 'start must be contiguous int32 of shape (nworld + 1,) on the pages\' device')
+    return MxChunk(start.data_ptr(), shape[0], 0)
+
+
+def _rows(pages, x, heads, name):
+    """MxRows of a tensor (..., heads, head_dim) whose token dimensions step evenly."""
+    kind = _TYPES.get(x.dtype, 3)
+    _require(kind < 3, '%s must be float32, bfloat16 or float16, got %s', name, x.dtype)
+    shape, stride = x.shape, x.stride()
+    _require(len(shape) in (3, 4) and shape[-1] == pages.struct.head_dim and (heads is None or shape[-2] == heads),
+             '%s has the wrong heads or head_dim: %s', name, tuple(shape))
+    _require(x.device == pages.device, '%s must be on the pages\' device', name)
+    _require(stride[-1] == 1 or shape[-1] == 1, '%s must be contiguous along head_dim', name)
+    if len(shape) == 4:
+        _require(shape[0] <= 1 or shape[1] == 0 or stride[0] == shape[1] * stride[1],
+                 '%s: the rows of all worlds must step evenly', name)
+        token = stride[1] if shape[1] > 1 or shape[0] <= 1 else stride[0]
+    else:
+        token = stride[0]
+    return MxRows(x.data_ptr(), token, stride[-2], shape[-2], kind)
+
+
+def _on(pages, stream):
+    if stream is None:
+        stream = torch.cuda.current_stream(pages.device)
+    return stream.cuda_stream
+
+
+def write(pages, k, v, start=None, *, stream=None):
+    """Store the chunk's keys and values (float32, bfloat16 or float16; any strides whose tokens step evenly
+    and whose head_dim is contiguous).  8-bit pages take, per 32 values along head_dim, the least power of two
+    at which all are within the codes' range, and round to nearest even; a block with an infinity or NaN
+    is stored as NaN.  Chunk tokens without a place (a chunk longer than its world's length, a table entry
+    that names no page) are left out."""
+    s = pages.struct
+    _require(k.shape == v.shape and k.dtype == v.dtype, 'k and v must have one shape and type')
+    chunk = _chunk(pages, k.shape[:-2], start)
+    a, b = _rows(pages, k, s.kv_heads, 'k'), _rows(pages, v, s.kv_heads, 'v')
+    with torch.cuda.device(pages.device):
+        native.check(load().mx_episode_write(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b),
+                                             _on(pages, stream)), 'mx_episode_write')
+
+
+def read(pages, start=None, *, count=None, tokens=None, dtype=torch.bfloat16, stream=None):
+    """The chunk's keys and values: ``(nworld, count, kv_heads, head_dim)``, or packed ``(tokens, kv_heads,
+    head_dim)`` with ``start``; each value rounded once to ``dtype``.  Tokens without a place read as zeros."""
+    s = pages.struct
+    _require(dtype in _TYPES and dtype != torch.float8_e4m3fn, 'read returns float32, bfloat16 or float16')
+    if start is None:
+        _require(count is not None and tokens is None and count >= 0, 'give count (every world), or start and tokens')
+        shape = (s.nworld, count)
+    else:
+        _require(tokens is not None and count is None and tokens >= 0, 'give count (every world), or start and tokens')
+        shape = (tokens,)
+    chunk = _chunk(pages, shape, start)
+    with torch.cuda.device(pages.device), torch.cuda.stream(stream):
+        k, v = (torch.empty(shape + (s.kv_heads, s.head_dim), dtype=dtype, device=pages.device) for _ in range(2))
+        a, b = _rows(pages, k, s.kv_heads, 'k'), _rows(pages, v, s.kv_heads, 'v')
+        native.check(load().mx_episode_read(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b),
+                                            _on(pages, stream)), 'mx_episode_read')
+    return k, v
+
+
+def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale=None, out=None, lse=None,
+           stream=None):
+    """Softmax attention of the chunk's queries over their worlds' tokens, in 32 bits.
+
+    Query head h uses key head ``h // (heads / kv_heads)``.  The query at position p (of its world's tokens)
+    sees the tokens ``j <= p``, or with ``causal=False`` all of them (a step's tokens see each other), and
+    with ``window`` > 0 only those with ``j > p - window``.  ``scale``: 1 / sqrt(head_dim) by default.  A query
+    that sees nothing gives zeros (and ``lse`` -inf).  ``q`` is bfloat16 or float16, the pages' type unless
+    those are 8-bit.  ``max_count`` (with ``start``): the largest chunk of a world, if known; rows beyond it are
+    not computed.  ``out`` (like q) and ``lse`` (float32, q's shape without head_dim, contiguous) are written
+    if given.  Returns out.  The same inputs give the same bits."""
+    s = pages.struct
+    chunk = _chunk(pages, q.shape[:-2], start)
+    rows = _rows(pages, q, None, 'q')
+    heads = rows.heads
+    _require(rows.type in (1, 2) and (s.type == 3 or s.type == rows.type),
+             'q must be bfloat16 or float16, and of the pages\' type unless those are 8-bit: %s on %s', q.dtype, pages.k.dtype)
+    _require(heads > 0 and heads % s.kv_heads == 0, 'q has %d heads, not a multiple of the pages\' %d', heads, s.kv_heads)
+    _require(0 <= window < 2 ** 31, 'window must be 0 (none) or a number of tokens, got %s', window)
+    scale = 1.0 / math.sqrt(s.head_dim) if scale is None else float(scale)
+    _require(math.isfinite(scale), 'scale must be finite')
+    if max_count is None:
+        max_count = chunk.tokens if start is not None else chunk.count
+    _require(0 <= max_count < 2 ** 31, 'max_count must be a number of tokens, got %s', max_count)
+    with torch.cuda.device(pages.device), torch.cuda.stream(stream):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=pages.device)
+        else:
+            _require(out.shape == q.shape and out.dtype == q.dtype, 'out must have q\'s shape and type')
+        if lse is not None:
+            _require(lse.dtype == torch.float32 and lse.shape == q.shape[:-1] and lse.is_contiguous()
+                     and lse.device == pages.device, 'lse must be contiguous float32 of q\'s shape without head_dim')
+        a = MxAttention(rows, _rows(pages, out, heads, 'out'), None if lse is None else lse.data_ptr(), None, 0,
+                        max_count, int(bool(causal)), window, scale)
+        lib = load()
+        need = lib.mx_episode_workspace(ct.byref(s), ct.byref(chunk), ct.byref(a))
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=pages.device)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+        native.check(lib.mx_episode_attend(ct.byref(s), ct.byref(chunk), ct.byref(a), _on(pages, stream)),
+                     'mx_episode_attend')
+    return out
