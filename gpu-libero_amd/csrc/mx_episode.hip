@@ -1,5 +1,6 @@
 // The episode memory's entry points: writing to and reading from the pages, joining the parts of a
 // split attention, and the host side of all four calls.
+#include <cmath>
 #include <type_traits>
 #include "mx_episode_types.h"
 #include "mx_episode_launch.h"
@@ -227,9 +228,9 @@ int chunk_check(const MxPages* p, const MxChunk* c) {
   return 0;
 }
 
-bool rows_aligned(const MxRows* r) {
+bool rows_aligned(const MxRows* r, int bytes) {
   const int64_t s = size_of(r->type);
-  return !(((uintptr_t)r->data | (uintptr_t)(r->token_stride * s) | (uintptr_t)(r->head_stride * s)) & 15);
+  return !(((uintptr_t)r->data | (uintptr_t)(r->token_stride * s) | (uintptr_t)(r->head_stride * s)) & (bytes - 1));
 }
 
 int rows_check(const MxRows* r, int heads, bool any) {
@@ -257,7 +258,7 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
   uint8_t *pages[2] = {(uint8_t*)p->k, (uint8_t*)p->v}, *scales[2] = {p->k_scale, p->v_scale};
   for (int i = 0; i < 2; i++)
     a.of[i] = Copy{pages[i], scales[i], (const uint8_t*)rows[i]->data, rows[i]->token_stride, rows[i]->head_stride,
-                   rows_aligned(rows[i])};
+                   rows_aligned(rows[i], 16)};
   a.table = p->table; a.length = p->length; a.start = c->start;
   a.nworld = p->nworld; a.npage = p->npage; a.width = p->width; a.kv_heads = p->kv_heads;
   a.page_shift = page_shift(p); a.tokens = c->tokens; a.count = c->count;
@@ -301,8 +302,12 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   a.nworld = p->nworld; a.npage = p->npage; a.width = p->width; a.kv_heads = p->kv_heads;
   a.page_shift = page_shift(p); a.tokens = c->tokens; a.count = c->count;
   a.heads = heads; a.group = heads / p->kv_heads;
-  a.causal = m->causal != 0; a.window = m->window; a.scale2 = m->scale * kLog2e;
-  a.q_vector = rows_aligned(&m->q);
+  a.causal = m->causal != 0; a.window = m->window; 
+  // a scale of 0 becomes one that no score is noticed under: a hidden key's -infinity has to stay
+  a.scale2 = fmaxf(fabsf(m->scale) * kLog2e, 1e-37f);
+  a.negate = m->scale < 0.f;
+  a.q_vector = rows_aligned(&m->q, 16);
+  a.o_vector = rows_aligned(&m->out, 8);
   const int most = c->start ? m->max_count : (m->max_count < c->count ? m->max_count : c->count);
   a.max_count = most < c->tokens ? most : c->tokens;
   launch.tiles = 0;
@@ -320,6 +325,7 @@ int choose(Attend& a, Launch& launch) {
   const int64_t rows = (int64_t)a.max_count * a.group;
   launch.blocks = rows <= 16 ? 1 : rows <= 32 || launch.head_dim == 256 ? 2 : 4;
   launch.rows = 16 * launch.blocks;
+  if (rows > 64 && launch.head_dim <= 128) launch.rows = kManyRows;
   const int64_t tiles = a.start ? (int64_t)a.tokens * a.group / launch.rows + a.nworld
                                 : ((rows + launch.rows - 1) / launch.rows) * a.nworld;
   int64_t keys = (int64_t)a.width << a.page_shift;

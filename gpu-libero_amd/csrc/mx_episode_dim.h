@@ -1,6 +1,7 @@
 // The attention kernels of one head_dim, and their launcher.
 #pragma once
 #include "mx_episode_few.h"
+#include "mx_episode_many.h"
 #include "mx_episode_launch.h"
 
 namespace mxe {
@@ -9,6 +10,11 @@ template <int D, int kType, bool kFp8>
 int attend_typed(const Attend& a, const Launch& launch, void* stream) {
   const dim3 grid(launch.grid), block(256);
   const hipStream_t s = (hipStream_t)stream;
+  if constexpr (D <= 128)
+    if (launch.rows == kManyRows) {
+      hipLaunchKernelGGL((attend_many<kType, kFp8, D>), grid, block, 0, s, a);
+      return (int)hipGetLastError();
+    }
   if (launch.blocks == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1>), grid, block, 0, s, a);
   else if (launch.blocks == 2) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2>), grid, block, 0, s, a);
   else if constexpr (D <= 128) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 4>), grid, block, 0, s, a);

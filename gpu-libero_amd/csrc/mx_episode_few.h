@@ -63,12 +63,7 @@ __global__ __launch_bounds__(256) void attend_few(const Attend a) {
 #pragma unroll
     for (int c = 0; c < kC; c++) {
       const int d = c < 2 * kPairs ? 64 * (c / 2) + 16 * quarter + 8 * (c & 1) : 32 * c + 8 * quarter;
-      if (a.q_vector) {
-        q[b][c] = *(const V8*)(from + d);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) q[b][c][j] = from[d + j];
-      }
+      q[b][c] = load_query<E>(a, from + d);
     }
   }
 

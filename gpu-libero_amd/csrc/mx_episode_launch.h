@@ -5,6 +5,8 @@
 
 namespace mxe {
 
+constexpr int kManyRows = 128;              // rows of a tile of attend_many
+
 struct Launch {
   int type, head_dim, blocks, rows, tiles;    // blocks of 16 rows to a tile
   bool fp8;

@@ -92,9 +92,32 @@ struct Attend {
   int64_t q_token, q_head, o_token, o_head;
   int nworld, npage, width, kv_heads, page_shift, tokens, count, max_count, heads, group;
   int causal, window, tiles, splits, split_keys;
-  float scale2;                      // scale * log2(e): probabilities are powers of two
-  bool q_vector;                     // q's rows are 16-byte aligned
+  float scale2;                      // |scale| * log2(e), not 0: probabilities are powers of two
+  bool negate;                       // scale < 0: the queries change their sign
+  bool q_vector, o_vector;           // q's rows are 16-byte aligned, out's 8-byte
 };
+
+// Eight values of a query
+template <class E> __device__ inline typename E::V8 load_query(const Attend& a, const typename E::T* from) {
+  typename E::V8 x;
+  if (a.q_vector) {
+    x = *(const typename E::V8*)from;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = from[j];
+  }
+  return a.negate ? -x : x;
+}
+
+// One value of V: of the key at element `at` / D of its pages
+template <class E, bool kFp8, int D> __device__ inline float value_at(const Attend& a, int64_t at, int d) {
+  if constexpr (kFp8) {
+    const unsigned byte = a.v_scale[at * (D / 32) + d / 32];
+    return (float)E::template from_fp8<false>(nan_codes(a.v[at * D + d], byte), scale_of(byte == 255 ? 127 : byte))[0];
+  } else {
+    return (float)((const typename E::T*)a.v)[at * D + d];
+  }
+}
 
 // The world of a tile.  Ragged chunks: world w has the tile numbers from start[w] group / rows + w on,
 // at least as many as its rows need, so that the tile of a block follows from `start` by a search,
