@@ -9,7 +9,7 @@ namespace mxe {
 
 // ---------------------------------------------------------------------------- write and read
 struct Copy {
-  uint8_t *pages, *scales;       // of k (blockIdx.y = 0) or v
+  uint8_t *pages, *scales;       // of k or v
   const uint8_t* rows;
   int64_t token_stride, head_stride;
   bool vector;                   // rows are 16-byte aligned
@@ -17,27 +17,13 @@ struct Copy {
 struct Move {
   Copy of[2];
   const int32_t *table, *length, *start;
-  int nworld, npage, width, kv_heads, page_shift, tokens, count;
+  int nworld, npage, width, kv_heads, head_dim, page_shift, tokens, count, tokens_each;
 };
 
-// The slot of packed row `token`, as (page * kv_heads * page_tokens + slot) without the head; -1: none
-__device__ inline int64_t slot_of(const Move& a, int token) {
-  int world, place, count;
-  if (!a.start) {
-    world = token / a.count;
-    place = token - world * a.count;
-    count = a.count;
-  } else {
-    int low = 0, high = a.nworld;
-    while (high - low > 1) {
-      const int middle = (low + high) >> 1;
-      if (a.start[middle] <= token) low = middle; else high = middle;
-    }
-    world = low;
-    place = token - a.start[low];
-    count = a.start[low + 1] - a.start[low];
-    if (place < 0 || place >= count) return -1;
-  }
+// The slot of packed row `token` of a world's chunk, as (page * kv_heads * page_tokens + slot) without the
+// head; -1: none
+__device__ inline int64_t slot_of(const Move& a, int world, int place, int count) {
+  if (place < 0 || place >= count) return -1;
   const int position = max(a.length[world], 0) - count + place;
   if (position < 0 || (position >> a.page_shift) >= a.width) return -1;
   const int page = a.table[(int64_t)world * a.width + (position >> a.page_shift)];
@@ -45,117 +31,173 @@ __device__ inline int64_t slot_of(const Move& a, int token) {
   return (((int64_t)page * a.kv_heads) << a.page_shift) + (position & ((1 << a.page_shift) - 1));
 }
 
-template <class T> __device__ inline void load8(const T* from, bool vector, float (&x)[8]) {
-  if (vector) {
-    if constexpr (sizeof(T) == 4) {
-      const f4 a = *(const f4*)from, b = *(const f4*)(from + 4);
-#pragma unroll
-      for (int j = 0; j < 4; j++) x[j] = a[j], x[4 + j] = b[j];
-    } else {
-      typedef T T8 __attribute__((ext_vector_type(8)));
-      const T8 a = *(const T8*)from;
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = (float)a[j];
+// The slots of `tokens` (at most 64) packed rows from `first` on, by the lanes of one wave.  Ragged chunks:
+// the first row's world by a search with 64 probes at a time, the others' from there, mostly the same.
+__device__ inline void find_slots(const Move& a, int first, int tokens, int64_t* slots) {
+  const int lane = threadIdx.x, token = first + lane;
+  if (!a.start) {
+    if (lane < tokens) {
+      const int world = token / a.count;
+      slots[lane] = slot_of(a, world, token - world * a.count, a.count);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = (float)from[j];
+    return;
+  }
+  int low = 0, high = a.nworld;
+  while (high - low > 1) {
+    const int step = (high - low + 63) >> 6, probe = low + lane * step;
+    const int passed = max(1, (int)__popcll(__ballot(probe < high && a.start[probe] <= first)));
+    low += (passed - 1) * step;
+    high = min(high, low + step);
+  }
+  if (lane < tokens) {
+    if (a.start[low + 1] <= token) {
+      high = a.nworld;
+      while (high - low > 1) {
+        const int middle = (low + high) >> 1;
+        if (a.start[middle] <= token) low = middle; else high = middle;
+      }
+    }
+    slots[lane] = slot_of(a, low, token - a.start[low], a.start[low + 1] - a.start[low]);
   }
 }
 
-// One thread moves eight values of one head of one token; the four threads of a scale's block are
-// neighbours.  Bound by memory; nothing is shared, so threads go in the order of the rows.
-template <class T, int kStore>
-__global__ __launch_bounds__(256) void write_rows(const Move a, int head_dim) {
-  const Copy c = a.of[blockIdx.y];
-  const int per = head_dim / 8;
-  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = item / per;
-  const int d = (int)(item - row * per) * 8;
-  const int64_t token = row / a.kv_heads;
-  const int head = (int)(row - token * a.kv_heads);
-  if (token >= a.tokens) return;                        // whole blocks of four threads leave together
-  const int64_t slot = slot_of(a, (int)token);
-  if (slot < 0) return;
-  float x[8];
-  load8((const T*)c.rows + token * c.token_stride + head * c.head_stride + d, c.vector, x);
-  const int64_t at = slot + ((int64_t)head << a.page_shift);
+template <class T, int N> __device__ inline void load_row(const T* from, bool vector, float (&x)[N]) {
+  if (vector) {
+    constexpr int kEach = 16 / sizeof(T);
+    typedef T V __attribute__((ext_vector_type(kEach)));
+#pragma unroll
+    for (int j = 0; j < N; j += kEach) {
+      const V v = *(const V*)(from + j);
+#pragma unroll
+      for (int e = 0; e < kEach; e++) x[j + e] = (float)v[e];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j++) x[j] = (float)from[j];
+  }
+}
+
+template <class T, int N> __device__ inline void store_row(T* to, bool vector, const float (&x)[N]) {
+  if (vector) {
+    constexpr int kEach = 16 / sizeof(T);
+    typedef T V __attribute__((ext_vector_type(kEach)));
+#pragma unroll
+    for (int j = 0; j < N; j += kEach) {
+      V v;
+#pragma unroll
+      for (int e = 0; e < kEach; e++) v[e] = (T)x[j + e];
+      *(V*)(to + j) = v;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j++) to[j] = (T)x[j];
+  }
+}
+
+// `at`: element in the pages; at / 32 is the scale's place, as head_dim is a multiple of 32
+template <int kStore, int N> __device__ inline void load_page(const Copy& c, int64_t at, float (&x)[N]) {
+  if constexpr (kStore == MX_TYPE_FP8) {
+    const u4 w = *(const u4*)(c.pages + at);
+    const unsigned byte = c.scales[at / MX_SCALE_BLOCK];
+    const float scale = byte == 255 ? NAN : __uint_as_float(byte ? byte << 23 : 0x400000u);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const f2 p = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false), q = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
+      x[4 * j] = p[0] * scale;
+      x[4 * j + 1] = p[1] * scale;
+      x[4 * j + 2] = q[0] * scale;
+      x[4 * j + 3] = q[1] * scale;
+    }
+  } else {
+    load_row((const typename Elem<kStore>::T*)c.pages + at, true, x);
+  }
+}
+
+// All threads take part, with at < 0 where there is nothing to store: two neighbours share a scale
+template <int kStore, int N> __device__ inline void store_page(const Copy& c, int64_t at, float (&x)[N]) {
   if constexpr (kStore == MX_TYPE_FP8) {
     // the largest magnitude of the block, as the bits of a float that is not negative: they order
     // like integers, infinities and NaN above all numbers
     unsigned top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+    for (int j = 0; j < N; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
     top = max(top, (unsigned)__shfl_xor((int)top, 1));
-    top = max(top, (unsigned)__shfl_xor((int)top, 2));
     // 448 = 1.75 * 2^8: the exponent less 8, and one more above a fraction of 1.75
     const bool finite = top < 0x7f800000u;
     const int e = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), -117);
     const float inverse = __uint_as_float((unsigned)(127 - e) << 23);
-    if (!finite)
+    if (at < 0) return;
+    u4 w;
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = 0.f;
-    u2 w;
-    unsigned y = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inverse, x[1] * inverse, 0, false);
-    w.x = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inverse, x[3] * inverse, y, true);
-    y = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] * inverse, x[5] * inverse, 0, false);
-    w.y = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] * inverse, x[7] * inverse, y, true);
-    *(u2*)(c.pages + at * head_dim + d) = w;
-    if ((d & 31) == 0) c.scales[at * (head_dim / 32) + d / 32] = finite ? (uint8_t)(e + 127) : 255;
+    for (int j = 0; j < 4; j++) {
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = finite ? x[4 * j + i] * inverse : 0.f;
+      const unsigned half = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      w[j] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], half, true);
+    }
+    *(u4*)(c.pages + at) = w;
+    if (at % MX_SCALE_BLOCK == 0) c.scales[at / MX_SCALE_BLOCK] = finite ? (uint8_t)(e + 127) : 255;
   } else {
-    typedef typename Elem<kStore>::T S;
-    typename Elem<kStore>::V8 y;
-#pragma unroll
-    for (int j = 0; j < 8; j++) y[j] = (S)x[j];
-    *(typename Elem<kStore>::V8*)((S*)c.pages + at * head_dim + d) = y;
+    if (at >= 0) store_row((typename Elem<kStore>::T*)c.pages + at, true, x);
   }
 }
 
-template <class T, int kStore>
-__global__ __launch_bounds__(256) void read_rows(const Move a, int head_dim) {
-  const Copy c = a.of[blockIdx.y];
-  const int per = head_dim / 8;
-  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = item / per;
-  const int d = (int)(item - row * per) * 8;
-  const int64_t token = row / a.kv_heads;
-  const int head = (int)(row - token * a.kv_heads);
-  if (token >= a.tokens) return;
-  const int64_t slot = slot_of(a, (int)token);
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0) {
-    const int64_t at = slot + ((int64_t)head << a.page_shift);
-    if constexpr (kStore == MX_TYPE_FP8) {
-      const u2 w = *(const u2*)(c.pages + at * head_dim + d);
-      const unsigned byte = c.scales[at * (head_dim / 32) + d / 32];
-      const float scale = byte == 255 ? NAN : __uint_as_float(byte ? byte << 23 : 0x400000u);
-      const f2 p = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, false), q = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true);
-      const f2 r = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, false), s = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, true);
-      x[0] = p[0] * scale; x[1] = p[1] * scale; x[2] = q[0] * scale; x[3] = q[1] * scale;
-      x[4] = r[0] * scale; x[5] = r[1] * scale; x[6] = s[0] * scale; x[7] = s[1] * scale;
-    } else {
-      load8((const typename Elem<kStore>::T*)c.pages + at * head_dim + d, true, x);
-    }
-  }
-  T* to = (T*)c.rows + token * c.token_stride + head * c.head_stride + d;
-  if (c.vector) {
-    if constexpr (sizeof(T) == 4) {
-      *(f4*)to = f4{x[0], x[1], x[2], x[3]};
-      *(f4*)(to + 4) = f4{x[4], x[5], x[6], x[7]};
-    } else {
-      typedef T T8 __attribute__((ext_vector_type(8)));
-      T8 y;
+// A workgroup moves `tokens_each` packed tokens of all heads, keys and values: its first threads find
+// their slots, then every thread moves pieces of kPer values in the order of the rows, kItems of keys and
+// kItems of values under way at once.  Nothing is computed but the scales: bound by memory.
+template <int kStore> struct Pieces { static constexpr int kPer = kStore == MX_TYPE_FP8 ? 16 : 8; };
+constexpr int kMostTokens = 64;                         // of a workgroup: their slots are kept in LDS
+
+template <class T, int kStore, int kItems, bool kWrite>
+__global__ __launch_bounds__(256) void move_rows(const Move a) {
+  constexpr int kPer = Pieces<kStore>::kPer;
+  __shared__ int64_t slots[kMostTokens];
+  const int first = blockIdx.x * a.tokens_each, tokens = min(a.tokens - first, a.tokens_each);
+  if (threadIdx.x < 64) find_slots(a, first, tokens, slots);
+  __syncthreads();
+  const int per = a.head_dim / kPer, row = a.kv_heads * per, items = tokens * row;
+  for (int base = threadIdx.x; base < items; base += 256 * kItems) {
+    float x[kItems][2][kPer];
+    int64_t at[kItems], to[2][kItems];
+    bool is[kItems];
 #pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = (T)x[j];
-      *(T8*)to = y;
-    }
-  } else {
+    for (int i = 0; i < kItems; i++) {
+      const int item = base + 256 * i;
+      is[i] = item < items;
+      const int token = (is[i] ? item : 0) / row, rest = (is[i] ? item : 0) - token * row;
+      const int head = rest / per, d = (rest - head * per) * kPer;
+      const int64_t slot = slots[token];
+      at[i] = slot < 0 ? -1 : (slot + ((int64_t)head << a.page_shift)) * a.head_dim + d;
 #pragma unroll
-    for (int j = 0; j < 8; j++) to[j] = (T)x[j];
+      for (int y = 0; y < 2; y++)
+        to[y][i] = (int64_t)(first + token) * a.of[y].token_stride + head * a.of[y].head_stride + d;
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; i++)
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        if (kWrite ? is[i] : is[i] && at[i] >= 0) {
+          if constexpr (kWrite) load_row<T, kPer>((const T*)a.of[y].rows + to[y][i], a.of[y].vector, x[i][y]);
+          else load_page<kStore, kPer>(a.of[y], at[i], x[i][y]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPer; j++) x[i][y][j] = 0.f;
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < kItems; i++)
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        if constexpr (kWrite) store_page<kStore, kPer>(a.of[y], is[i] ? at[i] : -1, x[i][y]);
+        else if (is[i]) store_row<T, kPer>((T*)a.of[y].rows + to[y][i], a.of[y].vector, x[i][y]);
+      }
   }
 }
 
 // ---------------------------------------------------------------------------- joining the parts
+constexpr int kMostSplits = 256;
+
 // Whether a packed row belongs to a world's chunk, and is not beyond max_count in it
 __device__ inline bool covered(const Attend& a, int token) {
   if (!a.start) return token % a.count < a.max_count;
@@ -168,42 +210,60 @@ __device__ inline bool covered(const Attend& a, int token) {
   return a.start[low] >= 0 && place >= 0 && token < a.start[low + 1] && place < a.max_count;
 }
 
-// A row's parts in the order of their keys, whatever order they were computed in: a wave takes every
-// fourth part of a row with its lanes along head_dim, then the four waves' sums are joined.
-template <class T>
-__global__ __launch_bounds__(256) void join_parts(const Attend a, int head_dim) {
-  __shared__ float o[4][256], ls[4];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+// A row's parts in the order of their keys, whatever order they were computed in.  A workgroup takes one
+// row: its waves find the parts' maximum and shares together, then each thread adds up every kLanes-th part
+// of four neighbouring values, and the threads' sums are joined in turn.
+template <class T, int D>
+__global__ __launch_bounds__(256) void join_parts(const Attend a) {
+  constexpr int kQuads = D / 4, kLanes = 256 / kQuads;
+  __shared__ float share[kMostSplits];
+  __shared__ __attribute__((aligned(16))) f4 o[kLanes][kQuads];
   const int64_t row = blockIdx.x, rows = (int64_t)a.tokens * a.heads;
-  // rows that no tile covers (no world's chunk, or beyond max_count) have no parts
   const int64_t token = row / a.heads;
   const int h = (int)(row - token * a.heads);
-  if (!covered(a, (int)token)) return;
+  if (!covered(a, (int)token)) return;                  // has no parts
+  const int lane = threadIdx.x & 63;
+  f2 ml[kMostSplits / 64];
   float most = -INFINITY;
-  for (int s = 0; s < a.splits; s++) most = fmaxf(most, a.part_ml[2 * (s * rows + row)]);
+#pragma unroll
+  for (int i = 0; i < kMostSplits / 64; i++) {          // every wave, all parts
+    const int s = lane + 64 * i;
+    ml[i] = s < a.splits ? *(const f2*)(a.part_ml + 2 * (s * rows + row)) : f2{-INFINITY, 0.f};
+    most = fmaxf(most, ml[i][0]);
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) most = fmaxf(most, __shfl_xor(most, x));
   const float zero = most == -INFINITY ? 0.f : most;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int s = wave; s < a.splits; s += 4) {
-    const int64_t at = s * rows + row;
-    const f2 ml = *(const f2*)(a.part_ml + 2 * at);
-    if (ml[1] == 0.f) continue;                         // no key of its own: its sums were not written
-    const float share = __builtin_amdgcn_exp2f(ml[0] - zero);
-    l += ml[1] * share;
+  float l = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (lane + 64 * j < head_dim) sum[j] += a.part[at * head_dim + lane + 64 * j] * share;
+  for (int i = 0; i < kMostSplits / 64; i++) {
+    // a part without a key of its own has no sums: they were not written
+    const float w = ml[i][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i][0] - zero);
+    l += ml[i][1] * w;
+    if (threadIdx.x < 64) share[lane + 64 * i] = ml[i][1] == 0.f ? -1.f : w;
   }
 #pragma unroll
-  for (int j = 0; j < 4; j++) o[wave][lane + 64 * j] = sum[j];
-  if (lane == 0) ls[wave] = l;
+  for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
   __syncthreads();
-  const int d = threadIdx.x;
-  l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
-  if (d < head_dim) {
-    const float x = (o[0][d] + o[1][d]) + (o[2][d] + o[3][d]);
-    ((T*)a.out)[token * a.o_token + (int64_t)h * a.o_head + d] = (T)(l == 0.f ? 0.f : x * (1.f / l));
+  const int quad = threadIdx.x % kQuads, first = threadIdx.x / kQuads;
+  f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+  if (first < kLanes)
+#pragma unroll 4
+    for (int s = first; s < a.splits; s += kLanes) {
+      const float w = share[s];
+      if (w != -1.f) sum += *(const f4*)(a.part + (s * rows + row) * D + 4 * quad) * w;
+    }
+  if (first < kLanes) o[first][quad] = sum;
+  __syncthreads();
+  if (threadIdx.x < kQuads) {
+#pragma unroll
+    for (int i = 1; i < kLanes; i++) sum += o[i][quad];
+    const float inverse = 1.f / l;
+    T* to = (T*)a.out + token * a.o_token + (int64_t)h * a.o_head + 4 * quad;
+#pragma unroll
+    for (int e = 0; e < 4; e++) to[e] = (T)(l == 0.f ? 0.f : sum[e] * inverse);
   }
-  if (a.lse && d == 0) a.lse[row] = l == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(l)) * kLn2;
+  if (a.lse && threadIdx.x == 0) a.lse[row] = l == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -252,8 +312,13 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
   }
   if (k->type != v->type) return MX_ERR_INVALID;
   if (!c->tokens) return 0;
-  const int64_t items = (int64_t)c->tokens * p->kv_heads * (p->head_dim / 8);
-  if ((items + 255) / 256 > INT32_MAX) return MX_ERR_DOMAIN;
+  // pieces of a token, and tokens of a workgroup: a few pieces to each thread, as soon as there are
+  // workgroups for every CU
+  const int pieces = p->kv_heads * (p->head_dim / (p->type == MX_TYPE_FP8 ? 16 : 8));
+  const int64_t all = (int64_t)c->tokens * pieces;
+  const int items = all >= 4 * 256 * 1024 ? 4 : 1;
+  int each = 256 * items / pieces;
+  each = each < 1 ? 1 : each > kMostTokens ? kMostTokens : each;
   Move a{};
   uint8_t *pages[2] = {(uint8_t*)p->k, (uint8_t*)p->v}, *scales[2] = {p->k_scale, p->v_scale};
   for (int i = 0; i < 2; i++)
@@ -262,13 +327,13 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
   a.table = p->table; a.length = p->length; a.start = c->start;
   a.nworld = p->nworld; a.npage = p->npage; a.width = p->width; a.kv_heads = p->kv_heads;
   a.page_shift = page_shift(p); a.tokens = c->tokens; a.count = c->count;
-  const dim3 grid((unsigned)((items + 255) / 256), 2);
+  a.head_dim = p->head_dim; a.tokens_each = each;
+  const dim3 grid((unsigned)((c->tokens + (int64_t)each - 1) / each));
   auto go = [&](auto t, auto store) {
     typedef decltype(t) T;
-    if constexpr (kWrite)
-      hipLaunchKernelGGL((write_rows<T, decltype(store)::value>), grid, dim3(256), 0, (hipStream_t)stream, a, p->head_dim);
-    else
-      hipLaunchKernelGGL((read_rows<T, decltype(store)::value>), grid, dim3(256), 0, (hipStream_t)stream, a, p->head_dim);
+    constexpr int kStore = decltype(store)::value;
+    if (items == 4) hipLaunchKernelGGL((move_rows<T, kStore, 4, kWrite>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((move_rows<T, kStore, 1, kWrite>), grid, dim3(256), 0, (hipStream_t)stream, a);
   };
   auto by_store = [&](auto t) {
     if (p->type == MX_TYPE_FP8) go(t, std::integral_constant<int, MX_TYPE_FP8>());
@@ -338,6 +403,7 @@ int choose(Attend& a, Launch& launch) {
   int64_t splits = (1024 + groups - 1) / groups;
   const int64_t most = (keys + 255) / 256;
   splits = splits < most ? splits : most;
+  if (splits > kMostSplits) splits = kMostSplits;
   const int64_t each = ((keys + splits - 1) / splits + 127) / 128 * 128;
   splits = (keys + each - 1) / each;
   if (groups * splits > INT32_MAX) return MX_ERR_DOMAIN;
@@ -395,10 +461,18 @@ int mx_episode_attend(const MxPages* pages, const MxChunk* chunk, const MxAttent
                                              : mxe::attend256(a, launch, stream);
   if (started || a.splits < 2) return started;
   const dim3 grid((unsigned)((int64_t)a.tokens * a.heads));
-  if (launch.type == MX_TYPE_BF16)
-    hipLaunchKernelGGL(mxe::join_parts<__bf16>, grid, dim3(256), 0, (hipStream_t)stream, a, launch.head_dim);
-  else
-    hipLaunchKernelGGL(mxe::join_parts<_Float16>, grid, dim3(256), 0, (hipStream_t)stream, a, launch.head_dim);
+  const auto join = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (launch.type == MX_TYPE_BF16) hipLaunchKernelGGL((mxe::join_parts<__bf16, D>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((mxe::join_parts<_Float16, D>), grid, dim3(256), 0, (hipStream_t)stream, a);
+  };
+  switch (launch.head_dim) {
+    case 32: join(std::integral_constant<int, 32>()); break;
+    case 64: join(std::integral_constant<int, 64>()); break;
+    case 96: join(std::integral_constant<int, 96>()); break;
+    case 128: join(std::integral_constant<int, 128>()); break;
+    default: join(std::integral_constant<int, 256>());
+  }
   return (int)hipGetLastError();
 }
 

@@ -95,7 +95,7 @@ class Pages:
     of two from 16 to 4096, head_dim one of 32, 64, 96, 128, 256.  The tensors stay the caller's, and are
     held here."""
 
-    __slots__ = ('k', 'v', 'table', 'length', 'k_scale', 'v_scale', 'struct', 'device')
+    __slots__ = ('k', 'v', 'table', 'length', 'k_scale', 'v_scale', 'struct', 'device', 'index')
 
     def __init__(self, k, v, table, length, k_scale=None, v_scale=None):
         _require(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype,
@@ -127,7 +127,7 @@ class Pages:
         for t in (v, table, length, k_scale, v_scale):
             _require(t is None or t.device == device, 'pages, scales, table and length must be on one device')
         self.k, self.v, self.table, self.length, self.k_scale, self.v_scale = k, v, table, length, k_scale, v_scale
-        self.device = device
+        self.device, self.index = device, device.index
         self.struct = MxPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if kind == 3 else None,
                               v_scale.data_ptr() if kind == 3 else None, table.data_ptr(), length.data_ptr(),
                               table.shape[0], npage, table.shape[1], kv, dim, tokens, kind)
@@ -137,37 +137,40 @@ def _chunk(pages, shape, start):
     """MxChunk of rows of this shape (without heads and head_dim)."""
     nworld = pages.struct.nworld
     if start is None:
-        _require(len(shape) == 2 and shape[0] == nworld,
-                 'rows must be (nworld, n, heads, head_dim), or packed (tokens, heads, head_dim) with start')
-        return MxChunk(None, shape[0] * shape[1], shape[1])
+        if len(shape) != 2 or shape[0] != nworld:
+            raise ValueError('rows must be (nworld, n, heads, head_dim), or packed (tokens, heads, head_dim) with start')
+        return MxChunk(None, nworld * shape[1], shape[1])
     _require(len(shape) == 1, 'rows with start must be packed: (tokens, heads, head_dim)')
     _require(start.dtype == torch.int32 and start.shape == (nworld + 1,) and start.is_contiguous()
              and start.device == pages.device, 'start must be contiguous int32 of shape (nworld + 1,) on the pages\' device')
     return MxChunk(start.data_ptr(), shape[0], 0)
 
 
-def _rows(pages, x, heads, name):
+def _rows(pages, x, shape, name):
     """MxRows of a tensor (..., heads, head_dim) whose token dimensions step evenly."""
     kind = _TYPES.get(x.dtype, 3)
-    _require(kind < 3, '%s must be float32, bfloat16 or float16, got %s', name, x.dtype)
-    shape, stride = x.shape, x.stride()
-    _require(len(shape) in (3, 4) and shape[-1] == pages.struct.head_dim and (heads is None or shape[-2] == heads),
-             '%s has the wrong heads or head_dim: %s', name, tuple(shape))
-    _require(x.device == pages.device, '%s must be on the pages\' device', name)
-    _require(stride[-1] == 1 or shape[-1] == 1, '%s must be contiguous along head_dim', name)
+    stride = x.stride()
+    if kind == 3 or shape[-1] != pages.struct.head_dim or x.device != pages.device or stride[-1] != 1:
+        _require(kind < 3, '%s must be float32, bfloat16 or float16, got %s', name, x.dtype)
+        _require(shape[-1] == pages.struct.head_dim, '%s has the wrong head_dim: %s', name, tuple(shape))
+        _require(x.device == pages.device, '%s must be on the pages\' device', name)
+        _require(stride[-1] == 1, '%s must be contiguous along head_dim', name)
+    token = stride[-3]
     if len(shape) == 4:
-        _require(shape[0] <= 1 or shape[1] == 0 or stride[0] == shape[1] * stride[1],
-                 '%s: the rows of all worlds must step evenly', name)
-        token = stride[1] if shape[1] > 1 or shape[0] <= 1 else stride[0]
-    else:
-        token = stride[0]
+        if shape[1] == 1:
+            token = stride[0]
+        elif shape[0] > 1 and shape[1] > 1 and stride[0] != shape[1] * token:
+            raise ValueError('%s: the rows of all worlds must step evenly' % name)
     return MxRows(x.data_ptr(), token, stride[-2], shape[-2], kind)
 
 
-def _on(pages, stream):
-    if stream is None:
-        stream = torch.cuda.current_stream(pages.device)
-    return stream.cuda_stream
+# the current stream's handle, without a Stream object around it where torch offers that
+_current = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _elsewhere(pages, stream):
+    """Whether a call has to change to the pages' device, or to a stream that is not the current one."""
+    return stream is not None or torch.cuda.current_device() != pages.index
 
 
 def write(pages, k, v, start=None, *, stream=None):
@@ -176,32 +179,40 @@ def write(pages, k, v, start=None, *, stream=None):
     at which all are within the codes' range, and round to nearest even; a block with an infinity or NaN
     is stored as NaN.  Chunk tokens without a place (a chunk longer than its world's length, a table entry
     that names no page) are left out."""
-    s = pages.struct
-    _require(k.shape == v.shape and k.dtype == v.dtype, 'k and v must have one shape and type')
-    chunk = _chunk(pages, k.shape[:-2], start)
-    a, b = _rows(pages, k, s.kv_heads, 'k'), _rows(pages, v, s.kv_heads, 'v')
-    with torch.cuda.device(pages.device):
-        native.check(load().mx_episode_write(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b),
-                                             _on(pages, stream)), 'mx_episode_write')
+    if _elsewhere(pages, stream):
+        with torch.cuda.device(pages.device), torch.cuda.stream(stream):
+            return write(pages, k, v, start)
+    s, shape = pages.struct, k.shape
+    if shape != v.shape or k.dtype != v.dtype or len(shape) < 3 or shape[-2] != s.kv_heads:
+        raise ValueError('k and v must have one type and one shape, with %d heads: %s, %s' % (s.kv_heads, tuple(shape), tuple(v.shape)))
+    chunk = _chunk(pages, shape[:-2], start)
+    a, b = _rows(pages, k, shape, 'k'), _rows(pages, v, shape, 'v')
+    rc = load().mx_episode_write(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b), _current(pages.index))
+    if rc:
+        native.check(rc, 'mx_episode_write')
 
 
 def read(pages, start=None, *, count=None, tokens=None, dtype=torch.bfloat16, stream=None):
     """The chunk's keys and values: ``(nworld, count, kv_heads, head_dim)``, or packed ``(tokens, kv_heads,
     head_dim)`` with ``start``; each value rounded once to ``dtype``.  Tokens without a place read as zeros."""
+    if _elsewhere(pages, stream):
+        with torch.cuda.device(pages.device), torch.cuda.stream(stream):
+            return read(pages, start, count=count, tokens=tokens, dtype=dtype)
     s = pages.struct
-    _require(dtype in _TYPES and dtype != torch.float8_e4m3fn, 'read returns float32, bfloat16 or float16')
-    if start is None:
-        _require(count is not None and tokens is None and count >= 0, 'give count (every world), or start and tokens')
-        shape = (s.nworld, count)
-    else:
-        _require(tokens is not None and count is None and tokens >= 0, 'give count (every world), or start and tokens')
-        shape = (tokens,)
+    kind = _TYPES.get(dtype, 3)
+    _require(kind < 3, 'read returns float32, bfloat16 or float16')
+    many, none = (count, tokens) if start is None else (tokens, count)
+    _require(many is not None and none is None and many >= 0, 'give count (every world), or start and tokens')
+    shape = (s.nworld, count) if start is None else (tokens,)
     chunk = _chunk(pages, shape, start)
-    with torch.cuda.device(pages.device), torch.cuda.stream(stream):
-        k, v = (torch.empty(shape + (s.kv_heads, s.head_dim), dtype=dtype, device=pages.device) for _ in range(2))
-        a, b = _rows(pages, k, s.kv_heads, 'k'), _rows(pages, v, s.kv_heads, 'v')
-        native.check(load().mx_episode_read(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b),
-                                            _on(pages, stream)), 'mx_episode_read')
+    shape += (s.kv_heads, s.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=pages.device)
+    v = torch.empty_like(k)
+    step = s.kv_heads * s.head_dim
+    a, b = (MxRows(x.data_ptr(), step, s.head_dim, s.kv_heads, kind) for x in (k, v))
+    rc = load().mx_episode_read(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b), _current(pages.index))
+    if rc:
+        native.check(rc, 'mx_episode_read')
     return k, v
 
 
@@ -216,34 +227,39 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
     those are 8-bit.  ``max_count`` (with ``start``): the largest chunk of a world, if known; rows beyond it are
     not computed.  ``out`` (like q) and ``lse`` (float32, q's shape without head_dim, contiguous) are written
     if given.  Returns out.  The same inputs give the same bits."""
-    s = pages.struct
-    chunk = _chunk(pages, q.shape[:-2], start)
-    rows = _rows(pages, q, None, 'q')
-    heads = rows.heads
-    _require(rows.type in (1, 2) and (s.type == 3 or s.type == rows.type),
-             'q must be bfloat16 or float16, and of the pages\' type unless those are 8-bit: %s on %s', q.dtype, pages.k.dtype)
-    _require(heads > 0 and heads % s.kv_heads == 0, 'q has %d heads, not a multiple of the pages\' %d', heads, s.kv_heads)
+    if _elsewhere(pages, stream):
+        with torch.cuda.device(pages.device), torch.cuda.stream(stream):
+            return attend(pages, q, start, max_count=max_count, causal=causal, window=window, scale=scale, out=out, lse=lse)
+    s, shape = pages.struct, q.shape
+    chunk = _chunk(pages, shape[:-2], start)
+    rows = _rows(pages, q, shape, 'q')
+    if not (rows.type == s.type or s.type == 3 and rows.type) or rows.heads < 1 or rows.heads % s.kv_heads:
+        _require(rows.heads > 0 and rows.heads % s.kv_heads == 0, 'q has %d heads, not a multiple of the pages\' %d',
+                 rows.heads, s.kv_heads)
+        raise ValueError('q must be bfloat16 or float16, and of the pages\' type unless those are 8-bit: %s on %s'
+                         % (q.dtype, pages.k.dtype))
     _require(0 <= window < 2 ** 31, 'window must be 0 (none) or a number of tokens, got %s', window)
-    scale = 1.0 / math.sqrt(s.head_dim) if scale is None else float(scale)
+    scale = s.head_dim ** -0.5 if scale is None else float(scale)
     _require(math.isfinite(scale), 'scale must be finite')
     if max_count is None:
         max_count = chunk.tokens if start is not None else chunk.count
     _require(0 <= max_count < 2 ** 31, 'max_count must be a number of tokens, got %s', max_count)
-    with torch.cuda.device(pages.device), torch.cuda.stream(stream):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=pages.device)
-        else:
-            _require(out.shape == q.shape and out.dtype == q.dtype, 'out must have q\'s shape and type')
-        if lse is not None:
-            _require(lse.dtype == torch.float32 and lse.shape == q.shape[:-1] and lse.is_contiguous()
-                     and lse.device == pages.device, 'lse must be contiguous float32 of q\'s shape without head_dim')
-        a = MxAttention(rows, _rows(pages, out, heads, 'out'), None if lse is None else lse.data_ptr(), None, 0,
-                        max_count, int(bool(causal)), window, scale)
-        lib = load()
-        need = lib.mx_episode_workspace(ct.byref(s), ct.byref(chunk), ct.byref(a))
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=pages.device)
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), need
-        native.check(lib.mx_episode_attend(ct.byref(s), ct.byref(chunk), ct.byref(a), _on(pages, stream)),
-                     'mx_episode_attend')
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _require(out.shape == shape and out.dtype == q.dtype, 'out must have q\'s shape and type')
+    a = MxAttention(rows, _rows(pages, out, shape, 'out'), None, None, 0, max_count, 1 if causal else 0, window, scale)
+    if lse is not None:
+        _require(lse.dtype == torch.float32 and lse.shape == shape[:-1] and lse.is_contiguous()
+                 and lse.device == pages.device, 'lse must be contiguous float32 of q\'s shape without head_dim')
+        a.lse = lse.data_ptr()
+    lib = _LIB or load()
+    refs = ct.byref(s), ct.byref(chunk), ct.byref(a)
+    need = lib.mx_episode_workspace(*refs)
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=pages.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+    rc = lib.mx_episode_attend(*refs, _current(pages.index))
+    if rc:
+        native.check(rc, 'mx_episode_attend')
     return out
