@@ -14,8 +14,11 @@
 
 namespace mxe {
 
+// Waves of a SIMD to leave registers for
+constexpr int few_waves(int D, int blocks) { return blocks == 1 && D <= 64 ? 4 : blocks <= 2 && D <= 128 ? 2 : 1; }
+
 template <int kType, bool kFp8, int D, int kBlocks>
-__global__ __launch_bounds__(256) void attend_few(const Attend a) {
+__global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const Attend a) {
   typedef Elem<kType> E;
   typedef typename E::T T;
   typedef typename E::V8 V8;
@@ -97,7 +100,6 @@ __global__ __launch_bounds__(256) void attend_few(const Attend a) {
   };
 
   u4 kreg[2][kFp8 ? kPairs + 1 : kC];
-  u2 kodd[2];
   unsigned kbyte[2][kFp8 ? kPairs + 1 : 1];
   u4 vreg[kVLoads];
   unsigned vbyte[kFp8 ? kVLoads : 1];
@@ -118,7 +120,8 @@ __global__ __launch_bounds__(256) void attend_few(const Attend a) {
           kbyte[s][c] = scale[2 * c + (quarter >> 1)];
         }
         if constexpr (kC & 1) {
-          kodd[s] = *(const u2*)(from + 32 * (kC - 1) + 8 * quarter);
+          const u2 w = *(const u2*)(from + 32 * (kC - 1) + 8 * quarter);
+          kreg[s][kPairs] = u4{w.x, w.y, 0, 0};
           kbyte[s][kPairs] = scale[kC - 1];
         }
       } else {
@@ -130,8 +133,7 @@ __global__ __launch_bounds__(256) void attend_few(const Attend a) {
 #pragma unroll
     for (int j = 0; j < kVLoads; j++) {
       const int x = j * 64 + lane, key_in = x / (D / kVPer), d = (x - key_in * (D / kVPer)) * kVPer;
-      const Keys& s = keys[key_in >> 4];
-      const int64_t at = s.at + min(key_in & 15, s.left);
+      const int64_t at = key_in < 16 ? keys[0].at + min(key_in, keys[0].left) : keys[1].at + min(key_in - 16, keys[1].left);
       if constexpr (kFp8) {
         vreg[j] = *(const u4*)(a.v + at * D + d);
         vbyte[j] = a.v_scale[at * kC + d / 32];
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(256) void attend_few(const Attend a) {
             const u4 w = kreg[u][c / 2];
             x = from_fp8<E>(c & 1 ? u2{w.z, w.w} : u2{w.x, w.y}, kbyte[u][c / 2]);
           } else {
-            x = from_fp8<E>(kodd[u], kbyte[u][kPairs]);
+            x = from_fp8<E>(u2{kreg[u][kPairs].x, kreg[u][kPairs].y}, kbyte[u][kPairs]);
           }
         } else {
           x = __builtin_bit_cast(V8, kreg[u][c]);
@@ -176,47 +178,36 @@ __global__ __launch_bounds__(256) void attend_few(const Attend a) {
     // probability times an infinity is no remainder).  8-bit values have no infinity, and a NaN need not be
     // kept from rows that all see it.
     unsigned wild = 0;
-    V8 vx[kVLoads][kVPer / 8];
 #pragma unroll
     for (int j = 0; j < kVLoads; j++) {
-      const int x = j * 64 + lane, key_in = x / (D / kVPer);
+      const int x = j * 64 + lane, key_in = x / (D / kVPer), d = (x - key_in * (D / kVPer)) * kVPer;
+      V8 v[kVPer / 8];
       if constexpr (kFp8) {
-        vx[j][0] = from_fp8<E>(u2{vreg[j].x, vreg[j].y}, vbyte[j]);
-        vx[j][1] = from_fp8<E>(u2{vreg[j].z, vreg[j].w}, vbyte[j]);
+        v[0] = from_fp8<E>(u2{vreg[j].x, vreg[j].y}, vbyte[j]);
+        v[1] = from_fp8<E>(u2{vreg[j].z, vreg[j].w}, vbyte[j]);
       } else {
-        vx[j][0] = __builtin_bit_cast(V8, vreg[j]);
+        v[0] = __builtin_bit_cast(V8, vreg[j]);
       }
-      const bool none = edge && (key + key_in >= end || !(key_in < 16 ? is0 : is1));
 #pragma unroll
       for (int e = 0; e < kVPer / 8; e++) {
-        u4 words = __builtin_bit_cast(u4, vx[j][e]);
-        if (edge && none) words = u4{0, 0, 0, 0};
-        if (!kFp8 || edge)
+        u4 words = __builtin_bit_cast(u4, v[e]);
+        if (edge && (key + key_in >= end || !(key_in < 16 ? is0 : is1))) words = u4{0, 0, 0, 0};
+        if (!kFp8 || edge) {
+          unsigned off = 0;
 #pragma unroll
-          for (int y = 0; y < 4; y++) wild |= not_finite<E>(words[y]);
-        vx[j][e] = __builtin_bit_cast(V8, words);
+          for (int y = 0; y < 4; y++) off |= not_finite<E>(words[y]);
+          off &= 0x80008000u;
+          if (off)
+#pragma unroll
+            for (int y = 0; y < 4; y++) words[y] = finite_or_zero<E>(words[y]);
+          wild |= off;
+        }
+        *(u4*)(vs + key_in * kStride + d + 8 * e) = words;
       }
     }
-    const bool repair = __ballot((wild & 0x80008000u) != 0);
-    auto store = [&](bool clean) {
-#pragma unroll
-      for (int j = 0; j < kVLoads; j++) {
-        const int x = j * 64 + lane, key_in = x / (D / kVPer), d = (x - key_in * (D / kVPer)) * kVPer;
-#pragma unroll
-        for (int e = 0; e < kVPer / 8; e++) {
-          s8 bits = __builtin_bit_cast(s8, vx[j][e]);
-          if (clean) {
-#pragma unroll
-            for (int y = 0; y < 8; y++)
-              if ((bits[y] & E::kExponent) == E::kExponent) bits[y] = 0;
-          }
-          *(s8*)(vs + key_in * kStride + d + 8 * e) = bits;
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    };
-    store(repair);
+    const bool repair = __ballot(wild != 0) != 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     // the next keys are on their way while these are weighed
     const int now = key;
     if (key + 128 < end) load(key + 128);
@@ -272,23 +263,22 @@ __global__ __launch_bounds__(256) void attend_few(const Attend a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (repair) {
-      // rows that see a value that is not finite get it added; the others' products had a zero for it
-      store(false);
-      for (int k = 0; k < 32; k++) {
+      // the products had zeros for these values: the rows that see them get them added
+      for (int k = now; k < min(now + 32, end); k++) {
+        const int page = table[k >> a.page_shift];
+        if ((unsigned)page >= (unsigned)a.npage) continue;
+        const int64_t at = (((int64_t)page * a.kv_heads + head) << a.page_shift) + (k & page_mask);
 #pragma unroll
-        for (int b = 0; b < kBlocks; b++) {
-          const bool sees = now + k >= low_r[b] && now + k < high_r[b];
+        for (int c = 0; c < D / 16; c++)
 #pragma unroll
-          for (int c = 0; c < D / 16; c++)
+          for (int i = 0; i < 4; i++) {
+            const float value = value_at<E, kFp8, D>(a, at, 16 * c + 4 * quarter + i);
+            if (!(fabsf(value) < INFINITY))
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const float value = (float)vs[k * kStride + 16 * c + 4 * quarter + i];
-              if (sees && !(fabsf(value) < INFINITY)) o[b][c][i] += value;
-            }
-        }
+              for (int b = 0; b < kBlocks; b++)
+                if (k >= low_r[b] && k < high_r[b]) o[b][c][i] += value;
+          }
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
     }
   }
 

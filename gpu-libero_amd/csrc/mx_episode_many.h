@@ -164,8 +164,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
           for (int y = 0; y < 4; y++) {
             const unsigned off = not_finite<E>(words[y]) & 0x80008000u;
             wild |= off;
-            if (off & 0x8000u) words[y] &= 0xffff0000u;
-            if (off & 0x80000000u) words[y] &= 0xffffu;
+            if (off) words[y] = finite_or_zero<E>(words[y]);
           }
         *(V8*)&sh.k[buffer][key_in * Shared::kStrideK + d + 8 * e] = k[e];
         *(u4*)&sh.v[buffer][key_in * Shared::kStrideV + d + 8 * e] = words;

@@ -64,6 +64,11 @@ template <class E> __device__ inline unsigned not_finite(unsigned w) {
   return (w & e) + (last | last << 16);
 }
 
+template <class E> __device__ inline unsigned finite_or_zero(unsigned w) {
+  const unsigned off = not_finite<E>(w);
+  return w & ~((off & 0x8000u ? 0xffffu : 0u) | (off & 0x80000000u ? 0xffff0000u : 0u));
+}
+
 // E8M0: byte b stands for 2^(b - 127); 255 for NaN, which the codes then carry (nan_codes)
 __device__ inline float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
 __device__ inline unsigned nan_codes(unsigned w, unsigned byte) { return byte == 255 ? 0x7f7f7f7fu : w; }
