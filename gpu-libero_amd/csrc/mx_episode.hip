@@ -384,8 +384,12 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   return choose(a, launch);
 }
 
-// Keys that one row of tiles can see at most, and how they are split: enough workgroups for every CU
-// to hold several, in shares of at least 256 keys.
+// Which kernel, how many tiles, and into how many parts each tile's keys are split: where the tiles leave
+// room, as many as the card holds workgroups at once (two per CU, four where heads of up to 64 values leave
+// the registers), unless one workgroup is done with its keys in about the time that a second launch to
+// join the parts takes.  Two worlds of up to 131072 quantised tokens, 8
+// key heads of 128 values: 256 workgroups 77.9 us, 512 54.0, 1024 55.5, 2048 63.1; heads of 64: 512 35.4,
+// 1024 30.7, 2048 33.1.
 int choose(Attend& a, Launch& launch) {
   const int64_t rows = (int64_t)a.max_count * a.group;
   launch.blocks = rows <= 16 ? 1 : rows <= 32 || launch.head_dim == 256 ? 2 : 4;
@@ -398,18 +402,15 @@ int choose(Attend& a, Launch& launch) {
     const int64_t spanned = (int64_t)a.window + launch.rows / a.group + 1;
     keys = keys < spanned ? keys : spanned;
   }
-  keys += 31;                                            // the first key goes down to a multiple of 32
   const int64_t groups = tiles * a.kv_heads;
-  int64_t splits = (1024 + groups - 1) / groups;
-  const int64_t most = (keys + 255) / 256;
+  const int room = launch.head_dim <= 64 ? 1024 : 512;
+  int64_t splits = keys * launch.head_dim <= 131072 ? 1 : (room + groups - 1) / groups;
+  const int64_t most = (keys + 31) / kLeastKeys + 1;     // the first key goes down to a multiple of 32
   splits = splits < most ? splits : most;
   if (splits > kMostSplits) splits = kMostSplits;
-  const int64_t each = ((keys + splits - 1) / splits + 127) / 128 * 128;
-  splits = (keys + each - 1) / each;
   if (groups * splits > INT32_MAX) return MX_ERR_DOMAIN;
   a.tiles = (int)tiles;
   a.splits = (int)splits;
-  a.split_keys = (int)(each < INT32_MAX ? each : INT32_MAX);
   launch.tiles = a.tiles;
   launch.grid = (unsigned)(groups * splits);
   return 0;

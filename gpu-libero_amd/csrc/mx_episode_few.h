@@ -47,10 +47,9 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
   int first_low, first_high, last_low, last_high;
   limits(a, t, t.row / a.group, first_low, first_high);
   limits(a, t, last_row / a.group, last_low, last_high);
-  const int all_low = last_low, all_high = first_high, high = last_high;
-  const int base = first_low & ~31;
-  const int begin = base + split * a.split_keys;
-  const int end = a.splits > 1 ? (int)min((long long)high, (long long)begin + a.split_keys) : high;
+  const int all_low = last_low, all_high = first_high;
+  int begin, end;
+  split_range(a, split, first_low, last_high, begin, end);
 
   // this lane's rows
   int low_r[kBlocks], high_r[kBlocks];

@@ -73,8 +73,8 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
   int first_low, first_high, last_low, last_high;
   limits(a, t, t.row / a.group, first_low, first_high);
   limits(a, t, last_row / a.group, last_low, last_high);
-  const int begin = (first_low & ~31) + split * a.split_keys;
-  const int end = a.splits > 1 ? (int)min((long long)last_high, (long long)begin + a.split_keys) : last_high;
+  int begin, end;
+  split_range(a, split, first_low, last_high, begin, end);
 
   // this wave's and lane's rows
   const int wave_row = t.row + 32 * wave, r = wave_row + n32;

@@ -96,7 +96,7 @@ struct Attend {
   float *lse, *part, *part_ml;       // part: [split][token][head][D]; part_ml: [split][token][head][2]
   int64_t q_token, q_head, o_token, o_head;
   int nworld, npage, width, kv_heads, page_shift, tokens, count, max_count, heads, group;
-  int causal, window, tiles, splits, split_keys;
+  int causal, window, tiles, splits;
   float scale2;                      // |scale| * log2(e), not 0: probabilities are powers of two
   bool negate;                       // scale < 0: the queries change their sign
   bool q_vector, o_vector;           // q's rows are 16-byte aligned, out's 8-byte
@@ -171,6 +171,20 @@ __device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, T
   t.position = length - count;
   t.length = (int)min((long long)length, (long long)a.width << a.page_shift);
   return true;
+}
+
+// The part of the keys [low, high) of a tile that a split takes: the same number for each, in steps of 128
+// keys, and no fewer than kLeastKeys (the last ones may have none).  By the world's own keys and not by
+// the most that the table can hold, so that long and short worlds both keep all splits at work.
+constexpr int kLeastKeys = 256;
+__device__ inline void split_range(const Attend& a, int split, int low, int high, int& begin, int& end) {
+  begin = low & ~31;
+  end = high;
+  if (a.splits == 1) return;
+  const int each = max(kLeastKeys, (int)(((unsigned)max(high - begin, 0) / (unsigned)a.splits + 128u) & ~127u));
+  const long long from = begin + (long long)split * each;
+  begin = (int)min(from, (long long)max(high, 0));
+  end = (int)min(from + each, (long long)high);
 }
 
 // The keys [low, high) that the chunk's token i sees
