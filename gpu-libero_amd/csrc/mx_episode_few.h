@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
     for (int c = 0; c < D / 16; c++) o[b][c] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int32_t* table = a.table + (int64_t)t.world * a.width;
+  Fixed* table = fixed(a.table + (int64_t)t.world * a.width);
   const int page_mask = (1 << a.page_shift) - 1;
 
   // The 16 keys from `key` on lie in one page: its number, or 0 with the keys marked absent

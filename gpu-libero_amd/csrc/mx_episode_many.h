@@ -21,7 +21,6 @@ struct ManyShared {
   static constexpr int kStrideV = D + (D == 128 || D == 64 ? 32 : 0);
   typename E::T k[2][kManyKeys * kStrideK];
   typename E::T v[2][kManyKeys * kStrideV];
-  int is[2][4];                               // whether the 16 keys have a page
   int wild[2][4];                             // by wave: an infinity or NaN among the values it brought
 };
 
@@ -42,7 +41,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
   typedef ManyShared<E, D> Shared;
   constexpr int kC = D / 16, kTiles = D / 32;
   constexpr int kPer = kFp8 ? 16 : 8, kChunks = D / kPer, kLoads = (kManyKeys * kChunks + 255) / 256;
-  constexpr bool kWhole = kManyKeys * kChunks % 256 == 0;
+  constexpr bool kWhole = kManyKeys * kChunks % 256 == 0, kOneGroup = 16 * kChunks % 64 == 0;
   __shared__ __attribute__((aligned(16))) Shared sh;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -103,43 +102,52 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
     for (int i = 0; i < 16; i++) o[c][i] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  // ---- bringing keys and values: each thread a 16-byte piece of kLoads keys and of their values
-  const int32_t* table = a.table + (int64_t)t.world * a.width;
+  // ---- bringing keys and values: each thread a 16-byte piece of kLoads keys and of their values.  16 keys
+  // from a multiple of 16 on lie in one page, so that addresses are a wave's own but for an offset of 32 bits.
+  Fixed* table = fixed(a.table + (int64_t)t.world * a.width);
   const int page_mask = (1 << a.page_shift) - 1;
-  int page[kLoads];
+  const int64_t row_bytes = kFp8 ? D : 2 * D;
+  int page[4];
   u4 kreg[kLoads], vreg[kLoads];
   unsigned kbyte[kFp8 ? kLoads : 1], vbyte[kFp8 ? kLoads : 1];
-  bool held[kLoads];                          // the key exists
   const auto key_of = [&](int j) { return (j * 256 + (int)threadIdx.x) / kChunks; };
   const auto piece_of = [&](int j) { return (j * 256 + (int)threadIdx.x) % kChunks; };
+  const auto first_of = [&](int key, int g) { return min(key + 16 * g, (end - 1) & ~15); };
   auto look_up = [&](int key) {
 #pragma unroll
-    for (int j = 0; j < kLoads; j++) page[j] = table[min(key + key_of(j), end - 1) >> a.page_shift];
+    for (int g = 0; g < 4; g++) page[g] = table[first_of(key, g) >> a.page_shift];
   };
   auto load = [&](int key) {
+    int64_t base[4];
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int in = (unsigned)page[g] < (unsigned)a.npage ? page[g] : 0;
+      base[g] = (((int64_t)in * a.kv_heads + head) << a.page_shift) + (first_of(key, g) & page_mask);
+    }
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
-      const int at_key = min(key + key_of(j), end - 1);
-      const bool is = (unsigned)page[j] < (unsigned)a.npage;
-      held[j] = is && key + key_of(j) < end;
-      const int64_t at = (((int64_t)(is ? page[j] : 0) * a.kv_heads + head) << a.page_shift) + (at_key & page_mask);
-      if (kWhole || key_of(j) < kManyKeys) {
-        if constexpr (kFp8) {
-          kreg[j] = *(const u4*)(a.k + at * D + piece_of(j) * 16);
-          vreg[j] = *(const u4*)(a.v + at * D + piece_of(j) * 16);
-          kbyte[j] = a.k_scale[at * kTiles + piece_of(j) / 2];
-          vbyte[j] = a.v_scale[at * kTiles + piece_of(j) / 2];
-        } else {
-          kreg[j] = *(const u4*)((const T*)a.k + at * D + piece_of(j) * 8);
-          vreg[j] = *(const u4*)((const T*)a.v + at * D + piece_of(j) * 8);
-        }
+      if (!kWhole && key_of(j) >= kManyKeys) continue;
+      // the group of 16 keys: the wave's, or where a wave's pieces straddle two, the lane's
+      const int group = kOneGroup ? (j * 256 + 64 * wave) / (16 * kChunks) : key_of(j) / 16;
+      int64_t at = base[0];
+#pragma unroll
+      for (int g = 1; g < 4; g++) at = group == g ? base[g] : at;
+      const unsigned row = min(key_of(j) % 16, end - 1 - first_of(key, group));
+      const unsigned offset = row * (unsigned)row_bytes + piece_of(j) * 16;
+      kreg[j] = *(const u4*)(a.k + at * row_bytes + offset);
+      vreg[j] = *(const u4*)(a.v + at * row_bytes + offset);
+      if constexpr (kFp8) {
+        const unsigned byte = row * kTiles + piece_of(j) / 2;
+        kbyte[j] = (a.k_scale + at * kTiles)[byte];
+        vbyte[j] = (a.v_scale + at * kTiles)[byte];
       }
     }
   };
-  // keys that only some rows of the workgroup see, or that are not there, are masked below
-  auto is_edge = [&](int key) { return key < last_low || key + kManyKeys > first_high || key + kManyKeys > end; };
-  auto store = [&](int buffer, int key) {
-    const bool edge = is_edge(key);
+  // Into LDS: values of keys that are not there as zeros, and, where only some rows of the workgroup see a
+  // key, infinities and NaN too (those rows get them added below).  `all`: every key is there.
+  auto is_edge = [&](int key) { return key < last_low || key + kManyKeys > first_high; };
+  auto store = [&](int buffer, int key, unsigned present) {
+    const bool edge = is_edge(key), all = present == 15u && key + kManyKeys <= end;
     unsigned wild = 0;
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
@@ -155,42 +163,60 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
         k[0] = __builtin_bit_cast(V8, kreg[j]);
         v[0] = __builtin_bit_cast(V8, vreg[j]);
       }
+      if (edge || !all) {
+        const bool none = key + key_in >= end || !(present >> (key_in / 16) & 1);
 #pragma unroll
-      for (int e = 0; e < kPer / 8; e++) {
-        u4 words = __builtin_bit_cast(u4, v[e]);
-        if (!held[j]) words = u4{0, 0, 0, 0};
-        if (edge)
+        for (int e = 0; e < kPer / 8; e++) {
+          u4 words = __builtin_bit_cast(u4, v[e]);
 #pragma unroll
           for (int y = 0; y < 4; y++) {
-            const unsigned off = not_finite<E>(words[y]) & 0x80008000u;
-            wild |= off;
-            if (off) words[y] = finite_or_zero<E>(words[y]);
+            if (none) words[y] = 0;
+            wild |= not_finite<E>(words[y]) & 0x80008000u;
+            words[y] = finite_or_zero<E>(words[y]);
           }
-        *(V8*)&sh.k[buffer][key_in * Shared::kStrideK + d + 8 * e] = k[e];
-        *(u4*)&sh.v[buffer][key_in * Shared::kStrideV + d + 8 * e] = words;
+          v[e] = __builtin_bit_cast(V8, words);
+        }
       }
-      if (piece_of(j) == 0 && key_in % 16 == 0) sh.is[buffer][key_in / 16] = (unsigned)page[j] < (unsigned)a.npage;
+#pragma unroll
+      for (int e = 0; e < kPer / 8; e++) {
+        *(V8*)&sh.k[buffer][key_in * Shared::kStrideK + d + 8 * e] = k[e];
+        *(V8*)&sh.v[buffer][key_in * Shared::kStrideV + d + 8 * e] = v[e];
+      }
     }
-    const int any = __ballot(wild != 0) != 0;
-    if (lane == 0) sh.wild[buffer][wave] = any;
+    if (edge || !all) {
+      const int any = __ballot(wild != 0) != 0;
+      if (lane == 0) sh.wild[buffer][wave] = any;
+    }
+  };
+  auto pages_there = [&]() {
+    unsigned bits = 0;
+#pragma unroll
+    for (int g = 0; g < 4; g++) bits |= ((unsigned)page[g] < (unsigned)a.npage ? 1u : 0u) << g;
+    return bits;
   };
 
   typedef __attribute__((address_space(3))) s4* TrPtr;
   int key = begin, buffer = 0;
+  unsigned present = 0;
   if (key < end) {
     look_up(key);
     load(key);
-    store(0, key);
+    present = pages_there();
+    if (key + kManyKeys < end) look_up(key + kManyKeys);
+    store(0, key, present);
   }
   for (; key < end; key += kManyKeys, buffer ^= 1) {
     const bool more = key + kManyKeys < end;
-    if (more) look_up(key + kManyKeys);
     __syncthreads();
-    if (more) load(key + kManyKeys);
+    unsigned next_present = 0;
+    if (more) {
+      load(key + kManyKeys);
+      next_present = pages_there();
+      if (key + 2 * kManyKeys < end) look_up(key + 2 * kManyKeys);
+    }
     if (rows_here && key < wave_high && key + kManyKeys > wave_low) {
-      const bool is0 = sh.is[buffer][0], is1 = sh.is[buffer][1], is2 = sh.is[buffer][2], is3 = sh.is[buffer][3];
-      const bool edge = key < wave_all_low || key + kManyKeys > wave_all_high || key + kManyKeys > end ||
-                        !(is0 & is1 & is2 & is3);
+      const bool there = present == 15u && key + kManyKeys <= end;
+      const bool edge = key < wave_all_low || key + kManyKeys > wave_all_high || !there;
       f16v s[2];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
@@ -206,8 +232,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             const int at = key + 32 * u + 8 * (i / 4) + 4 * half + i % 4;
-            const bool is = u ? (i < 8 ? is2 : is3) : (i < 8 ? is0 : is1);
-            if (!(is && at >= low_r && at < high_r && at < end)) s[u][i] = -INFINITY;
+            if (!((present >> (2 * u + i / 8) & 1) && at >= low_r && at < high_r && at < end)) s[u][i] = -INFINITY;
           }
       }
       float top = -INFINITY;
@@ -225,16 +250,16 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
       }
       const float zero = m == -INFINITY ? 0.f : m;
       V8 p[2][2];
-      float sum = 0.f;
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], a.scale2, -zero));
-          sum += x;
+          sum[u] += x;
           p[u][i / 8][i % 8] = (T)x;
         }
-      l += sum;
+      l += sum[0] + sum[1];
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -247,7 +272,8 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
             const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TrPtr)(at + 8 * Shared::kStrideV));
             o[c] = E::mfma32(__builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), p[u][b], o[c]);
           }
-      if (sh.wild[buffer][0] | sh.wild[buffer][1] | sh.wild[buffer][2] | sh.wild[buffer][3]) {
+      if ((!there || is_edge(key)) &&
+          (sh.wild[buffer][0] | sh.wild[buffer][1] | sh.wild[buffer][2] | sh.wild[buffer][3])) {
         // values that are not finite went in as zeros: the rows that see them get them added
         for (int k = key; k < min(key + kManyKeys, end); k++) {
           const int in = table[k >> a.page_shift];
@@ -263,7 +289,8 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend a) {
         }
       }
     }
-    if (more) store(buffer ^ 1, key + kManyKeys);
+    if (more) store(buffer ^ 1, key + kManyKeys, next_present);
+    present = next_present;
   }
 
   if (!row_here) return;

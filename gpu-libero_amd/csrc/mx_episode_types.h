@@ -31,6 +31,11 @@ typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// Tables, lengths and starts do not change while a kernel runs: where an index is a wave's own, its load goes
+// through the scalar cache
+typedef __attribute__((address_space(4))) const int32_t Fixed;
+__device__ inline Fixed* fixed(const int32_t* p) { return (Fixed*)(uintptr_t)p; }
+
 template <int kType> struct Elem;
 template <> struct Elem<MX_TYPE_BF16> {
   typedef __bf16 T;
@@ -157,17 +162,17 @@ __device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, T
     low = __builtin_amdgcn_readfirstlane(low);
     t.world = low;
     const long long row = (tile - tile_base(a, low, rows_per_tile)) * rows_per_tile;
-    token = a.start[low];
-    const int end = min(a.start[low + 1], a.tokens);
+    token = fixed(a.start)[low];
+    const int stop = fixed(a.start)[low + 1], end = min(stop, a.tokens);
     if (token < 0 || end <= token || row < 0 || row >= (long long)(end - token) * a.group) return false;
     t.row = (int)row;
-    count = a.start[low + 1] - token;
+    count = stop - token;
     t.rows = (int)min((long long)min(end - token, a.max_count) * a.group, (long long)INT32_MAX);
   }
   if (!a.start) t.rows = a.max_count * a.group;
   if (t.row >= t.rows) return false;
   t.token = token;
-  const int length = max(a.length[t.world], 0);
+  const int length = max(fixed(a.length)[t.world], 0);
   t.position = length - count;
   t.length = (int)min((long long)length, (long long)a.width << a.page_shift);
   return true;
