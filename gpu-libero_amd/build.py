@@ -19,7 +19,8 @@ SOURCES = [HERE / 'csrc' / 'mx_step.hip', HERE / 'csrc' / 'mx_step_slab.hip', HE
            HERE / 'csrc' / 'mx_step_f64.hip', HERE / 'csrc' / 'mx_episode.hip'] + [
            HERE / 'csrc' / ('mx_episode_d%d.hip' % d) for d in (32, 64, 96, 128, 256)]
 HEADERS = [HERE / 'csrc' / h for h in ('mx_math.h', 'mx_image.h', 'mx_collide.h', 'mx_convex.h', 'mx_episode_types.h',
-                                       'mx_episode_few.h', 'mx_episode_many.h', 'mx_episode_launch.h', 'mx_episode_dim.h')] + [
+                                       'mx_episode_few.h', 'mx_episode_many.h',
+                                       'mx_episode_stage.h', 'mx_episode_launch.h', 'mx_episode_dim.h')] + [
            ROOT / 'include' / 'mx_physics.h', ROOT / 'include' / 'mx_episode.h']
 
 HIPCC_FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared',

@@ -392,9 +392,9 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 // 1024 30.7, 2048 33.1.
 int choose(Attend& a, Launch& launch) {
   const int64_t rows = (int64_t)a.max_count * a.group;
-  launch.blocks = rows <= 16 ? 1 : rows <= 32 || launch.head_dim == 256 ? 2 : 4;
+  launch.blocks = rows <= 16 ? 1 : 2;
   launch.rows = 16 * launch.blocks;
-  if (rows > 64 && launch.head_dim <= 128) launch.rows = kManyRows;
+  if (rows > 32 && launch.head_dim <= 128) launch.rows = kManyRows;
   const int64_t tiles = a.start ? (int64_t)a.tokens * a.group / launch.rows + a.nworld
                                 : ((rows + launch.rows - 1) / launch.rows) * a.nworld;
   int64_t keys = (int64_t)a.width << a.page_shift;
@@ -405,7 +405,7 @@ int choose(Attend& a, Launch& launch) {
   const int64_t groups = tiles * a.kv_heads;
   const int room = launch.head_dim <= 64 ? 1024 : 512;
   int64_t splits = keys * launch.head_dim <= 131072 ? 1 : (room + groups - 1) / groups;
-  const int64_t most = (keys + 31) / kLeastKeys + 1;     // the first key goes down to a multiple of 32
+  const int64_t most = (keys + 63) / kLeastKeys + 1;     // the first key goes down to a multiple of 64
   splits = splits < most ? splits : most;
   if (splits > kMostSplits) splits = kMostSplits;
   if (groups * splits > INT32_MAX) return MX_ERR_DOMAIN;

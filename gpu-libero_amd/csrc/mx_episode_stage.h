@@ -1,0 +1,291 @@
+// Bringing 64 keys and their values at a time into LDS, for workgroups of 256 threads.
+//
+// 16-bit pages go from memory to LDS without passing registers (each wave 1 KB at a time, lane after lane), so
+// the rows in LDS are as long as in the pages; what keeps the reads off each other's banks is the order of a row's
+// 16-byte pieces, which each row has its own of: reads of one piece of 16 rows, and transposing reads of
+// four pieces of four rows, fall into all 64 banks once.  8-bit pages are converted on the way.
+#pragma once
+#include <cstddef>
+#include "mx_episode_types.h"
+
+namespace mxe {
+
+constexpr int kManyKeys = 64;
+
+template <class E, int D>
+struct Staged {
+  static constexpr int kPieces = D / 8;       // of a row; 16 of them pass over all banks
+  typename E::T k[kManyKeys * D], v[kManyKeys * D];
+  int wild[4];                                // by wave: an infinity or NaN among the values it brought
+
+  // the place of piece p of a row, and (they are pairs) the piece at a place
+  static __device__ __forceinline__ int place_k(int row, int p) {
+    if constexpr (D == 96) return p + (row >> 2 & 3) < 12 ? p + (row >> 2 & 3) : p + (row >> 2 & 3) - 12;
+    else if constexpr (D < 128) return p ^ (row / (16 / kPieces) & (kPieces - 1));
+    else return p ^ (row & 15);
+  }
+  static __device__ __forceinline__ int piece_k(int row, int at) {
+    if constexpr (D == 96) return at - (row >> 2 & 3) >= 0 ? at - (row >> 2 & 3) : at - (row >> 2 & 3) + 12;
+    else return place_k(row, at);
+  }
+  static __device__ __forceinline__ int place_v(int row, int p) {
+    if constexpr (D >= 128) return p ^ 4 * (row & 3);
+    else if constexpr (D == 64) return p ^ 4 * (row >> 1 & 1);
+    else return p;
+  }
+};
+
+// The 64 keys of a step start at a multiple of 64: pages of 64 tokens and more (kLarge) hold them all, smaller
+// ones a multiple of 16 of them, so that addresses are a wave's own but for an offset of 32 bits.  Page numbers are
+// asked for a step before the loads that need them.
+template <class E, bool kFp8, bool kLarge, int D>
+struct Stage {
+  typedef typename E::T T;
+  typedef typename E::V8 V8;
+  typedef Staged<E, D> Shared;
+  static constexpr int kPer = kFp8 ? 16 : 8, kChunks = D / kPer, kLoads = (kManyKeys * kChunks + 255) / 256;
+  static constexpr bool kWhole = kManyKeys * kChunks % 256 == 0, kOneGroup = 16 * kChunks % 64 == 0;
+  static constexpr int kPages = kLarge ? 1 : 4;
+  static constexpr int kRowBytes = kFp8 ? D : 2 * D, kScales = D / MX_SCALE_BLOCK;
+
+  const Attend& a;
+  Fixed* table;
+  int head, end;
+  int page[kPages];                           // of all keys, or of each 16 of them
+  unsigned from_k[kLoads], from_v[kLoads];    // this thread's pieces, from the first key's row
+  u4 kreg[kFp8 ? kLoads : 1], vreg[kFp8 ? kLoads : 1];
+  unsigned kbyte[kFp8 ? kLoads : 1], vbyte[kFp8 ? kLoads : 1];
+
+  __device__ __forceinline__ Stage(const Attend& a, int world, int head, int end)
+      : a(a), table(fixed(a.table + (int64_t)world * a.width)), head(head), end(end) {
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      const int row = key_of(j), at = piece_of(j);
+      from_k[j] = row * kRowBytes + (kFp8 ? at : Shared::piece_k(row, at)) * 16;
+      from_v[j] = row * kRowBytes + (kFp8 ? at : Shared::place_v(row, at)) * 16;
+    }
+  }
+
+  // Each thread has kLoads pieces of kPer values: of which key of the 64, and the how manieth of its row
+  static __device__ __forceinline__ int key_of(int j) { return (j * 256 + (int)threadIdx.x) / kChunks; }
+  static __device__ __forceinline__ int piece_of(int j) { return (j * 256 + (int)threadIdx.x) % kChunks; }
+  static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+  __device__ __forceinline__ int first_of(int key, int g) const { return min(key + 16 * g, (end - 1) & ~15); }
+  __device__ __forceinline__ int64_t row_of(int page, int key) const {
+    return (((int64_t)page * a.kv_heads + head) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+  }
+
+  __device__ __forceinline__ void look_up(int key) {
+#pragma unroll
+    for (int g = 0; g < kPages; g++) page[g] = table[(kLarge ? key : first_of(key, g)) >> a.page_shift];
+  }
+
+  // The pages that are there, a bit for each 16 keys
+  __device__ __forceinline__ unsigned present() const {
+    unsigned bits = 0;
+#pragma unroll
+    for (int g = 0; g < kPages; g++) bits |= ((unsigned)page[g] < (unsigned)a.npage ? kLarge ? 15u : 1u : 0u) << g;
+    return bits;
+  }
+
+  // From memory into LDS, a wave's 64 pieces one after the other from `to` on.  As the builtin, but for the
+  // waits that the compiler would put before every LDS read that follows, whatever it reads: arrived() waits.
+  static __device__ __forceinline__ void into_lds(const uint8_t* base, unsigned offset, unsigned place) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place), "v"(offset), "s"(base)
+                 : "memory", "m0");
+  }
+  static __device__ __forceinline__ void arrived() {
+    if constexpr (!kFp8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+
+  // `to`: the LDS address of the buffer
+  __device__ __forceinline__ void bring(unsigned to, int j, int64_t at, unsigned k, unsigned v, unsigned scale) {
+    const uint8_t *from_k = a.k + at * kRowBytes, *from_v = a.v + at * kRowBytes;
+    if constexpr (kFp8) {
+      kreg[j] = *(const u4*)(from_k + k);
+      vreg[j] = *(const u4*)(from_v + v);
+      kbyte[j] = (a.k_scale + at * kScales)[scale];
+      vbyte[j] = (a.v_scale + at * kScales)[scale];
+    } else {
+      to += (j * 256 + 64 * wave()) * 16;
+      into_lds(from_k, k, to + offsetof(Shared, k));
+      into_lds(from_v, v, to + offsetof(Shared, v));
+    }
+  }
+
+  // Starts the loads of 64 keys from `key` on; keys at and beyond `end` repeat the last one's address
+  __device__ __forceinline__ void load(unsigned to, int key) {
+    if (kLarge && key + kManyKeys <= end) {
+      const int64_t at = row_of((unsigned)page[0] < (unsigned)a.npage ? page[0] : 0, key);
+#pragma unroll
+      for (int j = 0; j < kLoads; j++)
+        if (kWhole || key_of(j) < kManyKeys) bring(to, j, at, from_k[j], from_v[j], key_of(j) * kScales + piece_of(j) / 2);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      if (!kWhole && key_of(j) >= kManyKeys) continue;
+      if constexpr (kLarge) {
+        const int64_t at = row_of((unsigned)page[0] < (unsigned)a.npage ? page[0] : 0, key);
+        // rows beyond the last: that one's piece instead
+        const int row = min(key_of(j), end - 1 - key);
+        const unsigned back = (key_of(j) - row) * kRowBytes;
+        bring(to, j, at, from_k[j] - back, from_v[j] - back, row * kScales + piece_of(j) / 2);
+      } else {
+        // the group of 16 keys: the wave's, or where a wave's pieces straddle two, the lane's
+        const int group = kOneGroup ? (j * 256 + 64 * wave()) / (16 * kChunks) : key_of(j) / 16;
+        const int first = first_of(key, group);
+        int in = page[0];
+#pragma unroll
+        for (int g = 1; g < kPages; g++) in = group == g ? page[g] : in;
+        if constexpr (kOneGroup) in = __builtin_amdgcn_readfirstlane(in);
+        const int64_t at = row_of((unsigned)in < (unsigned)a.npage ? in : 0, first);
+        const int row = min(key_of(j) % 16, end - 1 - first);
+        const unsigned back = (key_of(j) - row) * kRowBytes;
+        bring(to, j, at, from_k[j] - back, from_v[j] - back, row * kScales + piece_of(j) / 2);
+      }
+    }
+  }
+
+  // 8-bit pages: what load() brought into registers, converted, into LDS.  `careful`: see clean().
+  __device__ __forceinline__ void store(Shared& to, int key, unsigned there, bool careful) {
+    if constexpr (kFp8) {
+      unsigned wild = 0;
+#pragma unroll
+      for (int j = 0; j < kLoads; j++) {
+        if (!kWhole && key_of(j) >= kManyKeys) continue;
+        const int row = key_of(j);
+        const bool none = careful && (key + row >= end || !(there >> (row / 16) & 1));
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int p = 2 * piece_of(j) + e;
+          *(V8*)&to.k[row * D + Shared::place_k(row, p) * 8] =
+              from_fp8<E>(e ? u2{kreg[j].z, kreg[j].w} : u2{kreg[j].x, kreg[j].y}, kbyte[j]);
+          u4 v = __builtin_bit_cast(u4, from_fp8<E>(e ? u2{vreg[j].z, vreg[j].w} : u2{vreg[j].x, vreg[j].y}, vbyte[j]));
+          if (careful) wild |= cleaned(v, none);
+          *(u4*)&to.v[row * D + Shared::place_v(row, p) * 8] = v;
+        }
+      }
+      if (careful) flag(to, wild);
+    }
+  }
+
+  // Some of the keys are not there, or not seen by all rows: values of the former become zeros, and infinities and
+  // NaN too (the rows that see them get them added, by repair()).  16-bit pages: in LDS, each thread what
+  // it brought, after its loads are done and before a barrier.
+  __device__ __forceinline__ void clean(Shared& to, int key, unsigned there) {
+    unsigned wild = 0;
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      if (!kWhole && key_of(j) >= kManyKeys) continue;
+      const int row = key_of(j);
+      u4* at = (u4*)&to.v[(j * 256 + threadIdx.x) * 8];
+      u4 v = *at;
+      wild |= cleaned(v, key + row >= end || !(there >> (row / 16) & 1));
+      *at = v;
+    }
+    flag(to, wild);
+  }
+
+  static __device__ __forceinline__ unsigned cleaned(u4& v, bool none) {
+    unsigned wild = 0;
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+      if (none) v[y] = 0;
+      wild |= not_finite<E>(v[y]) & 0x80008000u;
+      v[y] = finite_or_zero<E>(v[y]);
+    }
+    return wild;
+  }
+  __device__ __forceinline__ void flag(Shared& to, unsigned wild) const {
+    const int any = __ballot(wild != 0) != 0;
+    if ((threadIdx.x & 63) == 0) to.wild[threadIdx.x >> 6] = any;
+  }
+
+  // Values of the keys [key, stop) that are not finite, added to the output of a lane's row if it sees the key
+  // (o in the layout of 32x32 products).
+  __device__ __forceinline__ void repair(int key, int stop, int low_r, int high_r, f16v (&o)[D / 32]) const {
+    const int half = (threadIdx.x & 63) >> 5;
+    for (int k = key; k < min(stop, end); k++) {
+      const int in = table[k >> a.page_shift];
+      if ((unsigned)in >= (unsigned)a.npage || !(k >= low_r && k < high_r)) continue;
+      const int64_t at = row_of(in, k);
+#pragma unroll
+      for (int c = 0; c < D / 32; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float value = value_at<E, kFp8, D>(a, at, 32 * c + 8 * (i / 4) + 4 * half + i % 4);
+          if (!(fabsf(value) < INFINITY)) o[c][i] += value;
+        }
+    }
+  }
+};
+
+__device__ __forceinline__ float both_halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_halves_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Where the 32 rows of a wave end up: their parts, or the output.  o, m, l as the kernels keep them (m and l
+// in powers of two; l of this lane's half of the keys).
+template <class E, int D>
+__device__ __forceinline__ void finish_row(const Attend& a, int split, int token, int query_head, float m, float l,
+                                  const f16v (&o)[D / 32]) {
+  typedef typename E::T T;
+  const int half = (threadIdx.x & 63) >> 5;
+  l = both_halves_sum(l);
+  const int64_t row_at = (int64_t)token * a.heads + query_head;
+  if (a.splits > 1) {
+    const int64_t at = (int64_t)split * a.tokens * a.heads + row_at;
+    if (l != 0.f)
+#pragma unroll
+      for (int c = 0; c < D / 32; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *(f4*)(a.part + at * D + 32 * c + 2 * i + 4 * half) = f4{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]};
+    if (half == 0) *(f2*)(a.part_ml + 2 * at) = f2{m, l};
+    return;
+  }
+  const float inverse = 1.f / l;
+  T* to = (T*)a.out + (int64_t)token * a.o_token + (int64_t)query_head * a.o_head;
+#pragma unroll
+  for (int c = 0; c < D / 32; c++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      T x[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = (T)(l == 0.f ? 0.f : o[c][i + e] * inverse);
+      if (a.o_vector) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        *(T4*)(to + 32 * c + 2 * i + 4 * half) = T4{x[0], x[1], x[2], x[3]};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) to[32 * c + 2 * i + 4 * half + e] = x[e];
+      }
+    }
+  if (a.lse && half == 0) a.lse[row_at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Blocks go to the XCDs in turn: where the key heads of all worlds divide among the eight, those of one
+// stay on one XCD, whose L2 then holds their keys and values.  Last rows first: under a causal mask they
+// have the most keys.
+__device__ __forceinline__ void place(const Attend& a, int& split, int& head, int& tile) {
+  unsigned block = blockIdx.x;
+  split = block % a.splits;
+  block /= a.splits;
+  const int per = a.tiles / a.nworld;
+  if (!a.start && (a.nworld * a.kv_heads) % 8 == 0) {
+    const int i = block >> 3, pair = (block & 7) + 8 * (i / per);
+    head = pair % a.kv_heads;
+    tile = pair / a.kv_heads * per + per - 1 - i % per;
+  } else {
+    head = block % a.kv_heads;
+    tile = a.tiles - 1 - block / a.kv_heads;
+  }
+}
+
+}  // namespace mxe

@@ -107,6 +107,12 @@ struct Attend {
   bool q_vector, o_vector;           // q's rows are 16-byte aligned, out's 8-byte
 };
 
+// A kernel's only argument, read where it is used: as a by-value parameter all of it would be in scalar
+// registers from the first instruction to the last, and the loops' own values would be spilled for it.
+__device__ __forceinline__ const Attend& arguments() {
+  return *(const Attend*)(__attribute__((address_space(4))) const Attend*)__builtin_amdgcn_kernarg_segment_ptr();
+}
+
 // Eight values of a query
 template <class E> __device__ inline typename E::V8 load_query(const Attend& a, const typename E::T* from) {
   typename E::V8 x;
@@ -183,7 +189,7 @@ __device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, T
 // the most that the table can hold, so that long and short worlds both keep all splits at work.
 constexpr int kLeastKeys = 256;
 __device__ inline void split_range(const Attend& a, int split, int low, int high, int& begin, int& end) {
-  begin = low & ~31;
+  begin = low & ~63;
   end = high;
   if (a.splits == 1) return;
   const int each = max(kLeastKeys, (int)(((unsigned)max(high - begin, 0) / (unsigned)a.splits + 128u) & ~127u));
