@@ -263,3 +263,143 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
     if rc:
         native.check(rc, 'mx_episode_attend')
     return out
+
+
+class Chunk:
+    """New tokens of an :class:`EpisodeCache`: of all its worlds the same number (``start`` None; rows are
+    ``(nworld, count, heads, head_dim)``), or ``counts[w]`` of world w (rows ``(tokens, heads, head_dim)``, packed
+    world by world, ``start`` on the device)."""
+
+    __slots__ = ('counts', 'tokens', 'count', 'start')
+
+    def __init__(self, counts, start):
+        self.counts, self.start = counts, start
+        self.tokens, self.count = int(counts.sum()), int(counts.max())
+
+    @property
+    def shape(self):
+        """The rows' leading shape."""
+        return (self.tokens,) if self.start is not None else (len(self.counts), self.count)
+
+
+class EpisodeCache:
+    """The episode memory of a batch of worlds, for a policy of ``layers`` attention layers.
+
+    ``tokens``: the most tokens of one world.  ``pages``: how many pages of ``page_tokens`` tokens all worlds
+    share (by default enough for every world at its longest; worlds in different phases of their episodes do
+    with about half).  ``storage``: 'fp8' (quantised, a scale per 32 values), 'bf16' or 'f16'.
+
+    Each step, :meth:`extend` makes room for the new tokens; then, layer by layer, :meth:`write` stores their keys and
+    values and :meth:`attend` attends from their queries.  :meth:`reset` empties worlds, as
+    ``HipBatchEnv.reset(id)`` restarts them.  Tables and lengths live on the device (``table``, ``length``), with a
+    copy on the host (``lengths``) that room is made by; pages are not cleared, their old contents are never read."""
+
+    def __init__(self, nworld, *, kv_heads, head_dim, tokens, layers=1, storage='fp8', page_tokens=64, pages=None,
+                 device='cuda:0'):
+        _require(storage in STORAGE, 'storage must be one of %s, got %s', sorted(STORAGE), storage)
+        _require(nworld > 0 and tokens > 0 and layers > 0 and kv_heads > 0, 'nworld, tokens, layers and kv_heads must be positive')
+        _require(head_dim in HEAD_DIMS, 'head_dim must be one of %s, got %s', HEAD_DIMS, head_dim)
+        _require(16 <= page_tokens <= 4096 and not page_tokens & (page_tokens - 1),
+                 'page_tokens must be a power of two from 16 to 4096, got %s', page_tokens)
+        width = -(-tokens // page_tokens)
+        pages = nworld * width if pages is None else int(pages)
+        _require(pages > 0, 'pages must be positive, got %s', pages)
+        device = torch.device(device)
+        if device.type == 'cuda' and device.index is None:
+            device = torch.device('cuda', torch.cuda.current_device())
+        self.nworld, self.tokens, self.page_tokens, self.device = nworld, int(tokens), page_tokens, device
+        self.table = torch.full((nworld, width), -1, dtype=torch.int32, device=device)
+        self.length = torch.zeros(nworld, dtype=torch.int32, device=device)
+        self.lengths = np.zeros(nworld, np.int64)
+        self._table = np.full((nworld, width), -1, np.int32)
+        self._free = np.arange(pages - 1, -1, -1, dtype=np.int32)     # a stack; its first _left are free
+        self._left = pages
+        shape = (pages, kv_heads, page_tokens, head_dim)
+        self.layers = []
+        for _ in range(layers):
+            k, v = (torch.empty(shape, dtype=STORAGE[storage], device=device) for _ in range(2))
+            scales = [torch.empty(shape[:3] + (head_dim // SCALE_BLOCK,), dtype=torch.uint8, device=device)
+                      for _ in range(2 if storage == 'fp8' else 0)]
+            self.layers.append(Pages(k, v, self.table, self.length, *scales))
+
+    @property
+    def free_pages(self):
+        return self._left
+
+    def _ids(self, id):
+        ids = np.arange(self.nworld) if id is None else np.atleast_1d(np.asarray(id, np.int64))
+        if ids.ndim != 1 or np.any((ids < 0) | (ids >= self.nworld)) or len(np.unique(ids)) != len(ids):
+            raise ValueError('invalid world ids')
+        return ids
+
+    def extend(self, count=1, id=None):
+        """Makes room for ``count`` (a number, or one for each world of ``id``) new tokens of the worlds ``id`` (all by
+        default) and returns their :class:`Chunk`.  Raises ValueError where a world would pass ``tokens`` and RuntimeError
+        when the pages do not suffice; nothing has changed then."""
+        ids = self._ids(id)
+        new = np.broadcast_to(np.asarray(count, np.int64), ids.shape)
+        _require(not np.any(new < 0), 'count must not be negative')
+        before = self.lengths[ids]
+        _require(not np.any(before + new > self.tokens), 'a world would hold more than %d tokens', self.tokens)
+        first, last = -(-before // self.page_tokens), -(-(before + new) // self.page_tokens)
+        need = last - first
+        total = int(need.sum())
+        if total > self._left:
+            raise RuntimeError('episode memory: %d more pages needed, %d free' % (total, self._left))
+        if total:
+            world = np.repeat(ids, need)
+            slot = np.repeat(first, need) + np.arange(total) - np.repeat(np.cumsum(need) - need, need)
+            page = self._free[self._left - total:self._left][::-1].copy()
+            self._left -= total
+            self._table[world, slot] = page
+            where = torch.from_numpy(world * self._table.shape[1] + slot).to(self.device)
+            self.table.view(-1)[where] = torch.from_numpy(page).to(self.device)
+        self.lengths[ids] += new
+        counts = np.zeros(self.nworld, np.int64)
+        counts[ids] = new
+        if len(ids) and len(ids) == self.nworld and np.all(new == new[0]):
+            if new[0]:
+                self.length.add_(int(new[0]))
+            return Chunk(counts, None)
+        both = np.zeros(2 * self.nworld + 1, np.int32)                # one upload: the chunk's starts, the lengths
+        both[1:self.nworld + 1] = np.cumsum(counts)
+        both[self.nworld + 1:] = self.lengths
+        both = torch.from_numpy(both).to(self.device)
+        self.length.copy_(both[self.nworld + 1:])
+        return Chunk(counts, both[:self.nworld + 1])
+
+    def reset(self, id=None):
+        """Empties the worlds ``id`` (all by default); their pages are free again."""
+        ids = self._ids(id)
+        if not len(ids):
+            return
+        rows = self._table[ids]
+        pages = rows[rows >= 0]
+        self._free[self._left:self._left + len(pages)] = pages
+        self._left += len(pages)
+        self._table[ids] = -1
+        self.lengths[ids] = 0
+        where = torch.from_numpy(ids).to(self.device)
+        self.table[where] = -1
+        self.length[where] = 0
+
+    def write(self, chunk, k, v, layer=0, *, stream=None):
+        """:func:`write` of the chunk's keys and values to a layer."""
+        write(self.layers[layer], k, v, chunk.start, stream=stream)
+
+    def attend(self, chunk, q, layer=0, **options):
+        """:func:`attend` from the chunk's queries to a layer; options as there."""
+        if chunk.start is not None:
+            options.setdefault('max_count', chunk.count)
+        return attend(self.layers[layer], q, chunk.start, **options)
+
+    def read(self, id=None, layer=0, *, dtype=torch.bfloat16, stream=None):
+        """The keys and values of the worlds ``id`` (all by default) as a layer stands for them, packed in the order of
+        the worlds, and the rows' starts (numpy, one more than ids): ``(k, v, starts)``."""
+        ids = np.sort(self._ids(id))
+        counts = np.zeros(self.nworld, np.int64)
+        counts[ids] = self.lengths[ids]
+        start = np.concatenate([[0], np.cumsum(counts)])
+        k, v = read(self.layers[layer], torch.from_numpy(start.astype(np.int32)).to(self.device), tokens=int(start[-1]),
+                    dtype=dtype, stream=stream)
+        return k, v, np.concatenate([start[ids], start[-1:]])
