@@ -99,14 +99,14 @@ template <int kStore, int N> __device__ inline void load_page(const Copy& c, int
   if constexpr (kStore == MX_TYPE_FP8) {
     const u4 w = *(const u4*)(c.pages + at);
     const unsigned byte = c.scales[at / MX_SCALE_BLOCK];
-    const float scale = byte == 255 ? NAN : __uint_as_float(byte ? byte << 23 : 0x400000u);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const f2 p = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false), q = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
-      x[4 * j] = p[0] * scale;
-      x[4 * j + 1] = p[1] * scale;
-      x[4 * j + 2] = q[0] * scale;
-      x[4 * j + 3] = q[1] * scale;
+      const f2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale_of(byte), false);
+      const f2 q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale_of(byte), true);
+      x[4 * j] = p[0];
+      x[4 * j + 1] = p[1];
+      x[4 * j + 2] = q[0];
+      x[4 * j + 3] = q[1];
     }
   } else {
     load_row((const typename Elem<kStore>::T*)c.pages + at, true, x);

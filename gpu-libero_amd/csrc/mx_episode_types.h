@@ -74,21 +74,15 @@ template <class E> __device__ inline unsigned finite_or_zero(unsigned w) {
   return w & ~((off & 0x8000u ? 0xffffu : 0u) | (off & 0x80000000u ? 0xffff0000u : 0u));
 }
 
-// E8M0: byte b stands for 2^(b - 127); 255 for NaN, which the codes then carry (nan_codes)
+// E8M0: byte b stands for 2^(b - 127), 255 for NaN.  The scaled conversions take the exponent of their scale in
+// this sense, with 255 giving NaN whatever the code and 0 giving 2^-127 (run over all of these).
 __device__ inline float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
-__device__ inline unsigned nan_codes(unsigned w, unsigned byte) { return byte == 255 ? 0x7f7f7f7fu : w; }
 
 template <class E> __device__ inline typename E::V8 from_fp8(u2 w, unsigned byte) {
-  typedef typename E::V8 V8;
-  const float s = scale_of(byte == 255 ? 127 : byte);
-  w.x = nan_codes(w.x, byte);
-  w.y = nan_codes(w.y, byte);
+  const float s = scale_of(byte);
   const auto a = E::template from_fp8<false>(w.x, s), b = E::template from_fp8<true>(w.x, s);
   const auto c = E::template from_fp8<false>(w.y, s), d = E::template from_fp8<true>(w.y, s);
-  V8 r;
-  r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1];
-  r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
-  return r;
+  return typename E::V8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // The kernels' arguments, by value.  `rows` are (token, head of the group) pairs of one key head, in
@@ -129,7 +123,7 @@ template <class E> __device__ inline typename E::V8 load_query(const Attend& a, 
 template <class E, bool kFp8, int D> __device__ inline float value_at(const Attend& a, int64_t at, int d) {
   if constexpr (kFp8) {
     const unsigned byte = a.v_scale[at * (D / 32) + d / 32];
-    return (float)E::template from_fp8<false>(nan_codes(a.v[at * D + d], byte), scale_of(byte == 255 ? 127 : byte))[0];
+    return (float)E::template from_fp8<false>(a.v[at * D + d], scale_of(byte))[0];
   } else {
     return (float)((const typename E::T*)a.v)[at * D + d];
   }

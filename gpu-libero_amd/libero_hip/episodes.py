@@ -31,8 +31,9 @@ from . import native
 
 SCALE_BLOCK = 32                      # values along head_dim that share a scale in 8-bit pages
 HEAD_DIMS = (32, 64, 96, 128, 256)
+ERR_WORKSPACE = -5
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
-_SIZES = {0: 4, 1: 2, 2: 2, 3: 1}
+_PAGE_TOKENS = frozenset(1 << i for i in range(4, 13))
 STORAGE = {'bf16': torch.bfloat16, 'f16': torch.float16, 'fp8': torch.float8_e4m3fn}
 
 EXPORTS = ['mx_pages_bytes', 'mx_chunk_bytes', 'mx_rows_bytes', 'mx_attention_bytes', 'mx_episode_write',
@@ -95,42 +96,57 @@ class Pages:
     of two from 16 to 4096, head_dim one of 32, 64, 96, 128, 256.  The tensors stay the caller's, and are
     held here."""
 
-    __slots__ = ('k', 'v', 'table', 'length', 'k_scale', 'v_scale', 'struct', 'device', 'index')
+    __slots__ = ('k', 'v', 'table', 'length', 'k_scale', 'v_scale', 'struct', 'index')
 
     def __init__(self, k, v, table, length, k_scale=None, v_scale=None):
-        _require(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype,
-                 'k and v pages must have one shape (npage, kv_heads, page_tokens, head_dim) and type')
-        kind = _TYPES.get(k.dtype, 0)
-        _require(kind > 0, 'pages must be bfloat16, float16 or float8_e4m3fn, got %s', k.dtype)
-        npage, kv, tokens, dim = k.shape
-        _require(dim in HEAD_DIMS, 'head_dim must be one of %s, got %d', HEAD_DIMS, dim)
-        _require(16 <= tokens <= 4096 and not tokens & (tokens - 1),
-                 'page_tokens must be a power of two from 16 to 4096, got %d', tokens)
-        _require(npage > 0 and 0 < kv <= 1024, 'pages need at least one page and 1 to 1024 heads')
-        device = k.device
-        _require(device.type == 'cuda', 'pages must be on the GPU')
-        _require(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.numel() > 0,
-                 'table must be contiguous int32 of shape (nworld, pages of a world)')
-        _require(length.dtype == torch.int32 and length.shape == table.shape[:1] and length.is_contiguous(),
-                 'length must be contiguous int32 of shape (nworld,)')
-        _require(npage * tokens < 2 ** 31 and table.shape[1] * tokens < 2 ** 31,
-                 'npage * page_tokens and the tokens of a table row must be below 2^31')
-        _require(k.is_contiguous() and v.is_contiguous() and not (k.data_ptr() | v.data_ptr()) & 15,
-                 'pages must be contiguous and 16-byte aligned')
+        # one condition for what is as it should be; what is not is named by _refuse_pages
+        shape, tables, kind, index = k.shape, table.shape, _TYPES.get(k.dtype, 0), k.get_device()
+        if not (kind and index >= 0 and len(shape) == 4 and len(tables) == 2 and v.shape == shape and v.dtype == k.dtype
+                and shape[3] in HEAD_DIMS and shape[2] in _PAGE_TOKENS and shape[0] > 0 and 0 < shape[1] <= 1024
+                and tables[0] > 0 and tables[1] > 0 and length.shape == tables[:1]
+                and table.dtype == torch.int32 and length.dtype == torch.int32
+                and shape[0] * shape[2] < 2 ** 31 and tables[1] * shape[2] < 2 ** 31
+                and v.get_device() == index and table.get_device() == index and length.get_device() == index
+                and k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and length.is_contiguous()
+                and (k_scale is None and v_scale is None) == (kind != 3)):
+            _refuse_pages(k, v, table, length, k_scale, v_scale)
+        at_k, at_v = k.data_ptr(), v.data_ptr()
+        _require(not (at_k | at_v) & 15, 'pages must be 16-byte aligned')
+        scale_k = scale_v = None
         if kind == 3:
-            shape = (npage, kv, tokens, dim // SCALE_BLOCK)
-            for s in (k_scale, v_scale):
-                _require(s is not None and s.dtype == torch.uint8 and s.shape == shape and s.is_contiguous(),
-                         '8-bit pages need contiguous uint8 scales of shape %s', shape)
-        else:
-            _require(k_scale is None and v_scale is None, 'only 8-bit pages have scales')
-        for t in (v, table, length, k_scale, v_scale):
-            _require(t is None or t.device == device, 'pages, scales, table and length must be on one device')
+            scales = shape[:3] + (shape[3] // SCALE_BLOCK,)
+            for x in (k_scale, v_scale):
+                if x is None or x.dtype != torch.uint8 or x.shape != scales or not x.is_contiguous() or x.get_device() != index:
+                    raise ValueError('8-bit pages need contiguous uint8 scales of shape %s on their device' % (tuple(scales),))
+            scale_k, scale_v = k_scale.data_ptr(), v_scale.data_ptr()
         self.k, self.v, self.table, self.length, self.k_scale, self.v_scale = k, v, table, length, k_scale, v_scale
-        self.device, self.index = device, device.index
-        self.struct = MxPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if kind == 3 else None,
-                              v_scale.data_ptr() if kind == 3 else None, table.data_ptr(), length.data_ptr(),
-                              table.shape[0], npage, table.shape[1], kv, dim, tokens, kind)
+        self.index = index
+        self.struct = MxPages(at_k, at_v, scale_k, scale_v, table.data_ptr(), length.data_ptr(), tables[0], shape[0],
+                              tables[1], shape[1], shape[3], shape[2], kind)
+
+    @property
+    def device(self):
+        return self.k.device
+
+
+def _refuse_pages(k, v, table, length, k_scale, v_scale):
+    _require(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype,
+             'k and v pages must have one shape (npage, kv_heads, page_tokens, head_dim) and type')
+    _require(_TYPES.get(k.dtype, 0) > 0, 'pages must be bfloat16, float16 or float8_e4m3fn, got %s', k.dtype)
+    npage, kv, tokens, dim = k.shape
+    _require(dim in HEAD_DIMS, 'head_dim must be one of %s, got %d', HEAD_DIMS, dim)
+    _require(tokens in _PAGE_TOKENS, 'page_tokens must be a power of two from 16 to 4096, got %d', tokens)
+    _require(npage > 0 and 0 < kv <= 1024, 'pages need at least one page and 1 to 1024 heads')
+    _require(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.numel() > 0,
+             'table must be contiguous int32 of shape (nworld, pages of a world)')
+    _require(length.dtype == torch.int32 and length.shape == table.shape[:1] and length.is_contiguous(),
+             'length must be contiguous int32 of shape (nworld,)')
+    _require(npage * tokens < 2 ** 31 and table.shape[1] * tokens < 2 ** 31,
+             'npage * page_tokens and the tokens of a table row must be below 2^31')
+    _require(k.is_contiguous() and v.is_contiguous(), 'pages must be contiguous')
+    _require((k_scale is None) == (v_scale is None) == (k.dtype != torch.float8_e4m3fn),
+             '8-bit pages have scales for k and v, others have none')
+    raise ValueError('pages, table and length must be on one GPU')
 
 
 def _chunk(pages, shape, start):
@@ -142,7 +158,7 @@ def _chunk(pages, shape, start):
         return MxChunk(None, nworld * shape[1], shape[1])
     _require(len(shape) == 1, 'rows with start must be packed: (tokens, heads, head_dim)')
     _require(start.dtype == torch.int32 and start.shape == (nworld + 1,) and start.is_contiguous()
-             and start.device == pages.device, 'start must be contiguous int32 of shape (nworld + 1,) on the pages\' device')
+             and start.get_device() == pages.index, 'start must be contiguous int32 of shape (nworld + 1,) on the pages\' device')
     return MxChunk(start.data_ptr(), shape[0], 0)
 
 
@@ -150,10 +166,10 @@ def _rows(pages, x, shape, name):
     """MxRows of a tensor (..., heads, head_dim) whose token dimensions step evenly."""
     kind = _TYPES.get(x.dtype, 3)
     stride = x.stride()
-    if kind == 3 or shape[-1] != pages.struct.head_dim or x.device != pages.device or stride[-1] != 1:
+    if kind == 3 or shape[-1] != pages.struct.head_dim or x.get_device() != pages.index or stride[-1] != 1:
         _require(kind < 3, '%s must be float32, bfloat16 or float16, got %s', name, x.dtype)
         _require(shape[-1] == pages.struct.head_dim, '%s has the wrong head_dim: %s', name, tuple(shape))
-        _require(x.device == pages.device, '%s must be on the pages\' device', name)
+        _require(x.get_device() == pages.index, '%s must be on the pages\' device', name)
         _require(stride[-1] == 1, '%s must be contiguous along head_dim', name)
     token = stride[-3]
     if len(shape) == 4:
@@ -238,12 +254,13 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
                  rows.heads, s.kv_heads)
         raise ValueError('q must be bfloat16 or float16, and of the pages\' type unless those are 8-bit: %s on %s'
                          % (q.dtype, pages.k.dtype))
-    _require(0 <= window < 2 ** 31, 'window must be 0 (none) or a number of tokens, got %s', window)
-    scale = s.head_dim ** -0.5 if scale is None else float(scale)
-    _require(math.isfinite(scale), 'scale must be finite')
+    if scale is None:
+        scale = s.head_dim ** -0.5
     if max_count is None:
         max_count = chunk.tokens if start is not None else chunk.count
-    _require(0 <= max_count < 2 ** 31, 'max_count must be a number of tokens, got %s', max_count)
+    if not (0 <= window < 2 ** 31 and 0 <= max_count < 2 ** 31 and math.isfinite(scale)):
+        raise ValueError('window (0: none) and max_count must be numbers of tokens and scale finite: %s, %s, %s'
+                         % (window, max_count, scale))
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
@@ -251,15 +268,15 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
     a = MxAttention(rows, _rows(pages, out, shape, 'out'), None, None, 0, max_count, 1 if causal else 0, window, scale)
     if lse is not None:
         _require(lse.dtype == torch.float32 and lse.shape == shape[:-1] and lse.is_contiguous()
-                 and lse.device == pages.device, 'lse must be contiguous float32 of q\'s shape without head_dim')
+                 and lse.get_device() == pages.index, 'lse must be contiguous float32 of q\'s shape without head_dim')
         a.lse = lse.data_ptr()
-    lib = _LIB or load()
-    refs = ct.byref(s), ct.byref(chunk), ct.byref(a)
-    need = lib.mx_episode_workspace(*refs)
-    if need:
+    lib, refs, raw = _LIB or load(), (ct.byref(s), ct.byref(chunk), ct.byref(a)), _current(pages.index)
+    rc = lib.mx_episode_attend(*refs, raw)
+    if rc == ERR_WORKSPACE:               # the keys are split: found before any launch
+        need = lib.mx_episode_workspace(*refs)
         workspace = torch.empty(need, dtype=torch.uint8, device=pages.device)
         a.workspace, a.workspace_bytes = workspace.data_ptr(), need
-    rc = lib.mx_episode_attend(*refs, _current(pages.index))
+        rc = lib.mx_episode_attend(*refs, raw)
     if rc:
         native.check(rc, 'mx_episode_attend')
     return out
