@@ -61,10 +61,18 @@ __device__ inline void find_slots(const Move& a, int first, int tokens, int64_t*
   }
 }
 
+// A thread's piece of a row in bytes, and how many pieces of keys and of values it has under way.  8-bit pages: 32
+// bytes, so that a thread's codes are 8 or 16 at once, except for reads into single precision, which are bound
+// by their own stores.  us, measured with 16 and 32 bytes: 500 histories of 8-bit pages into bf16 180 and 152, 67 chunks of
+// single precision written to 8-bit pages and read back 61 and 69 (16 for the read alone 59); one and two under way:
+// 500 histories of bf16 173 and 185, the 67 chunks 61 and 59.
+constexpr int piece_bytes(bool fp8, bool write, int size) { return fp8 && (write || size < 4) ? 32 : 16; }
+constexpr int pieces_ahead(int size) { return size == 4 ? 2 : 1; }
+
 template <class T, int N> __device__ inline void load_row(const T* from, bool vector, float (&x)[N]) {
+  constexpr int kEach = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  typedef T V __attribute__((ext_vector_type(kEach)));
   if (vector) {
-    constexpr int kEach = 16 / sizeof(T);
-    typedef T V __attribute__((ext_vector_type(kEach)));
 #pragma unroll
     for (int j = 0; j < N; j += kEach) {
       const V v = *(const V*)(from + j);
@@ -77,16 +85,19 @@ template <class T, int N> __device__ inline void load_row(const T* from, bool ve
   }
 }
 
-template <class T, int N> __device__ inline void store_row(T* to, bool vector, const float (&x)[N]) {
+// kPast: past the caches.  Rows that were read out are many; 262 MB of 8-bit pages into 524 MB of rows 183 us
+// through the caches, 152 past them, and 69 or 61 for 34 + 137 MB.
+template <bool kPast, class T, int N> __device__ inline void store_row(T* to, bool vector, const float (&x)[N]) {
+  constexpr int kEach = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  typedef T V __attribute__((ext_vector_type(kEach)));
   if (vector) {
-    constexpr int kEach = 16 / sizeof(T);
-    typedef T V __attribute__((ext_vector_type(kEach)));
 #pragma unroll
     for (int j = 0; j < N; j += kEach) {
       V v;
 #pragma unroll
       for (int e = 0; e < kEach; e++) v[e] = (T)x[j + e];
-      *(V*)(to + j) = v;
+      if constexpr (kPast) __builtin_nontemporal_store(v, (V*)(to + j));
+      else *(V*)(to + j) = v;
     }
   } else {
 #pragma unroll
@@ -97,12 +108,13 @@ template <class T, int N> __device__ inline void store_row(T* to, bool vector, c
 // `at`: element in the pages; at / 32 is the scale's place, as head_dim is a multiple of 32
 template <int kStore, int N> __device__ inline void load_page(const Copy& c, int64_t at, float (&x)[N]) {
   if constexpr (kStore == MX_TYPE_FP8) {
-    const u4 w = *(const u4*)(c.pages + at);
-    const unsigned byte = c.scales[at / MX_SCALE_BLOCK];
+    typedef unsigned W __attribute__((ext_vector_type(N / 4)));
+    const W w = *(const W*)(c.pages + at);
+    const float scale = scale_of(c.scales[at / MX_SCALE_BLOCK]);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const f2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale_of(byte), false);
-      const f2 q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale_of(byte), true);
+    for (int j = 0; j < N / 4; j++) {
+      const f2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale, false);
+      const f2 q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale, true);
       x[4 * j] = p[0];
       x[4 * j + 1] = p[1];
       x[4 * j + 2] = q[0];
@@ -113,45 +125,45 @@ template <int kStore, int N> __device__ inline void load_page(const Copy& c, int
   }
 }
 
-// All threads take part, with at < 0 where there is nothing to store: two neighbours share a scale
-template <int kStore, int N> __device__ inline void store_page(const Copy& c, int64_t at, float (&x)[N]) {
+// All threads take part, with at < 0 where there is nothing to store: neighbours share a scale
+template <int kStore, int N> __device__ inline void store_page(const Copy& c, int64_t at, const float (&x)[N]) {
   if constexpr (kStore == MX_TYPE_FP8) {
     // the largest magnitude of the block, as the bits of a float that is not negative: they order
     // like integers, infinities and NaN above all numbers
     unsigned top = 0;
 #pragma unroll
     for (int j = 0; j < N; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
-    top = max(top, (unsigned)__shfl_xor((int)top, 1));
+#pragma unroll
+    for (int lanes = 1; lanes < MX_SCALE_BLOCK / N; lanes *= 2) top = max(top, (unsigned)__shfl_xor((int)top, lanes));
     // 448 = 1.75 * 2^8: the exponent less 8, and one more above a fraction of 1.75
     const bool finite = top < 0x7f800000u;
     const int e = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), -117);
     const float inverse = __uint_as_float((unsigned)(127 - e) << 23);
     if (at < 0) return;
-    u4 w;
+    typedef unsigned W __attribute__((ext_vector_type(N / 4)));
+    W w;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < N / 4; j++) {
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) y[i] = finite ? x[4 * j + i] * inverse : 0.f;
       const unsigned half = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
       w[j] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], half, true);
     }
-    *(u4*)(c.pages + at) = w;
+    *(W*)(c.pages + at) = w;
     if (at % MX_SCALE_BLOCK == 0) c.scales[at / MX_SCALE_BLOCK] = finite ? (uint8_t)(e + 127) : 255;
   } else {
-    if (at >= 0) store_row((typename Elem<kStore>::T*)c.pages + at, true, x);
+    if (at >= 0) store_row<false>((typename Elem<kStore>::T*)c.pages + at, true, x);
   }
 }
 
 // A workgroup moves `tokens_each` packed tokens of all heads, keys and values: its first threads find
-// their slots, then every thread moves pieces of kPer values in the order of the rows, kItems of keys and
-// kItems of values under way at once.  Nothing is computed but the scales: bound by memory.
-template <int kStore> struct Pieces { static constexpr int kPer = kStore == MX_TYPE_FP8 ? 16 : 8; };
+// their slots, then every thread moves pieces in the order of the rows.  Nothing is computed but the scales: bound by memory.
 constexpr int kMostTokens = 64;                         // of a workgroup: their slots are kept in LDS
 
-template <class T, int kStore, int kItems, bool kWrite>
+template <class T, int kStore, bool kWrite>
 __global__ __launch_bounds__(256) void move_rows(const Move a) {
-  constexpr int kPer = Pieces<kStore>::kPer;
+  constexpr int kPer = piece_bytes(kStore == MX_TYPE_FP8, kWrite, sizeof(T)) / sizeof(T), kItems = pieces_ahead(sizeof(T));
   __shared__ int64_t slots[kMostTokens];
   const int first = blockIdx.x * a.tokens_each, tokens = min(a.tokens - first, a.tokens_each);
   if (threadIdx.x < 64) find_slots(a, first, tokens, slots);
@@ -190,7 +202,7 @@ __global__ __launch_bounds__(256) void move_rows(const Move a) {
 #pragma unroll
       for (int y = 0; y < 2; y++) {
         if constexpr (kWrite) store_page<kStore, kPer>(a.of[y], is[i] ? at[i] : -1, x[i][y]);
-        else if (is[i]) store_row<T, kPer>((T*)a.of[y].rows + to[y][i], a.of[y].vector, x[i][y]);
+        else if (is[i]) store_row<true>((T*)a.of[y].rows + to[y][i], a.of[y].vector, x[i][y]);
       }
   }
 }
@@ -312,12 +324,9 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
   }
   if (k->type != v->type) return MX_ERR_INVALID;
   if (!c->tokens) return 0;
-  // pieces of a token, and tokens of a workgroup: a few pieces to each thread, as soon as there are
-  // workgroups for every CU
-  const int pieces = p->kv_heads * (p->head_dim / (p->type == MX_TYPE_FP8 ? 16 : 8));
-  const int64_t all = (int64_t)c->tokens * pieces;
-  const int items = all >= 4 * 256 * 1024 ? 4 : 1;
-  int each = 256 * items / pieces;
+  // pieces of a token, and tokens of a workgroup
+  const int size = size_of(k->type), pieces = p->kv_heads * p->head_dim * size / piece_bytes(p->type == MX_TYPE_FP8, kWrite, size);
+  int each = 256 * pieces_ahead(size) / pieces;
   each = each < 1 ? 1 : each > kMostTokens ? kMostTokens : each;
   Move a{};
   uint8_t *pages[2] = {(uint8_t*)p->k, (uint8_t*)p->v}, *scales[2] = {p->k_scale, p->v_scale};
@@ -332,8 +341,7 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
   auto go = [&](auto t, auto store) {
     typedef decltype(t) T;
     constexpr int kStore = decltype(store)::value;
-    if (items == 4) hipLaunchKernelGGL((move_rows<T, kStore, 4, kWrite>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((move_rows<T, kStore, 1, kWrite>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((move_rows<T, kStore, kWrite>), grid, dim3(256), 0, (hipStream_t)stream, a);
   };
   auto by_store = [&](auto t) {
     if (p->type == MX_TYPE_FP8) go(t, std::integral_constant<int, MX_TYPE_FP8>());
