@@ -267,11 +267,12 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
         const int page = table[k >> a.page_shift];
         if ((unsigned)page >= (unsigned)a.npage) continue;
         const int64_t at = (((int64_t)page * a.kv_heads + head) << a.page_shift) + (k & page_mask);
+        const uint8_t *row = a.v + at * (kFp8 ? D : 2 * D), *scale = a.v_scale + at * kC;
 #pragma unroll
         for (int c = 0; c < D / 16; c++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const float value = value_at<E, kFp8, D>(a, at, 16 * c + 4 * quarter + i);
+            const float value = value_at<E, kFp8>(row, scale, 16 * c + 4 * quarter + i);
             if (!(fabsf(value) < INFINITY))
 #pragma unroll
               for (int b = 0; b < kBlocks; b++)

@@ -12,14 +12,19 @@
 
 namespace mxe {
 
+constexpr int many_keys(int D) { return 64; }
+constexpr int many_waves(int D) { return D <= 32 ? 4 : D <= 96 ? 3 : 2; }
+
 template <int kType, bool kFp8, bool kLarge, int D>
-__global__ __launch_bounds__(256, 2) void attend_many(const Attend) {
+__global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) {
   const Attend& a = arguments();
   typedef Elem<kType> E;
   typedef typename E::T T;
   typedef typename E::V8 V8;
-  typedef Staged<E, D> Shared;
-  constexpr int kC = D / 16, kTiles = D / 32;
+  constexpr int kKeys = many_keys(D), kC = D / 16, kTiles = D / 32, kU = kKeys / 32;
+  typedef Staged<E, kKeys, D> Shared;
+  typedef Stage<E, kFp8, kLarge, kKeys, D> Bring;
+  constexpr unsigned kAll = Bring::kAll;
   __shared__ __attribute__((aligned(1024))) Shared sh[2];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -63,10 +68,11 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend) {
     for (int i = 0; i < 16; i++) o[c][i] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  Stage<E, kFp8, kLarge, D> stage(a, t.world, head, end);
+  const float scale2 = a.scale2;
+  Bring stage(a, t.world, head, end);
   // keys that are not there, or that only some rows of the workgroup see
   const auto careful = [&](int key, unsigned there) {
-    return key < last_low || key + kManyKeys > first_high || there != 15u || key + kManyKeys > end;
+    return key < last_low || key + kKeys > first_high || there != kAll || key + kKeys > end;
   };
   // where this lane reads: a key's pieces, and for V^T the four keys and 4 of 16 values of its 16 lanes
   int from_k[kC], from_v[kTiles];
@@ -85,33 +91,33 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend) {
     stage.look_up(key);
     stage.load(at_lds, key);
     present = stage.present();
-    if (key + kManyKeys < end) stage.look_up(key + kManyKeys);
+    if (key + kKeys < end) stage.look_up(key + kKeys);
     stage.store(sh[0], key, present, careful(key, present));
   }
-  for (; key < end; key += kManyKeys, buffer ^= 1) {
-    const bool more = key + kManyKeys < end, mind = careful(key, present);
+  for (; key < end; key += kKeys, buffer ^= 1) {
+    const bool more = key + kKeys < end, mind = careful(key, present);
     stage.arrived();
     if (!kFp8 && mind) stage.clean(sh[buffer], key, present);
     __syncthreads();
     unsigned next_present = 0;
     if (more) {
-      stage.load(at_lds + (buffer ? 0 : (unsigned)sizeof(Shared)), key + kManyKeys);
+      stage.load(at_lds + (buffer ? 0 : (unsigned)sizeof(Shared)), key + kKeys);
       next_present = stage.present();
-      if (key + 2 * kManyKeys < end) stage.look_up(key + 2 * kManyKeys);
+      if (key + 2 * kKeys < end) stage.look_up(key + 2 * kKeys);
     }
-    if (rows_here && key < wave_high && key + kManyKeys > wave_low) {
+    if (rows_here && key < wave_high && key + kKeys > wave_low) {
       const T *ks = sh[buffer].k, *vs = sh[buffer].v;
-      f16v s[2];
+      f16v s[kU];
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
+      for (int u = 0; u < kU; u++) {
 #pragma unroll
         for (int i = 0; i < 16; i++) s[u][i] = 0.f;
 #pragma unroll
         for (int c = 0; c < kC; c++) s[u] = E::mfma32(*(const V8*)(ks + from_k[c] + 32 * u * D), q[c], s[u]);
       }
-      if (mind && (key < wave_all_low || key + kManyKeys > wave_all_high || present != 15u || key + kManyKeys > end)) {
+      if (mind && (key < wave_all_low || key + kKeys > wave_all_high || present != kAll || key + kKeys > end)) {
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int u = 0; u < kU; u++)
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             const int at = key + 32 * u + 8 * (i / 4) + 4 * half + i % 4;
@@ -120,10 +126,10 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend) {
       }
       float top = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int u = 0; u < kU; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
-      top = both_halves_max(top) * a.scale2;
+      top = both_halves_max(top) * scale2;
       if (__ballot(top > m + 8.f)) {
         const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
         m = next;
@@ -132,19 +138,19 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend) {
         for (int c = 0; c < kTiles; c++) o[c] *= shrink;
       }
       const float zero = m == -INFINITY ? 0.f : m;
-      V8 p[2][2];
+      V8 p[kU][2];
       float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int u = 0; u < kU; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], a.scale2, -zero));
-          sum[u] += x;
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale2, -zero));
+          sum[i & 1] += x;
           p[u][i / 8][i % 8] = (T)x;
         }
       l += sum[0] + sum[1];
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int u = 0; u < kU; u++)
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -155,9 +161,9 @@ __global__ __launch_bounds__(256, 2) void attend_many(const Attend) {
             o[c] = E::mfma32(__builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), p[u][b], o[c]);
           }
       if (mind && (sh[buffer].wild[0] | sh[buffer].wild[1] | sh[buffer].wild[2] | sh[buffer].wild[3]))
-        stage.repair(key, key + kManyKeys, low_r, high_r, o);
+        stage.repair(key, key + kKeys, low_r, high_r, o);
     }
-    if (more) stage.store(sh[buffer ^ 1], key + kManyKeys, next_present, careful(key + kManyKeys, next_present));
+    if (more) stage.store(sh[buffer ^ 1], key + kKeys, next_present, careful(key + kKeys, next_present));
     present = next_present;
   }
 

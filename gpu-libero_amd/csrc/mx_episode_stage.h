@@ -1,4 +1,4 @@
-// Bringing 64 keys and their values at a time into LDS, for workgroups of 256 threads.
+// Bringing kKeys (32 or 64) keys and their values at a time into LDS, for workgroups of 256 threads.
 //
 // 16-bit pages go from memory to LDS without passing registers (each wave 1 KB at a time, lane after lane), so
 // the rows in LDS are as long as in the pages; what keeps the reads off each other's banks is the order of a row's
@@ -10,12 +10,10 @@
 
 namespace mxe {
 
-constexpr int kManyKeys = 64;
-
-template <class E, int D>
+template <class E, int kKeys, int D>
 struct Staged {
   static constexpr int kPieces = D / 8;       // of a row; 16 of them pass over all banks
-  typename E::T k[kManyKeys * D], v[kManyKeys * D];
+  typename E::T k[kKeys * D], v[kKeys * D];
   int wild[4];                                // by wave: an infinity or NaN among the values it brought
 
   // the place of piece p of a row, and (they are pairs) the piece at a place
@@ -35,29 +33,39 @@ struct Staged {
   }
 };
 
-// The 64 keys of a step start at a multiple of 64: pages of 64 tokens and more (kLarge) hold them all, smaller
-// ones a multiple of 16 of them, so that addresses are a wave's own but for an offset of 32 bits.  Page numbers are
+// The keys of a step start at a multiple of their number: pages of 64 tokens and more (kLarge) hold them all,
+// smaller ones a multiple of 16 of them, so that addresses are a wave's own but for an offset of 32 bits.  Page numbers are
 // asked for a step before the loads that need them.
-template <class E, bool kFp8, bool kLarge, int D>
+template <class E, bool kFp8, bool kLarge, int kKeys, int D>
 struct Stage {
   typedef typename E::T T;
   typedef typename E::V8 V8;
-  typedef Staged<E, D> Shared;
-  static constexpr int kPer = kFp8 ? 16 : 8, kChunks = D / kPer, kLoads = (kManyKeys * kChunks + 255) / 256;
-  static constexpr bool kWhole = kManyKeys * kChunks % 256 == 0, kOneGroup = 16 * kChunks % 64 == 0;
-  static constexpr int kPages = kLarge ? 1 : 4;
+  typedef Staged<E, kKeys, D> Shared;
+  static constexpr int kPer = kFp8 ? 16 : 8, kChunks = D / kPer, kLoads = (kKeys * kChunks + 255) / 256;
+  static constexpr bool kWhole = kKeys * kChunks % 256 == 0, kOneGroup = 16 * kChunks % 64 == 0;
+  static constexpr int kPages = kLarge ? 1 : kKeys / 16;
+  static constexpr unsigned kAll = (1u << kKeys / 16) - 1;
   static constexpr int kRowBytes = kFp8 ? D : 2 * D, kScales = D / MX_SCALE_BLOCK;
 
-  const Attend& a;
+  // what a step needs of the arguments, kept in registers
   Fixed* table;
-  int head, end;
+  const uint8_t *k, *v, *k_scale, *v_scale;   // of this head in page 0
+  unsigned page_bytes, scale_bytes;           // from page to page
+  int page_shift, npage, end;
   int page[kPages];                           // of all keys, or of each 16 of them
   unsigned from_k[kLoads], from_v[kLoads];    // this thread's pieces, from the first key's row
   u4 kreg[kFp8 ? kLoads : 1], vreg[kFp8 ? kLoads : 1];
   unsigned kbyte[kFp8 ? kLoads : 1], vbyte[kFp8 ? kLoads : 1];
 
   __device__ __forceinline__ Stage(const Attend& a, int world, int head, int end)
-      : a(a), table(fixed(a.table + (int64_t)world * a.width)), head(head), end(end) {
+      : table(fixed(a.table + (int64_t)world * a.width)), page_shift(a.page_shift), npage(a.npage), end(end) {
+    const int64_t rows = (int64_t)head << page_shift;
+    k = a.k + rows * kRowBytes;
+    v = a.v + rows * kRowBytes;
+    k_scale = a.k_scale + rows * kScales;
+    v_scale = a.v_scale + rows * kScales;
+    page_bytes = ((unsigned)a.kv_heads << page_shift) * kRowBytes;      // at most 1024 heads of 4096 tokens of 512 bytes
+    scale_bytes = ((unsigned)a.kv_heads << page_shift) * kScales;
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
       const int row = key_of(j), at = piece_of(j);
@@ -66,25 +74,21 @@ struct Stage {
     }
   }
 
-  // Each thread has kLoads pieces of kPer values: of which key of the 64, and the how manieth of its row
+  // Each thread has kLoads pieces of kPer values: of which key, and the how manieth of its row
   static __device__ __forceinline__ int key_of(int j) { return (j * 256 + (int)threadIdx.x) / kChunks; }
   static __device__ __forceinline__ int piece_of(int j) { return (j * 256 + (int)threadIdx.x) % kChunks; }
   static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
   __device__ __forceinline__ int first_of(int key, int g) const { return min(key + 16 * g, (end - 1) & ~15); }
-  __device__ __forceinline__ int64_t row_of(int page, int key) const {
-    return (((int64_t)page * a.kv_heads + head) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-  }
-
   __device__ __forceinline__ void look_up(int key) {
 #pragma unroll
-    for (int g = 0; g < kPages; g++) page[g] = table[(kLarge ? key : first_of(key, g)) >> a.page_shift];
+    for (int g = 0; g < kPages; g++) page[g] = table[(kLarge ? key : first_of(key, g)) >> page_shift];
   }
 
   // The pages that are there, a bit for each 16 keys
   __device__ __forceinline__ unsigned present() const {
     unsigned bits = 0;
 #pragma unroll
-    for (int g = 0; g < kPages; g++) bits |= ((unsigned)page[g] < (unsigned)a.npage ? kLarge ? 15u : 1u : 0u) << g;
+    for (int g = 0; g < kPages; g++) bits |= ((unsigned)page[g] < (unsigned)npage ? kLarge ? kAll : 1u : 0u) << g;
     return bits;
   }
 
@@ -98,52 +102,48 @@ struct Stage {
     if constexpr (!kFp8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
 
-  // `to`: the LDS address of the buffer
-  __device__ __forceinline__ void bring(unsigned to, int j, int64_t at, unsigned k, unsigned v, unsigned scale) {
-    const uint8_t *from_k = a.k + at * kRowBytes, *from_v = a.v + at * kRowBytes;
+  // `to`: the LDS address of the buffer; `first`: the key in page `in` that the offsets start from
+  __device__ __forceinline__ void bring(unsigned to, int j, int in, int first, unsigned at_k, unsigned at_v, unsigned at_scale) {
+    const unsigned page = (unsigned)in < (unsigned)npage ? in : 0, row = first & ((1 << page_shift) - 1);
+    const uint64_t at = (uint64_t)page * page_bytes + row * (unsigned)kRowBytes;
     if constexpr (kFp8) {
-      kreg[j] = *(const u4*)(from_k + k);
-      vreg[j] = *(const u4*)(from_v + v);
-      kbyte[j] = (a.k_scale + at * kScales)[scale];
-      vbyte[j] = (a.v_scale + at * kScales)[scale];
+      kreg[j] = *(const u4*)(k + at + at_k);
+      vreg[j] = *(const u4*)(v + at + at_v);
+      const uint64_t scale = (uint64_t)page * scale_bytes + row * (unsigned)kScales;
+      kbyte[j] = (k_scale + scale)[at_scale];
+      vbyte[j] = (v_scale + scale)[at_scale];
     } else {
       to += (j * 256 + 64 * wave()) * 16;
-      into_lds(from_k, k, to + offsetof(Shared, k));
-      into_lds(from_v, v, to + offsetof(Shared, v));
+      into_lds(k + at, at_k, to + offsetof(Shared, k));
+      into_lds(v + at, at_v, to + offsetof(Shared, v));
     }
   }
 
-  // Starts the loads of 64 keys from `key` on; keys at and beyond `end` repeat the last one's address
+  // Starts the loads of the keys from `key` on; keys at and beyond `end` repeat the last one's address
   __device__ __forceinline__ void load(unsigned to, int key) {
-    if (kLarge && key + kManyKeys <= end) {
-      const int64_t at = row_of((unsigned)page[0] < (unsigned)a.npage ? page[0] : 0, key);
+    if (kLarge && key + kKeys <= end) {
 #pragma unroll
       for (int j = 0; j < kLoads; j++)
-        if (kWhole || key_of(j) < kManyKeys) bring(to, j, at, from_k[j], from_v[j], key_of(j) * kScales + piece_of(j) / 2);
+        if (kWhole || key_of(j) < kKeys)
+          bring(to, j, page[0], key, from_k[j], from_v[j], key_of(j) * kScales + piece_of(j) / 2);
       return;
     }
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
-      if (!kWhole && key_of(j) >= kManyKeys) continue;
-      if constexpr (kLarge) {
-        const int64_t at = row_of((unsigned)page[0] < (unsigned)a.npage ? page[0] : 0, key);
-        // rows beyond the last: that one's piece instead
-        const int row = min(key_of(j), end - 1 - key);
-        const unsigned back = (key_of(j) - row) * kRowBytes;
-        bring(to, j, at, from_k[j] - back, from_v[j] - back, row * kScales + piece_of(j) / 2);
-      } else {
+      if (!kWhole && key_of(j) >= kKeys) continue;
+      // rows beyond the last: that one's piece instead
+      int in = page[0], first = key, row = min(key_of(j), end - 1 - key);
+      if constexpr (!kLarge) {
         // the group of 16 keys: the wave's, or where a wave's pieces straddle two, the lane's
         const int group = kOneGroup ? (j * 256 + 64 * wave()) / (16 * kChunks) : key_of(j) / 16;
-        const int first = first_of(key, group);
-        int in = page[0];
 #pragma unroll
         for (int g = 1; g < kPages; g++) in = group == g ? page[g] : in;
         if constexpr (kOneGroup) in = __builtin_amdgcn_readfirstlane(in);
-        const int64_t at = row_of((unsigned)in < (unsigned)a.npage ? in : 0, first);
-        const int row = min(key_of(j) % 16, end - 1 - first);
-        const unsigned back = (key_of(j) - row) * kRowBytes;
-        bring(to, j, at, from_k[j] - back, from_v[j] - back, row * kScales + piece_of(j) / 2);
+        first = first_of(key, group);
+        row = min(key_of(j) % 16, end - 1 - first);
       }
+      const unsigned back = (key_of(j) - row) * kRowBytes;
+      bring(to, j, in, first, from_k[j] - back, from_v[j] - back, row * kScales + piece_of(j) / 2);
     }
   }
 
@@ -153,7 +153,7 @@ struct Stage {
       unsigned wild = 0;
 #pragma unroll
       for (int j = 0; j < kLoads; j++) {
-        if (!kWhole && key_of(j) >= kManyKeys) continue;
+        if (!kWhole && key_of(j) >= kKeys) continue;
         const int row = key_of(j);
         const bool none = careful && (key + row >= end || !(there >> (row / 16) & 1));
 #pragma unroll
@@ -177,7 +177,7 @@ struct Stage {
     unsigned wild = 0;
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
-      if (!kWhole && key_of(j) >= kManyKeys) continue;
+      if (!kWhole && key_of(j) >= kKeys) continue;
       const int row = key_of(j);
       u4* at = (u4*)&to.v[(j * 256 + threadIdx.x) * 8];
       u4 v = *at;
@@ -206,15 +206,17 @@ struct Stage {
   // (o in the layout of 32x32 products).
   __device__ __forceinline__ void repair(int key, int stop, int low_r, int high_r, f16v (&o)[D / 32]) const {
     const int half = (threadIdx.x & 63) >> 5;
-    for (int k = key; k < min(stop, end); k++) {
-      const int in = table[k >> a.page_shift];
-      if ((unsigned)in >= (unsigned)a.npage || !(k >= low_r && k < high_r)) continue;
-      const int64_t at = row_of(in, k);
+    for (int j = key; j < min(stop, end); j++) {
+      const int in = table[j >> page_shift];
+      if ((unsigned)in >= (unsigned)npage || !(j >= low_r && j < high_r)) continue;
+      const int row = j & ((1 << page_shift) - 1);
+      const uint8_t *from = v + (uint64_t)in * page_bytes + row * (unsigned)kRowBytes;
+      const uint8_t* scale = v_scale + (uint64_t)in * scale_bytes + row * (unsigned)kScales;
 #pragma unroll
       for (int c = 0; c < D / 32; c++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float value = value_at<E, kFp8, D>(a, at, 32 * c + 8 * (i / 4) + 4 * half + i % 4);
+          const float value = value_at<E, kFp8>(from, scale, 32 * c + 8 * (i / 4) + 4 * half + i % 4);
           if (!(fabsf(value) < INFINITY)) o[c][i] += value;
         }
     }

@@ -119,14 +119,10 @@ template <class E> __device__ inline typename E::V8 load_query(const Attend& a, 
   return a.negate ? -x : x;
 }
 
-// One value of V: of the key at element `at` / D of its pages
-template <class E, bool kFp8, int D> __device__ inline float value_at(const Attend& a, int64_t at, int d) {
-  if constexpr (kFp8) {
-    const unsigned byte = a.v_scale[at * (D / 32) + d / 32];
-    return (float)E::template from_fp8<false>(a.v[at * D + d], scale_of(byte))[0];
-  } else {
-    return (float)((const typename E::T*)a.v)[at * D + d];
-  }
+// One value of V, of the row at `row` with its scales at `scale`
+template <class E, bool kFp8> __device__ inline float value_at(const uint8_t* row, const uint8_t* scale, int d) {
+  if constexpr (kFp8) return (float)E::template from_fp8<false>(row[d], scale_of(scale[d / MX_SCALE_BLOCK]))[0];
+  else return (float)((const typename E::T*)row)[d];
 }
 
 // The world of a tile.  Ragged chunks: world w has the tile numbers from start[w] group / rows + w on,
