@@ -1,5 +1,5 @@
 // The episode memory's entry points: writing to and reading from the pages, joining the parts of a
-// split attention, and the host side of all four calls.
+// split attention, and the host side of all calls.  The attention itself: mx_episode_few.h, mx_episode_many.h.
 #include <cmath>
 #include <type_traits>
 #include "mx_episode_types.h"
@@ -289,7 +289,7 @@ int pages_check(const MxPages* p) {
   const int d = p->head_dim, t = p->page_tokens;
   if (d != 32 && d != 64 && d != 96 && d != 128 && d != 256) return MX_ERR_DOMAIN;
   if (t < 16 || t > 4096 || (t & (t - 1)) || p->kv_heads > 1024) return MX_ERR_DOMAIN;
-  if ((int64_t)p->npage * t > INT32_MAX || (int64_t)p->width * t > INT32_MAX) return MX_ERR_DOMAIN;
+  if ((int64_t)p->npage * t > INT32_MAX || (int64_t)p->width * t > 1 << 30) return MX_ERR_DOMAIN;
   if (((uintptr_t)p->k | (uintptr_t)p->v) & 15) return MX_ERR_INVALID;
   return 0;
 }
@@ -392,17 +392,21 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   return choose(a, launch);
 }
 
-// Which kernel, how many tiles, and into how many parts each tile's keys are split: where the tiles leave
-// room, as many as the card holds workgroups at once (two per CU, four where heads of up to 64 values leave
-// the registers), unless one workgroup is done with its keys in about the time that a second launch to
-// join the parts takes.  Two worlds of up to 131072 quantised tokens, 8
-// key heads of 128 values: 256 workgroups 77.9 us, 512 54.0, 1024 55.5, 2048 63.1; heads of 64: 512 35.4,
-// 1024 30.7, 2048 33.1.
+// Which kernel, by the rows that share a key head's keys and values.  us for 300 worlds of up to 700 tokens, 4 key
+// heads of 128 values, with 12, 24, 48 rows: attend_few of 16 rows 53, 76, 102 in bfloat16 and 33, 50, 69 with 8-bit
+// pages, of 32 rows 66, 68, 104 and 45, 48, 82, attend_many 61, 63, 69 and 63, 64, 72.  (Heads of 256 values: the
+// registers of attend_many do not hold them.)
+//
+// Into how many parts each tile's keys are split: where the tiles leave room, as many as the card holds
+// workgroups at once (two per CU, four where heads of up to 64 values leave the registers), unless one
+// workgroup is done with its keys in about the time that a second launch to join the parts takes.  Two
+// worlds of up to 131072 quantised tokens, 8 key heads of 128 values: 256 workgroups 77.9 us, 512 54.0, 1024
+// 55.5, 2048 63.1; heads of 64: 512 35.4, 1024 30.7, 2048 33.1.
 int choose(Attend& a, Launch& launch) {
   const int64_t rows = (int64_t)a.max_count * a.group;
+  const bool few = launch.head_dim > 128 || rows <= (launch.fp8 ? 32 : 16);
   launch.blocks = rows <= 16 ? 1 : 2;
-  launch.rows = 16 * launch.blocks;
-  if (rows > 32 && launch.head_dim <= 128) launch.rows = kManyRows;
+  launch.rows = few ? 16 * launch.blocks : kManyRows;
   const int64_t tiles = a.start ? (int64_t)a.tokens * a.group / launch.rows + a.nworld
                                 : ((rows + launch.rows - 1) / launch.rows) * a.nworld;
   int64_t keys = (int64_t)a.width << a.page_shift;
@@ -412,7 +416,7 @@ int choose(Attend& a, Launch& launch) {
   }
   const int64_t groups = tiles * a.kv_heads;
   const int room = launch.head_dim <= 64 ? 1024 : 512;
-  int64_t splits = keys * launch.head_dim <= 131072 ? 1 : (room + groups - 1) / groups;
+  int64_t splits = keys * (launch.head_dim > 64 ? launch.head_dim : 64) <= 131072 ? 1 : (room + groups - 1) / groups;
   const int64_t most = (keys + 63) / kLeastKeys + 1;     // the first key goes down to a multiple of 64
   splits = splits < most ? splits : most;
   if (splits > kMostSplits) splits = kMostSplits;

@@ -17,7 +17,7 @@ int attend_typed(const Attend& a, const Launch& launch, void* stream) {
       return (int)hipGetLastError();
     }
   if (launch.blocks == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2>), grid, block, 0, s, a);
+  else if constexpr (kFp8 || D > 128) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2>), grid, block, 0, s, a);
   return (int)hipGetLastError();
 }
 

@@ -16,10 +16,8 @@
 namespace mxe {
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
-typedef _Float16 hf4 __attribute__((ext_vector_type(4)));
 typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
@@ -192,7 +190,7 @@ __device__ inline void split_range(const Attend& a, int split, int low, int high
 __device__ inline void limits(const Attend& a, const Tile& t, int i, int& low, int& high) {
   const int position = t.position + i;
   high = position < 0 ? 0 : a.causal ? min(position + 1, t.length) : t.length;
-  low = a.window > 0 ? max(0, position - a.window + 1) : 0;
+  low = a.window > 0 && position >= a.window ? position - a.window + 1 : 0;
 }
 
 }  // namespace mxe

@@ -105,7 +105,7 @@ class Pages:
                 and shape[3] in HEAD_DIMS and shape[2] in _PAGE_TOKENS and shape[0] > 0 and 0 < shape[1] <= 1024
                 and tables[0] > 0 and tables[1] > 0 and length.shape == tables[:1]
                 and table.dtype == torch.int32 and length.dtype == torch.int32
-                and shape[0] * shape[2] < 2 ** 31 and tables[1] * shape[2] < 2 ** 31
+                and shape[0] * shape[2] < 2 ** 31 and tables[1] * shape[2] <= 2 ** 30
                 and v.get_device() == index and table.get_device() == index and length.get_device() == index
                 and k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and length.is_contiguous()
                 and (k_scale is None and v_scale is None) == (kind != 3)):
@@ -141,8 +141,8 @@ def _refuse_pages(k, v, table, length, k_scale, v_scale):
              'table must be contiguous int32 of shape (nworld, pages of a world)')
     _require(length.dtype == torch.int32 and length.shape == table.shape[:1] and length.is_contiguous(),
              'length must be contiguous int32 of shape (nworld,)')
-    _require(npage * tokens < 2 ** 31 and table.shape[1] * tokens < 2 ** 31,
-             'npage * page_tokens and the tokens of a table row must be below 2^31')
+    _require(npage * tokens < 2 ** 31 and table.shape[1] * tokens <= 2 ** 30,
+             'npage * page_tokens must be below 2^31 and the tokens of a table row at most 2^30')
     _require(k.is_contiguous() and v.is_contiguous(), 'pages must be contiguous')
     _require((k_scale is None) == (v_scale is None) == (k.dtype != torch.float8_e4m3fn),
              '8-bit pages have scales for k and v, others have none')

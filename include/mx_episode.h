@@ -42,7 +42,7 @@ extern "C" {
 /* Pages of keys and values: k, v [npage][kv_heads][page_tokens][head_dim], 16-byte aligned; scales (FP8,
  * otherwise null) [npage][kv_heads][page_tokens][head_dim / 32].  Token t of world w is slot
  * t % page_tokens of page table[w * width + t / page_tokens].  page_tokens: a power of two from 16 to
- * 4096; head_dim: 32, 64, 96, 128 or 256; npage * page_tokens and width * page_tokens below 2^31. */
+ * 4096; head_dim: 32, 64, 96, 128 or 256; npage * page_tokens below 2^31, width * page_tokens at most 2^30. */
 typedef struct MxPages {
   void *k, *v;
   uint8_t *k_scale, *v_scale;

@@ -58,7 +58,7 @@ class Call:
     ('nworld', 0, INVALID), ('npage', 0, INVALID), ('width', 0, INVALID), ('kv_heads', 0, INVALID),
     ('type', 0, INVALID), ('type', 3, INVALID), ('type', 9, INVALID), ('head_dim', 48, DOMAIN), ('head_dim', 512, DOMAIN),
     ('page_tokens', 8, DOMAIN), ('page_tokens', 48, DOMAIN), ('page_tokens', 8192, DOMAIN), ('npage', 2 ** 26, DOMAIN),
-    ('width', 2 ** 26, DOMAIN), ('kv_heads', 2000, DOMAIN)])
+    ('width', 2 ** 24 + 1, DOMAIN), ('kv_heads', 2000, DOMAIN)])
 def test_pages_are_checked(field, value, code):
     for entry in ('write', 'read', 'attend'):
         c = Call()

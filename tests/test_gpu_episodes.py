@@ -100,7 +100,7 @@ def compare(out, lse, want, kind):
     assert np.array_equal(np.isnan(ref), np.isnan(out)), 'NaN in other places'
     assert np.array_equal(ref[~fine & ~np.isnan(ref)], out[~fine & ~np.isnan(ref)])
     u = UNIT[kind]
-    error = np.abs(out - ref)[fine]
+    error = np.abs(out[fine] - ref[fine])
     bound = (u * np.abs(ref) + (u + 2.0 ** -12) * size)[fine] + 2.0 ** -24
     assert np.all(error <= bound), (error / bound).max()
     assert np.linalg.norm(error) <= (math.sqrt(2 / 3) * u + 2.0 ** -12) * np.linalg.norm(size[fine]) + 1e-30
@@ -190,6 +190,8 @@ def test_rows_without_keys(gpu_available):
     for causal in (True, False):
         check(world, [1, 1, 1, 1], 2, 'bf16', causal=causal, uniform=True)
         check(world, [2, 0, 9, 70], 2, 'bf16', causal=causal)          # positions -6.. and -30..
+        check(world, [2, 0, 9, 70], 2, 'bf16', causal=causal, window=2 ** 31 - 1)
+        check(world, [2, 0, 9, 70], 2, 'bf16', causal=causal, window=20)
     q = torch.ones((0, 2, 64), dtype=torch.bfloat16, device='cuda')
     assert episodes.attend(world.pages, q, torch.zeros(5, dtype=torch.int32, device='cuda')).shape == (0, 2, 64)
 
@@ -289,16 +291,18 @@ def test_other_stream_and_same_bits(gpu_available):
         compare(a, None, expected(world, q.cpu(), start), 'bf16')
 
 
-def test_captured_calls_follow_the_lengths(gpu_available):
-    """write and attend in a HIP graph: replays with other lengths and rows give what eager calls give."""
+@pytest.mark.parametrize('width,count', [(64, 1), (256, 1), (64, 30), (512, 30)])
+def test_captured_calls_follow_the_lengths(gpu_available, width, count):
+    """write and attend in a HIP graph, with the keys split (long tables) and not: replays with other lengths and
+    rows give what eager calls give."""
     import torch
-    print('case graph', flush=True)
-    world = World([600, 40, 1000], 2, 64, 16, 'bf16', seed=13, width=64)
+    print('case graph', width, count, flush=True)
+    world = World([600, 80, 1000], 2, 64, 16, 'bf16', seed=13, width=width)
     p = world.pages
     final = p.length.clone()
-    q = torch.randn((3, 1, 4, 64), device='cuda').bfloat16()
-    k, v = (torch.randn((3, 1, 2, 64), device='cuda').bfloat16() for _ in range(2))
-    out, lse = torch.empty_like(q), torch.empty((3, 1, 4), device='cuda')
+    q = torch.randn((3, count, 4, 64), device='cuda').bfloat16()
+    k, v = (torch.randn((3, count, 2, 64), device='cuda').bfloat16() for _ in range(2))
+    out, lse = torch.empty_like(q), torch.empty((3, count, 4), device='cuda')
     episodes.write(p, k, v)
     episodes.attend(p, q, out=out, lse=lse)
     torch.cuda.synchronize()
@@ -313,7 +317,7 @@ def test_captured_calls_follow_the_lengths(gpu_available):
         graph.replay()
         torch.cuda.synchronize()
         got, got_lse = out.clone(), lse.clone()
-        x, y = episodes.read(p, count=1)
+        x, y = episodes.read(p, count=count)
         assert torch.equal(x, k) and torch.equal(y, v)
         assert torch.equal(got, episodes.attend(p, q)) and bool(torch.isfinite(got_lse).all())
 
