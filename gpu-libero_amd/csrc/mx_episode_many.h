@@ -6,13 +6,25 @@
 //
 // The running maximum follows the scores only when one passes it by more than 2^8: until then the sums
 // are exact multiples of what they would be, and the output need not be rescaled.
+//
+// Two buffers: the next keys and values are on their way while these are weighed, one barrier a step.  Two
+// waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us), of
+// two workgroups, so that one's products run beside the other's softmax.
+// A prompt of 4 x 4096 tokens, 32 heads on 8 of 128 values, bfloat16: 597 us, 920 TFLOP/s, matrix
+// instructions 41 % and VALU 51 % busy; in copies of the kernel without the softmax's VALU work 533, without the loads
+// 530, without reading keys and values from LDS 495, with the matrix instructions alone 340: no one of them bounds it.
+// Tried and not kept: 64 rows to a wave (the compiler moves the outputs between the two halves of the register
+// file at every branch, 1100 us), 32 keys a step (700), eight waves to a workgroup (612), a wave's priority raised
+// around its products (591 to 615), reads of keys grouped ahead of the products (-1 %).
+// 16 worlds' 512 tokens over a window of 2000 in 8-bit pages, 16 heads on 2 of 64 values: 95 us, 640 TFLOP/s; a
+// head of 64 values has half the products to each power of two, and the VALU is 61 % busy.
 #pragma once
 #include "mx_episode_launch.h"
 #include "mx_episode_stage.h"
 
 namespace mxe {
 
-constexpr int many_keys(int D) { return 64; }
+constexpr int kManyKeys = 64;
 constexpr int many_waves(int D) { return D <= 32 ? 4 : D <= 96 ? 3 : 2; }
 
 template <int kType, bool kFp8, bool kLarge, int D>
@@ -21,7 +33,7 @@ __global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) 
   typedef Elem<kType> E;
   typedef typename E::T T;
   typedef typename E::V8 V8;
-  constexpr int kKeys = many_keys(D), kC = D / 16, kTiles = D / 32, kU = kKeys / 32;
+  constexpr int kKeys = kManyKeys, kC = D / 16, kTiles = D / 32, kU = kKeys / 32;
   typedef Staged<E, kKeys, D> Shared;
   typedef Stage<E, kFp8, kLarge, kKeys, D> Bring;
   constexpr unsigned kAll = Bring::kAll;

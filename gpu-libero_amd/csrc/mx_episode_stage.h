@@ -1,4 +1,4 @@
-// Bringing kKeys (32 or 64) keys and their values at a time into LDS, for workgroups of 256 threads.
+// Bringing kKeys keys and their values at a time into LDS, for workgroups of 256 threads.
 //
 // 16-bit pages go from memory to LDS without passing registers (each wave 1 KB at a time, lane after lane), so
 // the rows in LDS are as long as in the pages; what keeps the reads off each other's banks is the order of a row's
