@@ -16,8 +16,7 @@ for every world, or packed rows ``(tokens, heads, head_dim)`` with ``start`` (in
 w has the rows ``start[w]:start[w + 1]``.
 
 :class:`Pages` holds the tensors of one layer; :class:`EpisodeCache` keeps the pages of several layers, the
-worlds' tables and lengths, and hands out pages.  The reference has no counterpart: its policies
-(``libero/lifelong/``) recompute their history at every step.
+worlds' tables and lengths, and hands out pages.  The reference has no counterpart.
 """
 from __future__ import annotations
 
