@@ -1,9 +1,10 @@
 // Attention of few rows: the four waves of a workgroup each take 32 keys at a time of one world's key
 // head, for up to 16 * kBlocks rows (new tokens times the query heads that share the key head).
 //
-// One pass over the keys with a running maximum m, sum l and output O per row (in 32 bits):
+// One pass over the keys with a reference m, sum l and output O per row (in 32 bits):
 //   S^T = K Q^T (scores of 32 keys in two products' results, a row of the chunk per lane column),
-//   m' = max(m, S), p = 2^(S - m'), l' = l 2^(m - m') + sum p, O^T = O^T 2^(m - m') + V^T P^T.
+//   p = 2^(S - m), l = l + sum p, O^T = O^T + V^T P^T,
+// where m is the maximum of an early step, and moves (l and O with it) when a later one passes it too far.
 // With the scores transposed, a lane holds eight keys of its own row, which is the operand that the
 // second product wants if its keys are numbered 4 q + (0..3), 16 + 4 q + (0..3) for lane quarter q; V's
 // columns come in that order out of LDS by transposing reads, so probabilities never cross lanes.
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
   float m[kBlocks], l[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {
-    m[b] = -INFINITY;
+    m[b] = t.row + 16 * b + n16 < t.rows ? -INFINITY : 0.f;
     l[b] = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 16; c++) o[b][c] = f4{0.f, 0.f, 0.f, 0.f};
@@ -223,38 +224,43 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
     V8 p_high[kBlocks], p_low[kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; b++) {
-      float x[8], top = -INFINITY;
+      if (edge) {
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float y = s[b][u][i] * a.scale2;
-          if (edge) {
+          for (int i = 0; i < 4; i++) {
             const int at = now + 16 * u + 4 * quarter + i;
-            if (!(at >= low_r[b] && at < high_r[b] && at < end && (u ? is1 : is0))) y = -INFINITY;
+            if (!(at >= low_r[b] && at < high_r[b] && at < end && (u ? is1 : is0))) s[b][u][i] = -INFINITY;
           }
-          x[4 * u + i] = y;
-          top = fmaxf(top, y);
-        }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float next = fmaxf(m[b], top), zero = next == -INFINITY ? 0.f : next;
-      const float shrink = __builtin_amdgcn_exp2f(m[b] - zero);
-      m[b] = next;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float p = __builtin_amdgcn_exp2f(x[j] - zero);
-        sum += p;
-        const T h = (T)p;
-        p_high[b][j] = h;
-        p_low[b][j] = (T)(p - (float)h);
       }
-      l[b] = l[b] * shrink + sum;
-      if (__ballot(shrink != 1.f)) {
+      float sum;
+      const auto weigh = [&](float reference) __attribute__((always_inline)) {
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j / 4][j % 4], a.scale2, -reference));
+          sum += p;
+          const T h = (T)p;
+          p_high[b][j] = h;
+          p_low[b][j] = (T)(p - (float)h);
+        }
+      };
+      weigh(m[b]);
+      if (__ballot(!(sum <= kReferenceHolds))) {      // a new reference: see attend_many
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, s[b][j / 4][j % 4]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float before = m[b];
+        m[b] = fmaxf(m[b], top * a.scale2);
+        const float next = m[b] == -INFINITY ? 0.f : m[b], shrink = __builtin_amdgcn_exp2f(before - next);
+        l[b] *= shrink;
 #pragma unroll
         for (int c = 0; c < D / 16; c++) o[b][c] *= shrink;
+        weigh(next);
       }
+      l[b] += sum;
     }
 #pragma unroll
     for (int c = 0; c < D / 16; c++) {

@@ -4,8 +4,10 @@
 // that probabilities stay in their lanes), with 32x32 products and one 16-bit part of each probability:
 // here the matrix instructions are what bounds the kernel, and its error is that of the result's own rounding.
 //
-// The running maximum follows the scores only when one passes it by more than 2^8: until then the sums
-// are exact multiples of what they would be, and the output need not be rescaled.
+// The maximum is not looked for: the first step's stays the reference that powers of two are taken against,
+// until a lane's sum of a step passes 2^12 (or is no number); then the step's maximum is found, the outputs are rescaled
+// and the step is weighed again.  In 32 bits, and in bfloat16, weights up to 2^12 are as exact as those up to 1, and
+// float16 holds them; the sums that they are divided by have the same reference.
 //
 // Two buffers: the next keys and values are on their way while these are weighed, one barrier a step.  Two
 // waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us), of
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) 
   for (int c = 0; c < kTiles; c++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[c][i] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m = row_here ? -INFINITY : 0.f, l = 0.f;       // (a row that is not there never asks for a new reference)
 
   const float scale2 = a.scale2;
   Bring stage(a, t.world, head, end);
@@ -136,30 +138,34 @@ __global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) 
             if (!((present >> (2 * u + i / 8) & 1) && at >= low_r && at < high_r && at < end)) s[u][i] = -INFINITY;
           }
       }
-      float top = -INFINITY;
+      V8 p[kU][2];
+      float sum[2];
+      const auto weigh = [&](float reference) __attribute__((always_inline)) {
+        sum[0] = sum[1] = 0.f;
 #pragma unroll
-      for (int u = 0; u < kU; u++)
+        for (int u = 0; u < kU; u++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
-      top = both_halves_max(top) * scale2;
-      if (__ballot(top > m + 8.f)) {
-        const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
-        m = next;
+          for (int i = 0; i < 16; i++) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale2, -reference));
+            sum[i & 1] += x;
+            p[u][i / 8][i % 8] = (T)x;
+          }
+      };
+      weigh(m);
+      if (__ballot(!(sum[0] + sum[1] <= kReferenceHolds))) {
+        const float before = m;
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kU; u++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
+        m = fmaxf(m, both_halves_max(top) * scale2);
+        const float next = m == -INFINITY ? 0.f : m, shrink = __builtin_amdgcn_exp2f(before - next);
         l *= shrink;
 #pragma unroll
         for (int c = 0; c < kTiles; c++) o[c] *= shrink;
+        weigh(next);
       }
-      const float zero = m == -INFINITY ? 0.f : m;
-      V8 p[kU][2];
-      float sum[2] = {0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < kU; u++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale2, -zero));
-          sum[i & 1] += x;
-          p[u][i / 8][i % 8] = (T)x;
-        }
       l += sum[0] + sum[1];
 #pragma unroll
       for (int u = 0; u < kU; u++)
