@@ -3,8 +3,11 @@
 //
 // One pass over the keys with a reference m, sum l and output O per row (in 32 bits):
 //   S^T = K Q^T (scores of 32 keys in two products' results, a row of the chunk per lane column),
-//   p = 2^(S - m), l = l + sum p, O^T = O^T + V^T P^T,
-// where m is the maximum of an early step, and moves (l and O with it) when a later one passes it too far.
+//   p = 2^(S - m), l = l + sum p, O^T = O^T + V^T P^T.
+// The maximum is not looked for: the first step's stays the reference m until a lane's sum of a step passes 2^12
+// (or is no number); then the step's maximum is found, l and O are rescaled and the step is weighed again.  In 32
+// bits, and in bfloat16, weights up to 2^12 are as exact as those up to 1, and float16 holds them (210 -> 205 us for
+// the 4096 worlds below; attend_many, whose products run beside the powers of two, lost 3 % by it).
 // With the scores transposed, a lane holds eight keys of its own row, which is the operand that the
 // second product wants if its keys are numbered 4 q + (0..3), 16 + 4 q + (0..3) for lane quarter q; V's
 // columns come in that order out of LDS by transposing reads, so probabilities never cross lanes.
@@ -16,9 +19,9 @@
 // LDS of its own without a barrier, and the waves' results are joined once.  What counts is how many
 // waves a SIMD holds: keeping the values' words for the rare repair below took 130 registers and three
 // waves at 64 values a head, reading them again 120 and four (249 -> 216 us for 4096 worlds of up to
-// 1024 quantised tokens).  Single tokens, alternating inputs: those worlds (4 key heads of 64, 1.13 GB) 210 us, 5.4 TB/s, its
+// 1024 quantised tokens).  Single tokens, alternating inputs: those worlds (4 key heads of 64, 1.13 GB) 205 us, 5.5 TB/s, its
 // VALU 61 % busy with conversions and softmax; 500 worlds of up to 2048 tokens in bfloat16 (8 key heads of 128, 2.1 GB) 364 us, 5.8 TB/s;
-// two worlds, 131072 quantised tokens in all (277 MB), 50 us and 5 to join the parts.
+// two worlds, 131072 quantised tokens in all (277 MB), 49 us and 5 to join the parts.
 #pragma once
 #include "mx_episode_types.h"
 
@@ -246,7 +249,7 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
         }
       };
       weigh(m[b]);
-      if (__ballot(!(sum <= kReferenceHolds))) {      // a new reference: see attend_many
+      if (__ballot(!(sum <= kReferenceHolds))) {      // a new reference
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; j++) top = fmaxf(top, s[b][j / 4][j % 4]);

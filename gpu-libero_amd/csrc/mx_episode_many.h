@@ -4,10 +4,8 @@
 // that probabilities stay in their lanes), with 32x32 products and one 16-bit part of each probability:
 // here the matrix instructions are what bounds the kernel, and its error is that of the result's own rounding.
 //
-// The maximum is not looked for: the first step's stays the reference that powers of two are taken against,
-// until a lane's sum of a step passes 2^12 (or is no number); then the step's maximum is found, the outputs are rescaled
-// and the step is weighed again.  In 32 bits, and in bfloat16, weights up to 2^12 are as exact as those up to 1, and
-// float16 holds them; the sums that they are divided by have the same reference.
+// The running maximum follows the scores only when one passes it by more than 2^8: until then the sums
+// are exact multiples of what they would be, and the output need not be rescaled.
 //
 // Two buffers: the next keys and values are on their way while these are weighed, one barrier a step.  Two
 // waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us), of
@@ -17,7 +15,8 @@
 // 530, without reading keys and values from LDS 495, with the matrix instructions alone 340: no one of them bounds it.
 // Tried and not kept: 64 rows to a wave (the compiler moves the outputs between the two halves of the register
 // file at every branch, 1100 us), 32 keys a step (700), eight waves to a workgroup (612), a wave's priority raised
-// around its products (591 to 615), reads of keys grouped ahead of the products (-1 %).
+// around its products (591 to 615), reads of keys grouped ahead of the products (-1 %), the next step's scores
+// computed beside this one's softmax (650), the reference kept without a maximum (617).
 // 16 worlds' 512 tokens over a window of 2000 in 8-bit pages, 16 heads on 2 of 64 values: 95 us, 640 TFLOP/s; a
 // head of 64 values has half the products to each power of two, and the VALU is 61 % busy.
 #pragma once
@@ -80,7 +79,7 @@ __global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) 
   for (int c = 0; c < kTiles; c++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[c][i] = 0.f;
-  float m = row_here ? -INFINITY : 0.f, l = 0.f;       // (a row that is not there never asks for a new reference)
+  float m = -INFINITY, l = 0.f;
 
   const float scale2 = a.scale2;
   Bring stage(a, t.world, head, end);
@@ -138,34 +137,30 @@ __global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) 
             if (!((present >> (2 * u + i / 8) & 1) && at >= low_r && at < high_r && at < end)) s[u][i] = -INFINITY;
           }
       }
-      V8 p[kU][2];
-      float sum[2];
-      const auto weigh = [&](float reference) __attribute__((always_inline)) {
-        sum[0] = sum[1] = 0.f;
+      float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kU; u++)
+      for (int u = 0; u < kU; u++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale2, -reference));
-            sum[i & 1] += x;
-            p[u][i / 8][i % 8] = (T)x;
-          }
-      };
-      weigh(m);
-      if (__ballot(!(sum[0] + sum[1] <= kReferenceHolds))) {
-        const float before = m;
-        float top = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < kU; u++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
-        m = fmaxf(m, both_halves_max(top) * scale2);
-        const float next = m == -INFINITY ? 0.f : m, shrink = __builtin_amdgcn_exp2f(before - next);
+        for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
+      top = both_halves_max(top) * scale2;
+      if (__ballot(top > m + 8.f)) {
+        const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+        m = next;
         l *= shrink;
 #pragma unroll
         for (int c = 0; c < kTiles; c++) o[c] *= shrink;
-        weigh(next);
       }
+      const float zero = m == -INFINITY ? 0.f : m;
+      V8 p[kU][2];
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < kU; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale2, -zero));
+          sum[i & 1] += x;
+          p[u][i / 8][i % 8] = (T)x;
+        }
       l += sum[0] + sum[1];
 #pragma unroll
       for (int u = 0; u < kU; u++)

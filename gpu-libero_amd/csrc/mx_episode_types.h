@@ -176,7 +176,7 @@ __device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, T
 // keys, and no fewer than kLeastKeys (the last ones may have none).  By the world's own keys and not by
 // the most that the table can hold, so that long and short worlds both keep all splits at work.
 constexpr int kLeastKeys = 256;
-// A lane's sum of a step's weights up to which their reference is kept (see attend_many)
+// A lane's sum of a step's weights up to which attend_few keeps their reference
 constexpr float kReferenceHolds = 4096.f;
 __device__ inline void split_range(const Attend& a, int split, int low, int high, int& begin, int& end) {
   begin = low & ~63;
