@@ -375,7 +375,7 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   a.nworld = p->nworld; a.npage = p->npage; a.width = p->width; a.kv_heads = p->kv_heads;
   a.page_shift = page_shift(p); a.tokens = c->tokens; a.count = c->count;
   a.heads = heads; a.group = heads / p->kv_heads;
-  a.causal = m->causal != 0; a.window = m->window; 
+  a.causal = m->causal != 0; a.window = m->window;
   // a scale of 0 becomes one that no score is noticed under: a hidden key's -infinity has to stay
   a.scale2 = fmaxf(fabsf(m->scale) * kLog2e, 1e-37f);
   a.negate = m->scale < 0.f;

@@ -7,7 +7,7 @@
 // The maximum is not looked for: the first step's stays the reference m until a lane's sum of a step passes 2^12
 // (or is no number); then the step's maximum is found, l and O are rescaled and the step is weighed again.  In 32
 // bits, and in bfloat16, weights up to 2^12 are as exact as those up to 1, and float16 holds them (210 -> 205 us for
-// the 4096 worlds below; attend_many, whose products run beside the powers of two, lost 3 % by it).
+// the 4096 worlds below; attend_many, whose products run beside the powers of two, lost 2 % by it).
 // With the scores transposed, a lane holds eight keys of its own row, which is the operand that the
 // second product wants if its keys are numbered 4 q + (0..3), 16 + 4 q + (0..3) for lane quarter q; V's
 // columns come in that order out of LDS by transposing reads, so probabilities never cross lanes.
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
     // values into LDS, those of keys that do not exist as zeros
     const bool edge = key < all_low || key + 32 > all_high || key + 32 > end || !is0 || !is1;
     // an infinity or NaN among the values: added apart below, to the rows that see it (a remainder of a
-    // probability times an infinity is no remainder).  8-bit values have no infinity, and a NaN need not be
-    // kept from rows that all see it.
+    // probability times an infinity is no remainder).  8-bit values have no infinity in bfloat16, whose range is
+    // theirs (in float16 they do, beyond 65504), and a NaN need not be kept from rows that all see it.
     unsigned wild = 0;
 #pragma unroll
     for (int j = 0; j < kVLoads; j++) {
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
       for (int e = 0; e < kVPer / 8; e++) {
         u4 words = __builtin_bit_cast(u4, v[e]);
         if (edge && (key + key_in >= end || !(key_in < 16 ? is0 : is1))) words = u4{0, 0, 0, 0};
-        if (!kFp8 || edge) {
+        if (!kFp8 || kType == MX_TYPE_F16 || edge) {
           unsigned off = 0;
 #pragma unroll
           for (int y = 0; y < 4; y++) off |= not_finite<E>(words[y]);

@@ -243,6 +243,22 @@ def test_hidden_values_stay_hidden(gpu_available, count, bad):
     compare(torch.from_numpy(out[~seen]), None, (ref[~seen], None, size[~seen]), 'bf16')
 
 
+@pytest.mark.parametrize('count', [1, 40])
+@pytest.mark.parametrize('page', [16, 64])
+def test_quantised_values_beyond_float16(gpu_available, page, count):
+    """8-bit pages hold magnitudes that float16 does not: as float16 values they are infinities of their sign, and
+    so are the results of the queries that see them."""
+    print('case beyond float16', page, count, flush=True)
+    world = World([50, 300, 301], 1, 64, page, 'fp8', seed=18)
+    for w, token in ((0, 5), (1, 101), (2, 299)):
+        world.v[w][token, 0, :32] *= 2.0 ** 17
+        world.pages.v_scale[world.table[w, token // page], 0, token % page, 0] += 17
+    with np.errstate(over='ignore'):
+        world.v = [x.astype(np.float16).astype(np.float64) for x in world.v]
+    assert sum(np.isinf(x).sum() for x in world.v) > 30
+    check(world, [count] * 3, 2, 'f16')
+
+
 def test_scores_of_any_size(gpu_available):
     """Large scores of one sign, scale 0 and negative scale: the maximum is taken off first."""
     print('case scores', flush=True)
