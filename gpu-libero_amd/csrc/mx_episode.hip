@@ -327,7 +327,9 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
   // pieces of a token, and tokens of a workgroup
   const int size = size_of(k->type), pieces = p->kv_heads * p->head_dim * size / piece_bytes(p->type == MX_TYPE_FP8, kWrite, size);
   int each = 256 * pieces_ahead(size) / pieces;
-  each = each < 1 ? 1 : each > kMostTokens ? kMostTokens : each;
+  each = each < 1 ? 1 : each > kMostTokens || c->tokens / each >= kMostGroups ? kMostTokens : each;
+  const int64_t groups = (c->tokens + (int64_t)each - 1) / each;
+  if (groups > kMostGroups) return MX_ERR_DOMAIN;
   Move a{};
   uint8_t *pages[2] = {(uint8_t*)p->k, (uint8_t*)p->v}, *scales[2] = {p->k_scale, p->v_scale};
   for (int i = 0; i < 2; i++)
@@ -337,7 +339,7 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
   a.nworld = p->nworld; a.npage = p->npage; a.width = p->width; a.kv_heads = p->kv_heads;
   a.page_shift = page_shift(p); a.tokens = c->tokens; a.count = c->count;
   a.head_dim = p->head_dim; a.tokens_each = each;
-  const dim3 grid((unsigned)((c->tokens + (int64_t)each - 1) / each));
+  const dim3 grid((unsigned)groups);
   auto go = [&](auto t, auto store) {
     typedef decltype(t) T;
     constexpr int kStore = decltype(store)::value;
@@ -420,7 +422,7 @@ int choose(Attend& a, Launch& launch) {
   const int64_t most = (keys + 63) / kLeastKeys + 1;     // the first key goes down to a multiple of 64
   splits = splits < most ? splits : most;
   if (splits > kMostSplits) splits = kMostSplits;
-  if (groups * splits > INT32_MAX) return MX_ERR_DOMAIN;
+  if (groups * splits > kMostGroups) return MX_ERR_DOMAIN;
   a.tiles = (int)tiles;
   a.splits = (int)splits;
   launch.tiles = a.tiles;

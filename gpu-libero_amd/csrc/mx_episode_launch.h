@@ -7,6 +7,8 @@ namespace mxe {
 
 constexpr int kManyRows = 128;              // rows of a tile of attend_many
 
+constexpr int64_t kMostGroups = (1 << 24) - 1;   // workgroups of 256 of a launch: threads are counted in 32 bits
+
 struct Launch {
   int type, head_dim, blocks, rows, tiles;    // blocks of 16 rows to a tile
   bool fp8;

@@ -13,7 +13,8 @@
  * otherwise world w has the rows start[w] .. start[w + 1] of `tokens` rows (start[0] = 0,
  * start[nworld] = tokens, nondecreasing; rows outside `tokens` are never touched).  A chunk longer
  * than its world's length has only its last length[w] tokens; tokens beyond the table's reach, or
- * whose table entry names no page, are neither written nor seen, and read as zeros.
+ * whose table entry names no page, are neither written nor seen, and read as zeros.  Sizes that would take
+ * more than 2^24 - 1 workgroups of 256 threads (2^30 rows of one write) are MX_ERR_DOMAIN.
  */
 #ifndef MX_EPISODE_H
 #define MX_EPISODE_H

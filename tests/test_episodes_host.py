@@ -98,6 +98,20 @@ def test_rows_and_chunks_are_checked():
         assert getattr(c, entry)() == 0
 
 
+def test_more_workgroups_than_a_launch_holds():
+    """Threads of a launch are counted in 32 bits, so 2^24 - 1 workgroups of 256 are the most."""
+    c = Call()
+    c.pages.nworld, c.pages.kv_heads, c.pages.page_tokens, c.pages.width = 1 << 21, 8, 16, 1
+    rows = episodes.MxRows(c.at, 512, 64, 8, 1)
+    c.attention.q = c.attention.out = rows
+    c.chunk.tokens = c.pages.nworld
+    assert c.workspace() == 0 and c.attend() == DOMAIN
+    c = Call()                                            # 64 tokens to a workgroup are the most
+    c.pages.kv_heads = c.k.heads = c.v.heads = 1
+    c.chunk = episodes.MxChunk(c.at, 2 ** 31 - 1, 0)
+    assert c.write() == DOMAIN and c.read() == DOMAIN
+
+
 def test_workspace():
     """A long table and few rows are split along the keys, into a workspace that has to be there."""
     c = Call()

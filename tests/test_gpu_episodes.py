@@ -492,3 +492,18 @@ def test_refusals(gpu_available):
         with pytest.raises(ValueError):
             call()
             print('not refused:', i)
+
+
+def test_gradients_are_refused(gpu_available):
+    """There is no backward pass: a result that silently had no gradient would train nothing."""
+    import torch
+    print('case gradients', flush=True)
+    world = World([5, 20], 2, 64, 16, 'bf16', seed=19)
+    q = torch.randn((2, 1, 4, 64), device='cuda').bfloat16().requires_grad_()
+    kv = q[:, :, :2]
+    for call in (lambda: episodes.attend(world.pages, q), lambda: episodes.write(world.pages, kv, kv)):
+        with pytest.raises(ValueError, match='backward'):
+            call()
+    with torch.no_grad():
+        out = episodes.attend(world.pages, q)
+    assert not out.requires_grad and torch.equal(out, episodes.attend(world.pages, q.detach()))
