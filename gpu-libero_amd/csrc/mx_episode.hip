@@ -396,8 +396,9 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 
 // Which kernel, by the rows that share a key head's keys and values.  us for 300 worlds of up to 700 tokens, 4 key
 // heads of 128 values, with 12, 24, 48 rows: attend_few of 16 rows 53, 76, 102 in bfloat16 and 33, 50, 69 with 8-bit
-// pages, of 32 rows 66, 68, 104 and 45, 48, 82, attend_many 61, 63, 69 and 63, 64, 72.  (Heads of 256 values: the
-// registers of attend_many do not hold them.)
+// pages, of 32 rows 66, 68, 104 and 45, 48, 82, attend_many 61, 63, 69 and 63, 64, 72;
+// worlds of up to 512 tokens and heads of 256 values, with 12, 24, 48 rows: attend_few of 16 rows, then 32, 105, 162, 282
+// and 73, 134, 236, attend_many 154, 155, 162 and 224, 226, 239 (80 rows 173 and 251, attend_few 407 and 337).
 //
 // Into how many parts each tile's keys are split: where the tiles leave room, as many as the card holds
 // workgroups at once (two per CU, four where heads of up to 64 values leave the registers), unless one
@@ -406,7 +407,7 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 // 55.5, 2048 63.1; heads of 64: 512 35.4, 1024 30.7, 2048 33.1.
 int choose(Attend& a, Launch& launch) {
   const int64_t rows = (int64_t)a.max_count * a.group;
-  const bool few = launch.head_dim > 128 || rows <= (launch.fp8 ? 32 : 16);
+  const bool few = rows <= (launch.fp8 ? 32 : 16);
   launch.blocks = rows <= 16 ? 1 : 2;
   launch.rows = few ? 16 * launch.blocks : kManyRows;
   const int64_t tiles = a.start ? (int64_t)a.tokens * a.group / launch.rows + a.nworld

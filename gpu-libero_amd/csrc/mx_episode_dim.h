@@ -10,14 +10,13 @@ template <int D, int kType, bool kFp8>
 int attend_typed(const Attend& a, const Launch& launch, void* stream) {
   const dim3 grid(launch.grid), block(256);
   const hipStream_t s = (hipStream_t)stream;
-  if constexpr (D <= 128)
-    if (launch.rows == kManyRows) {
-      if (a.page_shift >= 6) hipLaunchKernelGGL((attend_many<kType, kFp8, true, D>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((attend_many<kType, kFp8, false, D>), grid, block, 0, s, a);
-      return (int)hipGetLastError();
-    }
+  if (launch.rows == kManyRows) {
+    if (a.page_shift >= 6) hipLaunchKernelGGL((attend_many<kType, kFp8, true, D>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attend_many<kType, kFp8, false, D>), grid, block, 0, s, a);
+    return (int)hipGetLastError();
+  }
   if (launch.blocks == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1>), grid, block, 0, s, a);
-  else if constexpr (kFp8 || D > 128) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2>), grid, block, 0, s, a);
+  else if constexpr (kFp8) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2>), grid, block, 0, s, a);
   return (int)hipGetLastError();
 }
 

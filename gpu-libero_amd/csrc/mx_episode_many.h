@@ -1,5 +1,5 @@
 // Attention of many rows: a workgroup takes 128 rows of one world's key head (new tokens times the query
-// heads that share the key head), each of its four waves 32 of them, and 64 keys at a time, which all four
+// heads that share the key head), each of its four waves 32 of them, and 64 keys at a time (32 of 256 values), which all four
 // read from LDS.  The mathematics is that of attend_few (one pass, running maximum, scores transposed so
 // that probabilities stay in their lanes), with 32x32 products and one 16-bit part of each probability:
 // here the matrix instructions are what bounds the kernel, and its error is that of the result's own rounding.
@@ -19,14 +19,18 @@
 // computed beside this one's softmax (650), the reference kept without a maximum (617).
 // 16 worlds' 512 tokens over a window of 2000 in 8-bit pages, 16 heads on 2 of 64 values: 95 us, 640 TFLOP/s; a
 // head of 64 values has half the products to each power of two, and the VALU is 61 % busy.
+// Heads of 256 values: the outputs and queries of 32 rows are 192 registers, so one wave per SIMD, whose
+// products nothing runs beside: 4 x 2048 tokens, 16 heads on 4, bfloat16: 295 us, 466 TFLOP/s (64 keys a step
+// 397, as many rows as attend_few takes at a time 915).
 #pragma once
 #include "mx_episode_launch.h"
 #include "mx_episode_stage.h"
 
 namespace mxe {
 
-constexpr int kManyKeys = 64;
-constexpr int many_waves(int D) { return D <= 32 ? 4 : D <= 96 ? 3 : 2; }
+// Keys of a step
+constexpr int many_keys(int D) { return D <= 128 ? 64 : 32; }
+constexpr int many_waves(int D) { return D <= 32 ? 4 : D <= 96 ? 3 : D <= 128 ? 2 : 1; }
 
 template <int kType, bool kFp8, bool kLarge, int D>
 __global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) {
@@ -34,7 +38,7 @@ __global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) 
   typedef Elem<kType> E;
   typedef typename E::T T;
   typedef typename E::V8 V8;
-  constexpr int kKeys = kManyKeys, kC = D / 16, kTiles = D / 32, kU = kKeys / 32;
+  constexpr int kKeys = many_keys(D), kC = D / 16, kTiles = D / 32, kU = kKeys / 32;
   typedef Staged<E, kKeys, D> Shared;
   typedef Stage<E, kFp8, kLarge, kKeys, D> Bring;
   constexpr unsigned kAll = Bring::kAll;

@@ -170,6 +170,17 @@ def test_uniform_chunks(gpu_available, count):
     check(world, [count] * 3, 3, 'bf16', window=65, uniform=True)
 
 
+@pytest.mark.parametrize('kind,store', [('f16', 'f16'), ('bf16', 'fp8')])
+@pytest.mark.parametrize('page,count', [(16, 17), (64, 33), (32, 70), (128, 140)])
+def test_chunks_of_wide_heads(gpu_available, page, count, kind, store):
+    """Heads of 256 values: pages on both sides of a step's keys, one part and several."""
+    print('case wide heads', page, count, kind, store, flush=True)
+    for width in (None, 2048 // page):
+        world = World([count, 700, count + 31], 2, 256, page, store, seed=20 + count, width=width)
+        check(world, [count] * 3, 4, kind, uniform=True)
+        check(world, [count, 1, count - 1], 4, kind, causal=False, window=100)
+
+
 @pytest.mark.parametrize('store', ['bf16', 'fp8'])
 @pytest.mark.parametrize('page', [16, 64, 1024])
 def test_long_keys_are_split(gpu_available, page, store):
