@@ -20,8 +20,8 @@
 // waves a SIMD holds: keeping the values' words for the rare repair below took 130 registers and three
 // waves at 64 values a head, reading them again 120 and four (249 -> 216 us for 4096 worlds of up to
 // 1024 quantised tokens).  Single tokens, alternating inputs: those worlds (4 key heads of 64, 1.13 GB) 205 us, 5.5 TB/s, its
-// VALU 61 % busy with conversions and softmax; 500 worlds of up to 2048 tokens in bfloat16 (8 key heads of 128, 2.1 GB) 364 us, 5.8 TB/s;
-// two worlds, 131072 quantised tokens in all (277 MB), 49 us and 5 to join the parts.
+// VALU 56 % busy with conversions and softmax; 500 worlds of up to 2048 tokens in bfloat16 (8 key heads of 128, 2.1 GB) 364 us, 5.8 TB/s;
+// two worlds, 131072 quantised tokens in all (277 MB), 47 us and 5 to join the parts.
 #pragma once
 #include "mx_episode_types.h"
 

@@ -14,9 +14,14 @@
 // instructions 41 % and VALU 51 % busy; in copies of the kernel without the softmax's VALU work 533, without the loads
 // 530, without reading keys and values from LDS 495, with the matrix instructions alone 340: no one of them bounds it.
 // Tried and not kept: 64 rows to a wave (the compiler moves the outputs between the two halves of the register
-// file at every branch, 1100 us), 32 keys a step (700), eight waves to a workgroup (612), a wave's priority raised
+// file at every branch, 1100 us; heads of 64 values hold them, and fewer workgroups run side by side: 8 x 4096 tokens 342 to 354,
+// 300 x 150 tokens 120 to 143, the window below 102 to 93), 32 keys a step (700), eight waves to a workgroup (612), a wave's priority raised
 // around its products (591 to 615), reads of keys grouped ahead of the products (-1 %), the next step's scores
 // computed beside this one's softmax (650), the reference kept without a maximum (617).
+// 300 ragged chunks of up to 41 tokens over up to 701, 12 heads on 4 of 96 values, float16 (161 MB): 57 us; the loads alone
+// 52, the rest alone 41, neither 22: what a workgroup waits for until its first keys are there, and that in two rounds of
+// workgroups (queries asked for after the first keys 55.6, but 59.3 instead of 58.5 in heads of 128; rows dealt to
+// other waves by block, the same).
 // 16 worlds' 512 tokens over a window of 2000 in 8-bit pages, 16 heads on 2 of 64 values: 95 us, 640 TFLOP/s; a
 // head of 64 values has half the products to each power of two, and the VALU is 61 % busy.
 // Heads of 256 values: the outputs and queries of 32 rows are 192 registers, so one wave per SIMD, whose
