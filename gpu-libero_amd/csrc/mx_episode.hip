@@ -362,7 +362,7 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   if (rc || (rc = chunk_check(p, c))) return rc;
   if (!m) return MX_ERR_INVALID;
   const int heads = m->q.heads;
-  if (heads < 1 || heads % p->kv_heads || m->max_count < 0 || m->window < 0) return MX_ERR_INVALID;
+  if (heads < 1 || heads % p->kv_heads || m->max_count < 0 || m->window < 0 || m->longest < 0) return MX_ERR_INVALID;
   if (heads / p->kv_heads > 1024) return MX_ERR_DOMAIN;
   if ((rc = rows_check(&m->q, heads, pointers && c->tokens > 0)) || (rc = rows_check(&m->out, heads, pointers && c->tokens > 0)))
     return rc;
@@ -391,6 +391,8 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   launch.type = m->q.type;
   launch.fp8 = p->type == MX_TYPE_FP8;
   launch.head_dim = p->head_dim;
+  launch.keys = (int64_t)p->width << a.page_shift;
+  if (m->longest && m->longest < launch.keys) launch.keys = m->longest;
   return choose(a, launch);
 }
 
@@ -405,6 +407,12 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 // workgroup is done with its keys in about the time that a second launch to join the parts takes.  Two
 // worlds of up to 131072 quantised tokens, 8 key heads of 128 values: 256 workgroups 77.9 us, 512 54.0, 1024
 // 55.5, 2048 63.1; heads of 64: 512 35.4, 1024 30.7, 2048 33.1.
+//
+// How many waves of attend_few share a tile: four, but one where there are waves' worth of tiles and their keys are few
+// (most of four waves would have none, and wait for each other).  us with four and one, up to 64, 256 and 400 keys:
+// 16384 tiles of 64 values, 8 bits, 66 and 27, 88 and 63, 109 and 94; 4096 tiles of 128 values, bfloat16, 43 and 20,
+// 70 and 60, 92 and 90; 2048 of those 23 and 12, 39 and 36, 50 and 53; 512 of them 10.8 and 10.9, 11.4 and 16.7, 15 and 23.
+constexpr int kShort = 256, kPlenty = 2048;
 int choose(Attend& a, Launch& launch) {
   const int64_t rows = (int64_t)a.max_count * a.group;
   const bool few = rows <= (launch.fp8 ? 32 : 16);
@@ -412,7 +420,7 @@ int choose(Attend& a, Launch& launch) {
   launch.rows = few ? 16 * launch.blocks : kManyRows;
   const int64_t tiles = a.start ? (int64_t)a.tokens * a.group / launch.rows + a.nworld
                                 : ((rows + launch.rows - 1) / launch.rows) * a.nworld;
-  int64_t keys = (int64_t)a.width << a.page_shift;
+  int64_t keys = launch.keys;
   if (a.window > 0 && a.causal) {
     const int64_t spanned = (int64_t)a.window + launch.rows / a.group + 1;
     keys = keys < spanned ? keys : spanned;
@@ -424,6 +432,7 @@ int choose(Attend& a, Launch& launch) {
   splits = splits < most ? splits : most;
   if (splits > kMostSplits) splits = kMostSplits;
   if (groups * splits > kMostGroups) return MX_ERR_DOMAIN;
+  launch.team = splits == 1 && keys <= kShort && groups >= kPlenty ? 1 : 4;
   a.tiles = (int)tiles;
   a.splits = (int)splits;
   launch.tiles = a.tiles;

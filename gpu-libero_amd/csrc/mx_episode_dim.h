@@ -15,8 +15,13 @@ int attend_typed(const Attend& a, const Launch& launch, void* stream) {
     else hipLaunchKernelGGL((attend_many<kType, kFp8, false, D>), grid, block, 0, s, a);
     return (int)hipGetLastError();
   }
-  if (launch.blocks == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1>), grid, block, 0, s, a);
-  else if constexpr (kFp8) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2>), grid, block, 0, s, a);
+  if (launch.blocks == 1) {
+    if (launch.team == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1, 1>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1, 4>), grid, block, 0, s, a);
+  } else if constexpr (kFp8) {
+    if (launch.team == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2, 1>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2, 4>), grid, block, 0, s, a);
+  }
   return (int)hipGetLastError();
 }
 

@@ -1,5 +1,6 @@
-// Attention of few rows: the four waves of a workgroup each take 32 keys at a time of one world's key
-// head, for up to 16 * kBlocks rows (new tokens times the query heads that share the key head).
+// Attention of few rows: the kTeam waves of a workgroup each take 32 keys at a time of one world's key
+// head, for up to 16 * kBlocks rows (new tokens times the query heads that share the key head).  kTeam is 4, or 1 for
+// many short histories, in which most of four waves would have no keys (see choose()).
 //
 // One pass over the keys with a reference m, sum l and output O per row (in 32 bits):
 //   S^T = K Q^T (scores of 32 keys in two products' results, a row of the chunk per lane column),
@@ -30,8 +31,8 @@ namespace mxe {
 // Waves of a SIMD to leave registers for
 constexpr int few_waves(int D, int blocks) { return blocks == 1 && D <= 64 ? 4 : blocks <= 2 && D <= 128 ? 2 : 1; }
 
-template <int kType, bool kFp8, int D, int kBlocks>
-__global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const Attend a) {
+template <int kType, bool kFp8, int D, int kBlocks, int kTeam>
+__global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(const Attend a) {
   typedef Elem<kType> E;
   typedef typename E::T T;
   typedef typename E::V8 V8;
@@ -39,12 +40,12 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
   constexpr int kStride = D + 16;                             // V's row in LDS: transposing reads of 16 rows hit all banks once
   constexpr int kVPer = kFp8 ? 16 : 8, kVLoads = 32 * D / kVPer / 64;
   constexpr int kPairs = kFp8 ? D / 64 : 0;                   // 8-bit keys: 16 bytes are the operands of two products
-  constexpr int kOStride = D + 4;
+  constexpr int kOStride = D + 4, kStep = 32 * kTeam;
   __shared__ __attribute__((aligned(16))) union Shared {
-    T v[4][32 * kStride];
-    float o[4][16 * kOStride];
+    T v[kTeam][32 * kStride];
+    float o[kTeam][16 * kOStride];
   } sh;
-  __shared__ float sh_m[4][kRows], sh_l[4][kRows];
+  __shared__ float sh_m[kTeam][kRows], sh_l[kTeam][kRows];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n16 = lane & 15, quarter = lane >> 4;
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
   typedef __attribute__((address_space(3))) s4* TrPtr;
   int key = begin + 32 * wave;
   if (key < end) load(key);
-  for (; key < end; key += 128) {
+  for (; key < end; key += kStep) {
     // scores
     f4 s[kBlocks][2];
     const bool is0 = keys[0].is, is1 = keys[1].is;
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
     __builtin_amdgcn_wave_barrier();
     // the next keys are on their way while these are weighed
     const int now = key;
-    if (key + 128 < end) load(key + 128);
+    if (key + kStep < end) load(key + kStep);
 
     V8 p_high[kBlocks], p_low[kBlocks];
 #pragma unroll
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
     }
   }
 
-  // join the four waves, 16 rows at a time
+  // join the waves, 16 rows at a time
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {
     l[b] += __shfl_xor(l[b], 16);
@@ -313,22 +314,23 @@ __global__ __launch_bounds__(256, few_waves(D, kBlocks)) void attend_few(const A
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {
     __syncthreads();
-    float top = fmaxf(fmaxf(sh_m[0][16 * b + n16], sh_m[1][16 * b + n16]),
-                      fmaxf(sh_m[2][16 * b + n16], sh_m[3][16 * b + n16]));
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kTeam; w++) top = fmaxf(top, sh_m[w][16 * b + n16]);
     if (top == -INFINITY) top = 0.f;
     const float shrink = __builtin_amdgcn_exp2f(m[b] - top);
 #pragma unroll
     for (int c = 0; c < D / 16; c++) *(f4*)&sh.o[wave][n16 * kOStride + 16 * c + 4 * quarter] = o[b][c] * shrink;
     __syncthreads();
-    for (int x = threadIdx.x; x < 16 * (D / 4); x += 256) {
+    for (int x = threadIdx.x; x < 16 * (D / 4); x += 64 * kTeam) {
       const int row = x / (D / 4), d = (x - row * (D / 4)) * 4, r = t.row + 16 * b + row;
       if (r >= t.rows) continue;
       f4 sum = f4{0.f, 0.f, 0.f, 0.f};
       float most = -INFINITY, total = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; w++) most = fmaxf(most, sh_m[w][16 * b + row]);
+      for (int w = 0; w < kTeam; w++) most = fmaxf(most, sh_m[w][16 * b + row]);
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
+      for (int w = 0; w < kTeam; w++) {
         sum += *(const f4*)&sh.o[w][row * kOStride + d];
         total += sh_l[w][16 * b + row] * __builtin_amdgcn_exp2f(sh_m[w][16 * b + row] - (most == -INFINITY ? 0.f : most));
       }

@@ -59,7 +59,7 @@ class MxRows(ct.Structure):
 class MxAttention(ct.Structure):
     _fields_ = [('q', MxRows), ('out', MxRows), ('lse', ct.c_void_p), ('workspace', ct.c_void_p),
                 ('workspace_bytes', ct.c_size_t), ('max_count', ct.c_int32), ('causal', ct.c_int32),
-                ('window', ct.c_int32), ('scale', ct.c_float)]
+                ('window', ct.c_int32), ('scale', ct.c_float), ('longest', ct.c_int32)]
 
 
 _LIB = None
@@ -237,7 +237,7 @@ def read(pages, start=None, *, count=None, tokens=None, dtype=torch.bfloat16, st
 
 
 def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale=None, out=None, lse=None,
-           stream=None):
+           longest=0, stream=None):
     """Softmax attention of the chunk's queries over their worlds' tokens, in 32 bits.
 
     Query head h uses key head ``h // (heads / kv_heads)``.  The query at position p (of its world's tokens)
@@ -245,11 +245,13 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
     with ``window`` > 0 only those with ``j > p - window``.  ``scale``: 1 / sqrt(head_dim) by default.  A query
     that sees nothing gives zeros (and ``lse`` -inf).  ``q`` is bfloat16 or float16, the pages' type unless
     those are 8-bit.  ``max_count`` (with ``start``): the largest chunk of a world, if known; rows beyond it are
-    not computed.  ``out`` (like q) and ``lse`` (float32, q's shape without head_dim, contiguous) are written
+    not computed.  ``longest``: the most tokens that a world has, if known; it says how to divide the work, and worlds that
+    are longer all the same only take longer.  ``out`` (like q) and ``lse`` (float32, q's shape without head_dim, contiguous) are written
     if given.  Returns out.  The same inputs give the same bits."""
     if _elsewhere(pages, stream):
         with torch.cuda.device(pages.device), torch.cuda.stream(stream):
-            return attend(pages, q, start, max_count=max_count, causal=causal, window=window, scale=scale, out=out, lse=lse)
+            return attend(pages, q, start, max_count=max_count, causal=causal, window=window, scale=scale, out=out, lse=lse,
+                          longest=longest)
     s, shape = pages.struct, q.shape
     chunk = _chunk(pages, shape[:-2], start)
     rows = _rows(pages, q, shape, 'q')
@@ -262,14 +264,15 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
         scale = s.head_dim ** -0.5
     if max_count is None:
         max_count = chunk.tokens if start is not None else chunk.count
-    if not (0 <= window < 2 ** 31 and 0 <= max_count < 2 ** 31 and math.isfinite(scale)):
-        raise ValueError('window (0: none) and max_count must be numbers of tokens and scale finite: %s, %s, %s'
-                         % (window, max_count, scale))
+    if not (0 <= window < 2 ** 31 and 0 <= max_count < 2 ** 31 and 0 <= longest < 2 ** 31 and math.isfinite(scale)):
+        raise ValueError('window (0: none), max_count and longest must be numbers of tokens and scale finite: %s, %s, %s, %s'
+                         % (window, max_count, longest, scale))
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _require(out.shape == shape and out.dtype == q.dtype, 'out must have q\'s shape and type')
-    a = MxAttention(rows, _rows(pages, out, shape, 'out'), None, None, 0, max_count, 1 if causal else 0, window, scale)
+    a = MxAttention(rows, _rows(pages, out, shape, 'out'), None, None, 0, max_count, 1 if causal else 0, window, scale,
+                    longest)
     if lse is not None:
         _require(lse.dtype == torch.float32 and lse.shape == shape[:-1] and lse.is_contiguous()
                  and lse.get_device() == pages.index, 'lse must be contiguous float32 of q\'s shape without head_dim')
@@ -289,12 +292,12 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
 class Chunk:
     """New tokens of an :class:`EpisodeCache`: of all its worlds the same number (``start`` None; rows are
     ``(nworld, count, heads, head_dim)``), or ``counts[w]`` of world w (rows ``(tokens, heads, head_dim)``, packed
-    world by world, ``start`` on the device)."""
+    world by world, ``start`` on the device).  ``longest``: the most tokens that a world had with them."""
 
-    __slots__ = ('counts', 'tokens', 'count', 'start')
+    __slots__ = ('counts', 'tokens', 'count', 'start', 'longest')
 
-    def __init__(self, counts, start):
-        self.counts, self.start = counts, start
+    def __init__(self, counts, start, longest=0):
+        self.counts, self.start, self.longest = counts, start, longest
         self.tokens, self.count = int(counts.sum()), int(counts.max())
 
     @property
@@ -376,18 +379,19 @@ class EpisodeCache:
             where = torch.from_numpy(world * self._table.shape[1] + slot).to(self.device)
             self.table.view(-1)[where] = torch.from_numpy(page).to(self.device)
         self.lengths[ids] += new
+        longest = int(self.lengths.max())
         counts = np.zeros(self.nworld, np.int64)
         counts[ids] = new
         if len(ids) and len(ids) == self.nworld and np.all(new == new[0]):
             if new[0]:
                 self.length.add_(int(new[0]))
-            return Chunk(counts, None)
+            return Chunk(counts, None, longest)
         both = np.zeros(2 * self.nworld + 1, np.int32)                # one upload: the chunk's starts, the lengths
         both[1:self.nworld + 1] = np.cumsum(counts)
         both[self.nworld + 1:] = self.lengths
         both = torch.from_numpy(both).to(self.device)
         self.length.copy_(both[self.nworld + 1:])
-        return Chunk(counts, both[:self.nworld + 1])
+        return Chunk(counts, both[:self.nworld + 1], longest)
 
     def reset(self, id=None):
         """Empties the worlds ``id`` (all by default); their pages are free again."""
@@ -412,6 +416,8 @@ class EpisodeCache:
         """:func:`attend` from the chunk's queries to a layer; options as there."""
         if chunk.start is not None:
             options.setdefault('max_count', chunk.count)
+        if not torch.cuda.is_current_stream_capturing():      # replays may come with longer worlds
+            options.setdefault('longest', chunk.longest)
         return attend(self.layers[layer], q, chunk.start, **options)
 
     def read(self, id=None, layer=0, *, dtype=torch.bfloat16, stream=None):

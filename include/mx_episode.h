@@ -83,7 +83,8 @@ int mx_episode_read(const MxPages* pages, const MxChunk* chunk, const MxRows* k,
  * in 32 bits.  A query that sees no key, or none with a score above -infinity, gives out 0 and lse
  * -infinity.  q and out have one type, BF16 or F16, which is the pages' too unless those are FP8 (whose
  * values are then taken in q's type).  max_count bounds n_w (a longer chunk's rows beyond it are not
- * computed); lse (tokens x heads floats) may be null.  workspace: mx_episode_workspace bytes, 16-byte
+ * computed).  longest: the most tokens that a world has, if the caller knows (0: not known); it says how to divide
+ * the work, and worlds that are longer all the same only take longer.  lse (tokens x heads floats) may be null.  workspace: mx_episode_workspace bytes, 16-byte
  * aligned, its contents undefined before and after (null when that is 0). */
 typedef struct MxAttention {
   MxRows q, out;
@@ -92,6 +93,7 @@ typedef struct MxAttention {
   size_t workspace_bytes;
   int32_t max_count, causal, window;
   float scale;
+  int32_t longest;
 } MxAttention;
 
 int mx_episode_attend(const MxPages* pages, const MxChunk* chunk, const MxAttention* a, void* stream);

@@ -193,6 +193,32 @@ def test_long_keys_are_split(gpu_available, page, store):
     check(world, [70, 1, 33, 0], 2, 'bf16', causal=False)
 
 
+@pytest.mark.parametrize('dim,kind,store', [(32, 'f16', 'f16'), (64, 'bf16', 'bf16'), (64, 'f16', 'fp8'), (96, 'bf16', 'fp8'),
+                                            (128, 'bf16', 'bf16'), (256, 'bf16', 'fp8')])
+def test_many_short_histories(gpu_available, dim, kind, store):
+    """Thousands of tiles with few keys: none, one, some on both sides of a step's 32; one block of rows and two."""
+    print('case short histories', dim, kind, store, flush=True)
+    lengths = np.arange(264) % 67
+    world = World(lengths, 8, dim, 16, store, seed=21)
+    check(world, [1] * 264, 16, kind, uniform=True)
+    check(world, (np.arange(264) % 4).tolist(), 24, kind, most=3)
+    check(world, [8 if store == 'fp8' else 4] * 264, 24, kind, causal=False, window=35, uniform=True)
+
+
+@pytest.mark.parametrize('longest', [1, 40, 300, 10 ** 9])
+def test_longest_is_only_a_guide(gpu_available, longest):
+    """Worlds longer than it says, in a table of any length, are seen whole."""
+    import torch
+    print('case longest', longest, flush=True)
+    for lengths, kv in (([300, 0, 17], 1), (np.r_[np.arange(255) % 20, [130, 300, 64, 33, 1]], 8)):
+        world = World(lengths, kv, 64, 16, 'bf16', seed=22, width=256)
+        counts = [1] * len(lengths)
+        q, start = queries(counts, 2 * kv, 64, 'bf16')
+        lse = torch.full((len(counts), 1, 2 * kv), 7.0, device='cuda')
+        out = episodes.attend(world.pages, q.cuda().unsqueeze(1), lse=lse, longest=longest)
+        compare(out, lse, expected(world, q, start), 'bf16')
+
+
 def test_rows_without_keys(gpu_available):
     """Empty worlds and chunks longer than their worlds: zeros and -inf, whatever the pages hold."""
     import torch
@@ -486,6 +512,7 @@ def test_refusals(gpu_available):
         lambda: episodes.attend(p, q[:, 0], start.long()), lambda: episodes.attend(p, q, window=-1),
         lambda: episodes.attend(p, q, scale=float('nan')), lambda: episodes.attend(p, q, out=q[:, :, :2]),
         lambda: episodes.attend(p, q, lse=torch.zeros((2, 1, 3), device='cuda')), lambda: episodes.attend(p, q, max_count=-1),
+        lambda: episodes.attend(p, q, longest=-1),
         lambda: episodes.attend(p, torch.zeros((2, 1, 64, 4), dtype=torch.bfloat16, device='cuda').transpose(2, 3)),
         lambda: episodes.write(p, q, q), lambda: episodes.write(p, kv, kv.float()), lambda: episodes.write(p, kv, kv[:, :0]),
         lambda: episodes.write(p, kv.double(), kv.double()), lambda: episodes.read(p), lambda: episodes.read(p, start),
