@@ -222,23 +222,39 @@ __device__ inline bool covered(const Attend& a, int token) {
   return a.start[low] >= 0 && place >= 0 && token < a.start[low + 1] && place < a.max_count;
 }
 
-// A row's parts in the order of their keys, whatever order they were computed in.  A workgroup takes one
-// row: its waves find the parts' maximum and shares together, then each thread adds up every kLanes-th part
-// of four neighbouring values, and the threads' sums are joined in turn.
-template <class T, int D>
+// A row's parts in the order of their keys, whatever order they were computed in.  kWaves of a workgroup's four take a
+// row: they find the parts' maximum and shares together, then each thread adds up every kLanes-th part of four
+// neighbouring values, and the threads' sums are joined in turn.  Four waves for the parts of a few rows; one
+// where there are rows enough for all waves (us for whole calls, with four and with one: 19632 rows of 32 values in
+// 7 parts 59 and 43, 60000 of 64 in 2 parts 170 and 124, 26880 of 128 in 3 parts 218 and 202).
+constexpr int kRowsForWaves = 4096;
+template <class T, int D, int kWaves>
 __global__ __launch_bounds__(256) void join_parts(const Attend a) {
-  constexpr int kQuads = D / 4, kLanes = 256 / kQuads;
-  __shared__ float share[kMostSplits];
-  __shared__ __attribute__((aligned(16))) f4 o[kLanes][kQuads];
-  const int64_t row = blockIdx.x, rows = (int64_t)a.tokens * a.heads;
+  constexpr int kQuads = D / 4, kLanes = 64 * kWaves / kQuads, kTeams = 4 / kWaves;
+  constexpr int kMost = kWaves == 1 ? 64 : kMostSplits;
+  __shared__ float sh_share[kTeams][kMost];
+  __shared__ __attribute__((aligned(16))) f4 sh_o[kTeams][kLanes][kQuads];
+  const int team = kWaves == 1 ? threadIdx.x >> 6 : 0, thread = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const auto meet = [] {
+    if constexpr (kWaves == 1) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  };
+  float* share = sh_share[team];
+  f4(*o)[kQuads] = sh_o[team];
+  const int64_t row = (int64_t)blockIdx.x * kTeams + team, rows = (int64_t)a.tokens * a.heads;
+  if (row >= rows) return;
   const int64_t token = row / a.heads;
   const int h = (int)(row - token * a.heads);
   if (!covered(a, (int)token)) return;                  // has no parts
   const int lane = threadIdx.x & 63;
-  f2 ml[kMostSplits / 64];
+  f2 ml[kMost / 64];
   float most = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kMostSplits / 64; i++) {          // every wave, all parts
+  for (int i = 0; i < kMost / 64; i++) {                // every wave, all parts
     const int s = lane + 64 * i;
     ml[i] = s < a.splits ? *(const f2*)(a.part_ml + 2 * (s * rows + row)) : f2{-INFINITY, 0.f};
     most = fmaxf(most, ml[i][0]);
@@ -248,16 +264,16 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
   const float zero = most == -INFINITY ? 0.f : most;
   float l = 0.f;
 #pragma unroll
-  for (int i = 0; i < kMostSplits / 64; i++) {
+  for (int i = 0; i < kMost / 64; i++) {
     // a part without a key of its own has no sums: they were not written
     const float w = ml[i][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i][0] - zero);
     l += ml[i][1] * w;
-    if (threadIdx.x < 64) share[lane + 64 * i] = ml[i][1] == 0.f ? -1.f : w;
+    if (thread < 64) share[lane + 64 * i] = ml[i][1] == 0.f ? -1.f : w;
   }
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
-  __syncthreads();
-  const int quad = threadIdx.x % kQuads, first = threadIdx.x / kQuads;
+  meet();
+  const int quad = thread % kQuads, first = thread / kQuads;
   f4 sum = f4{0.f, 0.f, 0.f, 0.f};
   if (first < kLanes)
 #pragma unroll 4
@@ -266,8 +282,8 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
       if (w != -1.f) sum += *(const f4*)(a.part + (s * rows + row) * D + 4 * quad) * w;
     }
   if (first < kLanes) o[first][quad] = sum;
-  __syncthreads();
-  if (threadIdx.x < kQuads) {
+  meet();
+  if (thread < kQuads) {
 #pragma unroll
     for (int i = 1; i < kLanes; i++) sum += o[i][quad];
     const float inverse = 1.f / l;
@@ -275,7 +291,7 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
 #pragma unroll
     for (int e = 0; e < 4; e++) to[e] = (T)(l == 0.f ? 0.f : sum[e] * inverse);
   }
-  if (a.lse && threadIdx.x == 0) a.lse[row] = l == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(l)) * kLn2;
+  if (a.lse && thread == 0) a.lse[row] = l == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -485,11 +501,20 @@ int mx_episode_attend(const MxPages* pages, const MxChunk* chunk, const MxAttent
                     : launch.head_dim == 128 ? mxe::attend128(a, launch, stream)
                                              : mxe::attend256(a, launch, stream);
   if (started || a.splits < 2) return started;
-  const dim3 grid((unsigned)((int64_t)a.tokens * a.heads));
+  const int64_t rows = (int64_t)a.tokens * a.heads;
+  const bool one = rows >= mxe::kRowsForWaves && a.splits <= 64;
+  const dim3 grid((unsigned)(one ? (rows + 3) / 4 : rows));
   const auto join = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (launch.type == MX_TYPE_BF16) hipLaunchKernelGGL((mxe::join_parts<__bf16, D>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((mxe::join_parts<_Float16, D>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    const auto go = [&](auto t, auto waves) {
+      hipLaunchKernelGGL((mxe::join_parts<decltype(t), D, decltype(waves)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    };
+    const auto by_rows = [&](auto t) {
+      if (one) go(t, std::integral_constant<int, 1>());
+      else go(t, std::integral_constant<int, 4>());
+    };
+    if (launch.type == MX_TYPE_BF16) by_rows((__bf16)0.f);
+    else by_rows((_Float16)0.f);
   };
   switch (launch.head_dim) {
     case 32: join(std::integral_constant<int, 32>()); break;

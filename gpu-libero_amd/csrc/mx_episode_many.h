@@ -8,7 +8,8 @@
 // are exact multiples of what they would be, and the output need not be rescaled.
 //
 // Two buffers: the next keys and values are on their way while these are weighed, one barrier a step.  Two
-// waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us), of
+// waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us,
+// but not for 96 in 8-bit pages, whose conversions then spill: 126 chunks 394 and 201 us), of
 // two workgroups, so that one's products run beside the other's softmax.
 // A prompt of 4 x 4096 tokens, 32 heads on 8 of 128 values, bfloat16: 597 us, 920 TFLOP/s, matrix
 // instructions 41 % and VALU 51 % busy; in copies of the kernel without the softmax's VALU work 533, without the loads
@@ -35,10 +36,10 @@ namespace mxe {
 
 // Keys of a step
 constexpr int many_keys(int D) { return D <= 128 ? 64 : 32; }
-constexpr int many_waves(int D) { return D <= 32 ? 4 : D <= 96 ? 3 : D <= 128 ? 2 : 1; }
+constexpr int many_waves(int D, bool fp8) { return D <= 32 ? 4 : D <= (fp8 ? 64 : 96) ? 3 : D <= 128 ? 2 : 1; }
 
 template <int kType, bool kFp8, bool kLarge, int D>
-__global__ __launch_bounds__(256, many_waves(D)) void attend_many(const Attend) {
+__global__ __launch_bounds__(256, many_waves(D, kFp8)) void attend_many(const Attend) {
   const Attend& a = arguments();
   typedef Elem<kType> E;
   typedef typename E::T T;

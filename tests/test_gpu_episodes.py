@@ -193,6 +193,17 @@ def test_long_keys_are_split(gpu_available, page, store):
     check(world, [70, 1, 33, 0], 2, 'bf16', causal=False)
 
 
+@pytest.mark.parametrize('dim,kind,store', [(32, 'f16', 'fp8'), (64, 'bf16', 'bf16'), (96, 'f16', 'f16'), (128, 'bf16', 'fp8'),
+                                            (256, 'bf16', 'bf16')])
+def test_parts_of_many_rows(gpu_available, dim, kind, store):
+    """Thousands of rows whose keys are split, most parts without any: worlds far shorter than their table."""
+    print('case parts', dim, kind, store, flush=True)
+    world = World([150, 700, 0, 137], 2, dim, 16, store, seed=23, width=256)
+    check(world, [130] * 4, 16, kind, uniform=True)
+    check(world, [130, 261, 0, 137], 16, kind, window=300)
+    check(world, [130, 129, 0, 5], 16, kind, causal=False)
+
+
 @pytest.mark.parametrize('dim,kind,store', [(32, 'f16', 'f16'), (64, 'bf16', 'bf16'), (64, 'f16', 'fp8'), (96, 'bf16', 'fp8'),
                                             (128, 'bf16', 'bf16'), (256, 'bf16', 'fp8')])
 def test_many_short_histories(gpu_available, dim, kind, store):
