@@ -179,7 +179,9 @@ constexpr int kLeastKeys = 256;
 // A lane's sum of a step's weights up to which attend_few keeps their reference
 constexpr float kReferenceHolds = 4096.f;
 __device__ inline void split_range(const Attend& a, int split, int low, int high, int& begin, int& end) {
-  begin = low & ~63;
+  // rows that see nothing may have a low beyond the table's reach, and up to 2^31 - 2: key numbers counted on from
+  // there would pass 32 bits, so that no range starts after its end (at most 2^30)
+  begin = min(low & ~63, max(high, 0));
   end = high;
   if (a.splits == 1) return;
   const int each = max(kLeastKeys, (int)(((unsigned)max(high - begin, 0) / (unsigned)a.splits + 128u) & ~127u));
