@@ -5,15 +5,16 @@
 // One pass over the keys with a reference m, sum l and output O per row (in 32 bits):
 //   S^T = K Q^T (scores of 32 keys in two products' results, a row of the chunk per lane column),
 //   p = 2^(S - m), l = l + sum p, O^T = O^T + V^T P^T.
-// The maximum is not looked for: the first step's stays the reference m until a lane's sum of a step passes 2^12
-// (or is no number); then the step's maximum is found, l and O are rescaled and the step is weighed again.  In 32
-// bits, and in bfloat16, weights up to 2^12 are as exact as those up to 1, and float16 holds them (210 -> 205 us for
+// The maximum is not looked for: the first step's stays the reference m until a lane's sum of a step passes
+// 2^12, in float16 65504 (or is no number); then the step's maximum is found, l and O are rescaled and the step is weighed again (see
+// Weights in mx_episode_types.h; 210 -> 205 us for
 // the 4096 worlds below; attend_many, whose products run beside the powers of two, lost 2 % by it).
 // With the scores transposed, a lane holds eight keys of its own row, which is the operand that the
 // second product wants if its keys are numbered 4 q + (0..3), 16 + 4 q + (0..3) for lane quarter q; V's
 // columns come in that order out of LDS by transposing reads, so probabilities never cross lanes.
 // They enter the product as two 16-bit parts, value and remainder, which costs matrix instructions
-// that a kernel bound by reading K and V has to spare, and keeps 16 bits of them.
+// that a kernel bound by reading K and V has to spare, and keeps 16 bits of them in bfloat16 and up to 22 in float16, whose
+// steps are never below 2^-24 (see Weights).
 //
 // Bound by memory, with a step's keys and values under way while the last one's are weighed: a wave reads keys as
 // the first product's operand straight from memory (a key to a lane, 16 bytes at a time), values through
@@ -250,14 +251,14 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
         }
       };
       weigh(m[b]);
-      if (__ballot(!(sum <= kReferenceHolds))) {      // a new reference
+      if (__ballot(!(sum <= E::kSumHolds))) {      // a new reference
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; j++) top = fmaxf(top, s[b][j / 4][j % 4]);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float before = m[b];
-        m[b] = fmaxf(m[b], top * a.scale2);
+        m[b] = fmaxf(m[b], top * a.scale2 - E::kTop);
         const float next = m[b] == -INFINITY ? 0.f : m[b], shrink = __builtin_amdgcn_exp2f(before - next);
         l[b] *= shrink;
 #pragma unroll

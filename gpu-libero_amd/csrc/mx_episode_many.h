@@ -4,8 +4,8 @@
 // that probabilities stay in their lanes), with 32x32 products and one 16-bit part of each probability:
 // here the matrix instructions are what bounds the kernel, and its error is that of the result's own rounding.
 //
-// The running maximum follows the scores only when one passes it by more than 2^8: until then the sums
-// are exact multiples of what they would be, and the output need not be rescaled.
+// The reference follows the scores only when one passes it by more than 2^8, in float16 2^15.9 (see Weights in
+// mx_episode_types.h): until then the sums are exact multiples of what they would be, and the output need not be rescaled.
 //
 // Two buffers: the next keys and values are on their way while these are weighed, one barrier a step.  Two
 // waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us,
@@ -153,8 +153,8 @@ __global__ __launch_bounds__(256, many_waves(D, kFp8)) void attend_many(const At
 #pragma unroll
         for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
       top = both_halves_max(top) * scale2;
-      if (__ballot(top > m + 8.f)) {
-        const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+      if (__ballot(top > m + E::kHolds)) {
+        const float next = fmaxf(m, top - E::kTop), shrink = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
         m = next;
         l *= shrink;
 #pragma unroll

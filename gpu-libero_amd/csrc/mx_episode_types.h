@@ -34,12 +34,20 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 typedef __attribute__((address_space(4))) const int32_t Fixed;
 __device__ inline Fixed* fixed(const int32_t* p) { return (Fixed*)(uintptr_t)p; }
 
+// Weights are 2^(score - reference), 16-bit operands of the second product.  A reference is set so that the
+// largest weight then is 2^kTop; attend_few keeps it until a lane's sum of a step passes kSumHolds, attend_many
+// until a weight would pass 2^kHolds.  In bfloat16, which has the range of 32 bits, any reference does.  float16
+// ends at 65504 and has full precision down to 2^-14, steps of 2^-24 below: with its largest weights from 2^12 on, those down
+// to 2^-26 of the largest (18 nats) are as exact as any, and those below 2^-37 (25 nats) are lost to the product,
+// though not to the sum of weights, which is in 32 bits.  (Largest weights of 1 lost all below 2^-25: 4095 values
+// 15 nats under one of zero were 2.6 % off.)
 template <int kType> struct Elem;
 template <> struct Elem<MX_TYPE_BF16> {
   typedef __bf16 T;
   typedef bf8 V8;
   typedef bf2 V2;
   static constexpr unsigned kExponent = 0x7f80;   // all ones in an infinity or NaN
+  static constexpr float kTop = 0.f, kSumHolds = 4096.f, kHolds = 8.f;   // see above
   static __device__ f4 mfma16(V8 a, V8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ f16v mfma32(V8 a, V8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   // two e4m3 codes (low or high half of w) times a power of two; exact: three fraction bits
@@ -52,6 +60,7 @@ template <> struct Elem<MX_TYPE_F16> {
   typedef hf8 V8;
   typedef hf2 V2;
   static constexpr unsigned kExponent = 0x7c00;
+  static constexpr float kTop = 12.f, kSumHolds = 65504.f, kHolds = 15.9f;
   static __device__ f4 mfma16(V8 a, V8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static __device__ f16v mfma32(V8 a, V8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   // exact from 2^-24 up to 65504, as any value of the queries' type
@@ -176,8 +185,6 @@ __device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, T
 // keys, and no fewer than kLeastKeys (the last ones may have none).  By the world's own keys and not by
 // the most that the table can hold, so that long and short worlds both keep all splits at work.
 constexpr int kLeastKeys = 256;
-// A lane's sum of a step's weights up to which attend_few keeps their reference
-constexpr float kReferenceHolds = 4096.f;
 __device__ inline void split_range(const Attend& a, int split, int low, int high, int& begin, int& end) {
   // rows that see nothing may have a low beyond the table's reach, and up to 2^31 - 2: key numbers counted on from
   // there would pass 32 bits, so that no range starts after its end (at most 2^30)

@@ -37,3 +37,60 @@ def test_lengths_up_to_32_bits(gpu_available, window, count):
             out = episodes.attend(world.pages, q.cuda(), torch.from_numpy(start).cuda(), causal=causal, window=window,
                                   max_count=count, lse=lse)
             compare(out, lse, (ref, ref_lse, size), 'bf16')
+
+
+def hot_and_cold(world, hot, gap):
+    """Queries of one value whose score (scale 1) is `gap` at each world's key `hot` and 0 at the others."""
+    import torch
+    for w in range(len(world.lengths)):
+        world.k[w][:, :, 0] = 0
+        world.k[w][hot[w], :, 0] = gap
+    page = world.pages.k.shape[2]
+    fp8 = world.pages.k.dtype == torch.float8_e4m3fn
+    values = world.pages.k.view(torch.uint8) if fp8 else world.pages.k
+    code = int(torch.tensor(float(gap)).to(torch.float8_e4m3fn).view(torch.uint8)) if fp8 else gap
+    for w in range(len(world.lengths)):
+        for t in range(world.lengths[w]):
+            where = (int(world.table[w, t // page]), slice(None), t % page)
+            values[where + (0,)] = code if t == hot[w] else 0
+            if fp8:
+                world.pages.k_scale[where + (0,)] = 127
+
+
+def first_value(counts, heads, dim, kind):
+    import torch
+    q, start = queries(counts, heads, dim, kind)
+    q.zero_()
+    q[..., 0] = 1
+    return q, torch.from_numpy(start).cuda()
+
+
+@pytest.mark.parametrize('gap', [10, 14, 18])
+@pytest.mark.parametrize('count', [1, 40])
+@pytest.mark.parametrize('kind,store', [('f16', 'f16'), ('f16', 'fp8'), ('bf16', 'bf16')])
+def test_small_weights_count(gpu_available, kind, store, count, gap):
+    """One key outweighs all others but has a value of zero: the output is made of the others' weights alone, each
+    exp(-gap) of the largest, which are operands of 16 bits as exact as any (float16: down to 2^-26 of the largest)."""
+    import torch
+    print('case small weights', kind, store, count, gap, flush=True)
+    for dim, width in ((64, None), (128, 512)):
+        world = World([600, 700], 1, dim, 16, store, seed=31, width=width)
+        hot = [5, 640]
+        hot_and_cold(world, hot, gap)
+        if store == 'fp8':                         # values of one sign, 64 times as large: small weights add up
+            world.pages.v.view(torch.uint8).bitwise_and_(0x7f)
+            world.pages.v_scale.add_(torch.where(world.pages.v_scale < 255, 6, 0).to(torch.uint8))
+        else:
+            world.pages.v.abs_().mul_(64)
+        for w in range(2):
+            world.v[w] = np.abs(world.v[w]) * 64
+            world.v[w][hot[w]] = 0
+            world.pages.v.view(torch.uint8 if store == 'fp8' else world.pages.v.dtype)[
+                int(world.table[w, hot[w] // 16]), :, hot[w] % 16] = 0
+        q, start = first_value([count] * 2, 4, dim, kind)
+        lse = torch.full(q.shape[:-1], 7.0, device='cuda')
+        out = episodes.attend(world.pages, q.cuda(), start, scale=1.0, lse=lse, max_count=count)
+        qd = q.double().numpy()
+        want = [attention(qd[w * count:(w + 1) * count], world.k[w], world.v[w], int(world.lengths[w]) - count, True, 0, 1.0)
+                for w in range(2)]
+        compare(out, lse, [np.concatenate(x) for x in zip(*want)], kind)
