@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
 #pragma unroll 4
     for (int s = first; s < a.splits; s += kLanes) {
       const float w = share[s];
-      if (w != -1.f) sum += *(const f4*)(a.part + (s * rows + row) * D + 4 * quad) * w;
+      if (w != -1.f) sum += rescaled(*(const f4*)(a.part + (s * rows + row) * D + 4 * quad), w);
     }
   if (first < kLanes) o[first][quad] = sum;
   meet();

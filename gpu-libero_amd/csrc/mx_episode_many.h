@@ -7,6 +7,10 @@
 // The reference follows the scores only when one passes it by more than 2^8, in float16 2^15.9 (see Weights in
 // mx_episode_types.h): until then the sums are exact multiples of what they would be, and the output need not be rescaled.
 //
+// An infinity or NaN among the values: steps that not all rows see take it out, and after the loop it is added to the rows
+// that see it.  The other steps multiply it, which gives the same unless its weight is 0 in 16 bits, or a later
+// rescale 0 in 32; so where there are outputs that are not finite, those are made anew from all values.
+//
 // Two buffers: the next keys and values are on their way while these are weighed, one barrier a step.  Two
 // waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us,
 // but not for 96 in 8-bit pages, whose conversions then spill: 126 chunks 394 and 201 us), of
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(256, many_waves(D, kFp8)) void attend_many(const At
   typedef __attribute__((address_space(3))) s4* TrPtr;
   typedef __attribute__((address_space(3))) Shared* LocalPtr;
   const unsigned at_lds = (unsigned)(uintptr_t)(LocalPtr)&sh[0];
-  int key = begin, buffer = 0;
+  int key = begin, buffer = 0, wild_from = end, wild_to = begin;       // steps whose values that are not finite were taken out
   unsigned present = 0;
   if (key < end) {
     stage.look_up(key);
@@ -183,13 +187,30 @@ __global__ __launch_bounds__(256, many_waves(D, kFp8)) void attend_many(const At
             const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TrPtr)(at + 8 * D));
             o[c] = E::mfma32(__builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), p[u][b], o[c]);
           }
-      if (mind && (sh[buffer].wild[0] | sh[buffer].wild[1] | sh[buffer].wild[2] | sh[buffer].wild[3]))
-        stage.repair(key, key + kKeys, low_r, high_r, o);
+      if (mind && (sh[buffer].wild[0] | sh[buffer].wild[1] | sh[buffer].wild[2] | sh[buffer].wild[3])) {
+        wild_from = min(wild_from, key);
+        wild_to = key + kKeys;
+      }
     }
     if (more) stage.store(sh[buffer ^ 1], key + kKeys, next_present, careful(key + kKeys, next_present));
     present = next_present;
   }
 
+  const float sum = both_halves_sum(l);
+  float off = 0.f;
+#pragma unroll
+  for (int c = 0; c < kTiles; c++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) off = __builtin_fmaf(o[c][i], 0.f, off);
+  if (__ballot(off != off && sum == sum)) {           // not because of the scores: left in
+#pragma unroll
+    for (int c = 0; c < kTiles; c++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[c][i] = fabsf(o[c][i]) < INFINITY ? o[c][i] : 0.f;
+    wild_from = begin;
+    wild_to = end;
+  }
+  stage.add_wild(wild_from, wild_to, low_r, high_r, o);
   if (row_here) finish_row<E, D>(a, split, t.token + token_in, query_head, m, l, o);
 }
 

@@ -171,7 +171,7 @@ struct Stage {
   }
 
   // Some of the keys are not there, or not seen by all rows: values of the former become zeros, and infinities and
-  // NaN too (the rows that see them get them added, by repair()).  16-bit pages: in LDS, each thread what
+  // NaN too (the rows that see them get them added, by add_wild()).  16-bit pages: in LDS, each thread what
   // it brought, after its loads are done and before a barrier.
   __device__ __forceinline__ void clean(Shared& to, int key, unsigned there) {
     unsigned wild = 0;
@@ -204,7 +204,7 @@ struct Stage {
 
   // Values of the keys [key, stop) that are not finite, added to the output of a lane's row if it sees the key
   // (o in the layout of 32x32 products).
-  __device__ __forceinline__ void repair(int key, int stop, int low_r, int high_r, f16v (&o)[D / 32]) const {
+  __device__ __forceinline__ void add_wild(int key, int stop, int low_r, int high_r, f16v (&o)[D / 32]) const {
     const int half = (threadIdx.x & 63) >> 5;
     for (int j = key; j < min(stop, end); j++) {
       const int in = table[j >> page_shift];

@@ -81,6 +81,16 @@ template <class E> __device__ inline unsigned finite_or_zero(unsigned w) {
   return w & ~((off & 0x8000u ? 0xffffu : 0u) | (off & 0x80000000u ? 0xffff0000u : 0u));
 }
 
+// A sum of weighted values, its weights made smaller: where the factor is 0 an infinity stays what it is, as its weight
+// is not zero but only beyond the range of 32 bits
+__device__ inline float rescaled(float x, float by) {
+  const float y = x * by;
+  return y == y ? y : x;
+}
+__device__ inline f4 rescaled(f4 x, float by) {
+  return f4{rescaled(x[0], by), rescaled(x[1], by), rescaled(x[2], by), rescaled(x[3], by)};
+}
+
 // E8M0: byte b stands for 2^(b - 127), 255 for NaN.  The scaled conversions take the exponent of their scale in
 // this sense, with 255 giving NaN whatever the code and 0 giving 2^-127 (run over all of these).
 __device__ inline float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }

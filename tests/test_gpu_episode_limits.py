@@ -94,3 +94,38 @@ def test_small_weights_count(gpu_available, kind, store, count, gap):
         want = [attention(qd[w * count:(w + 1) * count], world.k[w], world.v[w], int(world.lengths[w]) - count, True, 0, 1.0)
                 for w in range(2)]
         compare(out, lse, [np.concatenate(x) for x in zip(*want)], kind)
+
+
+@pytest.mark.parametrize('gap', [30, 120])
+@pytest.mark.parametrize('count', [1, 40])
+@pytest.mark.parametrize('dim,kind,store', [(32, 'f16', 'f16'), (64, 'bf16', 'bf16'), (64, 'bf16', 'fp8'), (96, 'f16', 'f16'),
+                                            (128, 'f16', 'fp8'), (128, 'bf16', 'fp8'), (256, 'bf16', 'bf16'), (256, 'f16', 'fp8')])
+def test_infinite_values_of_any_weight(gpu_available, dim, kind, store, count, gap):
+    """An infinity among the values gives the queries that see it an infinity, and a NaN a NaN, also where the key's
+    weight is beyond the reach of 16 bits or 32, before the keys that outweigh it and after, in their part and in others."""
+    import torch
+    print('case infinite values', dim, kind, store, count, gap, flush=True)
+    for width in (None, 512):
+        lengths = [300, 300, 700, 700, 2000, 90]
+        hot, cold = [0, 299 - count, 640, 5, 100, 1], [200, 7, 9, 600, 1900, 2]
+        world = World(lengths, 1, dim, 16, store, seed=32, width=width)
+        hot_and_cold(world, hot, gap)
+        for w in range(len(lengths)):
+            at = (int(world.table[w, cold[w] // 16]), 0, cold[w] % 16)
+            if store == 'fp8':                     # a block of scale 2^127, whose codes are 448 or -448
+                world.v[w][cold[w], 0, :32] = np.inf
+                world.v[w][cold[w], 0, 3] = -np.inf
+                world.pages.v.view(torch.uint8)[at][:32] = 0x7e
+                world.pages.v.view(torch.uint8)[at][3] = 0xfe
+                world.pages.v_scale[at][0] = 254
+            else:
+                for d, x in ((3, -np.inf), (4, np.inf), (dim - 1, np.nan)):
+                    world.v[w][cold[w], 0, d] = x
+                    world.pages.v[at][d] = x
+        q, start = first_value([count] * len(lengths), 3, dim, kind)
+        for causal in (True, False):
+            out = episodes.attend(world.pages, q.cuda(), start, scale=1.0, causal=causal, max_count=count)
+            qd = q.double().numpy()
+            want = [attention(qd[w * count:(w + 1) * count], world.k[w], world.v[w], int(world.lengths[w]) - count, causal, 0, 1.0)
+                    for w in range(len(lengths))]
+            compare(out, None, [np.concatenate(x) for x in zip(*want)], kind)
