@@ -210,9 +210,8 @@ __global__ __launch_bounds__(256) void move_rows(const Move a) {
 // ---------------------------------------------------------------------------- joining the parts
 constexpr int kMostSplits = 256;
 
-// Whether a packed row belongs to a world's chunk, and is not beyond max_count in it
+// Whether a packed row of ragged chunks belongs to a world's, and is not beyond max_count in it
 __device__ inline bool covered(const Attend& a, int token) {
-  if (!a.start) return token % a.count < a.max_count;
   int low = 0, high = a.nworld;
   while (high - low > 1) {
     const int middle = (low + high) >> 1;
@@ -245,11 +244,12 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
   };
   float* share = sh_share[team];
   f4(*o)[kQuads] = sh_o[team];
-  const int64_t row = (int64_t)blockIdx.x * kTeams + team, rows = (int64_t)a.tokens * a.heads;
+  const int64_t row = (int64_t)blockIdx.x * kTeams + team, rows = a.part_rows;
   if (row >= rows) return;
-  const int64_t token = row / a.heads;
-  const int h = (int)(row - token * a.heads);
-  if (!covered(a, (int)token)) return;                  // has no parts
+  int token = (int)(row / a.heads);                     // see part_row()
+  const int h = (int)(row - (int64_t)token * a.heads);
+  if (!a.start) token += token / a.max_count * (a.count - a.max_count);
+  else if (!covered(a, token)) return;                  // has no parts
   const int lane = threadIdx.x & 63;
   f2 ml[kMost / 64];
   float most = -INFINITY;
@@ -287,11 +287,11 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
 #pragma unroll
     for (int i = 1; i < kLanes; i++) sum += o[i][quad];
     const float inverse = 1.f / l;
-    T* to = (T*)a.out + token * a.o_token + (int64_t)h * a.o_head + 4 * quad;
+    T* to = (T*)a.out + (int64_t)token * a.o_token + (int64_t)h * a.o_head + 4 * quad;
 #pragma unroll
     for (int e = 0; e < 4; e++) to[e] = (T)(l == 0.f ? 0.f : sum[e] * inverse);
   }
-  if (a.lse && thread == 0) a.lse[row] = l == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(l)) * kLn2;
+  if (a.lse && thread == 0) a.lse[(int64_t)token * a.heads + h] = l == 0.f ? -INFINITY : (most + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -451,6 +451,8 @@ int choose(Attend& a, Launch& launch) {
   launch.team = splits == 1 && keys <= kShort && groups >= kPlenty ? 1 : 4;
   a.tiles = (int)tiles;
   a.splits = (int)splits;
+  // with parts there are fewer tiles than `room`, so at most 1024 of 128 rows
+  a.part_rows = splits > 1 ? (a.start ? a.tokens : a.nworld * a.max_count) * a.heads : 0;
   launch.tiles = a.tiles;
   launch.grid = (unsigned)(groups * splits);
   return 0;
@@ -458,7 +460,7 @@ int choose(Attend& a, Launch& launch) {
 
 size_t workspace_of(const Attend& a, const Launch& launch) {
   if (!launch.tiles || a.splits < 2) return 0;
-  return (size_t)a.splits * a.tokens * a.heads * (launch.head_dim + 2) * sizeof(float);
+  return (size_t)a.splits * a.part_rows * (launch.head_dim + 2) * sizeof(float);
 }
 
 }  // namespace mxe
@@ -493,7 +495,7 @@ int mx_episode_attend(const MxPages* pages, const MxChunk* chunk, const MxAttent
   if (bytes) {
     if (!m->workspace || m->workspace_bytes < bytes || ((uintptr_t)m->workspace & 15)) return MX_ERR_WORKSPACE;
     a.part = (float*)m->workspace;
-    a.part_ml = a.part + (size_t)a.splits * a.tokens * a.heads * launch.head_dim;
+    a.part_ml = a.part + (size_t)a.splits * a.part_rows * launch.head_dim;
   }
   const int started = launch.head_dim == 32 ? mxe::attend32(a, launch, stream)
                     : launch.head_dim == 64 ? mxe::attend64(a, launch, stream)
@@ -501,7 +503,7 @@ int mx_episode_attend(const MxPages* pages, const MxChunk* chunk, const MxAttent
                     : launch.head_dim == 128 ? mxe::attend128(a, launch, stream)
                                              : mxe::attend256(a, launch, stream);
   if (started || a.splits < 2) return started;
-  const int64_t rows = (int64_t)a.tokens * a.heads;
+  const int64_t rows = a.part_rows;
   const bool one = rows >= mxe::kRowsForWaves && a.splits <= 64;
   const dim3 grid((unsigned)(one ? (rows + 3) / 4 : rows));
   const auto join = [&](auto d) {

@@ -369,7 +369,7 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
       const int i = r / a.group, h = head * a.group + (r - i * a.group);
       const int64_t row_at = (int64_t)(t.token + i) * a.heads + h;
       if (a.splits > 1) {
-        const int64_t at = (int64_t)split * a.tokens * a.heads + row_at;
+        const int64_t at = (int64_t)split * a.part_rows + part_row(a, t, i, h);
         if (total != 0.f) *(f4*)(a.part + at * D + d) = sum;
         if (d == 0) *(f2*)(a.part_ml + 2 * at) = f2{most, total};
       } else {

@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256, many_waves(D, kFp8)) void attend_many(const At
     wild_to = end;
   }
   stage.add_wild(wild_from, wild_to, low_r, high_r, o);
-  if (row_here) finish_row<E, D>(a, split, t.token + token_in, query_head, m, l, o);
+  if (row_here) finish_row<E, D>(a, t, split, token_in, query_head, m, l, o);
 }
 
 }  // namespace mxe

@@ -235,14 +235,13 @@ __device__ __forceinline__ float both_halves_sum(float x) {
 // Where the 32 rows of a wave end up: their parts, or the output.  o, m, l as the kernels keep them (m and l
 // in powers of two; l of this lane's half of the keys).
 template <class E, int D>
-__device__ __forceinline__ void finish_row(const Attend& a, int split, int token, int query_head, float m, float l,
+__device__ __forceinline__ void finish_row(const Attend& a, const Tile& t, int split, int token_in, int query_head, float m, float l,
                                   const f16v (&o)[D / 32]) {
   typedef typename E::T T;
   const int half = (threadIdx.x & 63) >> 5;
   l = both_halves_sum(l);
-  const int64_t row_at = (int64_t)token * a.heads + query_head;
   if (a.splits > 1) {
-    const int64_t at = (int64_t)split * a.tokens * a.heads + row_at;
+    const int64_t at = (int64_t)split * a.part_rows + part_row(a, t, token_in, query_head);
     if (l != 0.f)
 #pragma unroll
       for (int c = 0; c < D / 32; c++)
@@ -253,7 +252,8 @@ __device__ __forceinline__ void finish_row(const Attend& a, int split, int token
     return;
   }
   const float inverse = 1.f / l;
-  T* to = (T*)a.out + (int64_t)token * a.o_token + (int64_t)query_head * a.o_head;
+  const int64_t token = t.token + token_in;
+  T* to = (T*)a.out + token * a.o_token + (int64_t)query_head * a.o_head;
 #pragma unroll
   for (int c = 0; c < D / 32; c++)
 #pragma unroll
@@ -269,7 +269,7 @@ __device__ __forceinline__ void finish_row(const Attend& a, int split, int token
         for (int e = 0; e < 4; e++) to[32 * c + 2 * i + 4 * half + e] = x[e];
       }
     }
-  if (a.lse && half == 0) a.lse[row_at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (a.lse && half == 0) a.lse[token * a.heads + query_head] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // Blocks go to the XCDs in turn: where the key heads of all worlds divide among the eight, those of one

@@ -109,10 +109,11 @@ struct Attend {
   const int32_t *table, *length, *start;
   const void* q;
   void* out;
-  float *lse, *part, *part_ml;       // part: [split][token][head][D]; part_ml: [split][token][head][2]
+  float *lse, *part, *part_ml;       // part: [split][row][D]; part_ml: [split][row][2]; rows: see part_row()
   int64_t q_token, q_head, o_token, o_head;
   int nworld, npage, width, kv_heads, page_shift, tokens, count, max_count, heads, group;
   int causal, window, tiles, splits;
+  int part_rows;                     // of one split
   float scale2;                      // |scale| * log2(e), not 0: probabilities are powers of two
   bool negate;                       // scale < 0: the queries change their sign
   bool q_vector, o_vector;           // q's rows are 16-byte aligned, out's 8-byte
@@ -189,6 +190,12 @@ __device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, T
   t.position = length - count;
   t.length = (int)min((long long)length, (long long)a.width << a.page_shift);
   return true;
+}
+
+// The row among the parts of query head h of the chunk's token i: chunks of one size have rows for max_count tokens
+// of each world, ragged ones for all packed tokens
+__device__ inline int64_t part_row(const Attend& a, const Tile& t, int i, int h) {
+  return (a.start ? t.token + i : t.world * a.max_count + i) * (int64_t)a.heads + h;
 }
 
 // The part of the keys [low, high) of a tile that a split takes: the same number for each, in steps of 128

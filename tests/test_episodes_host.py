@@ -159,3 +159,14 @@ def test_reference_attention():
     np.testing.assert_allclose(attention(q, k, v, 3, False, 0, 1.0)[0][0, 3], v[:, 1].mean(0))
     out, lse, _ = attention(q, k, v, -2, True, 0, 1.0)
     assert not out[:2].any() and np.all(np.isneginf(lse[:2])) and np.isfinite(lse[2]).all()
+
+
+def test_workspace_of_the_rows_that_are_computed():
+    """Chunks longer than max_count: the parts are of the computed rows, whatever the chunks hold beside them."""
+    c = Call()
+    c.pages.width = 4096
+    need = c.workspace()                                        # one token of each of two worlds
+    c.chunk.count, c.chunk.tokens = 2 ** 17, 2 ** 18
+    assert c.workspace() == need
+    c.attention.max_count = 3
+    assert c.workspace() > 0 and c.workspace() % (2 * 3 * 4 * (64 + 2) * 4) == 0

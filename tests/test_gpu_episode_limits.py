@@ -6,7 +6,7 @@ import pytest
 
 from episode_reference import attention
 from libero_hip import episodes
-from test_gpu_episodes import World, compare, queries
+from test_gpu_episodes import World, compare, expected, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,24 @@ def test_infinite_values_of_any_weight(gpu_available, dim, kind, store, count, g
             want = [attention(qd[w * count:(w + 1) * count], world.k[w], world.v[w], int(world.lengths[w]) - count, causal, 0, 1.0)
                     for w in range(len(lengths))]
             compare(out, None, [np.concatenate(x) for x in zip(*want)], kind)
+
+
+@pytest.mark.parametrize('most,count', [(1, 5), (3, 40), (40, 41), (60, 300)])
+@pytest.mark.parametrize('width', [64, 512])
+def test_fewer_rows_than_the_chunks_hold(gpu_available, width, most, count):
+    """max_count below the chunks' size, keys split and not: the rows before it are computed, the others not touched."""
+    import torch
+    print('case fewer rows', width, most, count, flush=True)
+    world = World([700, 301, 999], 2, 64, 16, 'bf16', seed=33, width=width)
+    q, start = queries([count] * 3, 4, 64, 'bf16')
+    want = expected(world, q, start)
+    here = np.arange(3 * count) % count < most
+    for ragged in (False, True):
+        shape = (3 * count,) if ragged else (3, count)
+        out = torch.full(shape + (4, 64), 9.0, dtype=torch.bfloat16, device='cuda')
+        lse = torch.full(shape + (4,), 7.0, device='cuda')
+        episodes.attend(world.pages, q.cuda().view(out.shape), torch.from_numpy(start).cuda() if ragged else None,
+                        max_count=most, out=out, lse=lse)
+        out, lse = out.cpu().view(q.shape), lse.cpu().view(q.shape[:-1])
+        compare(out[here], lse[here], [x[here] for x in want], 'bf16')
+        assert bool((out[~here] == 9).all()) and bool((lse[~here] == 7).all())
