@@ -88,6 +88,16 @@ def _require(ok, message, *args):
         raise ValueError(message % args)
 
 
+_REFUSED = {-1: 'arguments that do not fit', -2: 'sizes beyond its range (1024 query heads to a key head, 2^24 - 1 workgroups)'}
+
+
+def _check(rc, what):
+    """ValueError for what the library refuses, which it finds before any launch; RuntimeError for a failed launch."""
+    if rc < 0:
+        raise ValueError('%s: %s (%d)' % (what, _REFUSED.get(rc) or load().mx_error_string(rc).decode(), rc))
+    native.check(rc, what)
+
+
 class Pages:
     """One layer's pages and the worlds' tables into them.
 
@@ -209,7 +219,7 @@ def write(pages, k, v, start=None, *, stream=None):
     a, b = _rows(pages, k, shape, 'k'), _rows(pages, v, shape, 'v')
     rc = load().mx_episode_write(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b), _current(pages.index))
     if rc:
-        native.check(rc, 'mx_episode_write')
+        _check(rc, 'mx_episode_write')
 
 
 def read(pages, start=None, *, count=None, tokens=None, dtype=torch.bfloat16, stream=None):
@@ -232,7 +242,7 @@ def read(pages, start=None, *, count=None, tokens=None, dtype=torch.bfloat16, st
     a, b = (MxRows(x.data_ptr(), step, s.head_dim, s.kv_heads, kind) for x in (k, v))
     rc = load().mx_episode_read(ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(b), _current(pages.index))
     if rc:
-        native.check(rc, 'mx_episode_read')
+        _check(rc, 'mx_episode_read')
     return k, v
 
 
@@ -285,7 +295,7 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
         a.workspace, a.workspace_bytes = workspace.data_ptr(), need
         rc = lib.mx_episode_attend(*refs, raw)
     if rc:
-        native.check(rc, 'mx_episode_attend')
+        _check(rc, 'mx_episode_attend')
     return out
 
 
