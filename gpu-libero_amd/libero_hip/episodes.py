@@ -5,7 +5,9 @@ each world's episode has brought so far (instruction, observations, actions).  T
 pages of that memory: worlds differ in how far their episodes are, and a reset gives one world's pages back.
 
 Operators (``include/mx_episode.h``, on the current stream or ``stream``; they can be captured into a HIP
-graph, and read ``table``, ``length`` and ``start`` on the device):
+graph, and read ``table``, ``length`` and ``start`` on the device).  ``stream`` does not wait for the current one, nor that for
+it: the order is the caller's, as with any stream; tensors that are given may be dropped when the call returns, what it
+returns belongs to ``stream``:
 
 * :func:`write` stores a chunk's keys and values in the pages, in 16 bits or quantised to 8;
 * :func:`read` returns them as the pages stand for them;
@@ -203,6 +205,18 @@ def _elsewhere(pages, stream):
     return stream is not None or torch.cuda.current_device() != pages.index
 
 
+def _there(call, pages, stream, tensors, *args, **options):
+    """``call`` on the pages' device and on ``stream``, which then holds the memory of what it was given: a caller may
+    drop a tensor as soon as the call returns, long before ``stream`` comes to read it."""
+    with torch.cuda.device(pages.device), torch.cuda.stream(stream):
+        result = call(pages, *args, **options)
+        if stream is not None:
+            for x in (pages.k, pages.v, pages.k_scale, pages.v_scale, pages.table, pages.length) + tensors:
+                if x is not None:
+                    x.record_stream(stream)
+    return result
+
+
 def write(pages, k, v, start=None, *, stream=None):
     """Store the chunk's keys and values (float32, bfloat16 or float16; any strides whose tokens step evenly
     and whose head_dim is contiguous).  8-bit pages take, per 32 values along head_dim, the least power of two
@@ -210,8 +224,7 @@ def write(pages, k, v, start=None, *, stream=None):
     is stored as NaN.  Chunk tokens without a place (a chunk longer than its world's length, a table entry
     that names no page) are left out."""
     if _elsewhere(pages, stream):
-        with torch.cuda.device(pages.device), torch.cuda.stream(stream):
-            return write(pages, k, v, start)
+        return _there(write, pages, stream, (k, v, start), k, v, start)
     s, shape = pages.struct, k.shape
     if shape != v.shape or k.dtype != v.dtype or len(shape) < 3 or shape[-2] != s.kv_heads:
         raise ValueError('k and v must have one type and one shape, with %d heads: %s, %s' % (s.kv_heads, tuple(shape), tuple(v.shape)))
@@ -226,8 +239,7 @@ def read(pages, start=None, *, count=None, tokens=None, dtype=torch.bfloat16, st
     """The chunk's keys and values: ``(nworld, count, kv_heads, head_dim)``, or packed ``(tokens, kv_heads,
     head_dim)`` with ``start``; each value rounded once to ``dtype``.  Tokens without a place read as zeros."""
     if _elsewhere(pages, stream):
-        with torch.cuda.device(pages.device), torch.cuda.stream(stream):
-            return read(pages, start, count=count, tokens=tokens, dtype=dtype)
+        return _there(read, pages, stream, (start,), start, count=count, tokens=tokens, dtype=dtype)
     s = pages.struct
     kind = _TYPES.get(dtype, 3)
     _require(kind < 3, 'read returns float32, bfloat16 or float16')
@@ -259,9 +271,8 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
     are longer all the same only take longer.  ``out`` (like q) and ``lse`` (float32, q's shape without head_dim, contiguous) are written
     if given.  Returns out.  The same inputs give the same bits."""
     if _elsewhere(pages, stream):
-        with torch.cuda.device(pages.device), torch.cuda.stream(stream):
-            return attend(pages, q, start, max_count=max_count, causal=causal, window=window, scale=scale, out=out, lse=lse,
-                          longest=longest)
+        return _there(attend, pages, stream, (q, start, out, lse), q, start, max_count=max_count, causal=causal, window=window,
+                      scale=scale, out=out, lse=lse, longest=longest)
     s, shape = pages.struct, q.shape
     chunk = _chunk(pages, shape[:-2], start)
     rows = _rows(pages, q, shape, 'q')

@@ -26,3 +26,64 @@ def test_refusals_of_the_library_are_value_errors(gpu_available):
                        torch.ones(n, dtype=torch.int32, device='cuda'))
     with pytest.raises(ValueError, match='workgroups'):
         episodes.attend(p, pages[:1, :, :1].transpose(1, 2).expand(n, 1, 8, 32))
+
+
+def delayed(cycles=200_000_000):
+    """A stream that is busy for about a tenth of a second."""
+    import torch
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(cycles)
+    return side
+
+
+def filled(shape, dtype):
+    """Allocations of the current stream that take whatever memory has been given back."""
+    import torch
+    return [torch.full(shape, 77, dtype=dtype, device='cuda') for _ in range(3)]
+
+
+def test_tensors_may_be_dropped_after_a_call_on_another_stream(gpu_available):
+    """What a call on a stream of its own reads is kept for it, though the caller drops it and allocates anew."""
+    import torch
+    print('case dropped tensors', flush=True)
+    world = World([700, 301], 2, 64, 16, 'bf16', seed=41)
+    p = world.pages
+    q = torch.randn((70, 4, 64), device='cuda').bfloat16()
+    kv = [torch.randn((70, 2, 64), device='cuda').bfloat16() for _ in range(2)]
+    start = torch.tensor([0, 30, 70], dtype=torch.int32, device='cuda')
+    episodes.write(p, *kv, start)
+    want = episodes.attend(p, q, start)
+    episodes.write(p, kv[0] * 0, kv[1] * 0, start)
+    q2, first, k2, v2 = q.clone(), start.clone(), kv[0].clone(), kv[1].clone()
+    torch.cuda.synchronize()
+    side = delayed()
+    episodes.write(p, k2, v2, first, stream=side)
+    del k2, v2
+    read = episodes.read(p, first, tokens=70, stream=side)
+    out = episodes.attend(p, q2, first, stream=side)
+    del q2, first
+    junk = filled((70, 2, 64), torch.bfloat16), filled((70, 4, 64), torch.bfloat16), filled((3,), torch.int32)
+    assert not side.query()                        # the calls were still to come
+    torch.cuda.synchronize()
+    assert torch.equal(read[0], kv[0]) and torch.equal(read[1], kv[1]) and torch.equal(out, want)
+    del junk
+
+
+def test_cache_reads_on_another_stream(gpu_available):
+    """The rows' starts that EpisodeCache.read uploads itself stay whole until the stream has read them."""
+    import torch
+    print('case cache read elsewhere', flush=True)
+    c = episodes.EpisodeCache(6, kv_heads=2, head_dim=64, tokens=100, storage='bf16', page_tokens=16)
+    chunk = c.extend([50, 1, 20, 0, 100, 37], range(6))
+    k = torch.randn((chunk.tokens, 2, 64), device='cuda').bfloat16()
+    c.write(chunk, k, -k)
+    torch.cuda.synchronize()
+    side = delayed()
+    x, y, starts = c.read([0, 2, 5], stream=side)
+    junk = filled((7,), torch.int32)
+    assert not side.query()
+    torch.cuda.synchronize()
+    want = torch.cat([k[0:50], k[51:71], k[171:208]])
+    assert torch.equal(x, want) and torch.equal(y, -want) and starts.tolist() == [0, 50, 70, 107]
+    del junk
