@@ -337,7 +337,11 @@ class EpisodeCache:
     Each step, :meth:`extend` makes room for the new tokens; then, layer by layer, :meth:`write` stores their keys and
     values and :meth:`attend` attends from their queries.  :meth:`reset` empties worlds, as
     ``HipBatchEnv.reset(id)`` restarts them.  Tables and lengths live on the device (``table``, ``length``), with a
-    copy on the host (``lengths``) that room is made by; pages are not cleared, their old contents are never read."""
+    copy on the host (``lengths``) that room is made by; pages are not cleared, their old contents are never read.
+
+    :meth:`extend` and :meth:`reset` work on the current stream.  Calls on another one (``stream=``, or the current one then)
+    wait for the last of them, and the next of them waits for those calls.  Calls among each other (:meth:`write` on one
+    stream, :meth:`attend` on another) and their tensors are the caller's to order, and so are replays of a graph."""
 
     def __init__(self, nworld, *, kv_heads, head_dim, tokens, layers=1, storage='fp8', page_tokens=64, pages=None,
                  device='cuda:0'):
@@ -366,10 +370,53 @@ class EpisodeCache:
             scales = [torch.empty(shape[:3] + (head_dim // SCALE_BLOCK,), dtype=torch.uint8, device=device)
                       for _ in range(2 if storage == 'fp8' else 0)]
             self.layers.append(Pages(k, v, self.table, self.length, *scales))
+        # the stream of the last change and its handle; once calls come from others too, an event after that change and
+        # after the last call of each
+        self._home, self._handle, self._changed, self._used = None, 0, None, {}
+        if device.type == 'cuda':
+            self._change()
 
     @property
     def free_pages(self):
         return self._left
+
+    def _change(self):
+        """Before table and length change: the current stream waits for the calls that read them elsewhere."""
+        if self.device.type != 'cuda' or self._home is not None and not self._used and _current(self.device.index) == self._handle:
+            return
+        stream = torch.cuda.current_stream(self.device)
+        for handle, event in self._used.items():
+            if handle != stream.cuda_stream:
+                stream.wait_event(event)
+        self._used.clear()
+        if self._home is not None and self._handle != stream.cuda_stream:
+            stream.wait_stream(self._home)
+        self._home, self._handle = stream, stream.cuda_stream
+
+    def _change_done(self):
+        if self._changed is not None:
+            self._changed.record(self._home)
+
+    def _enter(self, stream, start=None):
+        """The stream of a call if that is not the last change's, for which it then waits."""
+        if (_current(self.device.index) if stream is None else stream.cuda_stream) == self._handle:
+            return None
+        stream = torch.cuda.current_stream(self.device) if stream is None else stream
+        with torch.cuda.stream(stream):
+            if torch.cuda.is_current_stream_capturing():
+                return None
+        if self._changed is None:
+            self._changed = self._home.record_event()
+        stream.wait_event(self._changed)
+        if start is not None:
+            start.record_stream(stream)
+        return stream
+
+    def _leave(self, stream):
+        if stream is not None:
+            event = self._used.get(stream.cuda_stream) or torch.cuda.Event()
+            event.record(stream)
+            self._used[stream.cuda_stream] = event
 
     def _ids(self, id):
         ids = np.arange(self.nworld) if id is None else np.atleast_1d(np.asarray(id, np.int64))
@@ -391,6 +438,7 @@ class EpisodeCache:
         total = int(need.sum())
         if total > self._left:
             raise RuntimeError('episode memory: %d more pages needed, %d free' % (total, self._left))
+        self._change()
         if total:
             world = np.repeat(ids, need)
             slot = np.repeat(first, need) + np.arange(total) - np.repeat(np.cumsum(need) - need, need)
@@ -406,12 +454,14 @@ class EpisodeCache:
         if len(ids) and len(ids) == self.nworld and np.all(new == new[0]):
             if new[0]:
                 self.length.add_(int(new[0]))
+            self._change_done()
             return Chunk(counts, None, longest)
         both = np.zeros(2 * self.nworld + 1, np.int32)                # one upload: the chunk's starts, the lengths
         both[1:self.nworld + 1] = np.cumsum(counts)
         both[self.nworld + 1:] = self.lengths
         both = torch.from_numpy(both).to(self.device)
         self.length.copy_(both[self.nworld + 1:])
+        self._change_done()
         return Chunk(counts, both[:self.nworld + 1], longest)
 
     def reset(self, id=None):
@@ -425,13 +475,17 @@ class EpisodeCache:
         self._left += len(pages)
         self._table[ids] = -1
         self.lengths[ids] = 0
+        self._change()
         where = torch.from_numpy(ids).to(self.device)
         self.table[where] = -1
         self.length[where] = 0
+        self._change_done()
 
     def write(self, chunk, k, v, layer=0, *, stream=None):
         """:func:`write` of the chunk's keys and values to a layer."""
+        other = self._enter(stream, chunk.start)
         write(self.layers[layer], k, v, chunk.start, stream=stream)
+        self._leave(other)
 
     def attend(self, chunk, q, layer=0, **options):
         """:func:`attend` from the chunk's queries to a layer; options as there."""
@@ -439,7 +493,10 @@ class EpisodeCache:
             options.setdefault('max_count', chunk.count)
         if not torch.cuda.is_current_stream_capturing():      # replays may come with longer worlds
             options.setdefault('longest', chunk.longest)
-        return attend(self.layers[layer], q, chunk.start, **options)
+        other = self._enter(options.get('stream'), chunk.start)
+        out = attend(self.layers[layer], q, chunk.start, **options)
+        self._leave(other)
+        return out
 
     def read(self, id=None, layer=0, *, dtype=torch.bfloat16, stream=None):
         """The keys and values of the worlds ``id`` (all by default) as a layer stands for them, packed in the order of
@@ -448,6 +505,8 @@ class EpisodeCache:
         counts = np.zeros(self.nworld, np.int64)
         counts[ids] = self.lengths[ids]
         start = np.concatenate([[0], np.cumsum(counts)])
+        other = self._enter(stream)
         k, v = read(self.layers[layer], torch.from_numpy(start.astype(np.int32)).to(self.device), tokens=int(start[-1]),
                     dtype=dtype, stream=stream)
+        self._leave(other)
         return k, v, np.concatenate([start[ids], start[-1:]])

@@ -87,3 +87,47 @@ def test_cache_reads_on_another_stream(gpu_available):
     want = torch.cat([k[0:50], k[51:71], k[171:208]])
     assert torch.equal(x, want) and torch.equal(y, -want) and starts.tolist() == [0, 50, 70, 107]
     del junk
+
+
+@pytest.mark.parametrize('given', [True, False])
+@pytest.mark.parametrize('busy', ['calls', 'changes', 'both'])
+def test_cache_calls_and_changes_keep_their_order(gpu_available, busy, given):
+    """Tables and lengths change on one stream, calls run on another: each sees the worlds as they were when it was
+    called, whichever stream is behind, with pages that go from world to world."""
+    import contextlib
+    import torch
+    print('case cache order', busy, given, flush=True)
+    n, heads, steps = 5, 4, 6
+    gen = torch.Generator('cuda').manual_seed(8)
+    rows = [[torch.randn((n, 3, 2, 64), generator=gen, device='cuda').bfloat16() for _ in range(2)]
+            + [torch.randn((n, 3, heads, 64), generator=gen, device='cuda').bfloat16()] for _ in range(steps)]
+
+    def play(side):
+        c = episodes.EpisodeCache(n, kv_heads=2, head_dim=64, tokens=64, storage='bf16', page_tokens=16, pages=9)
+        c.table.add_(0), c.length.add_(0)
+        torch.cuda.synchronize()
+        outs = []
+        for i, (k, v, q) in enumerate(rows):
+            if side is not None and busy != 'changes':
+                with torch.cuda.stream(side):
+                    torch.cuda._sleep(20_000_000)
+            if side is not None and busy != 'calls':
+                torch.cuda._sleep(20_000_000)
+            chunk = c.extend(3)
+            with contextlib.nullcontext() if given or side is None else torch.cuda.stream(side):
+                options = dict(stream=side) if given else {}
+                c.write(chunk, k, v, **options)
+                outs.append(c.attend(chunk, q, **options))
+            if i == 2:
+                c.reset([0, 3, 4])
+            if i == 3:
+                c.reset()
+        torch.cuda.synchronize()                     # calls among each other are the caller's to order
+        x, y, starts = c.read()
+        return outs + [x, y], starts
+
+    want, starts = play(None)
+    got, again = play(torch.cuda.Stream())
+    assert starts.tolist() == again.tolist() == [0, 6, 12, 18, 24, 30]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
