@@ -208,6 +208,7 @@ def _elsewhere(pages, stream):
 def _there(call, pages, stream, tensors, *args, **options):
     """``call`` on the pages' device and on ``stream``, which then holds the memory of what it was given: a caller may
     drop a tensor as soon as the call returns, long before ``stream`` comes to read it."""
+    _require(stream is None or stream.device == pages.device, 'stream must be on the pages\' device')
     with torch.cuda.device(pages.device), torch.cuda.stream(stream):
         result = call(pages, *args, **options)
         if stream is not None:
@@ -401,6 +402,7 @@ class EpisodeCache:
         """The stream of a call if that is not the last change's, for which it then waits."""
         if (_current(self.device.index) if stream is None else stream.cuda_stream) == self._handle:
             return None
+        _require(stream is None or stream.device == self.device, 'stream must be on the cache\'s device')
         stream = torch.cuda.current_stream(self.device) if stream is None else stream
         with torch.cuda.stream(stream):
             if torch.cuda.is_current_stream_capturing():

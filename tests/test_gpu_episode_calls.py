@@ -131,3 +131,19 @@ def test_cache_calls_and_changes_keep_their_order(gpu_available, busy, given):
     assert starts.tolist() == again.tolist() == [0, 6, 12, 18, 24, 30]
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_streams_of_other_devices_are_refused(gpu_available):
+    """A stream of another GPU was passed over for the current one without a word."""
+    import types
+    import torch
+    print('case stream of another device', flush=True)
+    other = types.SimpleNamespace(device=torch.device('cuda', 1), cuda_stream=1234567)
+    c = episodes.EpisodeCache(2, kv_heads=2, head_dim=64, tokens=10, storage='bf16')
+    chunk, p = c.extend(1), c.layers[0]
+    q = torch.zeros((2, 1, 2, 64), dtype=torch.bfloat16, device='cuda')
+    for call in (lambda: episodes.write(p, q, q, stream=other), lambda: episodes.read(p, count=1, stream=other),
+                 lambda: episodes.attend(p, q, stream=other), lambda: c.write(chunk, q, q, stream=other),
+                 lambda: c.attend(chunk, q, stream=other), lambda: c.read(stream=other)):
+        with pytest.raises(ValueError, match='device'):
+            call()
