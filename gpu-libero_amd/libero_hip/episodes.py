@@ -17,8 +17,8 @@ A chunk is the last tokens of each world's ``length``: ``(nworld, n, heads, head
 for every world, or packed rows ``(tokens, heads, head_dim)`` with ``start`` (int32, ``nworld + 1``): world
 w has the rows ``start[w]:start[w + 1]``.
 
-They are the memory of running episodes and have no backward pass: tensors whose gradients are being recorded
-are refused.
+They are the memory of running episodes and have no backward pass: tensors whose gradients are being recorded, or that
+carry a forward-mode tangent, are refused.
 
 :class:`Pages` holds the tensors of one layer; :class:`EpisodeCache` keeps the pages of several layers, the
 worlds' tables and lengths, and hands out pages.  The reference has no counterpart.
@@ -30,6 +30,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 
@@ -180,6 +181,8 @@ def _rows(pages, x, shape, name):
     """MxRows of a tensor (..., heads, head_dim) whose token dimensions step evenly."""
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError('%s: the episode memory has no backward pass; call it under torch.no_grad() or on a detached tensor' % name)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError('%s: the episode memory has no derivatives; give it the primal of a dual tensor' % name)
     kind = _TYPES.get(x.dtype, 3)
     stride = x.stride()
     if kind == 3 or shape[-1] != pages.struct.head_dim or x.get_device() != pages.index or stride[-1] != 1:

@@ -147,3 +147,19 @@ def test_streams_of_other_devices_are_refused(gpu_available):
                  lambda: c.attend(chunk, q, stream=other), lambda: c.read(stream=other)):
         with pytest.raises(ValueError, match='device'):
             call()
+
+
+def test_tangents_are_refused(gpu_available):
+    """A result without the tangent that its inputs had would be a derivative of zero."""
+    import torch
+    from torch.autograd import forward_ad
+    print('case tangents', flush=True)
+    p = World([5, 20], 2, 64, 16, 'bf16', seed=42).pages
+    q = torch.randn((2, 1, 4, 64), device='cuda').bfloat16()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: episodes.attend(p, dual), lambda: episodes.write(p, q[:, :, :2], dual[:, :, :2]),
+                     lambda: episodes.attend(p, q, out=forward_ad.make_dual(q.clone(), q))):
+            with pytest.raises(ValueError, match='dual'):
+                call()
+        assert torch.equal(episodes.attend(p, forward_ad.unpack_dual(dual).primal), episodes.attend(p, q))
