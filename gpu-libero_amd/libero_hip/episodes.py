@@ -125,6 +125,8 @@ class Pages:
                 and k.is_contiguous() and v.is_contiguous() and table.is_contiguous() and length.is_contiguous()
                 and (k_scale is None and v_scale is None) == (kind != 3)):
             _refuse_pages(k, v, table, length, k_scale, v_scale)
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            raise ValueError('pages: the episode memory has no backward pass; give it detached tensors')
         at_k, at_v = k.data_ptr(), v.data_ptr()
         _require(not (at_k | at_v) & 15, 'pages must be 16-byte aligned')
         scale_k = scale_v = None

@@ -163,3 +163,17 @@ def test_tangents_are_refused(gpu_available):
             with pytest.raises(ValueError, match='dual'):
                 call()
         assert torch.equal(episodes.attend(p, forward_ad.unpack_dual(dual).primal), episodes.attend(p, q))
+
+
+def test_pages_with_gradients_are_refused(gpu_available):
+    """Keys or values that are being trained would get no gradient from attend."""
+    import torch
+    print('case pages with gradients', flush=True)
+    p = World([5, 20], 2, 64, 16, 'bf16', seed=43).pages
+    trained = torch.nn.Parameter(p.v.clone())
+    for k, v in ((p.k, trained), (trained, p.v)):
+        with pytest.raises(ValueError, match='backward'):
+            episodes.Pages(k, v, p.table, p.length)
+    episodes.Pages(p.k, trained.detach(), p.table, p.length)
+    with torch.no_grad():
+        episodes.Pages(p.k, trained, p.table, p.length)
