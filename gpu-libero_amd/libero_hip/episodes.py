@@ -172,10 +172,12 @@ def _chunk(pages, shape, start):
     if start is None:
         if len(shape) != 2 or shape[0] != nworld:
             raise ValueError('rows must be (nworld, n, heads, head_dim), or packed (tokens, heads, head_dim) with start')
+        _require(nworld * shape[1] < 2 ** 31, 'a chunk has fewer than 2^31 rows: %d worlds of %d', nworld, shape[1])
         return MxChunk(None, nworld * shape[1], shape[1])
     _require(len(shape) == 1, 'rows with start must be packed: (tokens, heads, head_dim)')
     _require(start.dtype == torch.int32 and start.shape == (nworld + 1,) and start.is_contiguous()
              and start.get_device() == pages.index, 'start must be contiguous int32 of shape (nworld + 1,) on the pages\' device')
+    _require(shape[0] < 2 ** 31, 'a chunk has fewer than 2^31 rows: %d', shape[0])
     return MxChunk(start.data_ptr(), shape[0], 0)
 
 

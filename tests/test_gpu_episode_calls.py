@@ -177,3 +177,21 @@ def test_pages_with_gradients_are_refused(gpu_available):
     episodes.Pages(p.k, trained.detach(), p.table, p.length)
     with torch.no_grad():
         episodes.Pages(p.k, trained, p.table, p.length)
+
+
+def test_rows_beyond_32_bits_are_refused(gpu_available):
+    """2^32 rows were counted as none: nothing was written, and the call returned as if it had."""
+    import torch
+    print('case rows beyond 32 bits', flush=True)
+    p = World([5, 20], 2, 64, 16, 'bf16', seed=44).pages
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device='cuda')
+    x = torch.zeros((1, 1, 2, 64), dtype=torch.bfloat16, device='cuda')
+    for n in (2 ** 30, 2 ** 31):
+        with pytest.raises(ValueError, match='rows'):
+            episodes.write(p, x.expand(2, n, 2, 64), x.expand(2, n, 2, 64))
+        with pytest.raises(ValueError, match='rows'):
+            episodes.write(p, x[0].expand(2 * n, 2, 64), x[0].expand(2 * n, 2, 64), start)
+        with pytest.raises(ValueError, match='rows'):
+            episodes.read(p, count=n)
+        with pytest.raises(ValueError, match='rows'):
+            episodes.attend(p, x.expand(2, n, 2, 64))
