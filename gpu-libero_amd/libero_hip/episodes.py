@@ -318,6 +318,14 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
     return out
 
 
+def _captured(stream):
+    """Whether what is put on this stream (None: the current one) goes into a graph."""
+    if stream is None:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class Chunk:
     """New tokens of an :class:`EpisodeCache`: of all its worlds the same number (``start`` None; rows are
     ``(nworld, count, heads, head_dim)``), or ``counts[w]`` of world w (rows ``(tokens, heads, head_dim)``, packed
@@ -411,9 +419,8 @@ class EpisodeCache:
             return None
         _require(stream is None or stream.device == self.device, 'stream must be on the cache\'s device')
         stream = torch.cuda.current_stream(self.device) if stream is None else stream
-        with torch.cuda.stream(stream):
-            if torch.cuda.is_current_stream_capturing():
-                return None
+        if _captured(stream):
+            return None
         if self._changed is None:
             self._changed = self._home.record_event()
         stream.wait_event(self._changed)
@@ -497,12 +504,14 @@ class EpisodeCache:
         self._leave(other)
 
     def attend(self, chunk, q, layer=0, **options):
-        """:func:`attend` from the chunk's queries to a layer; options as there."""
-        if chunk.start is not None:
-            options.setdefault('max_count', chunk.count)
-        if not torch.cuda.is_current_stream_capturing():      # replays may come with longer worlds
+        """:func:`attend` from the chunk's queries to a layer; options as there.  ``max_count`` and ``longest`` are the chunk's
+        own, but not in a call that is captured: replays follow ``length`` and ``start``, whatever sizes they then have."""
+        stream = options.get('stream')
+        other = self._enter(stream, chunk.start)
+        if not _captured(stream):                             # replays may come with longer worlds, and larger chunks
+            if chunk.start is not None:
+                options.setdefault('max_count', chunk.count)
             options.setdefault('longest', chunk.longest)
-        other = self._enter(options.get('stream'), chunk.start)
         out = attend(self.layers[layer], q, chunk.start, **options)
         self._leave(other)
         return out

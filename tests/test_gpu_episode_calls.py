@@ -195,3 +195,30 @@ def test_rows_beyond_32_bits_are_refused(gpu_available):
             episodes.read(p, count=n)
         with pytest.raises(ValueError, match='rows'):
             episodes.attend(p, x.expand(2, n, 2, 64))
+
+
+def test_captured_attention_follows_larger_chunks(gpu_available):
+    """A graph of the cache's ragged attention, replayed with rows dealt to the worlds in other numbers than those it
+    was captured with: all rows are computed."""
+    import torch
+    print('case captured chunks', flush=True)
+    for heads, counts in ((2, [1, 5, 2]), (4, [10, 50, 30])):
+        c = episodes.EpisodeCache(3, kv_heads=2, head_dim=64, tokens=200, storage='bf16', page_tokens=16)
+        total = sum(counts)
+        past = c.extend(100)
+        c.write(past, *(torch.randn(past.shape + (2, 64), device='cuda').bfloat16() for _ in range(2)))
+        chunk = c.extend(counts)
+        c.write(chunk, *(torch.randn((total, 2, 64), device='cuda').bfloat16() for _ in range(2)))
+        q = torch.randn((total, heads, 64), device='cuda').bfloat16()
+        out = torch.empty_like(q)
+        c.attend(chunk, q, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.attend(chunk, q, out=out)
+        for new in (counts, [total - 2, 1, 1], [0, 0, total], [0, total, 0]):
+            chunk.start.copy_(torch.tensor([0, new[0], new[0] + new[1], total], dtype=torch.int32))
+            out.fill_(9)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, episodes.attend(c.layers[0], q, chunk.start))
