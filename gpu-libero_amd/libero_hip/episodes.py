@@ -300,6 +300,7 @@ def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _require(out.shape == shape and out.dtype == q.dtype, 'out must have q\'s shape and type')
+        _require(all(step or n < 2 for n, step in zip(shape, out.stride())), 'out has elements that share memory')
     a = MxAttention(rows, _rows(pages, out, shape, 'out'), None, None, 0, max_count, 1 if causal else 0, window, scale,
                     longest)
     if lse is not None:

@@ -222,3 +222,16 @@ def test_captured_attention_follows_larger_chunks(gpu_available):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, episodes.attend(c.layers[0], q, chunk.start))
+
+
+def test_results_that_share_memory_are_refused(gpu_available):
+    """An expanded out: rows would overwrite each other, the last one to come winning."""
+    import torch
+    print('case shared out', flush=True)
+    p = World([5, 20], 2, 64, 16, 'bf16', seed=45).pages
+    q = torch.randn((2, 1, 4, 64), device='cuda').bfloat16()
+    for out in (torch.zeros_like(q[:1]).expand(2, 1, 4, 64), torch.zeros_like(q[:, :, :1]).expand(2, 1, 4, 64)):
+        with pytest.raises(ValueError, match='share'):
+            episodes.attend(p, q, out=out)
+    out = torch.zeros((2, 4, 64), dtype=torch.bfloat16, device='cuda').as_strided((2, 1, 4, 64), (256, 0, 64, 1))
+    assert torch.equal(episodes.attend(p, q, out=out), episodes.attend(p, q))
