@@ -384,7 +384,7 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
     return rc;
   if (m->q.type != MX_TYPE_BF16 && m->q.type != MX_TYPE_F16) return MX_ERR_INVALID;
   if (m->out.type != m->q.type || (p->type != MX_TYPE_FP8 && p->type != m->q.type)) return MX_ERR_INVALID;
-  if (!(m->scale - m->scale == 0.f)) return MX_ERR_INVALID;    // not finite
+  if (!(fabsf(m->scale) * kLog2e < INFINITY)) return MX_ERR_INVALID;    // not finite, or not in base two
   a.k = (const uint8_t*)p->k; a.v = (const uint8_t*)p->v; a.k_scale = p->k_scale; a.v_scale = p->v_scale;
   a.table = p->table; a.length = p->length; a.start = c->start;
   a.q = m->q.data; a.out = m->out.data; a.lse = m->lse;

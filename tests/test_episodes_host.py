@@ -170,3 +170,14 @@ def test_workspace_of_the_rows_that_are_computed():
     assert c.workspace() == need
     c.attention.max_count = 3
     assert c.workspace() > 0 and c.workspace() % (2 * 3 * 4 * (64 + 2) * 4) == 0
+
+
+def test_scales_are_finite_in_base_two():
+    """The kernels take the scale times log2(e): 3e38 would become an infinity there, and scores of 0 NaN."""
+    for scale in (3e38, -3e38, float('inf'), float('nan')):
+        c = Call()
+        c.attention.scale = scale
+        assert c.attend() == INVALID and c.workspace() == 0
+    c = Call()
+    c.pages.width, c.attention.scale = 4096, 2.3e38
+    assert c.attend() == WORKSPACE
