@@ -94,9 +94,9 @@ struct Stage {
 
   // From memory into LDS, a wave's 64 pieces one after the other from `to` on.  As the builtin, but for the
   // waits that the compiler would put before every LDS read that follows, whatever it reads: arrived() waits.
+  // The place goes in as m0 itself (the compiler sets it), one wait state before its use.
   static __device__ __forceinline__ void into_lds(const uint8_t* base, unsigned offset, unsigned place) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place), "v"(offset), "s"(base)
-                 : "memory", "m0");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(place), "v"(offset), "s"(base) : "memory");
   }
   static __device__ __forceinline__ void arrived() {
     if constexpr (!kFp8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
