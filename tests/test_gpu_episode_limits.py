@@ -150,3 +150,32 @@ def test_fewer_rows_than_the_chunks_hold(gpu_available, width, most, count):
         out, lse = out.cpu().view(q.shape), lse.cpu().view(q.shape[:-1])
         compare(out[here], lse[here], [x[here] for x in want], 'bf16')
         assert bool((out[~here] == 9).all()) and bool((lse[~here] == 7).all())
+
+
+@pytest.mark.parametrize('store', ['bf16', 'fp8'])
+@pytest.mark.parametrize('page', [16, 64])
+def test_chunks_beyond_32_bits(gpu_available, page, store):
+    """Chunks of many rows over pages whose elements lie past 2^31 and 2^32."""
+    import torch
+    print('case far chunks', page, store, flush=True)
+    kv, dim = 4, 128
+    npage = 9_000_000 // page                                  # 4.6e9 elements
+    kind = {'bf16': torch.bfloat16, 'fp8': torch.float8_e4m3fn}[store]
+    k, v = (torch.zeros((npage, kv, page, dim), dtype=kind, device='cuda') for _ in range(2))
+    scales = [torch.zeros((npage, kv, page, 4), dtype=torch.uint8, device='cuda') for _ in range(2 if store == 'fp8' else 0)]
+    held = -(-150 // page)
+    ids = np.linspace(npage - 1, npage // 2, 2 * held).astype(np.int32).reshape(2, held)
+    pages = episodes.Pages(k, v, torch.from_numpy(ids).cuda(), torch.tensor([150, 137], dtype=torch.int32, device='cuda'), *scales)
+    x, y = (torch.randn((2, 137, kv, dim), device='cuda').bfloat16() for _ in range(2))
+    episodes.write(pages, x, y)
+    hk, hv = (g.double().cpu().numpy() for g in episodes.read(pages, count=137))
+    if store == 'bf16':
+        assert np.array_equal(hk, x.double().cpu().numpy()) and np.array_equal(hv, y.double().cpu().numpy())
+    q, _ = queries([137, 137], 8, dim, 'bf16')
+    lse = torch.empty((2, 137, 8), device='cuda')
+    out = episodes.attend(pages, q.cuda().view(2, 137, 8, dim), lse=lse)
+    pad = np.zeros((13, kv, dim))
+    qd = q.double().numpy()
+    want = [attention(qd[:137], np.concatenate([pad, hk[0]]), np.concatenate([pad, hv[0]]), 13, True, 0, dim ** -0.5),
+            attention(qd[137:], hk[1], hv[1], 0, True, 0, dim ** -0.5)]
+    compare(out, lse, [np.concatenate(z) for z in zip(*want)], 'bf16')
