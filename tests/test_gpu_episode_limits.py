@@ -6,7 +6,7 @@ import pytest
 
 from episode_reference import attention
 from libero_hip import episodes
-from test_gpu_episodes import World, compare, expected, queries
+from test_gpu_episodes import World, check, compare, expected, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +179,26 @@ def test_chunks_beyond_32_bits(gpu_available, page, store):
     want = [attention(qd[:137], np.concatenate([pad, hk[0]]), np.concatenate([pad, hv[0]]), 13, True, 0, dim ** -0.5),
             attention(qd[137:], hk[1], hv[1], 0, True, 0, dim ** -0.5)]
     compare(out, lse, [np.concatenate(z) for z in zip(*want)], 'bf16')
+
+
+@pytest.mark.parametrize('count', [6, 40, 300])
+@pytest.mark.parametrize('dim,kind,store', [(32, 'f16', 'f16'), (64, 'bf16', 'fp8'), (96, 'f16', 'f16'), (128, 'bf16', 'bf16'),
+                                            (128, 'f16', 'fp8'), (256, 'f16', 'f16')])
+def test_hidden_values_of_all_types(gpu_available, dim, kind, store, count):
+    """Infinities and NaN in values reach the queries that see them and no others (tokens later in the chunk, tokens that
+    have left the window), for every head size and type."""
+    import torch
+    print('case hidden values', dim, kind, store, count, flush=True)
+    for causal, window in ((True, 0), (True, 9), (False, 11)):
+        world = World([count, count + 21], 1, dim, 16, store, seed=34)
+        for w, token, at, bad in ((0, count - 2, 5, np.nan), (1, 12, dim - 1, np.inf), (1, count // 2, 17, -np.inf)):
+            where = (int(world.table[w, token // 16]), 0, token % 16)
+            if store == 'fp8':                     # a block of NaN
+                at = slice(at // 32 * 32, at // 32 * 32 + 32)
+                world.v[w][token, 0, at] = np.nan
+                world.pages.v_scale[where + (at.start // 32,)] = 255
+            else:
+                world.v[w][token, 0, at] = bad
+                world.pages.v[where + (at,)] = bad
+        check(world, [count, count], 3, kind, causal, window, seed=35)
+        check(world, [count, count - 4], 3, kind, causal, window, uniform=False, seed=36)
