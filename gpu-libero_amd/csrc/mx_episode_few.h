@@ -323,24 +323,33 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
       wild_to = end;
     }
   }
-  // the values that were taken out, added to the rows that see them
-  const bool wild_out = wild_from < wild_to;
+  // the values that were taken out, added to the rows that see them; 16 keys are looked through together
+  const bool wild_out = wild_from < wild_to;      // rare
   for (key = wild_from; key < wild_to; key += kStep)
-    for (int k = key; k < min(key + 32, end); k++) {
-      const int page = table[k >> a.page_shift];
-      if ((unsigned)page >= (unsigned)a.npage) continue;
-      const int64_t at = (((int64_t)page * a.kv_heads + head) << a.page_shift) + (k & page_mask);
-      const uint8_t *row = a.v + at * (kFp8 ? D : 2 * D), *scale = a.v_scale + at * kC;
+    for (int first = key; first < min(key + 32, end); first += 16) {     // 16 keys lie in one page
+      const Keys at = locate(first);
+      const uint8_t *from = a.v + at.at * (kFp8 ? D : 2 * D), *scale = a.v_scale + at.at * kC;
+      const int keys = min(16, end - first);
+      if (!at.is || !any_wild<E, kFp8>(from, scale, keys * (D / kVPer))) continue;
+      for (int j = 0; j < keys; j++)
 #pragma unroll
-      for (int c = 0; c < D / 16; c++)
+        for (int c = 0; c < D / 16; c++) {
+          const f4 x = values_at<E, kFp8>(from + j * (kFp8 ? D : 2 * D), scale + j * kC, 16 * c + 4 * quarter);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float value = value_at<E, kFp8>(row, scale, 16 * c + 4 * quarter + i);
-          if (!(fabsf(value) < INFINITY))
+          for (int b = 0; b < kBlocks; b++) {
+            const bool sees = first + j >= low_r[b] && first + j < high_r[b];
 #pragma unroll
-            for (int b = 0; b < kBlocks; b++)
-              if (k >= low_r[b] && k < high_r[b]) o[b][c][i] += value;
+            for (int i = 0; i < 4; i++) o[b][c][i] += sees && !(fabsf(x[i]) < INFINITY) ? x[i] : 0.f;
+          }
         }
+      bool open = false;                               // until all is NaN
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+        for (int c = 0; c < D / 16; c++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) open |= o[b][c][i] == o[b][c][i] && low_r[b] < high_r[b];
+      if (!__ballot(open)) wild_to = first;
     }
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {

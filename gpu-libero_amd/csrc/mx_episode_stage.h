@@ -203,22 +203,34 @@ struct Stage {
   }
 
   // Values of the keys [key, stop) that are not finite, added to the output of a lane's row if it sees the key
-  // (o in the layout of 32x32 products).
+  // (o in the layout of 32x32 products).  Sixteen keys, which lie in one page, are looked through together; it ends early
+  // when all is NaN.  (A prompt with one NaN 5.4 ms key by key.)
   __device__ __forceinline__ void add_wild(int key, int stop, int low_r, int high_r, f16v (&o)[D / 32]) const {
     const int half = (threadIdx.x & 63) >> 5;
-    for (int j = key; j < min(stop, end); j++) {
-      const int in = table[j >> page_shift];
-      if ((unsigned)in >= (unsigned)npage || !(j >= low_r && j < high_r)) continue;
-      const int row = j & ((1 << page_shift) - 1);
-      const uint8_t *from = v + (uint64_t)in * page_bytes + row * (unsigned)kRowBytes;
+    for (; key < min(stop, end); key += 16) {
+      const int in = table[key >> page_shift], keys = min(16, end - key);
+      if ((unsigned)in >= (unsigned)npage) continue;
+      const int row = key & ((1 << page_shift) - 1);
+      const uint8_t* from = v + (uint64_t)in * page_bytes + row * (unsigned)kRowBytes;
       const uint8_t* scale = v_scale + (uint64_t)in * scale_bytes + row * (unsigned)kScales;
+      if (!any_wild<E, kFp8>(from, scale, keys * kChunks)) continue;
+      bool open = false;
+      for (int j = 0; j < keys; j++) {
+        const bool sees = key + j >= low_r && key + j < high_r;
+#pragma unroll
+        for (int c = 0; c < D / 32; c++)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f4 x = values_at<E, kFp8>(from + j * kRowBytes, scale + j * kScales, 32 * c + 2 * i + 4 * half);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[c][i + e] += sees && !(fabsf(x[e]) < INFINITY) ? x[e] : 0.f;
+          }
+      }
 #pragma unroll
       for (int c = 0; c < D / 32; c++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float value = value_at<E, kFp8>(from, scale, 32 * c + 8 * (i / 4) + 4 * half + i % 4);
-          if (!(fabsf(value) < INFINITY)) o[c][i] += value;
-        }
+        for (int i = 0; i < 16; i++) open |= o[c][i] == o[c][i];
+      if (!__ballot(open && low_r < high_r)) return;
     }
   }
 };

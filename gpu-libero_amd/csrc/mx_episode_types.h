@@ -137,10 +137,35 @@ template <class E> __device__ inline typename E::V8 load_query(const Attend& a, 
   return a.negate ? -x : x;
 }
 
-// One value of V, of the row at `row` with its scales at `scale`
-template <class E, bool kFp8> __device__ inline float value_at(const uint8_t* row, const uint8_t* scale, int d) {
-  if constexpr (kFp8) return (float)E::template from_fp8<false>(row[d], scale_of(scale[d / MX_SCALE_BLOCK]))[0];
-  else return (float)((const typename E::T*)row)[d];
+// Four values of V from d on (a multiple of 4), of the row at `row` with its scales at `scale`
+template <class E, bool kFp8> __device__ inline f4 values_at(const uint8_t* row, const uint8_t* scale, int d) {
+  if constexpr (kFp8) {
+    const unsigned w = *(const unsigned*)(row + d);
+    const float s = scale_of(scale[d / MX_SCALE_BLOCK]);
+    const auto a = E::template from_fp8<false>(w, s), b = E::template from_fp8<true>(w, s);
+    return f4{(float)a[0], (float)a[1], (float)b[0], (float)b[1]};
+  } else {
+    typedef typename E::T T4 __attribute__((ext_vector_type(4)));
+    return __builtin_convertvector(*(const T4*)((const typename E::T*)row + d), f4);
+  }
+}
+
+// Whether there is an infinity or NaN among the first `pieces` of 16 bytes, by the lanes of a wave together
+template <class E, bool kFp8> __device__ inline bool any_wild(const uint8_t* from, const uint8_t* scale, int pieces) {
+  unsigned wild = 0;
+  for (int j = threadIdx.x & 63; j < pieces; j += 64) {
+    const u4 w = *(const u4*)(from + 16 * j);
+    if constexpr (kFp8) {
+      const u4 x = __builtin_bit_cast(u4, from_fp8<E>(u2{w.x, w.y}, scale[j / 2]));
+      const u4 y = __builtin_bit_cast(u4, from_fp8<E>(u2{w.z, w.w}, scale[j / 2]));
+#pragma unroll
+      for (int i = 0; i < 4; i++) wild |= not_finite<E>(x[i]) | not_finite<E>(y[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) wild |= not_finite<E>(w[i]);
+    }
+  }
+  return __ballot((wild & 0x80008000u) != 0) != 0;
 }
 
 // The world of a tile.  Ragged chunks: world w has the tile numbers from start[w] group / rows + w on,
