@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
 #pragma unroll
         for (int c = 0; c < D / 16; c++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) o[b][c][i] = fabsf(o[b][c][i]) < INFINITY ? o[b][c][i] : 0.f;
+          for (int i = 0; i < 4; i++) o[b][c][i] = set_aside(o[b][c][i]);
       wild_from = begin + 32 * wave;
       wild_to = end;
     }
@@ -351,6 +351,13 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
           for (int i = 0; i < 4; i++) open |= o[b][c][i] == o[b][c][i] && low_r[b] < high_r[b];
       if (!__ballot(open)) wild_to = first;
     }
+  if (wild_out)
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+      for (int c = 0; c < D / 16; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[b][c][i] = brought_back(o[b][c][i]);
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {
     __syncthreads();

@@ -206,11 +206,17 @@ __global__ __launch_bounds__(256, many_waves(D, kFp8)) void attend_many(const At
 #pragma unroll
     for (int c = 0; c < kTiles; c++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) o[c][i] = fabsf(o[c][i]) < INFINITY ? o[c][i] : 0.f;
+      for (int i = 0; i < 16; i++) o[c][i] = set_aside(o[c][i]);
     wild_from = begin;
     wild_to = end;
   }
-  stage.add_wild(wild_from, wild_to, low_r, high_r, o);
+  if (wild_from < wild_to) {
+    stage.add_wild(wild_from, wild_to, low_r, high_r, o);
+#pragma unroll
+    for (int c = 0; c < kTiles; c++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[c][i] = brought_back(o[c][i]);
+  }
   if (row_here) finish_row<E, D>(a, t, split, token_in, query_head, m, l, o);
 }
 

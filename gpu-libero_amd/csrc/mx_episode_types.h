@@ -9,6 +9,7 @@
 //             lane i of the group receives column i of the four rows.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <cfloat>
 #include <cstdint>
 #include "../../include/mx_physics.h"
 #include "../../include/mx_episode.h"
@@ -90,6 +91,11 @@ __device__ inline float rescaled(float x, float by) {
 __device__ inline f4 rescaled(f4 x, float by) {
   return f4{rescaled(x[0], by), rescaled(x[1], by), rescaled(x[2], by), rescaled(x[3], by)};
 }
+
+// Sums that are made anew from the values that are not finite: where none of those is found (finite ones have passed 32
+// bits) an infinity has to come out again.  It is kept as the largest finite number, to which they can be added.
+__device__ inline float set_aside(float x) { return fabsf(x) < INFINITY ? x : copysignf(FLT_MAX, x); }
+__device__ inline float brought_back(float x) { return fabsf(x) == FLT_MAX ? copysignf(INFINITY, x) : x; }
 
 // E8M0: byte b stands for 2^(b - 127), 255 for NaN.  The scaled conversions take the exponent of their scale in
 // this sense, with 255 giving NaN whatever the code and 0 giving 2^-127 (run over all of these).

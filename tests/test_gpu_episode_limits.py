@@ -202,3 +202,25 @@ def test_hidden_values_of_all_types(gpu_available, dim, kind, store, count):
                 world.pages.v[where + (at,)] = bad
         check(world, [count, count], 3, kind, causal, window, seed=35)
         check(world, [count, count - 4], 3, kind, causal, window, uniform=False, seed=36)
+
+
+@pytest.mark.parametrize('count', [1, 40])
+@pytest.mark.parametrize('store', ['bf16', 'fp8'])
+@pytest.mark.parametrize('dim', [64, 128])
+def test_sums_beyond_32_bits(gpu_available, dim, store, count):
+    """Finite values whose weighted sum passes 32 bits before it is divided: an infinity of their sign, or the value
+    itself where the kernel's order of sums holds it, but nothing smaller."""
+    import torch
+    print('case sums beyond 32 bits', dim, store, count, flush=True)
+    world = World([900, 700], 1, dim, 16, store, seed=37)
+    if store == 'fp8':
+        world.pages.v.view(torch.uint8).fill_(0x7e)             # 448 2^119
+        world.pages.v_scale.fill_(246)
+    else:
+        world.pages.v.fill_(2.9e38)
+    world.pages.v.view(torch.uint8 if store == 'fp8' else torch.int16)[..., dim // 2:] |= 0x80 if store == "fp8" else -32768
+    q, start = first_value([count] * 2, 4, dim, 'bf16')
+    q.zero_()
+    out = episodes.attend(world.pages, q.cuda(), torch.from_numpy(np.array([0, count, 2 * count], np.int32)).cuda(),
+                          max_count=count).float().cpu()
+    assert bool((out[..., :dim // 2] > 2.8e38).all()) and bool((out[..., dim // 2:] < -2.8e38).all())
