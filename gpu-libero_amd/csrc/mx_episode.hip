@@ -413,10 +413,10 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 }
 
 // Which kernel, by the rows that share a key head's keys and values.  us for 300 worlds of up to 700 tokens, 4 key
-// heads of 128 values, with 12, 24, 48 rows: attend_few of 16 rows 53, 76, 102 in bfloat16 and 33, 50, 69 with 8-bit
-// pages, of 32 rows 66, 68, 104 and 45, 48, 82, attend_many 61, 63, 69 and 63, 64, 72;
-// worlds of up to 512 tokens and heads of 256 values, with 12, 24, 48 rows: attend_few of 16 rows, then 32, 105, 162, 282
-// and 73, 134, 236, attend_many 154, 155, 162 and 224, 226, 239 (80 rows 173 and 251, attend_few 407 and 337).
+// heads of 128 values, with 12, 24, 48 rows: attend_few of 16 rows 52, 75, 101 in bfloat16 and 32, 48, 66 with 8-bit
+// pages, of 32 rows (8-bit pages only) 42, 44, 77, attend_many 57, 59, 63 and 54, 55, 60;
+// worlds of up to 512 tokens and heads of 256 values, with 12, 24, 48 rows: attend_few of 16 rows 106, 183, 265
+// and 75, 140, 204, of 32 rows 129, 137, 240, attend_many 122, 124, 131 and 136, 137, 143.
 //
 // Into how many parts each tile's keys are split: where the tiles leave room, as many as the card holds
 // workgroups at once (two per CU, four where heads of up to 64 values leave the registers), unless one

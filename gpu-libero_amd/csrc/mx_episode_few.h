@@ -13,17 +13,17 @@
 // second product wants if its keys are numbered 4 q + (0..3), 16 + 4 q + (0..3) for lane quarter q; V's
 // columns come in that order out of LDS by transposing reads, so probabilities never cross lanes.
 // They enter the product as two 16-bit parts, value and remainder, which costs matrix instructions
-// that a kernel bound by reading K and V has to spare, and keeps 16 bits of them in bfloat16 and up to 22 in float16, whose
+// that a kernel bound by reading K and V has to spare, and keeps 16 bits of them in bfloat16 and up to 20 in float16, whose
 // steps are never below 2^-24 (see Weights).
 //
 // Bound by memory, with a step's keys and values under way while the last one's are weighed: a wave reads keys as
 // the first product's operand straight from memory (a key to a lane, 16 bytes at a time), values through
 // LDS of its own without a barrier, and the waves' results are joined once.  What counts is how many
-// waves a SIMD holds: keeping the values' words for the rare repair below took 130 registers and three
+// waves a SIMD holds: keeping the values' words for the rare infinities below took 130 registers and three
 // waves at 64 values a head, reading them again 120 and four (249 -> 216 us for 4096 worlds of up to
 // 1024 quantised tokens).  Single tokens, alternating inputs: those worlds (4 key heads of 64, 1.13 GB) 205 us, 5.5 TB/s, its
-// VALU 56 % busy with conversions and softmax; 500 worlds of up to 2048 tokens in bfloat16 (8 key heads of 128, 2.1 GB) 364 us, 5.8 TB/s;
-// two worlds, 131072 quantised tokens in all (277 MB), 47 us and 5 to join the parts.
+// VALU 57 % busy with conversions and softmax; 500 worlds of up to 2048 tokens in bfloat16 (8 key heads of 128, 2.1 GB) 364 us, 5.8 TB/s;
+// two worlds, 131072 quantised tokens in all (277 MB), 48 us and 5 to join the parts.
 #pragma once
 #include "mx_episode_types.h"
 

@@ -2,7 +2,10 @@
 // heads that share the key head), each of its four waves 32 of them, and 64 keys at a time (32 of 256 values), which all four
 // read from LDS.  The mathematics is that of attend_few (one pass, running maximum, scores transposed so
 // that probabilities stay in their lanes), with 32x32 products and one 16-bit part of each probability:
-// here the matrix instructions are what bounds the kernel, and its error is that of the result's own rounding.
+// here the matrix instructions are part of what bounds the kernel, and a second product for the remainders would add
+// half of them again.  The rounding of the probabilities (2^-9 of each in bfloat16, 2^-12 in float16, at random) is of the size
+// of the result's own: against 64 bits the error is 1.3 times that of exact probabilities on a prompt, 1.4 times in a window of 2000
+// (0.0021 and 0.0016 of the norm, 0.0023 and 0.0017; float16 2.7e-4 and 2.1e-4).
 //
 // The reference follows the scores only when one passes it by more than 2^8, in float16 2^15.9 (see Weights in
 // mx_episode_types.h): until then the sums are exact multiples of what they would be, and the output need not be rescaled.
@@ -13,25 +16,29 @@
 //
 // Two buffers: the next keys and values are on their way while these are weighed, one barrier a step.  Two
 // waves per SIMD (three up to 96 values a head, where that took 300 ragged chunks from 52 to 47 us,
-// but not for 96 in 8-bit pages, whose conversions then spill: 126 chunks 394 and 201 us), of
+// but not for 96 in 8-bit pages, whose conversions then spill: 126 chunks 394 and 201 us, now 196), of
 // two workgroups, so that one's products run beside the other's softmax.
-// A prompt of 4 x 4096 tokens, 32 heads on 8 of 128 values, bfloat16: 597 us, 920 TFLOP/s, matrix
-// instructions 41 % and VALU 51 % busy; in copies of the kernel without the softmax's VALU work 533, without the loads
-// 530, without reading keys and values from LDS 495, with the matrix instructions alone 340: no one of them bounds it.
-// Tried and not kept: 64 rows to a wave (the compiler moves the outputs between the two halves of the register
+// A prompt of 4 x 4096 tokens, 32 heads on 8 of 128 values, bfloat16: 560 us, 980 TFLOP/s (554 to 613 on cards at other
+// clocks), matrix instructions 49 % and VALU 49 % busy; on a card at 554 to 566, in copies of the kernel without the softmax's VALU
+// work 501 to 507, without the loads 490 to 495, without reading keys and values from LDS 454, with the matrix instructions alone
+// 313: no one of them bounds it.  (With the scan for values that are not finite inside the loop 20 to 30 us more: the
+// compiler kept its addresses in scalar registers that it then spilled.)
+// Tried and not kept, beside a kernel of 597: 64 rows to a wave (the compiler moves the outputs between the two halves of the register
 // file at every branch, 1100 us; heads of 64 values hold them, and fewer workgroups run side by side: 8 x 4096 tokens 342 to 354,
 // 300 x 150 tokens 120 to 143, the window below 102 to 93), 32 keys a step (700), eight waves to a workgroup (612), a wave's priority raised
 // around its products (591 to 615), reads of keys grouped ahead of the products (-1 %), the next step's scores
 // computed beside this one's softmax (650), the reference kept without a maximum (617).
-// 300 ragged chunks of up to 41 tokens over up to 701, 12 heads on 4 of 96 values, float16 (161 MB): 57 us; the loads alone
-// 52, the rest alone 41, neither 22: what a workgroup waits for until its first keys are there, and that in two rounds of
-// workgroups (queries asked for after the first keys 55.6, but 59.3 instead of 58.5 in heads of 128; rows dealt to
+// 300 ragged chunks of up to 41 tokens over up to 701, 12 heads on 4 of 96 values, float16 (161 MB): 52 us; the loads alone
+// 47, the rest alone 39, neither 21: what a workgroup waits for until its first keys are there, and that in two rounds of
+// workgroups (queries asked for after the first keys 55.6 instead of 57.4 before, but 59.3 instead of 58.5 in heads of 128; rows dealt to
 // other waves by block, the same).
-// 16 worlds' 512 tokens over a window of 2000 in 8-bit pages, 16 heads on 2 of 64 values: 95 us, 640 TFLOP/s; a
-// head of 64 values has half the products to each power of two, and the VALU is 61 % busy.
+// 16 worlds' 512 tokens over a window of 2000 in 8-bit pages, 16 heads on 2 of 64 values: 98 us, 610 TFLOP/s; a
+// head of 64 values has half the products to each power of two, and the VALU is 62 % busy.  With pages of 16 or 32 tokens
+// 121: heads of 32 and 64 values then keep their page numbers in scratch memory (160 bytes a lane), as the compiler indexes
+// them at run time (heads of 128: 158 and 164).
 // Heads of 256 values: the outputs and queries of 32 rows are 192 registers, so one wave per SIMD, whose
-// products nothing runs beside: 4 x 2048 tokens, 16 heads on 4, bfloat16: 295 us, 466 TFLOP/s (64 keys a step
-// 397, as many rows as attend_few takes at a time 915).
+// products nothing runs beside, and which moves values between the halves of the register file: 4 x 2048 tokens, 16 heads on 4,
+// bfloat16: 233 us, 590 TFLOP/s (64 keys a step, as many rows as attend_few takes at a time: 397 and 915, beside 295 then).
 #pragma once
 #include "mx_episode_launch.h"
 #include "mx_episode_stage.h"

@@ -268,7 +268,9 @@ def read(pages, start=None, *, count=None, tokens=None, dtype=torch.bfloat16, st
 
 def attend(pages, q, start=None, *, max_count=None, causal=True, window=0, scale=None, out=None, lse=None,
            longest=0, stream=None):
-    """Softmax attention of the chunk's queries over their worlds' tokens, in 32 bits.
+    """Softmax attention of the chunk's queries over their worlds' tokens, with scores and sums in 32 bits; the
+    probabilities that multiply the values are rounded to q's type, in two parts for few rows and in one for many (see
+    ``include/mx_episode.h``).
 
     Query head h uses key head ``h // (heads / kv_heads)``.  The query at position p (of its world's tokens)
     sees the tokens ``j <= p``, or with ``causal=False`` all of them (a step's tokens see each other), and

@@ -80,12 +80,19 @@ int mx_episode_read(const MxPages* pages, const MxChunk* chunk, const MxRows* k,
  * h / (heads / kv_heads).  The query at position p = length[w] - n_w + i sees the keys j <= p (causal) or
  * j < length[w], and of those the `window` last up to its own position (j > p - window) when window > 0:
  *     out = sum_j exp(scale * q.k_j - m) v_j / sum_j exp(scale * q.k_j - m),  lse = m + log(sum)
- * in 32 bits.  A query that sees no key, or none with a score above -infinity, gives out 0 and lse
- * -infinity.  q and out have one type, BF16 or F16, which is the pages' too unless those are FP8 (whose
- * values are then taken in q's type).  max_count bounds n_w (a longer chunk's rows beyond it are not
- * computed).  longest: the most tokens that a world has, if the caller knows (0: not known); it says how to divide
- * the work, and worlds that are longer all the same only take longer.  lse (tokens x heads floats) may be null.  workspace: mx_episode_workspace bytes, 16-byte
- * aligned, its contents undefined before and after (null when that is 0). */
+ * A query that sees no key, or none with a score above -infinity, gives out 0 and lse -infinity.
+ *
+ * Scores, sums, lse and out before its one rounding are in 32 bits.  The probabilities that multiply the values are
+ * rounded to the queries' type: in two parts, value and remainder, where few rows (new tokens x query heads) share a key
+ * head (16, with 8-bit pages 32), in one where more do.  float16 probabilities below 2^-26 of a row's largest lose bits,
+ * those below 2^-37 count in the sum alone.  Sums of weighted values that pass 32 bits (bfloat16 values of 2^116 and more)
+ * are infinities.  An infinity or NaN in a value reaches all queries that see its key, whatever its weight, and no others.
+ *
+ * q and out have one type, BF16 or F16, which is the pages' too unless those are FP8 (whose values are then taken in q's
+ * type).  max_count bounds n_w (a longer chunk's rows beyond it are not computed).  longest: the most tokens that a world
+ * has, if the caller knows (0: not known); it says how to divide the work, and worlds that are longer all the same only
+ * take longer.  lse (tokens x heads floats) may be null.  workspace: mx_episode_workspace bytes, 16-byte aligned, its
+ * contents undefined before and after (null when that is 0). */
 typedef struct MxAttention {
   MxRows q, out;
   float* lse;
