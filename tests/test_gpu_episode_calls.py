@@ -235,3 +235,39 @@ def test_results_that_share_memory_are_refused(gpu_available):
             episodes.attend(p, q, out=out)
     out = torch.zeros((2, 4, 64), dtype=torch.bfloat16, device='cuda').as_strided((2, 1, 4, 64), (256, 0, 64, 1))
     assert torch.equal(episodes.attend(p, q, out=out), episodes.attend(p, q))
+
+
+def test_captured_on_the_stream_that_is_given(gpu_available):
+    """Calls with stream= that go into a graph on that stream, of the operators and of the cache: replays give what
+    eager calls give, and memory that was dropped since is not the graph's."""
+    import torch
+    print('case captured stream', flush=True)
+    side = torch.cuda.Stream()
+    c = episodes.EpisodeCache(3, kv_heads=2, head_dim=64, tokens=2000, storage='fp8')
+    past = c.extend([900, 40, 1500])
+    c.write(past, *(torch.randn(past.shape + (2, 64), device='cuda').bfloat16() for _ in range(2)))
+    chunk = c.extend(2)
+    k, v = (torch.randn((3, 2, 2, 64), device='cuda').bfloat16() for _ in range(2))
+    q = torch.randn((3, 2, 4, 64), device='cuda').bfloat16()
+    outs = [torch.empty_like(q) for _ in range(2)]
+
+    def calls():
+        c.write(chunk, k, v, stream=side)
+        c.attend(chunk, q, out=outs[0], stream=side)
+        episodes.attend(c.layers[0], q, out=outs[1], stream=side)
+
+    torch.cuda.synchronize()
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        calls()
+    for _ in range(3):
+        for x in (k, v, q):
+            x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        junk = filled((3, 2, 4, 64), torch.bfloat16)
+        want = episodes.attend(c.layers[0], q)
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+    del junk
