@@ -17,8 +17,10 @@ ROOT = HERE.parent
 LIBRARY = HERE / 'libmx_physics.so'
 SOURCES = [HERE / 'csrc' / 'mx_step.hip', HERE / 'csrc' / 'mx_step_slab.hip', HERE / 'csrc' / 'mx_step_slab4.hip',
            HERE / 'csrc' / 'mx_step_f64.hip', HERE / 'csrc' / 'mx_episode.hip'] + [
+           HERE / 'csrc' / ('mx_episode_%s.hip' % part) for part in ('rotary', 'room', 'recall')] + [
            HERE / 'csrc' / ('mx_episode_d%d.hip' % d) for d in (32, 64, 96, 128, 256)]
 HEADERS = [HERE / 'csrc' / h for h in ('mx_math.h', 'mx_image.h', 'mx_collide.h', 'mx_convex.h', 'mx_episode_types.h',
+                                       'mx_episode_move.h',
                                        'mx_episode_few.h', 'mx_episode_many.h',
                                        'mx_episode_stage.h', 'mx_episode_launch.h', 'mx_episode_dim.h')] + [
            ROOT / 'include' / 'mx_physics.h', ROOT / 'include' / 'mx_episode.h']

@@ -2,161 +2,12 @@
 // split attention, and the host side of all calls.  The attention itself: mx_episode_few.h, mx_episode_many.h.
 #include <cmath>
 #include <type_traits>
-#include "mx_episode_types.h"
+#include "mx_episode_move.h"
 #include "mx_episode_launch.h"
 
 namespace mxe {
 
 // ---------------------------------------------------------------------------- write and read
-struct Copy {
-  uint8_t *pages, *scales;       // of k or v
-  const uint8_t* rows;
-  int64_t token_stride, head_stride;
-  bool vector;                   // rows are 16-byte aligned
-};
-struct Move {
-  Copy of[2];
-  const int32_t *table, *length, *start;
-  int nworld, npage, width, kv_heads, head_dim, page_shift, tokens, count, tokens_each;
-};
-
-// The slot of packed row `token` of a world's chunk, as (page * kv_heads * page_tokens + slot) without the
-// head; -1: none
-__device__ inline int64_t slot_of(const Move& a, int world, int place, int count) {
-  if (place < 0 || place >= count) return -1;
-  const int position = max(a.length[world], 0) - count + place;
-  if (position < 0 || (position >> a.page_shift) >= a.width) return -1;
-  const int page = a.table[(int64_t)world * a.width + (position >> a.page_shift)];
-  if ((unsigned)page >= (unsigned)a.npage) return -1;
-  return (((int64_t)page * a.kv_heads) << a.page_shift) + (position & ((1 << a.page_shift) - 1));
-}
-
-// The slots of `tokens` (at most 64) packed rows from `first` on, by the lanes of one wave.  Ragged chunks:
-// the first row's world by a search with 64 probes at a time, the others' from there, mostly the same.
-__device__ inline void find_slots(const Move& a, int first, int tokens, int64_t* slots) {
-  const int lane = threadIdx.x, token = first + lane;
-  if (!a.start) {
-    if (lane < tokens) {
-      const int world = token / a.count;
-      slots[lane] = slot_of(a, world, token - world * a.count, a.count);
-    }
-    return;
-  }
-  int low = 0, high = a.nworld;
-  while (high - low > 1) {
-    const int step = (high - low + 63) >> 6, probe = low + lane * step;
-    const int passed = max(1, (int)__popcll(__ballot(probe < high && a.start[probe] <= first)));
-    low += (passed - 1) * step;
-    high = min(high, low + step);
-  }
-  if (lane < tokens) {
-    if (a.start[low + 1] <= token) {
-      high = a.nworld;
-      while (high - low > 1) {
-        const int middle = (low + high) >> 1;
-        if (a.start[middle] <= token) low = middle; else high = middle;
-      }
-    }
-    slots[lane] = slot_of(a, low, token - a.start[low], a.start[low + 1] - a.start[low]);
-  }
-}
-
-// A thread's piece of a row in bytes, and how many pieces of keys and of values it has under way.  8-bit pages: 32
-// bytes, so that a thread's codes are 8 or 16 at once, except for reads into single precision, which are bound
-// by their own stores.  us, measured with 16 and 32 bytes: 500 histories of 8-bit pages into bf16 180 and 152, 67 chunks of
-// single precision written to 8-bit pages and read back 61 and 69 (16 for the read alone 59); one and two under way:
-// 500 histories of bf16 173 and 185, the 67 chunks 61 and 59.
-constexpr int piece_bytes(bool fp8, bool write, int size) { return fp8 && (write || size < 4) ? 32 : 16; }
-constexpr int pieces_ahead(int size) { return size == 4 ? 2 : 1; }
-
-template <class T, int N> __device__ inline void load_row(const T* from, bool vector, float (&x)[N]) {
-  constexpr int kEach = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
-  typedef T V __attribute__((ext_vector_type(kEach)));
-  if (vector) {
-#pragma unroll
-    for (int j = 0; j < N; j += kEach) {
-      const V v = *(const V*)(from + j);
-#pragma unroll
-      for (int e = 0; e < kEach; e++) x[j + e] = (float)v[e];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; j++) x[j] = (float)from[j];
-  }
-}
-
-// kPast: past the caches.  Rows that were read out are many; 262 MB of 8-bit pages into 524 MB of rows 183 us
-// through the caches, 152 past them, and 69 or 61 for 34 + 137 MB.
-template <bool kPast, class T, int N> __device__ inline void store_row(T* to, bool vector, const float (&x)[N]) {
-  constexpr int kEach = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
-  typedef T V __attribute__((ext_vector_type(kEach)));
-  if (vector) {
-#pragma unroll
-    for (int j = 0; j < N; j += kEach) {
-      V v;
-#pragma unroll
-      for (int e = 0; e < kEach; e++) v[e] = (T)x[j + e];
-      if constexpr (kPast) __builtin_nontemporal_store(v, (V*)(to + j));
-      else *(V*)(to + j) = v;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; j++) to[j] = (T)x[j];
-  }
-}
-
-// `at`: element in the pages; at / 32 is the scale's place, as head_dim is a multiple of 32
-template <int kStore, int N> __device__ inline void load_page(const Copy& c, int64_t at, float (&x)[N]) {
-  if constexpr (kStore == MX_TYPE_FP8) {
-    typedef unsigned W __attribute__((ext_vector_type(N / 4)));
-    const W w = *(const W*)(c.pages + at);
-    const float scale = scale_of(c.scales[at / MX_SCALE_BLOCK]);
-#pragma unroll
-    for (int j = 0; j < N / 4; j++) {
-      const f2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale, false);
-      const f2 q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[j], scale, true);
-      x[4 * j] = p[0];
-      x[4 * j + 1] = p[1];
-      x[4 * j + 2] = q[0];
-      x[4 * j + 3] = q[1];
-    }
-  } else {
-    load_row((const typename Elem<kStore>::T*)c.pages + at, true, x);
-  }
-}
-
-// All threads take part, with at < 0 where there is nothing to store: neighbours share a scale
-template <int kStore, int N> __device__ inline void store_page(const Copy& c, int64_t at, const float (&x)[N]) {
-  if constexpr (kStore == MX_TYPE_FP8) {
-    // the largest magnitude of the block, as the bits of a float that is not negative: they order
-    // like integers, infinities and NaN above all numbers
-    unsigned top = 0;
-#pragma unroll
-    for (int j = 0; j < N; j++) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int lanes = 1; lanes < MX_SCALE_BLOCK / N; lanes *= 2) top = max(top, (unsigned)__shfl_xor((int)top, lanes));
-    // 448 = 1.75 * 2^8: the exponent less 8, and one more above a fraction of 1.75
-    const bool finite = top < 0x7f800000u;
-    const int e = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), -117);
-    const float inverse = __uint_as_float((unsigned)(127 - e) << 23);
-    if (at < 0) return;
-    typedef unsigned W __attribute__((ext_vector_type(N / 4)));
-    W w;
-#pragma unroll
-    for (int j = 0; j < N / 4; j++) {
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = finite ? x[4 * j + i] * inverse : 0.f;
-      const unsigned half = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-      w[j] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], half, true);
-    }
-    *(W*)(c.pages + at) = w;
-    if (at % MX_SCALE_BLOCK == 0) c.scales[at / MX_SCALE_BLOCK] = finite ? (uint8_t)(e + 127) : 255;
-  } else {
-    if (at >= 0) store_row<false>((typename Elem<kStore>::T*)c.pages + at, true, x);
-  }
-}
-
 // A workgroup moves `tokens_each` packed tokens of all heads, keys and values: its first threads find
 // their slots, then every thread moves pieces in the order of the rows.  Nothing is computed but the scales: bound by memory.
 constexpr int kMostTokens = 64;                         // of a workgroup: their slots are kept in LDS
@@ -373,7 +224,9 @@ int move(const MxPages* p, const MxChunk* c, const MxRows* k, const MxRows* v, v
 }
 
 // Checks, and the launch: which kernel, how many tiles, how the keys are split
-int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, Launch& launch, bool pointers) {
+int choose(Attend& a, Launch& launch);
+int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, Launch& launch, bool pointers,
+         const MxSelection* s, int block_shift) {
   int rc = pages_check(p);
   if (rc || (rc = chunk_check(p, c))) return rc;
   if (!m) return MX_ERR_INVALID;
@@ -409,6 +262,11 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   launch.head_dim = p->head_dim;
   launch.keys = (int64_t)p->width << a.page_shift;
   if (m->longest && m->longest < launch.keys) launch.keys = m->longest;
+  if (s) {
+    launch.listed = true;
+    a.blocks = s->blocks; a.lists = s->width; a.block_shift = block_shift;
+    launch.keys = (int64_t)s->width << block_shift;
+  }
   return choose(a, launch);
 }
 
@@ -430,11 +288,12 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 // 70 and 60, 92 and 90; 2048 of those 23 and 12, 39 and 36, 50 and 53; 512 of them 10.8 and 10.9, 11.4 and 16.7, 15 and 23.
 constexpr int kShort = 256, kPlenty = 2048;
 int choose(Attend& a, Launch& launch) {
-  const int64_t rows = (int64_t)a.max_count * a.group;
+  const int64_t rows = launch.listed ? a.group : (int64_t)a.max_count * a.group;
   const bool few = rows <= (launch.fp8 ? 32 : 16);
-  launch.blocks = rows <= 16 ? 1 : 2;
-  launch.rows = few ? 16 * launch.blocks : kManyRows;
-  const int64_t tiles = a.start ? (int64_t)a.tokens * a.group / launch.rows + a.nworld
+  launch.blocks = rows <= 16 || (launch.listed && !launch.fp8) ? 1 : 2;
+  launch.rows = few || launch.listed ? 16 * launch.blocks : kManyRows;
+  const int64_t tiles = launch.listed ? ((rows + launch.rows - 1) / launch.rows) * (a.start ? a.tokens : (int64_t)a.nworld * a.max_count)
+                      : a.start ? (int64_t)a.tokens * a.group / launch.rows + a.nworld
                                 : ((rows + launch.rows - 1) / launch.rows) * a.nworld;
   int64_t keys = launch.keys;
   if (a.window > 0 && a.causal) {
@@ -461,6 +320,45 @@ int choose(Attend& a, Launch& launch) {
 size_t workspace_of(const Attend& a, const Launch& launch) {
   if (!launch.tiles || a.splits < 2) return 0;
   return (size_t)a.splits * a.part_rows * (launch.head_dim + 2) * sizeof(float);
+}
+
+// The attention's launch, and that which joins the parts
+int attend_planned(Attend& a, const Launch& launch, const MxAttention* m, void* stream) {
+  const size_t bytes = workspace_of(a, launch);
+  if (bytes) {
+    if (!m->workspace || m->workspace_bytes < bytes || ((uintptr_t)m->workspace & 15)) return MX_ERR_WORKSPACE;
+    a.part = (float*)m->workspace;
+    a.part_ml = a.part + (size_t)a.splits * a.part_rows * launch.head_dim;
+  }
+  const int started = launch.head_dim == 32 ? attend32(a, launch, stream)
+                    : launch.head_dim == 64 ? attend64(a, launch, stream)
+                    : launch.head_dim == 96 ? attend96(a, launch, stream)
+                    : launch.head_dim == 128 ? attend128(a, launch, stream)
+                                             : attend256(a, launch, stream);
+  if (started || a.splits < 2) return started;
+  const int64_t rows = a.part_rows;
+  const bool one = rows >= kRowsForWaves && a.splits <= 64;
+  const dim3 grid((unsigned)(one ? (rows + 3) / 4 : rows));
+  const auto join = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    const auto go = [&](auto t, auto waves) {
+      hipLaunchKernelGGL((join_parts<decltype(t), D, decltype(waves)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    };
+    const auto by_rows = [&](auto t) {
+      if (one) go(t, std::integral_constant<int, 1>());
+      else go(t, std::integral_constant<int, 4>());
+    };
+    if (launch.type == MX_TYPE_BF16) by_rows((__bf16)0.f);
+    else by_rows((_Float16)0.f);
+  };
+  switch (launch.head_dim) {
+    case 32: join(std::integral_constant<int, 32>()); break;
+    case 64: join(std::integral_constant<int, 64>()); break;
+    case 96: join(std::integral_constant<int, 96>()); break;
+    case 128: join(std::integral_constant<int, 128>()); break;
+    default: join(std::integral_constant<int, 256>());
+  }
+  return (int)hipGetLastError();
 }
 
 }  // namespace mxe
@@ -490,42 +388,7 @@ int mx_episode_attend(const MxPages* pages, const MxChunk* chunk, const MxAttent
   mxe::Attend a{};
   mxe::Launch launch{};
   const int rc = mxe::plan(pages, chunk, m, a, launch, true);
-  if (rc || !launch.tiles) return rc;
-  const size_t bytes = mxe::workspace_of(a, launch);
-  if (bytes) {
-    if (!m->workspace || m->workspace_bytes < bytes || ((uintptr_t)m->workspace & 15)) return MX_ERR_WORKSPACE;
-    a.part = (float*)m->workspace;
-    a.part_ml = a.part + (size_t)a.splits * a.part_rows * launch.head_dim;
-  }
-  const int started = launch.head_dim == 32 ? mxe::attend32(a, launch, stream)
-                    : launch.head_dim == 64 ? mxe::attend64(a, launch, stream)
-                    : launch.head_dim == 96 ? mxe::attend96(a, launch, stream)
-                    : launch.head_dim == 128 ? mxe::attend128(a, launch, stream)
-                                             : mxe::attend256(a, launch, stream);
-  if (started || a.splits < 2) return started;
-  const int64_t rows = a.part_rows;
-  const bool one = rows >= mxe::kRowsForWaves && a.splits <= 64;
-  const dim3 grid((unsigned)(one ? (rows + 3) / 4 : rows));
-  const auto join = [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    const auto go = [&](auto t, auto waves) {
-      hipLaunchKernelGGL((mxe::join_parts<decltype(t), D, decltype(waves)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    };
-    const auto by_rows = [&](auto t) {
-      if (one) go(t, std::integral_constant<int, 1>());
-      else go(t, std::integral_constant<int, 4>());
-    };
-    if (launch.type == MX_TYPE_BF16) by_rows((__bf16)0.f);
-    else by_rows((_Float16)0.f);
-  };
-  switch (launch.head_dim) {
-    case 32: join(std::integral_constant<int, 32>()); break;
-    case 64: join(std::integral_constant<int, 64>()); break;
-    case 96: join(std::integral_constant<int, 96>()); break;
-    case 128: join(std::integral_constant<int, 128>()); break;
-    default: join(std::integral_constant<int, 256>());
-  }
-  return (int)hipGetLastError();
+  return rc || !launch.tiles ? rc : mxe::attend_planned(a, launch, m, stream);
 }
 
 }

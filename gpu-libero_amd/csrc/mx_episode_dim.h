@@ -10,6 +10,16 @@ template <int D, int kType, bool kFp8>
 int attend_typed(const Attend& a, const Launch& launch, void* stream) {
   const dim3 grid(launch.grid), block(256);
   const hipStream_t s = (hipStream_t)stream;
+  if (launch.listed) {
+    if (launch.blocks == 1) {
+      if (launch.team == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1, 1, true>), grid, dim3(64), 0, s, a);
+      else hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1, 4, true>), grid, block, 0, s, a);
+    } else if constexpr (kFp8) {
+      if (launch.team == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2, 1, true>), grid, dim3(64), 0, s, a);
+      else hipLaunchKernelGGL((attend_few<kType, kFp8, D, 2, 4, true>), grid, block, 0, s, a);
+    }
+    return (int)hipGetLastError();
+  }
   if (launch.rows == kManyRows) {
     if (a.page_shift >= 6) hipLaunchKernelGGL((attend_many<kType, kFp8, true, D>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((attend_many<kType, kFp8, false, D>), grid, block, 0, s, a);

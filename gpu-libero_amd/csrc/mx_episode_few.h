@@ -32,7 +32,9 @@ namespace mxe {
 // Waves of a SIMD to leave registers for
 constexpr int few_waves(int D, int blocks) { return blocks == 1 && D <= 64 ? 4 : blocks <= 2 && D <= 128 ? 2 : 1; }
 
-template <int kType, bool kFp8, int D, int kBlocks, int kTeam>
+// kListed: not over all keys of the world, but over those of the blocks that a token's list names (mx_episode_recall).  Keys
+// are then counted along the list; 16 of them lie in one block, and are where its number says.
+template <int kType, bool kFp8, int D, int kBlocks, int kTeam, bool kListed = false>
 __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(const Attend a) {
   typedef Elem<kType> E;
   typedef typename E::T T;
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
   block /= a.splits;
   const int head = block % a.kv_heads, tile = block / a.kv_heads;
   Tile t;
-  if (!find_tile(a, tile, kRows, t)) return;
+  if (!(kListed ? find_listed_tile(a, tile, kRows, t) : find_tile(a, tile, kRows, t))) return;
 
   // keys that any row of the tile sees, and keys that all its rows see
   const int last_row = min(t.row + kRows, t.rows) - 1;
@@ -65,7 +67,18 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
   limits(a, t, last_row / a.group, last_low, last_high);
   const int all_low = last_low, all_high = first_high;
   int begin, end;
-  split_range(a, split, first_low, last_high, begin, end);
+  Fixed* list = nullptr;
+  if constexpr (kListed) {
+    list = fixed(a.blocks + ((int64_t)(t.token + t.row / a.group) * a.kv_heads + head) * a.lists);
+    int named = 0;                                            // up to the last entry that names a block
+    for (int i = lane; i < a.lists; i += 64) named = list[i] >= 0 ? i + 1 : named;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) named = max(named, __shfl_xor(named, x));
+    named = __builtin_amdgcn_readfirstlane(named);
+    split_range(a, split, 0, last_high > 0 ? named << a.block_shift : 0, begin, end);
+  } else {
+    split_range(a, split, first_low, last_high, begin, end);
+  }
 
   // this lane's rows
   int low_r[kBlocks], high_r[kBlocks];
@@ -102,15 +115,24 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
   struct Keys {
     int64_t at;           // first key's element / D
     int left;             // keys up to `end`, less one (lanes beyond repeat the last)
+    int first;            // number of the first key in its world
     bool is;
   };
   auto locate = [&](int key) {
     Keys s;
-    const int from = min(key, (end - 1) & ~15);
-    const int page = table[from >> a.page_shift];
-    s.is = (unsigned)page < (unsigned)a.npage;
-    s.at = (((int64_t)(s.is ? page : 0) * a.kv_heads + head) << a.page_shift) + (from & page_mask);
+    int from = min(key, (end - 1) & ~15);
     s.left = end - 1 - from;
+    bool is = true;
+    if constexpr (kListed) {
+      const int block = list[from >> a.block_shift];
+      is = key < end && (unsigned)block < (unsigned)a.width << (a.page_shift - a.block_shift);
+      from = (is ? block << a.block_shift : 0) + (from & ((1 << a.block_shift) - 1));
+      is = is && from < last_high;
+    }
+    s.first = from;
+    const int page = table[from >> a.page_shift];
+    s.is = is && (unsigned)page < (unsigned)a.npage;
+    s.at = (((int64_t)(s.is ? page : 0) * a.kv_heads + head) << a.page_shift) + (from & page_mask);
     return s;
   };
 
@@ -167,6 +189,7 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
     // scores
     f4 s[kBlocks][2];
     const bool is0 = keys[0].is, is1 = keys[1].is;
+    const int at0 = kListed ? keys[0].first : key, at1 = kListed ? keys[1].first : key + 16;   // keys' numbers
 #pragma unroll
     for (int b = 0; b < kBlocks; b++) s[b][0] = s[b][1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -189,7 +212,8 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
       }
     }
     // values into LDS, those of keys that do not exist as zeros
-    const bool edge = key < all_low || key + 32 > all_high || key + 32 > end || !is0 || !is1;
+    const bool edge = kListed ? at0 + 16 > all_high || at1 + 16 > all_high || !is0 || !is1
+                              : key < all_low || key + 32 > all_high || key + 32 > end || !is0 || !is1;
     // an infinity or NaN among the values: taken out, and added after the loop to the rows that see it (a remainder of a
     // probability times an infinity is no remainder).  8-bit values have no infinity in bfloat16 but in blocks of
     // the largest scales (in float16 beyond 65504): there the steps that all rows see leave them in, to be found
@@ -208,7 +232,8 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
 #pragma unroll
       for (int e = 0; e < kVPer / 8; e++) {
         u4 words = __builtin_bit_cast(u4, v[e]);
-        if (edge && (key + key_in >= end || !(key_in < 16 ? is0 : is1))) words = u4{0, 0, 0, 0};
+        const bool beyond = kListed ? (key_in < 16 ? at0 + key_in : at1 + key_in - 16) >= last_high : key + key_in >= end;
+        if (edge && (beyond || !(key_in < 16 ? is0 : is1))) words = u4{0, 0, 0, 0};
         if (kTakeOut || edge) {
           unsigned off = 0;
 #pragma unroll
@@ -237,8 +262,8 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
         for (int u = 0; u < 2; u++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const int at = now + 16 * u + 4 * quarter + i;
-            if (!(at >= low_r[b] && at < high_r[b] && at < end && (u ? is1 : is0))) s[b][u][i] = -INFINITY;
+            const int at = (kListed ? (u ? at1 : at0) : now + 16 * u) + 4 * quarter + i;
+            if (!(at >= low_r[b] && at < high_r[b] && (kListed || at < end) && (u ? is1 : is0))) s[b][u][i] = -INFINITY;
           }
       }
       float sum;
@@ -329,7 +354,7 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
     for (int first = key; first < min(key + 32, end); first += 16) {     // 16 keys lie in one page
       const Keys at = locate(first);
       const uint8_t *from = a.v + at.at * (kFp8 ? D : 2 * D), *scale = a.v_scale + at.at * kC;
-      const int keys = min(16, end - first);
+      const int keys = min(16, kListed ? last_high - at.first : end - first);
       if (!at.is || !any_wild<E, kFp8>(from, scale, keys * (D / kVPer))) continue;
       for (int j = 0; j < keys; j++)
 #pragma unroll
@@ -337,7 +362,8 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
           const f4 x = values_at<E, kFp8>(from + j * (kFp8 ? D : 2 * D), scale + j * kC, 16 * c + 4 * quarter);
 #pragma unroll
           for (int b = 0; b < kBlocks; b++) {
-            const bool sees = first + j >= low_r[b] && first + j < high_r[b];
+            const int number = (kListed ? at.first : first) + j;
+            const bool sees = number >= low_r[b] && number < high_r[b];
 #pragma unroll
             for (int i = 0; i < 4; i++) o[b][c][i] += sees && !(fabsf(x[i]) < INFINITY) ? x[i] : 0.f;
           }

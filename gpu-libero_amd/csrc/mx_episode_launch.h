@@ -13,11 +13,24 @@ struct Launch {
   int type, head_dim, blocks, rows, tiles;    // blocks of 16 rows to a tile
   int team;                                   // waves of attend_few that share a tile
   int64_t keys;                               // the most that a world has, as far as the host knows
-  bool fp8;
+  bool fp8, listed;                           // listed: attention to listed blocks
   unsigned grid;
 };
 
-int choose(Attend& a, Launch& launch);
+// Checks and what a launch needs of an attention, all keys or (blocks, of 2^block_shift tokens) listed ones; its workspace;
+// and the launches (mx_episode.hip)
+int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, Launch& launch, bool pointers,
+         const MxSelection* s = nullptr, int block_shift = 0);
+size_t workspace_of(const Attend& a, const Launch& launch);
+int attend_planned(Attend& a, const Launch& launch, const MxAttention* m, void* stream);
+
+// Checks that all entry points share (mx_episode.hip)
+int size_of(int type);
+int pages_check(const MxPages* p);
+int chunk_check(const MxPages* p, const MxChunk* c);
+bool rows_aligned(const MxRows* r, int bytes);
+int rows_check(const MxRows* r, int heads, bool any);
+int page_shift(const MxPages* p);
 
 int attend32(const Attend& a, const Launch& launch, void* stream);
 int attend64(const Attend& a, const Launch& launch, void* stream);

@@ -123,6 +123,8 @@ struct Attend {
   float scale2;                      // |scale| * log2(e), not 0: probabilities are powers of two
   bool negate;                       // scale < 0: the queries change their sign
   bool q_vector, o_vector;           // q's rows are 16-byte aligned, out's 8-byte
+  const int32_t* blocks;             // of attention to listed blocks: (token, key head, entry), `lists` entries
+  int lists, block_shift;
 };
 
 // A kernel's only argument, read where it is used: as a by-value parameter all of it would be in scalar
@@ -182,6 +184,19 @@ struct Tile {
                                                    // in reach, position of the chunk's first token
 };
 
+// The last world whose rows begin at or before a packed row, by a search with 64 probes at a time
+__device__ inline int world_at(const int32_t* start, int nworld, int token) {
+  const int lane = threadIdx.x & 63;
+  int low = 0, high = nworld;
+  while (high - low > 1) {
+    const int step = (high - low + 63) >> 6, probe = low + lane * step;
+    const int passed = max(1, (int)__popcll(__ballot(probe < high && start[probe] <= token)));
+    low += (passed - 1) * step;
+    high = min(high, low + step);
+  }
+  return __builtin_amdgcn_readfirstlane(low);
+}
+
 __device__ inline long long tile_base(const Attend& a, int w, int rows_per_tile) {
   return (long long)a.start[w] * a.group / rows_per_tile + w;
 }
@@ -217,6 +232,32 @@ __device__ inline bool find_tile(const Attend& a, int tile, int rows_per_tile, T
   if (!a.start) t.rows = a.max_count * a.group;
   if (t.row >= t.rows) return false;
   t.token = token;
+  const int length = max(fixed(a.length)[t.world], 0);
+  t.position = length - count;
+  t.length = (int)min((long long)length, (long long)a.width << a.page_shift);
+  return true;
+}
+
+// The same for attention to listed blocks, where a tile has rows of one token alone: tokens by their packed row, each
+// with the tiles that its query heads need
+__device__ inline bool find_listed_tile(const Attend& a, int tile, int rows_per_tile, Tile& t) {
+  const int per = (a.group + rows_per_tile - 1) / rows_per_tile, token = tile / per;
+  int i, count;
+  if (!a.start) {
+    t.world = token / a.max_count;
+    i = token - t.world * a.max_count;
+    t.token = t.world * a.count;
+    count = a.count;
+  } else {
+    t.world = world_at(a.start, a.nworld, token);
+    t.token = fixed(a.start)[t.world];
+    const int stop = fixed(a.start)[t.world + 1];
+    i = token - t.token;
+    if (t.token < 0 || i < 0 || token >= min(stop, a.tokens) || i >= a.max_count) return false;
+    count = stop - t.token;
+  }
+  t.row = i * a.group + (tile - token * per) * rows_per_tile;
+  t.rows = (i + 1) * a.group;
   const int length = max(fixed(a.length)[t.world], 0);
   t.position = length - count;
   t.length = (int)min((long long)length, (long long)a.width << a.page_shift);

@@ -42,7 +42,11 @@ _PAGE_TOKENS = frozenset(1 << i for i in range(4, 13))
 STORAGE = {'bf16': torch.bfloat16, 'f16': torch.float16, 'fp8': torch.float8_e4m3fn}
 
 EXPORTS = ['mx_pages_bytes', 'mx_chunk_bytes', 'mx_rows_bytes', 'mx_attention_bytes', 'mx_episode_write',
-           'mx_episode_read', 'mx_episode_attend', 'mx_episode_workspace']
+           'mx_episode_read', 'mx_episode_attend', 'mx_episode_workspace',
+           'mx_rotary_bytes', 'mx_rotate', 'mx_episode_enter',
+           'mx_room_bytes', 'mx_room_change_bytes', 'mx_room_workspace', 'mx_room_update', 'mx_room_places',
+           'mx_summaries_bytes', 'mx_selection_bytes', 'mx_episode_summarise', 'mx_episode_select', 'mx_episode_recall',
+           'mx_recall_workspace']
 
 
 class MxPages(ct.Structure):
@@ -65,6 +69,28 @@ class MxAttention(ct.Structure):
                 ('window', ct.c_int32), ('scale', ct.c_float), ('longest', ct.c_int32)]
 
 
+class MxRotary(ct.Structure):
+    _fields_ = [('turn', ct.c_void_p), ('width', ct.c_int32), ('interleaved', ct.c_int32), ('amplitude', ct.c_float)]
+
+
+class MxRoom(ct.Structure):
+    _fields_ = ([(n, ct.c_void_p) for n in ('table', 'length', 'free', 'state')]
+                + [(n, ct.c_int32) for n in ('nworld', 'width', 'npage', 'page_tokens', 'tokens')])
+
+
+class MxRoomChange(ct.Structure):
+    _fields_ = [('count', ct.c_void_p), ('over', ct.c_void_p), ('start', ct.c_void_p), ('workspace', ct.c_void_p),
+                ('workspace_bytes', ct.c_size_t), ('each', ct.c_int32), ('rows', ct.c_int32)]
+
+
+class MxSummaries(ct.Structure):
+    _fields_ = [('codes', ct.c_void_p), ('exponent', ct.c_void_p), ('block_tokens', ct.c_int32)]
+
+
+class MxSelection(ct.Structure):
+    _fields_ = [('blocks', ct.c_void_p)] + [(n, ct.c_int32) for n in ('width', 'top', 'near', 'first', 'max_count', 'causal')]
+
+
 _LIB = None
 
 
@@ -73,7 +99,9 @@ def load():
     global _LIB
     if _LIB is None:
         lib = native.load()
-        for name, struct in (('pages', MxPages), ('chunk', MxChunk), ('rows', MxRows), ('attention', MxAttention)):
+        for name, struct in (('pages', MxPages), ('chunk', MxChunk), ('rows', MxRows), ('attention', MxAttention),
+                             ('rotary', MxRotary), ('room', MxRoom), ('room_change', MxRoomChange),
+                             ('summaries', MxSummaries), ('selection', MxSelection)):
             f = getattr(lib, 'mx_%s_bytes' % name)
             f.restype = ct.c_size_t
             if f() != ct.sizeof(struct):
@@ -82,6 +110,16 @@ def load():
         lib.mx_episode_attend.argtypes = [ct.c_void_p] * 4
         lib.mx_episode_workspace.argtypes = [ct.c_void_p] * 3
         lib.mx_episode_workspace.restype = ct.c_size_t
+        lib.mx_rotate.argtypes = [ct.c_void_p] * 3 + [ct.c_int32] * 2 + [ct.c_void_p] + [ct.c_int32] * 3 + [ct.c_void_p]
+        lib.mx_episode_enter.argtypes = [ct.c_void_p] * 8
+        lib.mx_room_workspace.argtypes = [ct.c_void_p]
+        lib.mx_room_update.argtypes = [ct.c_void_p] * 3
+        lib.mx_room_places.argtypes = [ct.c_void_p] * 6
+        lib.mx_episode_summarise.argtypes = [ct.c_void_p] * 4
+        lib.mx_episode_select.argtypes = [ct.c_void_p] * 6
+        lib.mx_episode_recall.argtypes = [ct.c_void_p] * 4 + [ct.c_int32, ct.c_void_p]
+        lib.mx_recall_workspace.argtypes = [ct.c_void_p] * 4 + [ct.c_int32]
+        lib.mx_room_workspace.restype = lib.mx_recall_workspace.restype = ct.c_size_t
         _LIB = lib
     return _LIB
 
@@ -225,6 +263,36 @@ def _there(call, pages, stream, tensors, *args, **options):
     return result
 
 
+def _on(device, stream, tensors, call):
+    """``call()`` on a device and a stream, as :func:`_there`."""
+    _require(stream is None or stream.device == device, 'stream must be on the tensors\' device')
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        result = call()
+        if stream is not None:
+            for x in tensors:
+                if x is not None:
+                    x.record_stream(stream)
+    return result
+
+
+def _overlap(a, b):
+    """Whether the memory from a tensor's first element to its last meets another's."""
+    if not a.numel() or not b.numel():
+        return False
+    first, second = a.data_ptr(), b.data_ptr()
+    reach = [x.element_size() * (1 + sum((n - 1) * step for n, step in zip(x.shape, x.stride()))) for x in (a, b)]
+    return first < second + reach[1] and second < first + reach[0]
+
+
+def _output(like, out, name='out'):
+    """``out`` for rows like ``like``: made here, or given and then checked."""
+    if out is None:
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    _require(out.shape == like.shape and out.dtype == like.dtype, '%s must have the rows\' shape and type', name)
+    _require(all(step or n < 2 for n, step in zip(like.shape, out.stride())), '%s has elements that share memory', name)
+    return out
+
+
 def write(pages, k, v, start=None, *, stream=None):
     """Store the chunk's keys and values (float32, bfloat16 or float16; any strides whose tokens step evenly
     and whose head_dim is contiguous).  8-bit pages take, per 32 values along head_dim, the least power of two
@@ -346,24 +414,12 @@ class Chunk:
         return (self.tokens,) if self.start is not None else (len(self.counts), self.count)
 
 
-class EpisodeCache:
-    """The episode memory of a batch of worlds, for a policy of ``layers`` attention layers.
-
-    ``tokens``: the most tokens of one world.  ``pages``: how many pages of ``page_tokens`` tokens all worlds
-    share (by default enough for every world at its longest; worlds in different phases of their episodes do
-    with about half).  ``storage``: 'fp8' (quantised, a scale per 32 values), 'bf16' or 'f16'.
-
-    Each step, :meth:`extend` makes room for the new tokens; then, layer by layer, :meth:`write` stores their keys and
-    values and :meth:`attend` attends from their queries.  :meth:`reset` empties worlds, as
-    ``HipBatchEnv.reset(id)`` restarts them.  Tables and lengths live on the device (``table``, ``length``), with a
-    copy on the host (``lengths``) that room is made by; pages are not cleared, their old contents are never read.
-
-    :meth:`extend` and :meth:`reset` work on the current stream.  Calls on another one (``stream=``, or the current one then)
-    wait for the last of them, and the next of them waits for those calls.  Calls among each other (:meth:`write` on one
-    stream, :meth:`attend` on another) and their tensors are the caller's to order, and so are replays of a graph."""
+class Layers:
+    """The pages of several layers, the worlds' tables and lengths, and the calls on them: what caches share whatever keeps
+    their books.  See :class:`EpisodeCache`."""
 
     def __init__(self, nworld, *, kv_heads, head_dim, tokens, layers=1, storage='fp8', page_tokens=64, pages=None,
-                 device='cuda:0'):
+                 device='cuda:0', block_tokens=None):
         _require(storage in STORAGE, 'storage must be one of %s, got %s', sorted(STORAGE), storage)
         _require(nworld > 0 and tokens > 0 and layers > 0 and kv_heads > 0, 'nworld, tokens, layers and kv_heads must be positive')
         _require(head_dim in HEAD_DIMS, 'head_dim must be one of %s, got %s', HEAD_DIMS, head_dim)
@@ -375,13 +431,9 @@ class EpisodeCache:
         device = torch.device(device)
         if device.type == 'cuda' and device.index is None:
             device = torch.device('cuda', torch.cuda.current_device())
-        self.nworld, self.tokens, self.page_tokens, self.device = nworld, int(tokens), page_tokens, device
+        self.nworld, self.tokens, self.page_tokens, self.device, self.pages = nworld, int(tokens), page_tokens, device, pages
         self.table = torch.full((nworld, width), -1, dtype=torch.int32, device=device)
         self.length = torch.zeros(nworld, dtype=torch.int32, device=device)
-        self.lengths = np.zeros(nworld, np.int64)
-        self._table = np.full((nworld, width), -1, np.int32)
-        self._free = np.arange(pages - 1, -1, -1, dtype=np.int32)     # a stack; its first _left are free
-        self._left = pages
         shape = (pages, kv_heads, page_tokens, head_dim)
         self.layers = []
         for _ in range(layers):
@@ -389,15 +441,15 @@ class EpisodeCache:
             scales = [torch.empty(shape[:3] + (head_dim // SCALE_BLOCK,), dtype=torch.uint8, device=device)
                       for _ in range(2 if storage == 'fp8' else 0)]
             self.layers.append(Pages(k, v, self.table, self.length, *scales))
+        self.summaries = None
+        if block_tokens is not None:
+            from . import recall
+            self.summaries = [recall.Summaries.make(x, block_tokens) for x in self.layers]
         # the stream of the last change and its handle; once calls come from others too, an event after that change and
         # after the last call of each
         self._home, self._handle, self._changed, self._used = None, 0, None, {}
         if device.type == 'cuda':
             self._change()
-
-    @property
-    def free_pages(self):
-        return self._left
 
     def _change(self):
         """Before table and length change: the current stream waits for the calls that read them elsewhere."""
@@ -442,6 +494,137 @@ class EpisodeCache:
         if ids.ndim != 1 or np.any((ids < 0) | (ids >= self.nworld)) or len(np.unique(ids)) != len(ids):
             raise ValueError('invalid world ids')
         return ids
+
+    @staticmethod
+    def _packed(chunk, x):
+        """Rows in the shape that the chunk's start wants."""
+        return x.flatten(0, 1) if chunk.start is not None and x.dim() == 4 else x
+
+    @staticmethod
+    def _bounds(chunk, stream, options, *names):
+        """What is known of the chunk, where replays of a captured call could not come with longer worlds, and larger
+        chunks."""
+        if getattr(chunk, 'bounded', False) or not _captured(stream):
+            if chunk.start is not None:
+                options.setdefault('max_count', chunk.count)
+            if 'longest' in names:
+                options.setdefault('longest', chunk.longest)
+
+    def _summarise(self, chunk, layer, stream):
+        if self.summaries is not None:
+            from . import recall
+            given = dict(count=chunk.count) if chunk.start is None else dict(tokens=chunk.tokens)
+            recall.summarise(self.summaries[layer], chunk.start, stream=stream, **given)
+
+    def write(self, chunk, k, v, layer=0, *, stream=None):
+        """:func:`write` of the chunk's keys and values to a layer, and the summaries of the blocks that they complete."""
+        other = self._enter(stream, chunk.start)
+        write(self.layers[layer], self._packed(chunk, k), self._packed(chunk, v), chunk.start, stream=stream)
+        self._summarise(chunk, layer, stream)
+        self._leave(other)
+
+    def enter(self, chunk, rotary, q, k, v, layer=0, *, out=None, stream=None):
+        """:func:`libero_hip.rotary.enter` of the chunk's rows to a layer, as :meth:`write`; returns the queries, turned."""
+        from . import rotary as operators
+        other = self._enter(stream, chunk.start)
+        given = None if out is None else self._packed(chunk, out)
+        _require(given is None or given.data_ptr() == out.data_ptr(), 'out: the rows of all worlds must step evenly')
+        turned = operators.enter(self.layers[layer], rotary, self._packed(chunk, q), self._packed(chunk, k), self._packed(chunk, v),
+                                 chunk.start, out=given, stream=stream)
+        self._summarise(chunk, layer, stream)
+        self._leave(other)
+        return turned.view(q.shape) if out is None else out
+
+    def attend(self, chunk, q, layer=0, **options):
+        """:func:`attend` from the chunk's queries to a layer; options as there.  ``max_count`` and ``longest`` are the chunk's
+        own, but not in a call that is captured: replays follow ``length`` and ``start``, whatever sizes they then have."""
+        stream = options.get('stream')
+        other = self._enter(stream, chunk.start)
+        self._bounds(chunk, stream, options, 'longest')
+        out = self._attended(chunk, q, options, lambda x: attend(self.layers[layer], x, chunk.start, **options))
+        self._leave(other)
+        return out
+
+    def recall(self, chunk, q, layer=0, *, top, near=1, first=0, **options):
+        """:func:`libero_hip.recall.select` of blocks for the chunk's queries and :func:`libero_hip.recall.recall` of them: attention
+        whose cost does not grow with the episode.  The cache has to be made with ``block_tokens``.  ``max_count`` as in
+        :meth:`attend`; ``scale`` must not be negative, as the blocks of the largest scores are chosen."""
+        from . import recall
+        _require(self.summaries is not None, 'the cache has no summaries: make it with block_tokens')
+        _require(options.get('scale') is None or options['scale'] >= 0, 'scale must not be negative, got %s', options.get('scale'))
+        stream = options.get('stream')
+        other = self._enter(stream, chunk.start)
+        self._bounds(chunk, stream, options)
+        both = {x: options[x] for x in ('causal', 'max_count', 'stream') if x in options}
+
+        def call(x):
+            blocks = recall.select(self.summaries[layer], x, chunk.start, top=top, near=near, first=first, **both)
+            return recall.recall(self.layers[layer], x, blocks, chunk.start, block_tokens=self.summaries[layer].block_tokens, **options)
+
+        out = self._attended(chunk, q, options, call)
+        self._leave(other)
+        return out
+
+    def _attended(self, chunk, q, options, call):
+        """A call with queries, ``out`` and ``lse`` in the shape that the chunk's start wants, and its result in q's."""
+        x = self._packed(chunk, q)
+        if x is q:
+            return call(q)
+        given = options.get('out')
+        for name in ('out', 'lse'):
+            if options.get(name) is not None:
+                y = options[name].flatten(0, 1)
+                _require(y.data_ptr() == options[name].data_ptr(), '%s: the rows of all worlds must step evenly', name)
+                options[name] = y
+        out = call(x)
+        return given if given is not None else out.view(q.shape)
+
+    def read(self, id=None, layer=0, *, dtype=torch.bfloat16, stream=None):
+        """The keys and values of the worlds ``id`` (all by default) as a layer stands for them, packed in the order of
+        the worlds, and the rows' starts (numpy, one more than ids): ``(k, v, starts)``."""
+        ids = np.sort(self._ids(id))
+        counts = np.zeros(self.nworld, np.int64)
+        counts[ids] = self.lengths[ids]
+        start = np.concatenate([[0], np.cumsum(counts)])
+        other = self._enter(stream)
+        k, v = read(self.layers[layer], torch.from_numpy(start.astype(np.int32)).to(self.device), tokens=int(start[-1]),
+                    dtype=dtype, stream=stream)
+        self._leave(other)
+        return k, v, np.concatenate([start[ids], start[-1:]])
+
+
+class EpisodeCache(Layers):
+    """The episode memory of a batch of worlds, for a policy of ``layers`` attention layers, with its books on the host
+    (:class:`libero_hip.room.DeviceEpisodeCache`: on the device).
+
+    ``tokens``: the most tokens of one world.  ``pages``: how many pages of ``page_tokens`` tokens all worlds
+    share (by default enough for every world at its longest; worlds in different phases of their episodes do
+    with about half).  ``storage``: 'fp8' (quantised, a scale per 32 values), 'bf16' or 'f16'.
+
+    ``block_tokens``: blocks of so many tokens are summarised as they are written, for :meth:`recall`.
+
+    Each step, :meth:`extend` makes room for the new tokens; then, layer by layer, :meth:`write` (with positions: :meth:`enter`) stores their keys and
+    values and :meth:`attend` (over long episodes: :meth:`recall`) attends from their queries.  :meth:`reset` empties worlds, as
+    ``HipBatchEnv.reset(id)`` restarts them.  Tables and lengths live on the device (``table``, ``length``), with a
+    copy on the host (``lengths``) that room is made by; pages are not cleared, their old contents are never read.
+
+    :meth:`extend` and :meth:`reset` work on the current stream.  Calls on another one (``stream=``, or the current one then)
+    wait for the last of them, and the next of them waits for those calls.  Calls among each other (:meth:`write` on one
+    stream, :meth:`attend` on another) and their tensors are the caller's to order, and so are replays of a graph."""
+
+    def __init__(self, nworld, *, kv_heads, head_dim, tokens, layers=1, storage='fp8', page_tokens=64, pages=None,
+                 device='cuda:0', block_tokens=None):
+        super().__init__(nworld, kv_heads=kv_heads, head_dim=head_dim, tokens=tokens, layers=layers, storage=storage,
+                         page_tokens=page_tokens, pages=pages, device=device, block_tokens=block_tokens)
+        pages, width = self.pages, self.table.shape[1]
+        self.lengths = np.zeros(nworld, np.int64)
+        self._table = np.full((nworld, width), -1, np.int32)
+        self._free = np.arange(pages - 1, -1, -1, dtype=np.int32)     # a stack; its first _left are free
+        self._left = pages
+
+    @property
+    def free_pages(self):
+        return self._left
 
     def extend(self, count=1, id=None):
         """Makes room for ``count`` (a number, or one for each world of ``id``) new tokens of the worlds ``id`` (all by
@@ -499,35 +682,3 @@ class EpisodeCache:
         self.table[where] = -1
         self.length[where] = 0
         self._change_done()
-
-    def write(self, chunk, k, v, layer=0, *, stream=None):
-        """:func:`write` of the chunk's keys and values to a layer."""
-        other = self._enter(stream, chunk.start)
-        write(self.layers[layer], k, v, chunk.start, stream=stream)
-        self._leave(other)
-
-    def attend(self, chunk, q, layer=0, **options):
-        """:func:`attend` from the chunk's queries to a layer; options as there.  ``max_count`` and ``longest`` are the chunk's
-        own, but not in a call that is captured: replays follow ``length`` and ``start``, whatever sizes they then have."""
-        stream = options.get('stream')
-        other = self._enter(stream, chunk.start)
-        if not _captured(stream):                             # replays may come with longer worlds, and larger chunks
-            if chunk.start is not None:
-                options.setdefault('max_count', chunk.count)
-            options.setdefault('longest', chunk.longest)
-        out = attend(self.layers[layer], q, chunk.start, **options)
-        self._leave(other)
-        return out
-
-    def read(self, id=None, layer=0, *, dtype=torch.bfloat16, stream=None):
-        """The keys and values of the worlds ``id`` (all by default) as a layer stands for them, packed in the order of
-        the worlds, and the rows' starts (numpy, one more than ids): ``(k, v, starts)``."""
-        ids = np.sort(self._ids(id))
-        counts = np.zeros(self.nworld, np.int64)
-        counts[ids] = self.lengths[ids]
-        start = np.concatenate([[0], np.cumsum(counts)])
-        other = self._enter(stream)
-        k, v = read(self.layers[layer], torch.from_numpy(start.astype(np.int32)).to(self.device), tokens=int(start[-1]),
-                    dtype=dtype, stream=stream)
-        self._leave(other)
-        return k, v, np.concatenate([start[ids], start[-1:]])

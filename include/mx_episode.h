@@ -109,6 +109,116 @@ int mx_episode_attend(const MxPages* pages, const MxChunk* chunk, const MxAttent
  * matter); 0 also for arguments that it refuses. */
 size_t mx_episode_workspace(const MxPages* pages, const MxChunk* chunk, const MxAttention* a);
 
+/* ---------------------------------------------------------------------------------------------- rotary positions
+ * A row at position p has the pairs of the first `width` values of each head turned by the angle p * turn[i], and
+ * multiplied by amplitude; the other values stay:
+ *     y_a = amplitude * (x_a cos - x_b sin),  y_b = amplitude * (x_a sin + x_b cos)
+ * Pair i is (i, i + width / 2), or with `interleaved` (2 i, 2 i + 1).  turn: width / 2 angles in radians, 64 bits, on the
+ * device.  The angle is reduced in 64 bits (off by 2^-52 of itself at most), sine, cosine and products are in 32 bits. */
+typedef struct MxRotary {
+  const double* turn;
+  int32_t width, interleaved;
+  float amplitude;
+} MxRotary;
+
+size_t mx_rotary_bytes(void);                /* sizeof(MxRotary) */
+
+/* Turn rows (F32, BF16 or F16; out of the same type) of head_dim values by positions[token % period], int32, or int64
+ * with `wide`; `back` turns by the negative angle, with the same amplitude: this is the gradient.  width is even, from 2 to
+ * head_dim, which is at most 1024.  x and out must not share memory. */
+int mx_rotate(const MxRotary* rotary, const MxRows* x, const MxRows* out, int32_t head_dim, int32_t tokens,
+              const void* positions, int32_t period, int32_t wide, int32_t back, void* stream);
+
+/* Turn the chunk's queries and keys by their rows' positions in their worlds (length[w] - n_w + i), the queries to `out`, the
+ * keys on into the pages, with the values beside them as mx_episode_write stores them; keys are rounded once, when they
+ * are stored.  All rows have one type.  Rows that belong to no world are left out, their places in `out` as they were. */
+int mx_episode_enter(const MxPages* pages, const MxChunk* chunk, const MxRotary* rotary, const MxRows* q, const MxRows* out,
+                     const MxRows* k, const MxRows* v, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- room for tokens
+ * The worlds' tables and lengths and the pages that none of them has: free[0 .. state[0]) is a stack of page numbers, of
+ * npage places.  state[1] collects what was refused (MX_ROOM_*); it is never cleared here.  A world has the pages of its
+ * first (length + page_tokens - 1) / page_tokens table entries and holds at most `tokens` tokens. */
+typedef struct MxRoom {
+  int32_t *table, *length, *free, *state;
+  int32_t nworld, width, npage, page_tokens, tokens;
+} MxRoom;
+
+#define MX_ROOM_TOKENS 1    /* a world would pass `tokens` (or the table), or fall below no token */
+#define MX_ROOM_PAGES  2    /* the free pages do not suffice */
+#define MX_ROOM_ROWS   4    /* more new rows than `rows` */
+
+/* A change of all worlds: those of `over` (nworld bytes, null: none) are emptied; then world w gets count[w] new tokens
+ * (count null: `each`), or gives back its last -count[w].  Pages come off the stack in the order of the worlds and their
+ * tokens, and go onto it in the opposite order, so that tokens taken back leave tables and stack as they were.
+ * If any world or the stack refuses, no world gets or gives back tokens, and state[1] says why; `over` is done all the
+ * same.  start (nworld + 1, null: not wanted) becomes the sums of the new tokens before each world (of a refused change,
+ * and for tokens given back, 0): the chunk to write and attend with.  rows: the most rows that the chunk may have.
+ * workspace: mx_room_workspace bytes, 16-byte aligned. */
+typedef struct MxRoomChange {
+  const int32_t* count;
+  const uint8_t* over;
+  int32_t* start;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t each, rows;
+} MxRoomChange;
+
+size_t mx_room_bytes(void);                  /* sizeof(MxRoom) */
+size_t mx_room_change_bytes(void);           /* sizeof(MxRoomChange) */
+size_t mx_room_workspace(const MxRoom* room);
+int mx_room_update(const MxRoom* room, const MxRoomChange* change, void* stream);
+
+/* World, position and slot (page * page_tokens + place in it) of each of the chunk's rows; -1, -1, -1 for rows that belong
+ * to no world, -1 as position for rows before the world's first token, and as slot for those without a place.  Of the
+ * room, table and length are read; free and state may be null. */
+int mx_room_places(const MxRoom* room, const MxChunk* chunk, int32_t* world, int32_t* position, int32_t* slot, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- recall
+ * Attention of a query to some blocks of block_tokens tokens (a power of two from 16 to page_tokens) of its world: the
+ * blocks whose summaries match it best, the latest ones, and the first ones.
+ *
+ * The summary of a block that is full is the mean m of its keys (in 64 bits): codes c = rint(m / 2^e), |c| <= 127, with
+ * the least e from -40 to 40 at which |m| is at most 127 * 2^e (codes beyond are cut off), and the byte e + 127; a block with a key that is
+ * not finite has the byte 255.  codes [npage][kv_heads][page_tokens / block_tokens][head_dim], 16-byte aligned, exponent without head_dim. */
+typedef struct MxSummaries {
+  int8_t* codes;
+  uint8_t* exponent;
+  int32_t block_tokens;
+} MxSummaries;
+
+/* What mx_episode_select chooses for each of the chunk's rows and key heads: of the world's blocks, those that begin at
+ * or before the last token that the query sees, the blocks [0, first); from the `near`-th block before the one behind the
+ * query's own on, all; and of those between the `top` with the largest scores, of equal ones the earlier.  The score of a block is
+ *     max over the query heads h of the key head of  (sum_d q_hd c_d) 2^(e_h + e),
+ * with q_h in codes of its own head by the rule above (a NaN counts as 0, an infinity as cut off): exact in 32 bits,
+ * the same on any machine.  The byte 255 stands above all scores, a table entry that names no page below.
+ * blocks: tokens x kv_heads x width, filled from the left in ascending order, then -1; all of it is written, -1 for rows that see nothing,
+ * belong to no world, or lie beyond max_count in it.  width is at least first + near + top, and more by
+ * (max_count + block_tokens - 2) / block_tokens where queries see tokens behind them (causal 0), and at most 4096; top at most 1024. */
+typedef struct MxSelection {
+  int32_t* blocks;
+  int32_t width, top, near, first, max_count, causal;
+} MxSelection;
+
+size_t mx_summaries_bytes(void);             /* sizeof(MxSummaries) */
+size_t mx_selection_bytes(void);             /* sizeof(MxSelection) */
+
+/* The summaries of the blocks that the chunk's tokens complete, from the keys in the pages. */
+int mx_episode_summarise(const MxPages* pages, const MxChunk* chunk, const MxSummaries* summaries, void* stream);
+
+int mx_episode_select(const MxPages* pages, const MxChunk* chunk, const MxSummaries* summaries, const MxRows* q,
+                      const MxSelection* selection, void* stream);
+
+/* mx_episode_attend over the keys of the listed blocks: s->blocks, s->width and block_tokens are read, the other numbers
+ * of s are not.  A block counts as often as it is listed; numbers that are no block of the world's table are left out.
+ * The probabilities are in two parts.  a->window must be 0. */
+int mx_episode_recall(const MxPages* pages, const MxChunk* chunk, const MxAttention* a, const MxSelection* s,
+                      int32_t block_tokens, void* stream);
+
+size_t mx_recall_workspace(const MxPages* pages, const MxChunk* chunk, const MxAttention* a, const MxSelection* s,
+                           int32_t block_tokens);
+
 #ifdef __cplusplus
 }
 #endif
