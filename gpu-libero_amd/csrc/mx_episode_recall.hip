@@ -145,12 +145,15 @@ struct Select {
   int64_t q_token, q_head;
   int nworld, npage, width, kv_heads, page_shift, block_shift, tokens, count, max_count, group;
   int lists, top, near, first;
-  int units;                     // rows times key heads
+  int units, tile;               // tiles of `tile` rows, times key heads
+  int pieces;                    // of 64 scores that a token has room for in LDS
   bool causal, q_vector;
 };
 
-constexpr int kRegisters = 8;    // scores of a lane, through LDS so that the loop over them is short
 constexpr int kMostTop = 1024;
+constexpr int kMostPieces = 32;  // of 64 scores: a wave has them in registers when it chooses
+constexpr int kMostTile = 4;     // tokens
+constexpr int kShare = 32;       // blocks that each wave of 16 may choose for the last to choose from
 
 __device__ inline unsigned sortable(float x) {
   const unsigned u = __float_as_uint(x);
@@ -166,13 +169,15 @@ template <int D> struct Queries {
   float scale[4];
 };
 
+// The rows from 16 * `part` on of `tokens` tokens times the group
 template <class T, int D>
-__device__ inline void load_queries(const Select& a, const T* rows, int tile, Queries<D>& q) {
-  const int lane = threadIdx.x & 63, n16 = lane & 15, quarter = lane >> 4, h = 16 * tile + n16;
+__device__ inline void load_queries(const Select& a, const T* rows, int tokens, int part, Queries<D>& q) {
+  const int lane = threadIdx.x & 63, n16 = lane & 15, quarter = lane >> 4, r = 16 * part + n16;
   constexpr int kValues = 16 * ((D + 63) / 64);
   float x[kValues];
-  const bool is = h < a.group;
-  const T* row = rows + (int64_t)(is ? h : 0) * a.q_head;
+  const bool is = r < tokens * a.group;
+  const int token = is ? r / a.group : 0, h = is ? r - token * a.group : 0;
+  const T* row = rows + (int64_t)token * a.q_token + (int64_t)h * a.q_head;
 #pragma unroll
   for (int i = 0; i < kValues; i += 8) {
     const int d = 64 * (i / 16) + 16 * quarter + i % 16;
@@ -207,182 +212,253 @@ __device__ inline void load_queries(const Select& a, const T* rows, int tile, Qu
   for (int i = 0; i < 4; i++) q.scale[i] = __shfl(scale, 4 * quarter + i);
 }
 
-// kTeam waves choose the blocks of a row and a key head (1: four such units to a workgroup).  They score 64 blocks at a time, by products of
-// 16 queries with 16 blocks, keep a score of each block, find the score of the last block chosen bit by
-// bit, counting with ballots, and write the blocks from there on in their order.  More blocks than registers hold
-// (only teams of 16) go in segments, the chosen ones of those before among the next.
-template <int kType, int D, int kTeam>
-__global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(const Select a) {
-  typedef typename Elem<kType>::T T;
-  constexpr int kSegment = 64 * kRegisters * kTeam, kParts = (D + 63) / 64;
-  constexpr bool kKeeps = kTeam == 16;
-  __shared__ unsigned scores[kTeam == 1 ? 4 : kTeam][kRegisters][64];
-  __shared__ int counts[2][kTeam], sh_above[2 * kTeam], sh_equal[2 * kTeam];
-  __shared__ unsigned kept_key[kKeeps ? kMostTop : 1];
-  __shared__ int kept_block[kKeeps ? kMostTop : 1];
-  const int wave = kTeam == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int team_wave = threadIdx.x >> 6, n16 = lane & 15, quarter = lane >> 4, thread = 64 * wave + lane;
-  const int unit = kTeam == 1 ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
-  if (unit >= a.units) return;
-  const int head = unit % a.kv_heads, token = unit / a.kv_heads;
-  int32_t* list = a.blocks + (int64_t)unit * a.lists;
-  const int world = a.start ? world_at(a.start, a.nworld, token) : token / a.count;
-  const int begin = a.start ? a.start[world] : world * a.count, count = a.start ? a.start[world + 1] - begin : a.count;
-  const int place = token - begin, length = max(a.length[world], 0), position = length - count + place;
-  const int reach = (int)min((long long)length, (long long)a.width << a.page_shift);
-  const bool is = begin >= 0 && place >= 0 && place < min(count, a.max_count) && position >= 0;
-  const int high = !is ? 0 : a.causal ? min(position + 1, reach) : reach;      // of the keys that are seen
-  const int blocks = (high + (1 << a.block_shift) - 1) >> a.block_shift;
-  const int near_from = min(max((is ? position >> a.block_shift : 0) - a.near + 1, 0), blocks);
-  const int from = min(a.first, near_from), candidates = near_from - from;
-  const int chosen = min(a.top, candidates);
-  // what is always listed, and what lies behind
-  for (int i = thread; i < a.lists; i += 64 * kTeam) {
-    if (i < from) list[i] = i;
-    else if (i >= from + chosen) list[i] = i - from - chosen < blocks - near_from ? near_from + i - from - chosen : -1;
-    else if (chosen == candidates) list[i] = i;
+// What a token may see: blocks up to `blocks`, of which those from near_from on and those before `from` are listed in any
+// case, and `chosen` of those between
+struct Seen {
+  int from, near_from, blocks, chosen;
+};
+
+__device__ inline Seen seen_by(const Select& a, bool is, int position, int reach) {
+  Seen s;
+  const int high = !is || position < 0 ? 0 : a.causal ? min(position + 1, reach) : reach;
+  s.blocks = (high + (1 << a.block_shift) - 1) >> a.block_shift;
+  s.near_from = min(max((max(position, 0) >> a.block_shift) - a.near + 1, 0), s.blocks);
+  s.from = min(a.first, s.near_from);
+  s.chosen = min(a.top, s.near_from - s.from);
+  return s;
+}
+
+// One wave: of `rows` rows of 64 keys (0: none) the `want` largest, of equal ones the first, in their order.  The first `kept`
+// are those of blocks chosen before, whose numbers are in kept_block; the others' follow from `base`.  The key of the last
+// one chosen is found bit by bit, counting with ballots, until as many as are wanted are above.
+template <int kRows, class Put>
+__device__ inline void choose_rows(const unsigned* keys, int rows, int want, Put put) {
+  const int lane = threadIdx.x & 63;
+  unsigned key[kRows];
+#pragma unroll
+  for (int j = 0; j < kRows; j++) key[j] = j < rows ? keys[64 * j + lane] : 0;
+  const auto count = [&](unsigned least) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kRows; j++) n += (int)__popcll(__ballot(key[j] >= least));
+    return n;
+  };
+  unsigned bound = 0;                              // keys above are chosen, and the first ones equal to it
+  int above = 0;
+  for (int bit = 31; bit >= 0; bit--) {
+    const unsigned trial = bound | 1u << bit;
+    const int n = count(trial);
+    if (n == want) {
+      bound = trial - 1;
+      above = n;
+      break;
+    }
+    if (n > want) bound = trial;
+    else above = n;                                // those with a larger key than `bound` may become
   }
-  if (chosen == candidates || !chosen) return;
+  const unsigned long long before = (1ull << lane) - 1;
+  int ties = want - above, at = 0;
+#pragma unroll
+  for (int j = 0; j < kRows; j++) {
+    if (j >= rows) break;
+    const unsigned long long x = __ballot(key[j] > bound), y = __ballot(key[j] == bound);
+    const int equal_before = (int)__popcll(y & before), taken = min((int)__popcll(y), ties);
+    if (key[j] > bound || (key[j] == bound && equal_before < ties))
+      put(at + (int)__popcll(x & before) + min(equal_before, ties), j, key[j]);
+    at += (int)__popcll(x) + taken;
+    ties -= taken;
+  }
+}
 
-  const T* rows = (const T*)a.q + (int64_t)token * a.q_token + (int64_t)head * a.group * a.q_head;
-  const int32_t* table = a.table + (int64_t)world * a.width;
-  const int per_shift = a.page_shift - a.block_shift, tiles = (a.group + 15) / 16;
-  Queries<D> q;
-  if (tiles == 1) load_queries<T, D>(a, rows, 0, q);
-  int kept = 0;
-  for (int segment = 0; segment < candidates; segment += kSegment) {
-    const int last = min(segment + kSegment, candidates);
-#pragma unroll 1
-    for (int j = 0; j < kRegisters; j++) {
-      const int base = segment + (wave * kRegisters + j) * 64;
-      if (base >= last) break;
-      i4 part[4][kParts];
-      int64_t entry[4];
-      bool there[4];
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const int block = from + min(base + 16 * t + n16, last - 1);
-        const int page = table[block >> per_shift];
-        there[t] = (unsigned)page < (unsigned)a.npage;
-        entry[t] = (((int64_t)(there[t] ? page : 0) * a.kv_heads + head) << per_shift) + (block & ((1 << per_shift) - 1));
-      }
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const int8_t* codes = a.codes + entry[t] * D;
-#pragma unroll
-        for (int c = 0; c < kParts; c++) {
-          const bool inside = 64 * c + 16 * quarter < D;
-          part[t][c] = *(const i4*)(codes + (inside ? 64 * c + 16 * quarter : 0));
-          if (!inside) part[t][c] = i4{0, 0, 0, 0};
-        }
-      }
-      // a lane's own block is that of its quarter's product
-      const int64_t mine = quarter == 0 ? entry[0] : quarter == 1 ? entry[1] : quarter == 2 ? entry[2] : entry[3];
-      const bool is_there = quarter == 0 ? there[0] : quarter == 1 ? there[1] : quarter == 2 ? there[2] : there[3];
-      const unsigned byte = a.exponent[mine];
-      float best = -INFINITY;
-      for (int tile = 0; tile < tiles; tile++) {
-        if (tiles > 1) load_queries<T, D>(a, rows, tile, q);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-          i4 sum = i4{0, 0, 0, 0};
-#pragma unroll
-          for (int c = 0; c < kParts; c++) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.codes[c], part[t][c], sum, 0, 0, 0);
-          float most = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 4; i++) most = q.scale[i] < 0.f ? most : fmaxf(most, (float)sum[i] * q.scale[i]);
-          most = fmaxf(most, __shfl_xor(most, 16));
-          most = fmaxf(most, __shfl_xor(most, 32));
-          best = t == quarter ? fmaxf(best, most) : best;
-        }
-      }
-      const float score = !is_there ? -INFINITY : byte == kNoNumber ? INFINITY : best * scale_of(byte);
-      scores[team_wave][j][lane] = base + lane < last ? sortable(score) : 0;
-    }
-    unsigned key[kRegisters];
-#pragma unroll
-    for (int j = 0; j < kRegisters; j++)        // a lane reads what it has written
-      key[j] = segment + (wave * kRegisters + j) * 64 < last ? scores[team_wave][j][lane] : 0;
-    unsigned old_key = 0;
-    int old_block = 0;
-    if constexpr (kKeeps) {
-      if (segment) __syncthreads();
-      if (thread < kept) {
-        old_key = kept_key[thread];
-        old_block = kept_block[thread];
-      }
-    }
-    const int want = min(a.top, last);            // of those seen so far
-
-    unsigned bound = 0;                           // the smallest key that is chosen
-    for (int bit = 31; bit >= 0; bit--) {
-      const unsigned trial = bound | 1u << bit;
-      int n = 0;
-#pragma unroll
-      for (int j = 0; j < kRegisters; j++) n += (int)__popcll(__ballot(key[j] >= trial));
-      if constexpr (kKeeps) n += (int)__popcll(__ballot(old_key >= trial));
-      if constexpr (kTeam > 1) {
-        if (lane == 0) counts[bit & 1][wave] = n;
-        __syncthreads();
-        n = 0;
-#pragma unroll
-        for (int w = 0; w < kTeam; w++) n += counts[bit & 1][w];
-      }
-      if (n >= want) bound = trial;
-    }
-    // how many are above it and equal to it: in the kept ones of each wave, then in the new ones
-    int above = 0, equal = 0;
-#pragma unroll
-    for (int j = 0; j < kRegisters; j++) {
-      above += (int)__popcll(__ballot(key[j] > bound));
-      equal += (int)__popcll(__ballot(key[j] == bound));
-    }
-    const unsigned long long old_above = kKeeps ? __ballot(old_key > bound) : 0;
-    const unsigned long long old_equal = kKeeps ? __ballot(old_key == bound && old_key) : 0;
-    int above_old = 0, equal_old = 0, above_new = 0, equal_new = 0, ties = want - above;
-    if constexpr (kTeam > 1) {
-      if (lane == 0) {
-        sh_above[wave] = (int)__popcll(old_above);
-        sh_equal[wave] = (int)__popcll(old_equal);
-        sh_above[kTeam + wave] = above;
-        sh_equal[kTeam + wave] = equal;
-      }
+// kTeam waves choose the blocks of up to kMostTile tokens of a world and a key head (1: four such units to a workgroup, of one token
+// each).  They score 64 blocks at a time for all of them, by products of 16 rows (tokens times query heads) with 16 summaries, into LDS; then a wave chooses for
+// each token.  More blocks than LDS has room for go in segments, the chosen ones of those before among the next.
+//
+// What bounds it: for a step's tokens a chain of loads that depend on each other (length, table, summaries), for prompts the
+// products and the counting.
+template <int kType, int D, int kTeam>
+__global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(const Select) {
+  // read where they are used: as a parameter they would be in scalar registers throughout, and those of the loops spilled
+  const Select& a = *(const Select*)(__attribute__((address_space(4))) const Select*)__builtin_amdgcn_kernarg_segment_ptr();
+  typedef typename Elem<kType>::T T;
+  constexpr int kParts = (D + 63) / 64, kTile = kTeam == 4 ? kMostTile : 1;
+  extern __shared__ unsigned scores[];            // [token][64 * pieces], then, where there are segments, the kept
+                                                  // blocks' numbers [token][kMostTop]
+  const int wave = kTeam == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n16 = lane & 15, quarter = lane >> 4;
+  const int team = kTeam == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int unit = kTeam == 1 ? blockIdx.x * 4 + team : blockIdx.x;
+  if (unit >= a.units) return;
+  const int head = unit % a.kv_heads, tile = unit / a.kv_heads, room = 64 * a.pieces;
+  unsigned* mine = scores + team * room;
+  int* kept_block = (int*)(scores + (kTeam == 1 ? 4 : a.tile) * room) + team * kMostTop;
+  const auto meet = [] {
+    if constexpr (kTeam == 1) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
       __syncthreads();
-      int all = 0;
-      for (int w = 0; w < 2 * kTeam; w++) {
-        const int x = sh_above[w], y = sh_equal[w];
-        all += x;
-        above_old += w < wave ? x : 0;
-        equal_old += w < wave ? y : 0;
-        above_new += w < kTeam + wave ? x : 0;
-        equal_new += w < kTeam + wave ? y : 0;
-      }
-      ties = want - all;
     }
-    const bool done = last == candidates;
-    const unsigned long long before = (1ull << lane) - 1;
-    const auto put = [&](bool above_it, bool equal_to_it, int above_before, int equal_before, unsigned value, int block) {
-      if (!(above_it || (equal_to_it && equal_before < ties))) return;
-      const int at = above_before + min(equal_before, ties);
-      if (done) {
-        if (from + at < a.lists) list[from + at] = block;
-      } else if constexpr (kKeeps) {
-        kept_key[at] = value;
-        kept_block[at] = block;
-      }
-    };
-    if constexpr (kKeeps)
-      put(old_key > bound, old_key == bound && old_key, above_old + (int)__popcll(old_above & before),
-          equal_old + (int)__popcll(old_equal & before), old_key, old_block);
+  };
+  // the tile's rows, those of one world at a time
+  const int tile_end = min((tile + 1) * a.tile, a.tokens);
+  for (int token = tile * a.tile, next; token < tile_end; token = next) {
+    const int world = a.start ? world_at(a.start, a.nworld, token) : token / a.count;
+    const int begin = a.start ? a.start[world] : world * a.count, stop = a.start ? a.start[world + 1] : begin + a.count;
+    const bool is = begin >= 0 && token >= begin && token < stop;
+    next = is ? min(stop, tile_end) : token + 1;
+    const int tokens = next - token, count = stop - begin, length = max(a.length[world], 0);
+    const int position = length - count + token - begin;
+    const int reach = (int)min((long long)length, (long long)a.width << a.page_shift);
+    int from[kTile], near_from[kTile];             // of each token
+    int low = INT32_MAX, high = 0;                 // of the blocks between which to choose
 #pragma unroll
-    for (int j = 0; j < kRegisters; j++) {
-      const unsigned long long x = __ballot(key[j] > bound), y = __ballot(key[j] == bound);
-      put(key[j] > bound, key[j] == bound, above_new + (int)__popcll(x & before), equal_new + (int)__popcll(y & before), key[j],
-          from + segment + (wave * kRegisters + j) * 64 + lane);
-      above_new += (int)__popcll(x);
-      equal_new += (int)__popcll(y);
+    for (int t = 0; t < kTile; t++) {
+      const Seen s = seen_by(a, is && t < tokens && token + t - begin < a.max_count, position + t, reach);
+      from[t] = s.from;
+      near_from[t] = s.near_from;
+      if (t >= tokens) continue;
+      // what is listed in any case, and what lies behind
+      int32_t* list = a.blocks + ((int64_t)(token + t) * a.kv_heads + head) * a.lists;
+      const bool all = s.chosen == s.near_from - s.from;
+      for (int i = 64 * wave + lane; i < a.lists; i += 64 * kTeam) {
+        if (i < s.from || (all && i < s.from + s.chosen)) list[i] = i;
+        else if (i >= s.from + s.chosen) list[i] = i - s.from - s.chosen < s.blocks - s.near_from ? s.near_from + i - s.from - s.chosen : -1;
+      }
+      if (all || !s.chosen) continue;
+      low = min(low, s.from);
+      high = max(high, s.near_from);
     }
-    kept = want;
+    if (low >= high) continue;
+    const int my_from = quarter == 0 ? from[0] : quarter == 1 ? from[kTile > 1] : quarter == 2 ? from[kTile / 2] : from[kTile - 1];
+    const int my_near_from = quarter == 0 ? near_from[0] : quarter == 1 ? near_from[kTile > 1] : quarter == 2 ? near_from[kTile / 2]
+                                                                                            : near_from[kTile - 1];
+
+    const T* rows = (const T*)a.q + (int64_t)token * a.q_token + (int64_t)head * a.group * a.q_head;
+    const int32_t* table = a.table + (int64_t)world * a.width;
+    const int per_shift = a.page_shift - a.block_shift, parts = (tokens * a.group + 15) / 16;
+    Queries<D> q;
+    if (parts == 1) load_queries<T, D>(a, rows, tokens, 0, q);
+    int kept = 0;
+    for (int segment = low; segment < high;) {
+      const bool segment_before = segment > low;
+      const int kept_rows = (kept + 63) >> 6, last = min(segment + 64 * (a.pieces - kept_rows), high);
+      const int rows_new = (last - segment + 63) >> 6;
+      // few of many: each wave chooses from neighbouring rows of its own first, so that one wave is left with a share of all
+      // (32 of 2048 blocks 26 -> 19 us)
+      const bool shared = kTeam == 16 && !segment_before && last == high && a.top <= kShare;
+      const int each = (rows_new + kTeam - 1) / kTeam;
+      // one piece at a time: with the next one's summaries under way a wave has half as many beside it (two pieces of 64
+      // values 15.5 -> 22.5 us)
+#pragma unroll 1
+      for (int row = shared ? wave * each : wave; row < (shared ? min((wave + 1) * each, rows_new) : rows_new); row += shared ? 1 : kTeam) {
+        const int base = segment + 64 * row;
+        i4 part[4][kParts];
+        unsigned byte[4];
+        bool there[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int block = min(base + 16 * u + n16, last - 1), page = table[block >> per_shift];
+          there[u] = (unsigned)page < (unsigned)a.npage;
+          const int64_t entry = (((int64_t)(there[u] ? page : 0) * a.kv_heads + head) << per_shift) + (block & ((1 << per_shift) - 1));
+          const int8_t* codes = a.codes + entry * D;
+#pragma unroll
+          for (int c = 0; c < kParts; c++) {
+            const bool inside = 64 * c + 16 * quarter < D;
+            part[u][c] = *(const i4*)(codes + (inside ? 64 * c + 16 * quarter : 0));
+            if (!inside) part[u][c] = i4{0, 0, 0, 0};
+          }
+          byte[u] = a.exponent[entry];
+        }
+        float best[4];                             // of the first token, where it has more rows than one product
+#pragma unroll
+        for (int u = 0; u < 4; u++) best[u] = -INFINITY;
+        for (int p = 0; p < parts; p++) {
+          if (parts > 1) load_queries<T, D>(a, rows, tokens, p, q);
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            i4 sum = i4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < kParts; c++) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.codes[c], part[u][c], sum, 0, 0, 0);
+            float row[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) row[i] = q.scale[i] < 0.f ? -INFINITY : (float)sum[i] * q.scale[i];
+            const int at = base + 16 * u + n16;
+            const auto store = [&](int from, int near_from, int t, float most) {
+              const float score = !there[u] ? -INFINITY : byte[u] == kNoNumber ? INFINITY : most * scale_of(byte[u]);
+              mine[t * room + 64 * kept_rows + at - segment] = at < last && at >= from && at < near_from ? sortable(score) : 0;
+            };
+            if (kTile > 1 && a.group == 4) {       // a quarter of the lanes has a token's rows
+              if (quarter < tokens) store(my_from, my_near_from, quarter, fmaxf(fmaxf(row[0], row[1]), fmaxf(row[2], row[3])));
+            } else {
+#pragma unroll
+              for (int t = 0; t < kTile; t++) {
+                if (t >= tokens) continue;
+                float most = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  const int r = 4 * quarter + i;
+                  most = fmaxf(most, tokens == 1 || (r >= t * a.group && r < (t + 1) * a.group) ? row[i] : -INFINITY);
+                }
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                if (parts > 1) most = best[u] = fmaxf(best[u], most);
+                if (quarter == 0 && p == parts - 1) store(from[t], near_from[t], t, most);
+              }
+            }
+          }
+        }
+      }
+      unsigned* share = scores + room;             // (only teams of 16, which have one token)
+      int* share_block = (int*)(share + kTeam * kShare);
+      if (shared) {
+        unsigned* keys = mine + 64 * wave * each;
+        const int own = max(min(each, rows_new - wave * each), 0);
+        if (lane < kShare) share[kShare * wave + lane] = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (own)
+          choose_rows<2>(keys, own, a.top, [&](int at, int j, unsigned key) {
+            share[kShare * wave + at] = key;
+            share_block[kShare * wave + at] = segment + 64 * (wave * each + j) + lane;
+          });
+      }
+      meet();
+      const bool done = last == high;
+      const int t = kTile > 1 ? wave : 0;          // a wave's own token
+      const Seen s = seen_by(a, is && t < tokens && token + t - begin < a.max_count, position + t, reach);
+      if (t < tokens && (kTile > 1 || wave == 0) && s.chosen && s.chosen < s.near_from - s.from) {
+        unsigned* keys = mine + t * room;
+        int* held = kept_block + t * kMostTop;
+        int32_t* list = a.blocks + ((int64_t)(token + t) * a.kv_heads + head) * a.lists + s.from;
+        const int listed = a.lists - s.from, used = kept_rows + (last - segment + 63) / 64;
+        const auto put = [&](int at, int j, unsigned key) {
+          const int block = shared ? share_block[64 * j + lane] : j < kept_rows ? held[64 * j + lane]
+                                                                               : segment + 64 * (j - kept_rows) + lane;
+          if (done) {
+            if (at < listed) list[at] = block;
+          } else {
+            keys[at] = key;
+            held[at] = block;
+          }
+        };
+        // a segment may not have as many yet as are wanted: keys of 0 are chosen then, and are no blocks' in the next
+        if (shared) choose_rows<(kTeam * kShare + 63) / 64>(share, kTeam * kShare / 64, s.chosen, put);
+        else if (used <= 2) choose_rows<2>(keys, used, s.chosen, put);
+        else if (used <= 8) choose_rows<8>(keys, used, s.chosen, put);
+        else if (used <= 16) choose_rows<16>(keys, used, s.chosen, put);
+        else choose_rows<kMostPieces>(keys, used, s.chosen, put);
+      }
+      segment = last;
+      kept = a.top;
+      if (!done) {
+        meet();
+        // behind the kept ones of a row nothing
+        for (int t = 0; t < min(tokens, kTile); t++)
+          for (int i = kept + 64 * wave + lane; i < ((kept + 63) & ~63); i += 64 * kTeam) mine[t * room + i] = 0;
+      }
+    }
+    meet();                                        // before the next world's scores
   }
 }
 
@@ -403,19 +479,16 @@ template <int D> void launch_summarise(const Summarise& a, int type, unsigned gr
   else go(std::integral_constant<int, MX_TYPE_F16>());
 }
 
-// Waves of a team, by the blocks that a world's table has room for
-int team_of(int64_t blocks) { return blocks <= 64 * kRegisters ? 1 : blocks <= 256 * kRegisters ? 4 : 16; }
-
-template <int D> void launch_select(const Select& a, int type, int team, unsigned groups, void* stream) {
+template <int D> void launch_select(const Select& a, int type, int team, unsigned groups, size_t lds, void* stream) {
   const auto go = [&](auto t, auto n) {
     constexpr int kTeam = decltype(n)::value;
-    hipLaunchKernelGGL((select_blocks<decltype(t)::value, D, kTeam>), dim3(groups), dim3(kTeam == 1 ? 256 : 64 * kTeam), 0,
+    hipLaunchKernelGGL((select_blocks<decltype(t)::value, D, kTeam>), dim3(groups), dim3(kTeam == 1 ? 256 : 64 * kTeam), lds,
                        (hipStream_t)stream, a);
   };
   const auto by_team = [&](auto t) {
     if (team == 1) go(t, std::integral_constant<int, 1>());
     else if (team == 4) go(t, std::integral_constant<int, 4>());
-    else go(t, std::integral_constant<int, 16>());
+    else if constexpr (D <= 128) go(t, std::integral_constant<int, 16>());
   };
   if (type == MX_TYPE_BF16) by_team(std::integral_constant<int, MX_TYPE_BF16>());
   else by_team(std::integral_constant<int, MX_TYPE_F16>());
@@ -492,13 +565,20 @@ int mx_episode_select(const MxPages* p, const MxChunk* c, const MxSummaries* s, 
   a.lists = m->width; a.top = m->top; a.near = m->near; a.first = m->first;
   a.causal = m->causal != 0;
   a.q_vector = rows_aligned(q, 16);
-  const int64_t units = (int64_t)c->tokens * p->kv_heads;
-  const int team = team_of((int64_t)p->width << (a.page_shift - a.block_shift));
+  // tokens side by side where worlds have many, so that they share the summaries' loads
+  const int64_t pieces = (((int64_t)p->width << (a.page_shift - a.block_shift)) + 63) / 64;
+  const int side = a.group > 8 ? 1 : 16 / a.group < kMostTile ? 16 / a.group : kMostTile;
+  a.tile = c->tokens >= (int64_t)2 * side * p->nworld ? side : 1;
+  a.pieces = (int)(pieces < kMostPieces ? pieces : kMostPieces);
+  const int64_t units = ((int64_t)c->tokens + a.tile - 1) / a.tile * p->kv_heads;
+  const int team = a.tile > 1 ? 4 : pieces <= 2 || units >= 4096 ? 1 : pieces < 16 || units >= 512 || p->head_dim > 128 ? 4 : 16;
   const int64_t groups = team == 1 ? (units + 3) / 4 : units;
   // threads are counted in 32 bits
   if (groups > (team == 16 ? kMostGroups / 4 : kMostGroups)) return MX_ERR_DOMAIN;
   a.units = (int)units;
-  by_head_dim(p->head_dim, [&](auto d) { launch_select<decltype(d)::value>(a, q->type, team, (unsigned)groups, stream); });
+  const size_t lds = sizeof(int) * (team == 1 ? 4 : a.tile) * (64 * a.pieces + (pieces > kMostPieces ? kMostTop : 0))
+                     + (team == 16 ? sizeof(int) * 2 * 16 * kShare : 0);
+  by_head_dim(p->head_dim, [&](auto d) { launch_select<decltype(d)::value>(a, q->type, team, (unsigned)groups, lds, stream); });
   return (int)hipGetLastError();
 }
 

@@ -2,9 +2,10 @@
 // their worlds, positions and slots.
 //
 // Where a world's pages come off the stack follows from the needs of all worlds before it, and whether they do at all from
-// everyone's.  There are few numbers to a world, so each workgroup reads all of them again for its prefix and the totals
-// instead of waiting for its neighbours; lengths then change in a second launch, which also hands out the pages that the
-// first has put on the stack.  Both are bound by their launches and by a few dependent loads.
+// everyone's.  One workgroup does all for up to 1024 worlds with few pages.  For more there are two launches: there are few
+// numbers to a world, so each workgroup reads all of them again for its prefix and the totals instead of waiting for its
+// neighbours; lengths then change in the second launch, which also hands out the pages that the first has put on the stack.
+// Bound by launches and by a few dependent loads.
 #include "mx_episode_move.h"
 #include "mx_episode_launch.h"
 
@@ -26,43 +27,57 @@ struct Change {
   bool refused;
 };
 
-__device__ inline Change change_of(const Room& a, int w) {
+__device__ inline Change change_of(const Room& a, int has, int by, bool over) {
   Change c;
-  const int pages = (1 << a.page_shift) - 1;
-  const long long reach = (long long)a.width << a.page_shift;
-  const int length = (int)min((long long)max(a.length[w], 0), reach);
-  c.base = a.over && a.over[w] ? 0 : length;
-  const int by = a.count ? a.count[w] : a.each;
-  const long long after = (long long)c.base + by;
-  c.refused = after < 0 || (by > 0 && after > min((long long)a.tokens, reach));
+  const int pages = (1 << a.page_shift) - 1, reach = a.width << a.page_shift;      // at most 2^30
+  const int length = min(max(has, 0), reach);
+  c.base = over ? 0 : length;
+  const unsigned after = (unsigned)c.base + (unsigned)by;                          // of no fewer than 0: below 2^32
+  c.refused = by < -c.base || (by > 0 && after > (unsigned)min(a.tokens, reach));
   c.after = c.refused ? c.base : (int)after;
-  c.held = (int)(((long long)length + pages) >> a.page_shift);
+  c.held = (length + pages) >> a.page_shift;
   c.kept = (min(c.base, c.after) + pages) >> a.page_shift;
   c.need = (c.after + pages) >> a.page_shift;
   c.rows = max(by, 0);
   return c;
 }
 
-// Sums over a workgroup of 256: those before the thread's and all of them
-template <class T> __device__ inline T sums_before(T x, T* sh, T& all) {
+__device__ inline Change change_of(const Room& a, int w) {
+  return change_of(a, a.length[w], a.count ? a.count[w] : a.each, a.over && a.over[w]);
+}
+
+// Sums over a workgroup of kMany values to a thread: those before the thread's, in place, and all of them
+template <int kThreads, int kMany>
+__device__ inline void sums_before(long long (&x)[kMany], long long (&sh)[kThreads / 64][kMany], long long (&all)[kMany]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T sum = x;
+  long long sum[kMany];
 #pragma unroll
-  for (int by = 1; by < 64; by *= 2) {
-    const T y = __shfl_up(sum, by);
-    if (lane >= by) sum += y;
-  }
-  if (lane == 63) sh[wave] = sum;
-  __syncthreads();
-  T before = sum - x;
-  all = 0;
+  for (int i = 0; i < kMany; i++) sum[i] = x[i];
 #pragma unroll
-  for (int w = 0; w < 4; w++) {
-    if (w < wave) before += sh[w];
-    all += sh[w];
-  }
+  for (int by = 1; by < 64; by *= 2)
+#pragma unroll
+    for (int i = 0; i < kMany; i++) {
+      const long long y = __shfl_up(sum[i], by);
+      if (lane >= by) sum[i] += y;
+    }
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < kMany; i++) sh[wave][i] = sum[i];
   __syncthreads();
-  return before;
+#pragma unroll
+  for (int i = 0; i < kMany; i++) {
+    x[i] = sum[i] - x[i];
+    all[i] = 0;
+  }
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; w++)
+#pragma unroll
+    for (int i = 0; i < kMany; i++) {
+      const long long y = sh[w][i];
+      x[i] += w < wave ? y : 0;
+      all[i] += y;
+    }
+  __syncthreads();
 }
 
 // Which of a workgroup's worlds a piece of work belongs to: the last w with before[w] <= i
@@ -75,114 +90,188 @@ __device__ inline int owner(const long long* before, int worlds, long long i) {
   return low;
 }
 
+// Why a change is refused, from the sums over all worlds
+__device__ inline int why_not(const Room& a, bool refused, long long left, long long back, long long need, long long rows) {
+  return (refused ? MX_ROOM_TOKENS : 0) | (need > min(left + back, (long long)a.npage) ? MX_ROOM_PAGES : 0)
+         | (rows > a.rows ? MX_ROOM_ROWS : 0);
+}
+
+// Of a world in a refused change only what has to go, goes
+__device__ inline void refuse(Change& c, bool over) {
+  c.after = c.base;
+  c.kept = over ? 0 : c.held;
+  c.need = c.kept;
+}
+
+// Pieces of work, `many` of them, that belong to a workgroup's worlds from before[o] on: their table entries count on from
+// from[o], and are moved in turn
+template <int kThreads, class Move>
+__device__ inline void each_entry(const Room& a, int first, int worlds, const long long* before, const int* from, long long many, Move move) {
+  for (long long i = threadIdx.x; i < many; i += kThreads) {
+    const int o = owner(before, worlds, i);
+    const long long slot = from[o] + i - before[o];
+    if (slot < a.width) move(a.table + (int64_t)(first + o) * a.width + slot, i);
+  }
+}
+
+// One workgroup, a world to a thread
+constexpr int kAlone = 1024;
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void update_alone(const Room a) {
+  __shared__ long long sh[kThreads / 64][4], before[kThreads];
+  __shared__ int from[kThreads];
+  const int w = threadIdx.x;
+  const bool mine = w < a.nworld, over = mine && a.over && a.over[w];
+  const long long left = min(max(a.state[0], 0), a.npage);
+  Change c{};
+  if (mine) c = change_of(a, w);
+  // pages back (of emptied worlds alone, and all), pages needed, rows
+  long long x[4] = {over ? c.held : 0, c.held - min(c.kept, c.held), c.need - c.kept, c.rows}, all[4];
+  sums_before<kThreads, 4>(x, sh, all);
+  const int why = why_not(a, __syncthreads_or(c.refused), left, all[1], all[2], all[3]);
+  if (why) refuse(c, over);
+  const long long back = why ? all[0] : all[1];
+  before[w] = why ? x[0] : x[1];
+  from[w] = min(c.kept, c.held);
+  if (a.start && mine) {
+    a.start[w] = why ? 0 : (int)x[3];
+    if (w == a.nworld - 1) a.start[a.nworld] = why ? 0 : (int)all[3];
+  }
+  const long long top = min(left + back, (long long)a.npage);
+  if (back) {                                     // the first page that comes back lies highest on the stack
+    __syncthreads();
+    each_entry<kThreads>(a, 0, a.nworld, before, from, back, [&](int32_t* entry, long long i) {
+      const long long at = left + back - 1 - i;
+      if (at >= 0 && at < a.npage) a.free[at] = *entry;
+      *entry = -1;
+    });
+    __syncthreads();
+  }
+  if (!why && all[2]) {
+    before[w] = x[2];
+    __syncthreads();
+    each_entry<kThreads>(a, 0, a.nworld, before, from, all[2], [&](int32_t* entry, long long i) {
+      if (top - 1 - i >= 0) *entry = a.free[top - 1 - i];
+    });
+  }
+  if (mine) a.length[w] = c.after;
+  if (w == 0) {
+    a.state[0] = (int)(why ? top : top - all[2]);
+    if (why) a.state[1] |= why;
+  }
+}
+
 constexpr int kMostWorlds = 256;                // of a workgroup
 
-// Totals, the pages that come back, and the rows' starts.  Whether tokens are refused decides which pages come back: those of
-// emptied worlds always, those of tokens given back only then.
+// Totals, the pages that come back, and the rows' starts
 __global__ __launch_bounds__(256) void update_count(const Room a) {
-  __shared__ long long sh[4], before[kMostWorlds];
-  __shared__ int from[kMostWorlds];
+  __shared__ long long sums[4][2], sh[4][2], before[kMostWorlds];
+  __shared__ int from[kMostWorlds], parts[4][6];
   const int first = blockIdx.x * a.worlds_each, worlds = min(a.nworld - first, a.worlds_each);
-  // sums over all worlds, and over those before this workgroup's: pages back (without and with tokens given back), pages
-  // needed, rows
-  long long all_over = 0, all_back = 0, all_need = 0, all_rows = 0, my_over = 0, my_back = 0, my_need = 0, my_rows = 0;
-  int refused = 0;
-  for (int w = threadIdx.x; w < a.nworld; w += 256) {
-    const Change c = change_of(a, w);
-    const int over = a.over && a.over[w] ? c.held : 0, back = c.held - min(c.kept, c.held), need = c.need - c.kept;
-    refused |= c.refused;
-    all_over += over;
-    all_back += back;
-    all_need += need;
-    all_rows += c.rows;
-    if (w < first) {
-      my_over += over;
-      my_back += back;
-      my_need += need;
-      my_rows += c.rows;
+  // sums over all worlds: pages needed and rows, in 64 bits as there may be any number of them; pages back (of emptied worlds alone,
+  // and all); and over those before this workgroup's: pages back, needed, and rows, which are right if the change is not
+  // refused
+  long long wide[2] = {0, 0};
+  int x[6] = {0, 0, 0, 0, 0, 0}, refused = 0;
+  constexpr int kAhead = 8;                       // worlds of a thread whose numbers are under way together
+  for (int base = threadIdx.x; base < a.nworld; base += kAhead * 256) {
+    int length[kAhead], count[kAhead];
+    bool over[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      const int w = base + u * 256;
+      const bool is = w < a.nworld;
+      length[u] = is ? a.length[w] : 0;
+      count[u] = !is ? 0 : a.count ? a.count[w] : a.each;
+      over[u] = is && a.over && a.over[w];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      const Change c = change_of(a, length[u], count[u], over[u]);
+      const int gone = over[u] ? c.held : 0, back = c.held - min(c.kept, c.held), need = c.need - c.kept;
+      const bool earlier = base + u * 256 < first;
+      refused |= c.refused;
+      wide[0] += need;
+      wide[1] += c.rows;
+      x[0] += gone;
+      x[1] += back;
+      x[2] += earlier ? gone : 0;
+      x[3] += earlier ? back : 0;
+      x[4] += earlier ? need : 0;
+      x[5] += earlier ? c.rows : 0;
     }
   }
-  long long none;
-  sums_before(all_over, sh, all_over);
-  sums_before(all_back, sh, all_back);
-  sums_before(all_need, sh, all_need);
-  sums_before(all_rows, sh, all_rows);
-  sums_before(my_over, sh, my_over);
-  sums_before(my_back, sh, my_back);
-  sums_before(my_need, sh, my_need);
-  sums_before(my_rows, sh, my_rows);
+#pragma unroll
+  for (int by = 1; by < 64; by *= 2) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) wide[i] += __shfl_xor(wide[i], by);
+#pragma unroll
+    for (int i = 0; i < 6; i++) x[i] += __shfl_xor(x[i], by);
+  }
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) sums[threadIdx.x >> 6][i] = wide[i];
+#pragma unroll
+    for (int i = 0; i < 6; i++) parts[threadIdx.x >> 6][i] = x[i];
+  }
+  refused = __syncthreads_or(refused);
+#pragma unroll
+  for (int i = 0; i < 2; i++) wide[i] = sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i];
+#pragma unroll
+  for (int i = 0; i < 6; i++) x[i] = parts[0][i] + parts[1][i] + parts[2][i] + parts[3][i];
   const long long left = min(max(a.state[0], 0), a.npage);
-  int why = __syncthreads_or(refused) ? MX_ROOM_TOKENS : 0;
-  if (all_need > min(left + all_back, (long long)a.npage)) why |= MX_ROOM_PAGES;
-  if (all_rows > a.rows) why |= MX_ROOM_ROWS;
-  const long long back_in_all = why ? all_over : all_back;
+  const int why = why_not(a, refused, left, x[1], wide[0], wide[1]);
+  const long long back_in_all = why ? x[0] : x[1];
 
   // this workgroup's worlds, one to a thread
   const int w = first + threadIdx.x;
   const bool mine = (int)threadIdx.x < worlds;
   Change c{};
   if (mine) c = change_of(a, w);
-  const int kept = !mine ? 0 : why ? (a.over && a.over[w] ? 0 : c.held) : min(c.kept, c.held);
-  const long long back = mine ? c.held - kept : 0, rows = mine && !why ? c.rows : 0;
-  long long total;
-  const long long back_before = sums_before(back, sh, total), rows_before = sums_before(rows, sh, none);
+  if (mine && why) refuse(c, a.over && a.over[w]);
+  const int kept = min(c.kept, c.held);
+  long long y[2] = {c.held - kept, c.rows}, total[2];
+  sums_before<256, 2>(y, sh, total);
   if (a.start && mine) {
-    a.start[w] = why ? 0 : (int)(my_rows + rows_before);
-    if (w == a.nworld - 1) a.start[a.nworld] = why ? 0 : (int)all_rows;
+    a.start[w] = why ? 0 : (int)(x[5] + y[1]);
+    if (w == a.nworld - 1) a.start[a.nworld] = why ? 0 : (int)wide[1];
   }
-  before[threadIdx.x] = back_before;
+  before[threadIdx.x] = y[0];
   from[threadIdx.x] = kept;
   __syncthreads();
   // the first page that comes back lies highest on the stack
-  const long long top = left + back_in_all - 1 - (why ? my_over : my_back);
-  for (long long i = threadIdx.x; i < total; i += 256) {
-    const int o = owner(before, worlds, i);
-    const long long slot = from[o] + i - before[o], at = top - i;
-    if (at >= 0 && at < a.npage && slot < a.width) a.free[at] = a.table[(int64_t)(first + o) * a.width + slot];
-  }
-  if (threadIdx.x == 0) {
-    a.found[blockIdx.x] = int4{(int)min(left + back_in_all, (long long)a.npage), (int)my_need, why, (int)all_need};
-  }
+  const long long top = left + back_in_all - 1 - (why ? x[2] : x[3]);
+  each_entry<256>(a, first, worlds, before, from, total[0], [&](const int32_t* entry, long long i) {
+    if (top - i >= 0 && top - i < a.npage) a.free[top - i] = *entry;
+  });
+  if (threadIdx.x == 0)
+    a.found[blockIdx.x] = int4{(int)max(min(left + back_in_all, (long long)a.npage), 0LL), x[4], why, (int)wide[0]};
 }
 
 // Tables and lengths
 __global__ __launch_bounds__(256) void update_tables(const Room a) {
-  __shared__ long long sh[4], before[kMostWorlds];
-  __shared__ int from[kMostWorlds];
+  __shared__ long long sh[4][2], before[kMostWorlds], given[kMostWorlds];
+  __shared__ int from[kMostWorlds], to[kMostWorlds];
   const int first = blockIdx.x * a.worlds_each, worlds = min(a.nworld - first, a.worlds_each);
   const int4 found = a.found[blockIdx.x];
   const int left = found.x, why = found.z, w = first + threadIdx.x;
   const bool mine = (int)threadIdx.x < worlds;
   Change c{};
   if (mine) c = change_of(a, w);
-  const bool over = mine && a.over && a.over[w];
-  if (why) {
-    c.after = c.base;
-    c.kept = over ? 0 : c.held;
-    c.need = c.kept;
-  }
-  const long long given = mine ? max(c.held - max(c.kept, c.need), 0) : 0;      // entries that name no page any more
-  const long long taken = mine ? max(c.need - c.kept, 0) : 0;
-  long long all;
-  const long long taken_before = sums_before(taken, sh, all);
-  before[threadIdx.x] = taken_before;
+  if (mine && why) refuse(c, a.over && a.over[w]);
+  // entries that get a page, and those that name none any more
+  long long x[2] = {max(c.need - c.kept, 0), max(c.held - max(c.kept, c.need), 0)}, all[2];
+  sums_before<256, 2>(x, sh, all);
+  before[threadIdx.x] = x[0];
+  given[threadIdx.x] = x[1];
   from[threadIdx.x] = c.kept;
+  to[threadIdx.x] = max(c.kept, c.need);
   __syncthreads();
-  for (long long i = threadIdx.x; i < all; i += 256) {
-    const int o = owner(before, worlds, i);
-    const long long slot = from[o] + i - before[o], at = left - 1 - found.y - i;
-    if (at >= 0 && slot < a.width) a.table[(int64_t)(first + o) * a.width + slot] = a.free[at];
-  }
-  __syncthreads();
-  const long long given_before = sums_before(given, sh, all);
-  before[threadIdx.x] = given_before;
-  from[threadIdx.x] = max(c.kept, c.need);
-  __syncthreads();
-  for (long long i = threadIdx.x; i < all; i += 256) {
-    const int o = owner(before, worlds, i);
-    const long long slot = from[o] + i - before[o];
-    if (slot < a.width) a.table[(int64_t)(first + o) * a.width + slot] = -1;
-  }
+  each_entry<256>(a, first, worlds, before, from, all[0], [&](int32_t* entry, long long i) {
+    const long long at = left - 1LL - found.y - i;
+    if (at >= 0) *entry = a.free[at];
+  });
+  each_entry<256>(a, first, worlds, given, to, all[1], [&](int32_t* entry, long long i) { *entry = -1; });
   if (mine) a.length[w] = c.after;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.state[0] = why ? left : left - found.w;
@@ -190,26 +279,87 @@ __global__ __launch_bounds__(256) void update_tables(const Room a) {
   }
 }
 
-// A row to a lane
+// Four neighbouring rows to a lane: they are mostly of one world and in one page
 struct Places {
   Move m;
   int32_t *world, *position, *slot;
+  bool vector;                   // the results are 16-byte aligned
 };
 
+constexpr int kRowsEach = 4, kStarts = 1024;
 __global__ __launch_bounds__(256) void find_places(const Places a) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long first = blockIdx.x * 256LL + 64 * wave;
-  if (first >= a.m.tokens) return;
-  const int lane = threadIdx.x & 63, tokens = (int)min(64LL, a.m.tokens - first), token = (int)first + lane;
-  const int world = world_of(a.m.start, a.m.nworld, a.m.count, (int)first, tokens);
-  if (world < 0) return;
-  const int begin = a.m.start ? a.m.start[world] : world * a.m.count, count = a.m.start ? a.m.start[world + 1] - begin : a.m.count;
-  const int place = token - begin;
-  const bool is = begin >= 0 && place >= 0 && place < count;
-  const int position = max(a.m.length[world], 0) - count + place;
-  a.world[token] = is ? world : -1;
-  a.position[token] = is ? max(position, -1) : -1;
-  a.slot[token] = is ? (int)slot_of(a.m, world, place, count) : -1;
+  const Move& m = a.m;
+  __shared__ int starts[kStarts];
+  const int rows_each = 256 * kRowsEach;
+  const int block = (int)((long long)blockIdx.x * rows_each), in_block = min(m.tokens - block, rows_each);
+  // the worlds of the workgroup's rows, and where their rows begin
+  int low = 0, high = m.nworld;
+  if (m.start && m.nworld >= kStarts) {
+    low = world_at(m.start, m.nworld, block);
+    high = world_at(m.start, m.nworld, block + in_block - 1) + 1;
+  }
+  const int many = high - low + 1;
+  const bool held = m.start && many <= kStarts;
+  if (held) {
+    for (int i = threadIdx.x; i < many; i += 256) starts[i] = m.start[low + i];
+    __syncthreads();
+  }
+  const auto start_of = [&](int world) { return held ? starts[world - low] : m.start[world]; };
+  const int in = kRowsEach * (int)threadIdx.x;
+  if (in >= in_block) return;
+  const int first = block + in;
+  int world = low, begin = 0, stop = 0, length = 0, page = -1, entry = -1;
+  const auto find = [&](int token) {               // from an earlier row's world on: mostly the same
+    if (m.start) {
+      int below = high;
+      if (start_of(world + 1) <= token)
+        while (below - world > 1) {
+          const int middle = (world + below) >> 1;
+          if (start_of(middle) <= token) world = middle; else below = middle;
+        }
+      begin = start_of(world);
+      stop = start_of(world + 1);
+    } else {
+      world = token / m.count;
+      begin = world * m.count;
+      stop = begin + m.count;
+    }
+    length = max(m.length[world], 0);
+    entry = -1;
+  };
+  find(first);
+  int32_t out[3][kRowsEach];
+  const int rows = min(kRowsEach, in_block - in);
+#pragma unroll
+  for (int i = 0; i < kRowsEach; i++) {
+    const int token = first + i;
+    if (i >= rows) continue;
+    if (token >= stop && world + 1 < high) find(token);
+    const bool is = begin >= 0 && token >= begin && token < stop;
+    const int position = length - (stop - begin) + token - begin;
+    int slot = -1;
+    if (is && position >= 0 && position >> m.page_shift < m.width) {
+      if (position >> m.page_shift != entry) {
+        entry = position >> m.page_shift;
+        page = m.table[(int64_t)world * m.width + entry];
+      }
+      if ((unsigned)page < (unsigned)m.npage) slot = (page << m.page_shift) + (position & ((1 << m.page_shift) - 1));
+    }
+    out[0][i] = is ? world : -1;
+    out[1][i] = is ? max(position, -1) : -1;
+    out[2][i] = slot;
+  }
+  int32_t* to[3] = {a.world + first, a.position + first, a.slot + first};
+#pragma unroll
+  for (int x = 0; x < 3; x++) {
+    if (a.vector && rows == kRowsEach) {
+      *(int4*)to[x] = int4{out[x][0], out[x][1], out[x][2], out[x][3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRowsEach; i++)
+        if (i < rows) to[x][i] = out[x][i];
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -227,6 +377,9 @@ int worlds_each(int nworld) {
   return each < 16 ? 16 : each;
 }
 
+// Whether one workgroup does all: its threads move all pages of all worlds at worst
+bool alone(const MxRoom* r) { return r->nworld <= kAlone && (int64_t)r->nworld * r->width <= 65536; }
+
 }  // namespace mxe
 
 extern "C" {
@@ -235,7 +388,7 @@ size_t mx_room_bytes(void) { return sizeof(MxRoom); }
 size_t mx_room_change_bytes(void) { return sizeof(MxRoomChange); }
 
 size_t mx_room_workspace(const MxRoom* room) {
-  if (mxe::room_check(room)) return 0;
+  if (mxe::room_check(room) || mxe::alone(room)) return 0;
   const int each = mxe::worlds_each(room->nworld);
   return (size_t)((room->nworld + each - 1) / each) * sizeof(int4);
 }
@@ -247,7 +400,7 @@ int mx_room_update(const MxRoom* room, const MxRoomChange* change, void* stream)
   if (!change || !room->free || !room->state || change->rows < 0) return MX_ERR_INVALID;
   if (room->nworld > kMostWorlds * 512) return MX_ERR_DOMAIN;
   const size_t bytes = mx_room_workspace(room);
-  if (!change->workspace || change->workspace_bytes < bytes || ((uintptr_t)change->workspace & 15)) return MX_ERR_WORKSPACE;
+  if (bytes && (!change->workspace || change->workspace_bytes < bytes || ((uintptr_t)change->workspace & 15))) return MX_ERR_WORKSPACE;
   Room a{};
   a.table = room->table; a.length = room->length; a.free = room->free; a.state = room->state;
   a.count = change->count; a.over = change->over; a.start = change->start;
@@ -256,6 +409,11 @@ int mx_room_update(const MxRoom* room, const MxRoomChange* change, void* stream)
   a.page_shift = __builtin_ctz(room->page_tokens);
   a.tokens = room->tokens; a.each = change->each; a.rows = change->rows;
   a.worlds_each = worlds_each(room->nworld);
+  if (!bytes) {
+    if (room->nworld <= 256) hipLaunchKernelGGL(update_alone<256>, dim3(1), dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(update_alone<kAlone>, dim3(1), dim3(kAlone), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+  }
   const dim3 grid((unsigned)((room->nworld + a.worlds_each - 1) / a.worlds_each));
   hipLaunchKernelGGL(update_count, grid, dim3(256), 0, (hipStream_t)stream, a);
   hipLaunchKernelGGL(update_tables, grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -275,7 +433,8 @@ int mx_room_places(const MxRoom* room, const MxChunk* c, int32_t* world, int32_t
   a.m.nworld = room->nworld; a.m.npage = room->npage; a.m.width = room->width; a.m.kv_heads = 1;
   a.m.page_shift = __builtin_ctz(room->page_tokens); a.m.tokens = c->tokens; a.m.count = c->count;
   a.world = world; a.position = position; a.slot = slot;
-  hipLaunchKernelGGL(find_places, dim3((unsigned)((c->tokens + 255LL) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+  a.vector = !(((uintptr_t)world | (uintptr_t)position | (uintptr_t)slot) & 15);
+  hipLaunchKernelGGL(find_places, dim3((unsigned)((c->tokens + 256LL * kRowsEach - 1) / (256 * kRowsEach))), dim3(256), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 

@@ -75,7 +75,7 @@ def summarise(summaries, start=None, *, count=None, tokens=None, stream=None):
     many, none = (count, tokens) if start is None else (tokens, count)
     _require(many is not None and none is None and many >= 0, 'give count (every world), or start and tokens')
     chunk = _chunk(pages, (pages.struct.nworld, count) if start is None else (tokens,), start)
-    rc = episodes.load().mx_episode_summarise(ct.byref(pages.struct), ct.byref(chunk), ct.byref(summaries.struct), _current(pages.index))
+    rc = (episodes._LIB or episodes.load()).mx_episode_summarise(ct.byref(pages.struct), ct.byref(chunk), ct.byref(summaries.struct), _current(pages.index))
     if rc:
         _check(rc, 'mx_episode_summarise')
 
@@ -106,12 +106,12 @@ def select(summaries, q, start=None, *, top, near=1, first=0, causal=True, max_c
     _require(listed <= MOST_LISTED, 'at most %d blocks can be listed, got %d: give max_count, the largest chunk of a world', MOST_LISTED, listed)
     shape = shape[:-2] + (s.kv_heads, listed)
     if out is None:
-        out = torch.empty(shape, dtype=torch.int32, device=pages.device)
+        out = torch.empty(shape, dtype=torch.int32, device=q.device)
     else:
         _require(out.dtype == torch.int32 and out.shape == shape and out.is_contiguous() and out.get_device() == pages.index,
                  'out must be contiguous int32 of shape %s on the pages\' device', tuple(shape))
     m = MxSelection(out.data_ptr(), listed, top, near, first, max_count, 1 if causal else 0)
-    rc = episodes.load().mx_episode_select(ct.byref(s), ct.byref(chunk), ct.byref(summaries.struct), ct.byref(rows), ct.byref(m),
+    rc = (episodes._LIB or episodes.load()).mx_episode_select(ct.byref(s), ct.byref(chunk), ct.byref(summaries.struct), ct.byref(rows), ct.byref(m),
                                            _current(pages.index))
     if rc:
         _check(rc, 'mx_episode_select')
@@ -157,7 +157,7 @@ def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal
                  and lse.get_device() == pages.index, 'lse must be contiguous float32 of q\'s shape without head_dim')
         a.lse = lse.data_ptr()
     m = MxSelection(blocks.data_ptr(), blocks.shape[-1])
-    lib, refs, raw = episodes.load(), (ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(m), block_tokens), _current(pages.index)
+    lib, refs, raw = episodes._LIB or episodes.load(), (ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(m), block_tokens), _current(pages.index)
     rc = lib.mx_episode_recall(*refs, raw)
     if rc == ERR_WORKSPACE:               # the keys are split: found before any launch
         need = lib.mx_recall_workspace(*refs)

@@ -33,7 +33,7 @@ class Room:
     refused (:data:`REFUSED`), until the caller sets it to 0.  ``tokens``: the most of a world, by default what its table
     reaches.  :func:`places` needs neither ``free`` nor ``state``.  The tensors stay the caller's, and are held here."""
 
-    __slots__ = ('table', 'length', 'free', 'state', 'struct', 'index')
+    __slots__ = ('table', 'length', 'free', 'state', 'struct', 'index', 'workspace')
 
     def __init__(self, table, length, npage, page_tokens, free=None, state=None, *, tokens=None):
         index = table.get_device()
@@ -57,6 +57,7 @@ class Room:
         self.table, self.length, self.free, self.state, self.index = table, length, free, state, index
         self.struct = MxRoom(table.data_ptr(), length.data_ptr(), None if free is None else free.data_ptr(),
                              None if state is None else state.data_ptr(), table.shape[0], table.shape[1], npage, page_tokens, tokens)
+        self.workspace = None             # bytes, once a change has asked
 
     @property
     def device(self):
@@ -98,11 +99,14 @@ def make_room(room, count, over=None, *, rows=None, stream=None):
         _require(over.dtype in (torch.bool, torch.uint8) and over.shape == (s.nworld,) and over.is_contiguous()
                  and over.get_device() == room.index, 'over must be contiguous bool of shape (nworld,) on the room\'s device')
         change.over = over.data_ptr()
-    lib = episodes.load()
-    need = lib.mx_room_workspace(ct.byref(s))
-    start = torch.empty(s.nworld + 1, dtype=torch.int32, device=room.device)
-    workspace = torch.empty(need, dtype=torch.uint8, device=room.device)
-    change.start, change.workspace, change.workspace_bytes, change.rows = start.data_ptr(), workspace.data_ptr(), need, rows
+    lib, device = episodes._LIB or episodes.load(), room.table.device
+    if room.workspace is None:
+        room.workspace = lib.mx_room_workspace(ct.byref(s))
+    start = torch.empty(s.nworld + 1, dtype=torch.int32, device=device)
+    if room.workspace:
+        workspace = torch.empty(room.workspace, dtype=torch.uint8, device=device)
+        change.workspace, change.workspace_bytes = workspace.data_ptr(), room.workspace
+    change.start, change.rows = start.data_ptr(), rows
     rc = lib.mx_room_update(ct.byref(s), ct.byref(change), _current(room.index))
     if rc:
         _check(rc, 'mx_room_update')
@@ -126,11 +130,16 @@ def places(room, start=None, *, count=None, tokens=None, stream=None):
                  and start.get_device() == room.index, 'start must be contiguous int32 of shape (nworld + 1,) on the room\'s device')
         _require(tokens < 2 ** 31, 'a chunk has fewer than 2^31 rows: %d', tokens)
         shape, chunk = (tokens,), MxChunk(start.data_ptr(), tokens, 0)
-    found = tuple(torch.empty(shape, dtype=torch.int32, device=room.device) for _ in range(3))
-    rc = episodes.load().mx_room_places(ct.byref(s), ct.byref(chunk), *(x.data_ptr() for x in found), _current(room.index))
+    rows = chunk.tokens
+    step = rows if rows < 4096 else rows + -rows % 4          # many rows: each of the three is 16-byte aligned
+    found = torch.empty((3, step), dtype=torch.int32, device=room.table.device)
+    at = found.data_ptr()
+    rc = (episodes._LIB or episodes.load()).mx_room_places(ct.byref(s), ct.byref(chunk), at, at + 4 * step, at + 8 * step, _current(room.index))
     if rc:
         _check(rc, 'mx_room_places')
-    return found
+    if step > rows:
+        found = found[:, :rows]
+    return (found if start is not None else found.unflatten(1, shape)).unbind(0)
 
 
 class DeviceChunk:

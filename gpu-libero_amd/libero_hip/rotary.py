@@ -98,12 +98,17 @@ def _stepping(x, name):
 
 
 def _turn(rotary, x, positions, back, out):
-    rows, to = _stepping(x, 'x'), _stepping(out, 'out')
-    tokens = x[..., 0, 0].numel() if x.shape[-2] and x.shape[-1] else 0
+    rows, shape = _stepping(x, 'x'), x.shape
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        to = MxRows(out.data_ptr(), shape[-2] * shape[-1], shape[-1], shape[-2], rows.type)
+    else:
+        to = _stepping(out, 'out')
+    tokens = shape[0] if len(shape) == 3 else shape[0] * shape[1]
     _require(tokens < 2 ** 31, 'fewer than 2^31 rows can be turned at once: %s', tokens)
-    if not tokens:
+    if not (tokens and rows.heads):
         return out
-    rc = episodes.load().mx_rotate(ct.byref(rotary.struct), ct.byref(rows), ct.byref(to), x.shape[-1], tokens, positions.data_ptr(),
+    rc = (episodes._LIB or episodes.load()).mx_rotate(ct.byref(rotary.struct), ct.byref(rows), ct.byref(to), x.shape[-1], tokens, positions.data_ptr(),
                                    positions.numel(), positions.dtype == torch.int64, back, _current(rotary.index))
     if rc:
         _check(rc, 'mx_rotate')
@@ -117,11 +122,13 @@ class _Rotate(torch.autograd.Function):
     def forward(ctx, x, positions, turn, rotary, back):
         ctx.save_for_backward(positions, turn)
         ctx.rotary, ctx.back = rotary, back
-        return _turn(rotary, x, positions, back, _output(x, None))
+        return _turn(rotary, x, positions, back, None)
 
     @staticmethod
     def backward(ctx, grad):
         positions, turn = ctx.saved_tensors
+        if not torch.is_grad_enabled():                  # no gradient of the gradient is wanted
+            return _turn(ctx.rotary, grad.contiguous(), positions, not ctx.back, None), None, None, None, None
         return _Rotate.apply(grad.contiguous(), positions, turn, ctx.rotary, not ctx.back), None, None, None, None
 
 
@@ -133,14 +140,15 @@ def rotate(rotary, x, positions, *, back=False, out=None, stream=None):
     ``back`` turns by the negative angles (with the same amplitude): that is the gradient, which autograd takes where x
     requires one; its own gradient is a rotation again.  ``out``, like x and apart from it, is written if given, where no
     gradient is recorded.  Returns out."""
-    device = x.device
-    _require(x.get_device() == rotary.index, 'x must be on the device of the angles')
-    _require(x.dim() in (3, 4) and rotary.struct.width <= x.shape[-1],
-             'x must be (..., tokens, heads, head_dim) with a head_dim of at least the %d values that turn: %s', rotary.struct.width,
-             tuple(x.shape))
-    _require(positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous() and positions.get_device() == rotary.index
-             and positions.shape in (x.shape[:-2], x.shape[-3:-2]),
-             'positions must be contiguous int32 or int64 on x\'s device, one to a row, or of shape (tokens,)')
+    shape = x.shape
+    if not (x.get_device() == rotary.index and len(shape) in (3, 4) and rotary.struct.width <= shape[-1]
+            and positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous()
+            and positions.get_device() == rotary.index and positions.shape in (shape[:-2], shape[-3:-2])):
+        _require(x.get_device() == rotary.index, 'x must be on the device of the angles')
+        _require(x.dim() in (3, 4) and rotary.struct.width <= x.shape[-1],
+                 'x must be (..., tokens, heads, head_dim) with a head_dim of at least the %d values that turn: %s',
+                 rotary.struct.width, tuple(x.shape))
+        raise ValueError('positions must be contiguous int32 or int64 on x\'s device, one to a row, or of shape (tokens,)')
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
         raise ValueError('x: there is no forward-mode derivative; rotate the tangent itself')
     recorded = x.requires_grad and torch.is_grad_enabled()
@@ -155,10 +163,10 @@ def rotate(rotary, x, positions, *, back=False, out=None, stream=None):
             if not (x.stride(-1) == 1 or x.shape[-1] == 1) or x.dim() == 4 and x.shape[0] > 1 and x.stride(0) != x.shape[1] * x.stride(1):
                 _stepping(x, 'x')
             return _Rotate.apply(x, positions, rotary.turn, rotary, bool(back))
-        return _turn(rotary, x, positions, bool(back), _output(x, out))
+        return _turn(rotary, x, positions, bool(back), out)
 
     if stream is not None or torch.cuda.current_device() != rotary.index:
-        return _on(device, stream, (x, positions, rotary.turn, out), call)
+        return _on(x.device, stream, (x, positions, rotary.turn, out), call)
     return call()
 
 
@@ -185,7 +193,7 @@ def enter(pages, rotary, q, k, v, start=None, *, out=None, stream=None):
         _require(not (_overlap(out, q) or _overlap(out, k) or _overlap(out, v)), 'out must be apart from q, k and v')
     out = _output(q, out)
     to = _rows(pages, out, q.shape, 'out')
-    rc = episodes.load().mx_episode_enter(ct.byref(s), ct.byref(chunk), ct.byref(rotary.struct), ct.byref(a), ct.byref(to),
+    rc = (episodes._LIB or episodes.load()).mx_episode_enter(ct.byref(s), ct.byref(chunk), ct.byref(rotary.struct), ct.byref(a), ct.byref(to),
                                           ct.byref(b), ct.byref(c), _current(pages.index))
     if rc:
         _check(rc, 'mx_episode_enter')
