@@ -95,10 +95,11 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
   };
   float* share = sh_share[team];
   f4(*o)[kQuads] = sh_o[team];
-  const int64_t row = (int64_t)blockIdx.x * kTeams + team, rows = a.part_rows;
-  if (row >= rows) return;
-  int token = (int)(row / a.heads);                     // see part_row()
-  const int h = (int)(row - (int64_t)token * a.heads);
+  const int64_t at = (int64_t)blockIdx.x * kTeams + team, sums = (int64_t)a.part_rows / a.heads * a.part_heads;
+  if (at >= sums) return;
+  int token = (int)(at / a.part_heads);                 // see part_row()
+  const int h = (int)(at - (int64_t)token * a.part_heads) + a.part_first;
+  const int64_t row = (int64_t)token * a.heads + h, rows = a.part_rows;
   if (!a.start) token += token / a.max_count * (a.count - a.max_count);
   else if (!covered(a, token)) return;                  // has no parts
   const int lane = threadIdx.x & 63;
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256) void join_parts(const Attend a) {
 #pragma unroll 4
     for (int s = first; s < a.splits; s += kLanes) {
       const float w = share[s];
-      if (w != -1.f) sum += rescaled(*(const f4*)(a.part + (s * rows + row) * D + 4 * quad), w);
+      if (w != -1.f) sum += rescaled(*(const f4*)(a.part + (s * sums + at) * D + 4 * quad), w);
     }
   if (first < kLanes) o[first][quad] = sum;
   meet();
@@ -270,6 +271,43 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   return choose(a, launch);
 }
 
+// Whether rows are gathered by the blocks that they share, so that a block's keys and values are read for up to 128 rows
+// at once and each row has as many parts as its list has entries, which are written and read again in 32 bits.  By what either way takes to an
+// entry of a token and key head, in ns: 0.3 and 0.075 (8 bits: 0.095) for each KB of the block's keys and values, or 0.45 for
+// each KB of the parts and 10 for each tile, a tenth more for marking and listing.  us, gathered and not, of 128 values in bfloat16 but where said, 19 blocks of 64 tokens listed:
+// 2048 tokens over 65536, 32 heads on 8, 475 and 911 (8-bit pages 443 and 555), 512 tokens 171 and 234, 256 tokens 124 and
+// 123; 4 x 1024 over 8192, 8 heads on 8, 265 and 1482, 32 on 4, 858 and 758, 32 on 8 of 256 values 1171 and 3808; 16 x 256 over
+// 8192, 16 on 4 of 64 values, 172 and 262 (163 and 201); 64 x 64 over 4096 205 and 240; 300 x 41 over 1024, 12 on 4 of 96 values, blocks of 32, 631 and 533.
+constexpr int64_t kMostParts = 1 << 25, kMostBytes = 1 << 30, kBatchBytes = 192 << 20;
+bool choose_gathered(Attend& a, Launch& launch) {
+  const int64_t blocks = (int64_t)a.width << (a.page_shift - a.block_shift), block = 1LL << a.block_shift;
+  const int64_t tokens = a.start ? a.tokens : (int64_t)a.nworld * a.max_count, rows = tokens * a.heads;
+  if (a.lists < 2 || a.lists > kMostSplits || a.group > kManyRows || a.max_count > 32768 || rows > INT32_MAX) return false;
+  const int many = kManyRows / a.group;
+  const double share = (double)tokens * a.lists / ((double)a.nworld * blocks);      // tokens to a block
+  const double kb = 2.0 * block * launch.head_dim * (launch.fp8 ? 1 : 2) / 1024, part_kb = 4.0 * a.group * launch.head_dim / 1024;
+  if (1.1 * (0.45 * part_kb + 10.0 * ceil(share / many) / share) > 0.3 + (launch.fp8 ? 0.095 : 0.075) * kb) return false;
+  const int64_t head_bytes = tokens * a.group * a.lists * launch.head_dim * 4;      // of a key head's sums
+  if (rows * a.lists > kMostParts || head_bytes > kMostBytes) return false;
+  // a tile for each full set of rows of a key head, and one that is not full for each block
+  const int64_t head_tiles = tokens * a.lists / many + a.nworld * blocks, tiles = head_tiles * a.kv_heads;
+  if (tiles > kMostGroups || (int64_t)a.nworld * a.kv_heads * ((a.max_count + 31) / 32) > kMostGroups) return false;
+  launch.gathered = true;
+  launch.rows = kManyRows;
+  launch.tiles = (int)tiles;
+  a.splits = a.lists;
+  a.part_rows = (int)rows;
+  // so many key heads at a time that their parts are still in the last cache when they are joined
+  const int64_t batches = (head_bytes * a.kv_heads + kBatchBytes - 1) / kBatchBytes;
+  a.batch_heads = batches >= a.kv_heads ? 1 : (int)((a.kv_heads + batches - 1) / batches);
+  a.words = (a.max_count + 31) / 32;
+  a.world_blocks = (int)blocks;
+  a.tiles_most = (int)head_tiles * a.batch_heads;
+  a.tiles = a.tiles_most;
+  launch.grid = (unsigned)a.tiles_most;
+  return true;
+}
+
 // Which kernel, by the rows that share a key head's keys and values.  us for 300 worlds of up to 700 tokens, 4 key
 // heads of 128 values, with 12, 24, 48 rows: attend_few of 16 rows 52, 75, 101 in bfloat16 and 32, 48, 66 with 8-bit
 // pages, of 32 rows (8-bit pages only) 42, 44, 77, attend_many 57, 59, 63 and 54, 55, 60;
@@ -288,6 +326,7 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 // 70 and 60, 92 and 90; 2048 of those 23 and 12, 39 and 36, 50 and 53; 512 of them 10.8 and 10.9, 11.4 and 16.7, 15 and 23.
 constexpr int kShort = 256, kPlenty = 2048;
 int choose(Attend& a, Launch& launch) {
+  if (launch.listed && choose_gathered(a, launch)) return 0;
   const int64_t rows = launch.listed ? a.group : (int64_t)a.max_count * a.group;
   const bool few = rows <= (launch.fp8 ? 32 : 16);
   launch.blocks = rows <= 16 || (launch.listed && !launch.fp8) ? 1 : 2;
@@ -310,6 +349,7 @@ int choose(Attend& a, Launch& launch) {
   launch.team = splits == 1 && keys <= kShort && groups >= kPlenty ? 1 : 4;
   a.tiles = (int)tiles;
   a.splits = (int)splits;
+  a.part_heads = a.heads;
   // with parts there are fewer tiles than `room`, so at most 1024 of 128 rows
   a.part_rows = splits > 1 ? (a.start ? a.tokens : a.nworld * a.max_count) * a.heads : 0;
   launch.tiles = a.tiles;
@@ -317,26 +357,47 @@ int choose(Attend& a, Launch& launch) {
   return 0;
 }
 
-size_t workspace_of(const Attend& a, const Launch& launch) {
-  if (!launch.tiles || a.splits < 2) return 0;
-  return (size_t)a.splits * a.part_rows * (launch.head_dim + 2) * sizeof(float);
+// Batches of key heads whose rows are gathered one after the other
+int batches_of(const Attend& a) { return (a.kv_heads + a.batch_heads - 1) / a.batch_heads; }
+
+// The workspace: sums, (maximum, sum of weights) of each part, and for gathered rows the tiles' numbers, tiles, their rows and marks
+struct Workspace {
+  size_t ml, counts, tiles, rows, marks, bytes;
+};
+Workspace workspace_for(const Attend& a, const Launch& launch) {
+  Workspace w{};
+  const size_t parts = (size_t)a.splits * a.part_rows;
+  if (!launch.gathered) {
+    w.ml = parts * launch.head_dim * sizeof(float);
+    w.bytes = w.ml + parts * 2 * sizeof(float);
+    return w;
+  }
+  const auto after = [](size_t at, size_t bytes) { return (at + bytes + 15) & ~(size_t)15; };
+  const size_t batches = batches_of(a), tiles = batches * a.tiles_most;
+  w.ml = after(0, (size_t)a.splits * (a.part_rows / a.heads) * a.batch_heads * a.group * launch.head_dim * sizeof(float));
+  w.counts = after(w.ml, parts * 2 * sizeof(float));
+  w.tiles = after(w.counts, batches * sizeof(int));
+  w.rows = after(w.tiles, tiles * sizeof(int4));
+  w.marks = after(w.rows, tiles * (kManyRows / a.group) * sizeof(int));
+  w.bytes = after(w.marks, (size_t)a.nworld * a.kv_heads * a.world_blocks * a.words * sizeof(unsigned));
+  return w;
 }
 
-// The attention's launch, and that which joins the parts
-int attend_planned(Attend& a, const Launch& launch, const MxAttention* m, void* stream) {
-  const size_t bytes = workspace_of(a, launch);
-  if (bytes) {
-    if (!m->workspace || m->workspace_bytes < bytes || ((uintptr_t)m->workspace & 15)) return MX_ERR_WORKSPACE;
-    a.part = (float*)m->workspace;
-    a.part_ml = a.part + (size_t)a.splits * a.part_rows * launch.head_dim;
-  }
-  const int started = launch.head_dim == 32 ? attend32(a, launch, stream)
-                    : launch.head_dim == 64 ? attend64(a, launch, stream)
-                    : launch.head_dim == 96 ? attend96(a, launch, stream)
-                    : launch.head_dim == 128 ? attend128(a, launch, stream)
-                                             : attend256(a, launch, stream);
-  if (started || a.splits < 2) return started;
-  const int64_t rows = a.part_rows;
+size_t workspace_of(const Attend& a, const Launch& launch) {
+  return !launch.tiles || a.splits < 2 ? 0 : workspace_for(a, launch).bytes;
+}
+
+int launch_attend(const Attend& a, const Launch& launch, void* stream) {
+  return launch.head_dim == 32 ? attend32(a, launch, stream)
+       : launch.head_dim == 64 ? attend64(a, launch, stream)
+       : launch.head_dim == 96 ? attend96(a, launch, stream)
+       : launch.head_dim == 128 ? attend128(a, launch, stream)
+                                : attend256(a, launch, stream);
+}
+
+// The attention's launches, and those which join the parts
+int launch_join(const Attend& a, const Launch& launch, void* stream) {
+  const int64_t rows = (int64_t)a.part_rows / a.heads * a.part_heads;
   const bool one = rows >= kRowsForWaves && a.splits <= 64;
   const dim3 grid((unsigned)(one ? (rows + 3) / 4 : rows));
   const auto join = [&](auto d) {
@@ -359,6 +420,34 @@ int attend_planned(Attend& a, const Launch& launch, const MxAttention* m, void* 
     default: join(std::integral_constant<int, 256>());
   }
   return (int)hipGetLastError();
+}
+
+int attend_planned(Attend& a, const Launch& launch, const MxAttention* m, void* stream) {
+  const size_t bytes = workspace_of(a, launch);
+  if (bytes) {
+    if (!m->workspace || m->workspace_bytes < bytes || ((uintptr_t)m->workspace & 15)) return MX_ERR_WORKSPACE;
+    const Workspace w = workspace_for(a, launch);
+    uint8_t* at = (uint8_t*)m->workspace;
+    a.part = (float*)at;
+    a.part_ml = (float*)(at + w.ml);
+    a.gathered_tiles = (int*)(at + w.counts);
+    a.gathered = (int4*)(at + w.tiles);
+    a.gathered_rows = (int*)(at + w.rows);
+    a.marks = (unsigned*)(at + w.marks);
+  }
+  if (!launch.gathered) {
+    const int rc = launch_attend(a, launch, stream);
+    return rc || a.splits < 2 ? rc : launch_join(a, launch, stream);
+  }
+  int rc = gather_rows(a, launch, stream);
+  for (a.batch = 0; !rc && a.batch < batches_of(a); a.batch++) {
+    const int first = a.batch * a.batch_heads, heads = a.kv_heads - first < a.batch_heads ? a.kv_heads - first : a.batch_heads;
+    a.part_first = first * a.group;
+    a.part_heads = heads * a.group;
+    rc = launch_attend(a, launch, stream);
+    if (!rc) rc = launch_join(a, launch, stream);
+  }
+  return rc;
 }
 
 }  // namespace mxe

@@ -10,6 +10,11 @@ template <int D, int kType, bool kFp8>
 int attend_typed(const Attend& a, const Launch& launch, void* stream) {
   const dim3 grid(launch.grid), block(256);
   const hipStream_t s = (hipStream_t)stream;
+  if (launch.gathered) {
+    if (a.page_shift >= 6) hipLaunchKernelGGL((attend_many<kType, kFp8, true, D, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attend_many<kType, kFp8, false, D, true>), grid, block, 0, s, a);
+    return (int)hipGetLastError();
+  }
   if (launch.listed) {
     if (launch.blocks == 1) {
       if (launch.team == 1) hipLaunchKernelGGL((attend_few<kType, kFp8, D, 1, 1, true>), grid, dim3(64), 0, s, a);

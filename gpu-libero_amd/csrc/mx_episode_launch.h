@@ -13,7 +13,7 @@ struct Launch {
   int type, head_dim, blocks, rows, tiles;    // blocks of 16 rows to a tile
   int team;                                   // waves of attend_few that share a tile
   int64_t keys;                               // the most that a world has, as far as the host knows
-  bool fp8, listed;                           // listed: attention to listed blocks
+  bool fp8, listed, gathered;                 // listed: attention to listed blocks; gathered: of rows that share one
   unsigned grid;
 };
 
@@ -22,6 +22,7 @@ struct Launch {
 int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, Launch& launch, bool pointers,
          const MxSelection* s = nullptr, int block_shift = 0);
 size_t workspace_of(const Attend& a, const Launch& launch);
+int gather_rows(Attend& a, const Launch& launch, void* stream);    // (mx_episode_recall.hip)
 int attend_planned(Attend& a, const Launch& launch, const MxAttention* m, void* stream);
 
 // Checks that all entry points share (mx_episode.hip)

@@ -462,6 +462,104 @@ __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(c
   }
 }
 
+// ---------------------------------------------------------------------------- rows gathered by their blocks
+// A workgroup takes 32 tokens of a world's chunk and a key head: the bits of all blocks that their lists name, collected in
+// LDS (so many blocks at a time), and written side by side: marks[world, key head][word][block].  Entries of whose keys
+// the row sees none get empty parts.
+constexpr int kMarked = 8192;
+__global__ __launch_bounds__(256) void mark_rows(const Attend a) {
+  __shared__ unsigned bits[kMarked];
+  const int word = blockIdx.x % a.words, pair = blockIdx.x / a.words, world = pair / a.kv_heads, head = pair - world * a.kv_heads;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i * a.batch_heads < a.kv_heads; i += 256) a.gathered_tiles[i] = 0;
+  const int begin = a.start ? a.start[world] : world * a.count, stop = a.start ? min(a.start[world + 1], a.tokens) : begin + a.count;
+  const int count = a.start ? a.start[world + 1] - begin : a.count, length = max(a.length[world], 0);
+  const int tokens = begin < 0 ? 0 : max(min(min(stop - begin, a.max_count) - 32 * word, 32), 0);
+  const int reach = (int)min((long long)length, (long long)a.width << a.page_shift);
+  unsigned* marks = a.marks + ((int64_t)pair * a.words + word) * a.world_blocks;
+  for (int first = 0; first < a.world_blocks; first += kMarked) {
+    const int many = min(a.world_blocks - first, kMarked);
+    for (int i = threadIdx.x; i < many; i += 256) bits[i] = 0;
+    __syncthreads();
+    for (int at = threadIdx.x; at < tokens * a.lists; at += 256) {
+      const int which = at / a.lists, entry = at - which * a.lists, i = 32 * word + which, position = length - count + i;
+      const int high = position < 0 ? 0 : a.causal ? min(position + 1, reach) : reach;
+      const int block = a.blocks[((int64_t)(begin + i) * a.kv_heads + head) * a.lists + entry];
+      if ((unsigned)block < (unsigned)a.world_blocks && block << a.block_shift < high) {
+        if ((unsigned)(block - first) < (unsigned)many) atomicOr(&bits[block - first], 1u << which);
+      } else if (!first) {
+        const int64_t row = (a.start ? begin + i : (int64_t)world * a.max_count + i) * a.heads + head * a.group;
+        for (int h = 0; h < a.group; h++) *(f2*)(a.part_ml + 2 * (entry * (int64_t)a.part_rows + row + h)) = f2{-INFINITY, 0.f};
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < many; i += 256) marks[first + i] = bits[i];
+  }
+}
+
+// A workgroup takes 16 blocks of a world's key head, a wave four of them in turn: how many tiles their tokens are, places for those in any
+// order among the others' of the batch, as each row's part is its own, and the tokens in their order.
+constexpr int kCounted = 16;
+__global__ __launch_bounds__(256) void list_tiles(const Attend a) {
+  __shared__ int sh_tokens[kCounted], sh_from[kCounted];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, many = kManyRows / a.group;
+  const int per = (a.world_blocks + kCounted - 1) / kCounted, pair = blockIdx.x / per, first = (blockIdx.x - pair * per) * kCounted;
+  const int batch = (pair % a.kv_heads) / a.batch_heads;
+  const unsigned* marks = a.marks + (int64_t)pair * a.words * a.world_blocks;
+  // the tokens of a block, by 16 threads
+  {
+    const int block = first + (threadIdx.x >> 4);
+    int tokens = 0;
+    if (block < a.world_blocks)
+      for (int w = threadIdx.x & 15; w < a.words; w += 16) tokens += __popc(marks[(int64_t)w * a.world_blocks + block]);
+#pragma unroll
+    for (int by = 1; by < 16; by *= 2) tokens += __shfl_xor(tokens, by);
+    if ((threadIdx.x & 15) == 0) sh_tokens[threadIdx.x >> 4] = tokens;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int tiles = lane < kCounted ? (sh_tokens[lane] + many - 1) / many : 0;
+    int sum = tiles;
+#pragma unroll
+    for (int by = 1; by < kCounted; by *= 2) {
+      const int y = __shfl_up(sum, by);
+      if (lane >= by) sum += y;
+    }
+    int from = 0;
+    if (lane == kCounted - 1 && sum) from = atomicAdd(a.gathered_tiles + batch, sum);
+    from = __shfl(from, kCounted - 1) + sum - tiles;
+    if (lane < kCounted) sh_from[lane] = from;
+  }
+  __syncthreads();
+  for (int i = wave; i < kCounted; i += 4) {
+    const int tokens = sh_tokens[i], tiles = (tokens + many - 1) / many;
+    if (!tokens || sh_from[i] + tiles > a.tiles_most) continue;
+    const int64_t from = (int64_t)batch * a.tiles_most + sh_from[i];
+    for (int j = lane; j < tiles; j += 64) a.gathered[from + j] = int4{pair, first + i, min(tokens - j * many, many), 0};
+    int* rows = a.gathered_rows + from * many;
+    int before = 0;                               // marked in the words before
+    for (int base = 0; base < a.words; base += 64) {
+      unsigned word = base + lane < a.words ? marks[(int64_t)(base + lane) * a.world_blocks + first + i] : 0;
+      int sum = __popc(word);
+#pragma unroll
+      for (int by = 1; by < 64; by *= 2) {
+        const int y = __shfl_up(sum, by);
+        if (lane >= by) sum += y;
+      }
+      for (int place = before + sum - __popc(word); word; word &= word - 1, place++) rows[place] = 32 * (base + lane) + __builtin_ctz(word);
+      before += __shfl(sum, 63);
+    }
+  }
+}
+
+int gather_rows(Attend& a, const Launch& launch, void* stream) {
+  const hipStream_t s = (hipStream_t)stream;
+  const unsigned pairs = a.nworld * a.kv_heads, per = (a.world_blocks + kCounted - 1) / kCounted;
+  hipLaunchKernelGGL(mark_rows, dim3(pairs * a.words), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(list_tiles, dim3(pairs * per), dim3(256), 0, s, a);
+  return (int)hipGetLastError();
+}
+
 // ---------------------------------------------------------------------------- host side
 int summaries_check(const MxPages* p, const MxSummaries* s) {
   if (!s || !s->codes || !s->exponent || ((uintptr_t)s->codes & 15)) return MX_ERR_INVALID;

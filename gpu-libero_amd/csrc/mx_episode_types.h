@@ -120,11 +120,20 @@ struct Attend {
   int nworld, npage, width, kv_heads, page_shift, tokens, count, max_count, heads, group;
   int causal, window, tiles, splits;
   int part_rows;                     // of one split
+  int part_heads, part_first;        // the query heads that `part` has, all but where rows are gathered
   float scale2;                      // |scale| * log2(e), not 0: probabilities are powers of two
   bool negate;                       // scale < 0: the queries change their sign
   bool q_vector, o_vector;           // q's rows are 16-byte aligned, out's 8-byte
   const int32_t* blocks;             // of attention to listed blocks: (token, key head, entry), `lists` entries
   int lists, block_shift;
+  // rows gathered by their blocks: the tokens of each (world and key head, block), a bit each in `words` words
+  // [pair][word][block]; tiles of (pair, block, number of tokens), how many of those there
+  // are, and their tokens, up to 128 / group of each tile
+  unsigned* marks;
+  int4* gathered;
+  int *gathered_tiles, *gathered_rows;
+  int words, world_blocks;
+  int tiles_most, batch, batch_heads;  // tiles that the key heads of a batch have room for; which batch; its key heads
 };
 
 // A kernel's only argument, read where it is used: as a by-value parameter all of it would be in scalar

@@ -500,3 +500,148 @@ def test_refusals(gpu_available):
         with pytest.raises(ValueError):
             call()
             print('not refused', i)
+
+
+# ------------------------------------------------------------------------------ rows that share blocks
+def gathers(world, counts, heads, listed, block, most=None):
+    """Whether the rows of such a call are gathered by their blocks: its workspace then has more than the parts' numbers."""
+    import ctypes as ct
+    import torch
+    s = world.pages.struct
+    tokens = int(np.sum(counts))
+    start = torch.zeros(len(counts) + 1, dtype=torch.int32, device='cuda')
+    chunk = episodes.MxChunk(start.data_ptr(), tokens, 0)
+    kind = s.type if s.type != 3 else 1
+    rows = episodes.MxRows(start.data_ptr(), heads * s.head_dim, s.head_dim, heads, kind)
+    a = episodes.MxAttention(rows, rows, None, None, 0, max(counts) if most is None else most, 1, 0, 0.1, 0)
+    m = episodes.MxSelection(start.data_ptr(), listed)
+    need = episodes.load().mx_recall_workspace(*(ct.byref(x) for x in (s, chunk, a, m)), block)
+    return need % (tokens * heads * (s.head_dim + 2) * 4) != 0
+
+
+@pytest.mark.parametrize('kind,store', [('bf16', 'bf16'), ('f16', 'f16'), ('bf16', 'fp8'), ('f16', 'fp8')])
+@pytest.mark.parametrize('dim,block,page,heads', [(32, 64, 64, 6), (64, 32, 32, 2), (96, 64, 128, 6), (128, 64, 64, 6),
+                                                  (128, 128, 256, 4), (256, 64, 64, 6), (256, 128, 128, 2)])
+def test_gathered_rows(gpu_available, dim, block, page, heads, kind, store):
+    """Chunks of hundreds of tokens, whose rows are gathered by the blocks that they share: full and partial tiles, blocks of
+    less than a step's keys, one step's and more; worlds of other lengths beside."""
+    print('case gathered', dim, block, page, heads, kind, store, flush=True)
+    world = World([700, 40, 0, 530], 2, dim, page, store, seed=dim + block)
+    counts = [260, 40, 0, 97]
+    assert gathers(world, counts, heads, 9, block)
+    for causal in (True, False):
+        check(world, counts, heads, kind, block, 4, 2, 3, causal)
+
+
+@pytest.mark.parametrize('group', [1, 2, 5, 7, 8])
+def test_gathered_groups(gpu_available, group):
+    print('case gathered group', group, flush=True)
+    world = World([600, 300], 3, 64, 128, 'bf16', seed=group)
+    assert gathers(world, [150, 150], 3 * group, 4, 128)
+    check(world, [150, 150], 3 * group, 'bf16', 128, 2, 1, 1, uniform=True)
+    check(world, [150, 33], 3 * group, 'bf16', 128, 2, 1, 1, causal=False)
+
+
+@pytest.mark.parametrize('store', ['bf16', 'fp8'])
+def test_gathered_lists_of_the_caller(gpu_available, store):
+    """Blocks listed twice, not at all, out of order, that are none; rows beyond max_count are left as they were."""
+    import torch
+    print('case gathered lists', store, flush=True)
+    rng = np.random.default_rng(3)
+    world = World([500, 310, 130], 2, 64, 64, store, seed=5)
+    counts = [200, 0, 130]
+    q, start = queries(counts, 4, 64, 'bf16')
+    blocks = rng.integers(-2, 11, (330, 2, 12)).astype(np.int32)
+    blocks[0, 0, :] = -1
+    blocks[1, 1, :2] = 2 ** 31 - 1, -2 ** 31
+    blocks[2, 0, :] = 0
+    blocks[200:, 1, 5] = blocks[200:, 1, 4]
+    assert gathers(world, counts, 4, 12, 64)
+    valid = np.where(blocks < 8, blocks, -1)
+    at = torch.from_numpy(start).cuda()
+    for causal in (True, False):
+        lse = torch.zeros((330, 4), device='cuda')
+        given = torch.from_numpy(blocks).cuda()
+        out = recall.recall(world.pages, q.cuda(), given, at, block_tokens=64, causal=causal, lse=lse)
+        want = listed_attention(world, q, start, valid, 64, causal)
+        compare(out, lse, want, 'bf16')
+        assert torch.equal(out, recall.recall(world.pages, q.cuda(), given, at, block_tokens=64, causal=causal))
+        target = torch.full_like(out, 7)
+        recall.recall(world.pages, q.cuda(), given, at, block_tokens=64, causal=causal, max_count=150, out=target)
+        assert bool((target[150:200] == 7).all())
+        keep = np.r_[0:150, 200:330]
+        compare(target[torch.from_numpy(keep).cuda()], None, [x[keep] for x in want], 'bf16')
+
+
+@pytest.mark.parametrize('bad,store', [(np.inf, 'bf16'), (np.nan, 'bf16'), (np.nan, 'fp8')])
+def test_gathered_hidden_values(gpu_available, bad, store):
+    """An infinity or NaN in a value reaches the gathered rows that see it and no others."""
+    import torch
+    print('case gathered hidden', bad, store, flush=True)
+    world = World([330, 290], 1, 64, 64, store, seed=6)
+    for w, t in ((0, 40), (0, 300), (1, 289)):
+        world.v[w][t, 0, 5 if store != 'fp8' else slice(0, 32)] = bad
+        if store == 'fp8':
+            world.pages.v_scale[world.table[w, t // 64], 0, t % 64, 0] = 255
+        else:
+            world.pages.v[world.table[w, t // 64], 0, t % 64] = torch.from_numpy(world.v[w][t, 0]).cuda().bfloat16()
+    q, start = queries([160, 200], 2, 64, 'bf16')
+    blocks = np.random.default_rng(0).integers(0, 6, (360, 1, 4)).astype(np.int32)
+    assert gathers(world, [160, 200], 2, 4, 64)
+    at = torch.from_numpy(start).cuda()
+    for causal in (True, False):
+        out = recall.recall(world.pages, q.cuda(), torch.from_numpy(blocks).cuda(), at, block_tokens=64, causal=causal)
+        compare(out, None, listed_attention(world, q, start, blocks, 64, causal), 'bf16')
+
+
+def test_gathered_pages_that_are_not_there(gpu_available):
+    import torch
+    print('case gathered missing', flush=True)
+    world = World([400], 1, 64, 64, 'bf16', seed=7)
+    world.pages.table[0, 1] = -1
+    q, start = queries([200], 2, 64, 'bf16')
+    blocks = np.tile(np.array([0, 1, 4, 6], np.int32), (200, 1, 1))
+    assert gathers(world, [200], 2, 4, 64)
+    out = recall.recall(world.pages, q.cuda(), torch.from_numpy(blocks).cuda(), torch.from_numpy(start).cuda(), block_tokens=64)
+    blocks[..., 1] = -1
+    compare(out, None, listed_attention(world, q, start, blocks, 64, True), 'bf16')
+
+
+def test_gathered_in_batches_of_heads(gpu_available):
+    """More parts than are kept at once: key heads in several batches, of which the last is smaller; and captured."""
+    import torch
+    print('case gathered batches', flush=True)
+    n, kv, dim = 8192, 3, 64
+    gen = torch.Generator('cuda').manual_seed(0)
+    k, v = (torch.randn((n // 64, kv, 64, dim), generator=gen, device='cuda').bfloat16() for _ in range(2))
+    p = episodes.Pages(k, v, torch.arange(n // 64, dtype=torch.int32, device='cuda')[None].contiguous(),
+                       torch.tensor([n], dtype=torch.int32, device='cuda'))
+    s = recall.Summaries.make(p, 64)
+    recall.summarise(s, count=n)
+    q = torch.randn((1, 4096, 4 * kv, dim), generator=gen, device='cuda').bfloat16()
+    blocks = recall.select(s, q, top=21, near=1, first=1)
+
+    def call():
+        lse = torch.empty(q.shape[:-1], device='cuda')
+        return recall.recall(p, q, blocks, block_tokens=64, lse=lse), lse
+
+    out, lse = call()
+    # a few rows at a time: few enough that they are not gathered
+    for at in (0, 1000, 4090):
+        some = torch.cat([q[:, at:at + 6]], 1).contiguous()
+        short = episodes.Pages(k, v, p.table, torch.tensor([n - 4096 + at + 6], dtype=torch.int32, device='cuda'))
+        few = torch.empty(some.shape[:-1], device='cuda')
+        want = recall.recall(short, some, blocks[:, at:at + 6].contiguous(), block_tokens=64, lse=few)
+        # both within 2^-8 of |out| and a little of sum p |v|, at most 2^-12, of the same
+        torch.testing.assert_close(out[:, at:at + 6].float(), want.float(), rtol=2.0 ** -7, atol=2.0 ** -10)
+        torch.testing.assert_close(lse[:, at:at + 6], few, rtol=2.0 ** -17, atol=2.0 ** -11)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for _ in range(3):
+        q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [x.clone() for x in got]
+        for a, b in zip(kept, call()):
+            assert torch.equal(a, b)
