@@ -67,14 +67,26 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
   limits(a, t, last_row / a.group, last_low, last_high);
   const int all_low = last_low, all_high = first_high;
   int begin, end;
-  Fixed* list = nullptr;
+  Fixed* table = fixed(a.table + (int64_t)t.world * a.width);
+  // listed blocks: the lanes hold 64 entries of the list and their pages (-1: none), so that a step finds its keys without a
+  // load (72 us instead of 73 for 1024 worlds' 11 blocks of 64 8-bit tokens)
+  int list_block = -1, list_page = -1, list_held = 0;
+  const auto hold = [&](int group) {
+    const int32_t* list = a.blocks + ((int64_t)(t.token + t.row / a.group) * a.kv_heads + head) * a.lists;
+    const int entry = 64 * group + lane;
+    list_block = entry < a.lists ? list[entry] : -1;
+    if ((unsigned)list_block >= (unsigned)a.width << (a.page_shift - a.block_shift)) list_block = -1;
+    const int page = a.table[(int64_t)t.world * a.width + (max(list_block, 0) >> (a.page_shift - a.block_shift))];
+    list_page = list_block >= 0 && (unsigned)page < (unsigned)a.npage ? page : -1;
+    list_held = group;
+  };
   if constexpr (kListed) {
-    list = fixed(a.blocks + ((int64_t)(t.token + t.row / a.group) * a.kv_heads + head) * a.lists);
     int named = 0;                                            // up to the last entry that names a block
-    for (int i = lane; i < a.lists; i += 64) named = list[i] >= 0 ? i + 1 : named;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) named = max(named, __shfl_xor(named, x));
-    named = __builtin_amdgcn_readfirstlane(named);
+    for (int group = (a.lists - 1) >> 6; group >= 0 && !named; group--) {
+      hold(group);
+      const uint64_t names = __ballot(list_block >= 0);
+      if (names) named = 64 * group + 64 - __builtin_clzll(names);
+    }
     split_range(a, split, 0, last_high > 0 ? named << a.block_shift : 0, begin, end);
   } else {
     split_range(a, split, first_low, last_high, begin, end);
@@ -108,7 +120,6 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
     for (int c = 0; c < D / 16; c++) o[b][c] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  Fixed* table = fixed(a.table + (int64_t)t.world * a.width);
   const int page_mask = (1 << a.page_shift) - 1;
 
   // The 16 keys from `key` on lie in one page: its number, or 0 with the keys marked absent
@@ -120,18 +131,20 @@ __global__ __launch_bounds__(64 * kTeam, few_waves(D, kBlocks)) void attend_few(
   };
   auto locate = [&](int key) {
     Keys s;
-    int from = min(key, (end - 1) & ~15);
+    int from = min(key, (end - 1) & ~15), page;
     s.left = end - 1 - from;
-    bool is = true;
     if constexpr (kListed) {
-      const int block = list[from >> a.block_shift];
-      is = key < end && (unsigned)block < (unsigned)a.width << (a.page_shift - a.block_shift);
-      from = (is ? block << a.block_shift : 0) + (from & ((1 << a.block_shift) - 1));
-      is = is && from < last_high;
+      const int entry = from >> a.block_shift;
+      if (entry >> 6 != list_held) hold(entry >> 6);
+      const int block = __builtin_amdgcn_readlane(list_block, entry & 63);
+      page = __builtin_amdgcn_readlane(list_page, entry & 63);
+      from = (max(block, 0) << a.block_shift) + (from & ((1 << a.block_shift) - 1));
+      s.is = key < end && page >= 0 && from < last_high;
+    } else {
+      page = table[from >> a.page_shift];
+      s.is = (unsigned)page < (unsigned)a.npage;
     }
     s.first = from;
-    const int page = table[from >> a.page_shift];
-    s.is = is && (unsigned)page < (unsigned)a.npage;
     s.at = (((int64_t)(s.is ? page : 0) * a.kv_heads + head) << a.page_shift) + (from & page_mask);
     return s;
   };

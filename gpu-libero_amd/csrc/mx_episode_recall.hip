@@ -23,6 +23,11 @@ __device__ inline int power_of(double most) {
   return min(max(e - 7 + (fraction > kMostCode / 128.0 ? 1 : 0), -kMostPower), kMostPower);
 }
 
+__device__ inline int power_of(float most) {               // most >= 0, its fraction and exponent as bits
+  const unsigned bits = __float_as_uint(most);
+  return min(max((int)(bits >> 23) - 126 - 7 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0), -kMostPower), kMostPower);
+}
+
 // ---------------------------------------------------------------------------- summaries
 struct Summarise {
   const uint8_t *k, *k_scale;
@@ -161,13 +166,21 @@ __device__ inline unsigned sortable(float x) {
 }
 
 // 16 queries of a key head (rows beyond the group are zeros) in codes, as operands of products of 64 values, the last of them
-// zeros where D is no multiple of 64; and the scales of the four rows that a lane has in a result, -1 for rows that are none.
+// zeros where D is no multiple of 64; and of the four rows that a lane has in a result the scales, and -infinity where there is no row.
 // (One product of 32 values in the place of the zeros: sums that went from a product of 64 into one of 32 were wrong now
 // and then in 96 values a head, in this loop and not by themselves.)
 template <int D> struct Queries {
   i4 codes[(D + 63) / 64];
-  float scale[4];
+  float scale[4], none[4];
 };
+
+// Of four lanes, 16 apart
+__device__ inline float quarters_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // The rows from 16 * `part` on of `tokens` tokens times the group
 template <class T, int D>
@@ -190,26 +203,29 @@ __device__ inline void load_queries(const Select& a, const T* rows, int tokens, 
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < kValues; i++) most = fmaxf(most, fabsf(x[i]));
-  most = fmaxf(most, __shfl_xor(most, 16));
-  most = fmaxf(most, __shfl_xor(most, 32));
-  const int e = power_of(most);
+  const int e = power_of(quarters_max(most));
+  const float by = __uint_as_float((unsigned)(127 - e) << 23);
   unsigned words[kValues / 4];
 #pragma unroll
   for (int i = 0; i < kValues / 4; i++) {
     unsigned w = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const float code = fminf(fmaxf(__builtin_rintf(ldexpf(x[4 * i + j], -e)), -(float)kMostCode), (float)kMostCode);
-      w |= ((unsigned)(int)code & 0xffu) << (8 * j);
+      // the sum's last bits are the nearest whole number's, of ties the even one's
+      const float code = __builtin_amdgcn_fmed3f(x[4 * i + j] * by, -(float)kMostCode, (float)kMostCode) + 12582912.f;
+      w |= (__float_as_uint(code) & 0xffu) << (8 * j);
     }
     words[i] = w;
   }
 #pragma unroll
   for (int c = 0; c < kValues / 16; c++)
     q.codes[c] = i4{(int)words[4 * c], (int)words[4 * c + 1], (int)words[4 * c + 2], (int)words[4 * c + 3]};
-  const float scale = is ? ldexpf(1.f, e) : -1.f;
+  const float scale = __uint_as_float((unsigned)(127 + e) << 23), none = is ? 0.f : -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 4; i++) q.scale[i] = __shfl(scale, 4 * quarter + i);
+  for (int i = 0; i < 4; i++) {
+    q.scale[i] = __shfl(scale, 4 * quarter + i);
+    q.none[i] = __shfl(none, 4 * quarter + i);
+  }
 }
 
 // What a token may see: blocks up to `blocks`, of which those from near_from on and those before `from` are listed in any
@@ -382,7 +398,7 @@ __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(c
             for (int c = 0; c < kParts; c++) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.codes[c], part[u][c], sum, 0, 0, 0);
             float row[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) row[i] = q.scale[i] < 0.f ? -INFINITY : (float)sum[i] * q.scale[i];
+            for (int i = 0; i < 4; i++) row[i] = __builtin_fmaf((float)sum[i], q.scale[i], q.none[i]);
             const int at = base + 16 * u + n16;
             const auto store = [&](int from, int near_from, int t, float most) {
               const float score = !there[u] ? -INFINITY : byte[u] == kNoNumber ? INFINITY : most * scale_of(byte[u]);
@@ -400,8 +416,7 @@ __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(c
                   const int r = 4 * quarter + i;
                   most = fmaxf(most, tokens == 1 || (r >= t * a.group && r < (t + 1) * a.group) ? row[i] : -INFINITY);
                 }
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
+                most = quarters_max(most);
                 if (parts > 1) most = best[u] = fmaxf(best[u], most);
                 if (quarter == 0 && p == parts - 1) store(from[t], near_from[t], t, most);
               }

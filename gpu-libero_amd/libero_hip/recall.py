@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import episodes
-from .episodes import (ERR_WORKSPACE, MxAttention, MxSelection, MxSummaries, _check, _chunk, _current, _elsewhere, _on, _output,
+from .episodes import (ERR_WORKSPACE, MxAttention, MxRows, MxSelection, MxSummaries, _check, _chunk, _current, _elsewhere, _on, _output,
                        _require, _rows)
 
 MOST_LISTED, MOST_TOP = 4096, 1024
@@ -150,8 +150,12 @@ def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal
         max_count = chunk.tokens if start is not None else chunk.count
     _require(0 <= max_count < 2 ** 31 and math.isfinite(scale), 'max_count must be a number of tokens and scale finite: %s, %s',
              max_count, scale)
-    out = _output(q, out)
-    a = MxAttention(rows, _rows(pages, out, shape, 'out'), None, None, 0, max_count, 1 if causal else 0, 0, scale, 0)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        to = MxRows(out.data_ptr(), rows.heads * s.head_dim, s.head_dim, rows.heads, rows.type)
+    else:
+        to = _rows(pages, _output(q, out), shape, 'out')
+    a = MxAttention(rows, to, None, None, 0, max_count, 1 if causal else 0, 0, scale, 0)
     if lse is not None:
         _require(lse.dtype == torch.float32 and lse.shape == shape[:-1] and lse.is_contiguous()
                  and lse.get_device() == pages.index, 'lse must be contiguous float32 of q\'s shape without head_dim')

@@ -189,10 +189,12 @@ def enter(pages, rotary, q, k, v, start=None, *, out=None, stream=None):
     chunk = _chunk(pages, shape[:-2], start)
     a, b, c = _rows(pages, q, q.shape, 'q'), _rows(pages, k, shape, 'k'), _rows(pages, v, shape, 'v')
     _require(a.heads > 0, 'q has no heads')
-    if out is not None:
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        to = MxRows(out.data_ptr(), a.heads * s.head_dim, s.head_dim, a.heads, a.type)
+    else:
         _require(not (_overlap(out, q) or _overlap(out, k) or _overlap(out, v)), 'out must be apart from q, k and v')
-    out = _output(q, out)
-    to = _rows(pages, out, q.shape, 'out')
+        to = _rows(pages, _output(q, out), q.shape, 'out')
     rc = (episodes._LIB or episodes.load()).mx_episode_enter(ct.byref(s), ct.byref(chunk), ct.byref(rotary.struct), ct.byref(a), ct.byref(to),
                                           ct.byref(b), ct.byref(c), _current(pages.index))
     if rc:
