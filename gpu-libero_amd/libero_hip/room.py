@@ -15,10 +15,11 @@ from __future__ import annotations
 
 import ctypes as ct
 
+import numpy as np
 import torch
 
 from . import episodes
-from .episodes import MxChunk, MxRoom, MxRoomChange, _PAGE_TOKENS, _check, _current, _on, _require
+from .episodes import MxChunk, MxRoom, MxRoomChange, _PAGE_TOKENS, _captured, _check, _current, _on, _require
 
 REFUSED = {1: 'a world would hold more tokens than it may, or fewer than none', 2: 'the free pages do not suffice',
            4: 'more new rows than there is space for'}
@@ -77,7 +78,8 @@ def make_room(room, count, over=None, *, rows=None, stream=None):
     leave tables and free pages as they were.  If a world would pass the room's tokens or fall below none, if the free
     pages do not suffice, or if there are more new tokens than ``rows`` (what the caller's tensors hold; for a tensor of counts
     as many as there may be), no world gets or gives back any token: ``start`` is all 0, so that nothing is written or
-    computed, and ``room.state[1]`` says why.  The worlds of ``over`` are empty all the same."""
+    computed, and ``room.state[1]`` says why.  The worlds of ``over`` are empty all the same.  Changes of one room from several
+    streams are the caller's to order."""
     if _away(room, stream):
         tensors = (count if torch.is_tensor(count) else None, over, room.table, room.length, room.free, room.state)
         return _on(room.device, stream, tensors, lambda: make_room(room, count, over, rows=rows))
@@ -92,9 +94,10 @@ def make_room(room, count, over=None, *, rows=None, stream=None):
         rows = 2 ** 31 - 1 if rows is None else rows
     else:
         _require(-2 ** 31 < count < 2 ** 31, 'count must be a number of tokens, got %s', count)
-        change.each = count
+        change.each = int(count)
         rows = min(s.nworld * max(count, 0), 2 ** 31 - 1) if rows is None else rows
     _require(0 <= rows < 2 ** 31, 'rows must be a number of rows, got %s', rows)
+    rows = int(rows)
     if over is not None:
         _require(over.dtype in (torch.bool, torch.uint8) and over.shape == (s.nworld,) and over.is_contiguous()
                  and over.get_device() == room.index, 'over must be contiguous bool of shape (nworld,) on the room\'s device')
@@ -167,35 +170,48 @@ class DeviceEpisodeCache(episodes.Layers):
         state = torch.tensor([self.pages, 0], dtype=torch.int32, device=self.device)
         self.room = Room(self.table, self.length, self.pages, self.page_tokens, free, state, tokens=self.tokens)
 
+    def _change(self):
+        if not _captured(None):               # replays are the caller's to order
+            super()._change()
+
+    def _change_done(self):
+        if not _captured(None):
+            super()._change_done()
+
     def extend(self, count=1, over=None, *, rows=None, most=None):
         """Empty the worlds of ``over``, then make room for new tokens of every world, as :func:`make_room`, and return their
-        chunk.  ``count``: a number, or int32 on the device, with ``rows`` (how many rows the step's tensors have) and ``most``
-        (the most of one world, if known)."""
+        chunk.  ``count``: a number, or int32 on the device, with ``rows`` (how many rows the step's tensors have; those beyond the
+        counts' sum belong to no world, and what is computed from them is not defined) and ``most`` (the most of one world,
+        if known: rows of a world beyond it are not attended from)."""
+        if torch.is_tensor(count):
+            _require(rows is not None, 'give rows with a tensor of counts')
+            most = rows if most is None else most
+            _require(0 <= most < 2 ** 31, 'most must be a number of tokens, got %s', most)
+            shape = (rows,)
+        else:
+            _require(count >= 0, 'count must not be negative; take tokens back with take_back')
+            _require(most is None and rows in (None, self.nworld * count), 'rows and most go with a tensor of counts')
+            most, rows = count, self.nworld * count
+            _require(rows < 2 ** 31, 'a chunk has fewer than 2^31 rows: %d worlds of %d', self.nworld, count)
+            shape = (self.nworld, count)
         self._change()
         start = make_room(self.room, count, over, rows=rows)
         self._change_done()
-        if torch.is_tensor(count):
-            _require(rows is not None, 'give rows with a tensor of counts')
-            return DeviceChunk(start, rows, rows if most is None else most, (rows,))
-        _require(count >= 0, 'count must not be negative; take tokens back with take_back')
-        return DeviceChunk(start, self.nworld * count, count, (self.nworld, count))
+        return DeviceChunk(start, rows, most, shape)
 
     def take_back(self, count):
-        """The last ``count`` tokens of every world (a number, or int32 on the device) are gone, as if they had never been."""
-        if torch.is_tensor(count):
-            count = -count
-        else:
-            _require(count >= 0, 'count must not be negative')
-            count = -count
+        """The last ``count`` tokens of every world (a number, or int32 on the device, none negative) are gone, as if they had
+        never been."""
+        _require(torch.is_tensor(count) or count >= 0, 'count must not be negative')
         self._change()
-        make_room(self.room, count)
+        make_room(self.room, -count, rows=0)
         self._change_done()
 
     def reset(self, over=None):
         """Empties the worlds of ``over`` (bool on the device; None: all)."""
+        self._change()
         if over is None:
             over = torch.ones(self.nworld, dtype=torch.bool, device=self.device)
-        self._change()
         make_room(self.room, 0, over)
         self._change_done()
 
@@ -203,19 +219,28 @@ class DeviceEpisodeCache(episodes.Layers):
         """:func:`places` of the chunk's rows, in the chunk's shape."""
         return tuple(x.view(chunk.shape) for x in places(self.room, chunk.start, tokens=chunk.tokens))
 
+    def _seen(self, x):
+        """A tensor's values after the last change, on the host."""
+        other = self._enter(None)
+        x = x.cpu()
+        self._leave(other)
+        return x
+
     def check(self):
         """Raises RuntimeError if a change was refused since the last call; waits for the device."""
-        why = int(self.room.state[1])
+        why = int(self._seen(self.room.state)[1])
         if why:
+            self._change()
             self.room.state[1] = 0
+            self._change_done()
             raise RuntimeError('episode memory: ' + '; '.join(text for bit, text in REFUSED.items() if why & bit))
 
     @property
     def free_pages(self):
         """How many pages are free; waits for the device."""
-        return int(self.room.state[0])
+        return int(self._seen(self.room.state)[0])
 
     @property
     def lengths(self):
         """The worlds' tokens (numpy); waits for the device."""
-        return self.length.cpu().numpy().astype('int64')
+        return self._seen(self.length).numpy().astype(np.int64)

@@ -645,3 +645,46 @@ def test_gathered_in_batches_of_heads(gpu_available):
         kept = [x.clone() for x in got]
         for a, b in zip(kept, call()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dim,kind,store', [(64, 'bf16', 'fp8'), (128, 'f16', 'f16'), (32, 'bf16', 'bf16')])
+def test_many_short_lists(gpu_available, dim, kind, store):
+    """Lists of few keys in thousands of worlds: one wave to a tile."""
+    print('case recall short lists', dim, kind, store, flush=True)
+    lengths = np.random.default_rng(dim).integers(0, 150, 1100)
+    world = World(lengths, 2, dim, 16, store, seed=dim)
+    check(world, [1] * 1100, 2, kind, 16, 3, 1, 1, uniform=True)
+
+
+def test_two_graphs_side_by_side(gpu_available):
+    """Two captured recalls, gathered and split, replayed at once on two streams: neither uses the other's memory."""
+    import torch
+    print('case recall two graphs', flush=True)
+    made = []
+    for seed, (lengths, count, top) in enumerate((([900, 700], 200, 4), ([20000, 9000], 1, 300))):
+        world = World(lengths, 2, 64, 64, 'bf16', seed=30 + seed)
+        s = summarised(world, 64 if count > 1 else 16)
+        q = torch.randn((2, count, 4, 64), device='cuda').bfloat16()
+
+        def call(world=world, s=s, q=q, top=top):
+            blocks = recall.select(s, q, top=top)
+            return recall.recall(world.pages, q, blocks, block_tokens=s.block_tokens)
+
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        made.append((graph, got, q, call, torch.cuda.Stream()))
+    for _ in range(4):
+        for _, _, q, _, _ in made:
+            q.normal_()
+        want = [call() for _, _, _, call, _ in made]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for graph, _, _, _, side in made:
+                with torch.cuda.stream(side):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for (_, got, _, _, _), x in zip(made, want):
+            assert torch.equal(got, x)

@@ -323,3 +323,58 @@ def test_refusals(gpu_available):
     with pytest.raises(ValueError, match='worlds'):
         room.make_room(many, 1)
     assert not length.any() and not state.any()
+
+
+def test_wrong_calls_change_nothing(gpu_available):
+    import torch
+    print('case room wrong calls', flush=True)
+    c = room.DeviceEpisodeCache(4, kv_heads=1, head_dim=32, tokens=50, storage='bf16', page_tokens=16)
+    c.extend(5)
+    before = [x.clone() for x in (c.table, c.length, c.room.state, c.room.free)]
+    two = torch.full((4,), 2, dtype=torch.int32, device='cuda')
+    for call in (lambda: c.extend(two), lambda: c.extend(-1), lambda: c.extend(1, rows=3), lambda: c.extend(1, most=1),
+                 lambda: c.extend(two.long(), rows=8), lambda: c.extend(two, rows=-1), lambda: c.extend(two, rows=8, most=-1),
+                 lambda: c.take_back(-1), lambda: c.reset(two), lambda: c.extend(1, two.bool()[:3]), lambda: c.extend(2 ** 31)):
+        with pytest.raises(ValueError):
+            call()
+    c.take_back(-two)                                # counts that are not to be: refused on the device
+    with pytest.raises(RuntimeError, match='more new rows'):
+        c.check()
+    for x, y in zip((c.table, c.length, c.room.state, c.room.free), before):
+        assert torch.equal(x, y)
+    assert c.extend(np.int64(2)).shape == (4, 2) and c.lengths.tolist() == [7] * 4
+
+
+@pytest.mark.parametrize('busy', ['changes', 'calls'])
+def test_device_cache_streams_keep_their_order(gpu_available, busy):
+    """Changes on one stream, calls and what the host reads on another, whichever is behind."""
+    import torch
+    print('case device cache order', busy, flush=True)
+    gen = torch.Generator('cuda').manual_seed(3)
+    rows = [[torch.randn((5, 3, h, 64), generator=gen, device='cuda').bfloat16() for h in (2, 2, 4)] for _ in range(5)]
+
+    def play(side):
+        c = room.DeviceEpisodeCache(5, kv_heads=2, head_dim=64, tokens=64, storage='bf16', page_tokens=16, pages=9, block_tokens=16)
+        torch.cuda.synchronize()
+        outs, lengths = [], []
+        for i, (k, v, q) in enumerate(rows):
+            if busy == 'calls' and side is not None:
+                with torch.cuda.stream(side):
+                    torch.cuda._sleep(20_000_000)
+            if busy == 'changes':
+                torch.cuda._sleep(20_000_000)
+            over = torch.tensor([i == 3, False, i == 2, False, i == 3], device='cuda')
+            chunk = c.extend(3, over)
+            options = dict(stream=side) if side is not None else {}
+            c.write(chunk, k, v, **options)
+            outs += [c.attend(chunk, q, **options), c.recall(chunk, q, top=1, **options)]
+            with torch.cuda.stream(side):
+                lengths.append(c.lengths.tolist())
+        torch.cuda.synchronize()
+        return outs, lengths
+
+    want, lengths = play(None)
+    got, again = play(torch.cuda.Stream())
+    assert lengths == again and lengths[3] == [3, 12, 6, 12, 3]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
