@@ -271,13 +271,15 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   return choose(a, launch);
 }
 
-// Whether rows are gathered by the blocks that they share, so that a block's keys and values are read for up to 128 rows
-// at once and each row has as many parts as its list has entries, which are written and read again in 32 bits.  By what either way takes to an
-// entry of a token and key head, in ns: 0.3 and 0.075 (8 bits: 0.095) for each KB of the block's keys and values, or 0.45 for
-// each KB of the parts and 10 for each tile, a tenth more for marking and listing.  us, gathered and not, of 128 values in bfloat16 but where said, 19 blocks of 64 tokens listed:
-// 2048 tokens over 65536, 32 heads on 8, 475 and 911 (8-bit pages 443 and 555), 512 tokens 171 and 234, 256 tokens 124 and
-// 123; 4 x 1024 over 8192, 8 heads on 8, 265 and 1482, 32 on 4, 858 and 758, 32 on 8 of 256 values 1171 and 3808; 16 x 256 over
-// 8192, 16 on 4 of 64 values, 172 and 262 (163 and 201); 64 x 64 over 4096 205 and 240; 300 x 41 over 1024, 12 on 4 of 96 values, blocks of 32, 631 and 533.
+// Whether rows are gathered by the blocks that they share, so that a block's keys and values are read for up to 128
+// rows at once and each row has as many parts as its list has entries, which are written and read again in 32 bits.  By
+// what either way takes to an entry of a token and key head, in ns: 0.3 and 0.075 (8 bits: 0.095) for each KB of the
+// block's keys and values, or 0.45 for each KB of the parts and 10 for each tile, a tenth more for marking and listing.
+// us, gathered and not, of 128 values in bfloat16 but where said, 19 blocks of 64 tokens listed: 2048 tokens over
+// 65536, 32 heads on 8, 475 and 911 (8-bit pages 443 and 555), 512 tokens 171 and 234, 256 tokens 124 and 123; 4 x 1024
+// over 8192, 8 heads on 8, 265 and 1482, 32 on 4, 858 and 758, 32 on 8 of 256 values 1171 and 3808; 16 x 256 over 8192,
+// 16 on 4 of 64 values, 172 and 262 (163 and 201); 64 x 64 over 4096 205 and 240; 300 x 41 over 1024, 12 on 4 of 96
+// values, blocks of 32, 631 and 533.
 constexpr int64_t kMostParts = 1 << 25, kMostBytes = 1 << 30, kBatchBytes = 192 << 20;
 bool choose_gathered(Attend& a, Launch& launch) {
   const int64_t blocks = (int64_t)a.width << (a.page_shift - a.block_shift), block = 1LL << a.block_shift;
@@ -360,7 +362,8 @@ int choose(Attend& a, Launch& launch) {
 // Batches of key heads whose rows are gathered one after the other
 int batches_of(const Attend& a) { return (a.kv_heads + a.batch_heads - 1) / a.batch_heads; }
 
-// The workspace: sums, (maximum, sum of weights) of each part, and for gathered rows the tiles' numbers, tiles, their rows and marks
+// The workspace: sums, (maximum, sum of weights) of each part, and for gathered rows the tiles' numbers, tiles, their
+// rows and marks
 struct Workspace {
   size_t ml, counts, tiles, rows, marks, bytes;
 };

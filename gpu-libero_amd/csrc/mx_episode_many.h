@@ -58,7 +58,11 @@ constexpr int many_keys(int D) { return D <= 128 ? 64 : 32; }
 constexpr int many_waves(int D, bool fp8) { return D <= 32 ? 4 : D <= (fp8 ? 64 : 96) ? 3 : D <= 128 ? 2 : 1; }
 
 // kListed: rows that share a block in their lists (mx_episode_recall), gathered from all of a chunk's tokens; the keys are
-// the block's alone, and what comes out is the part of each of those rows that has the place of the block in its list.
+// the block's alone, and what comes out is the part of each of those rows that has the place of the block in its list.  The
+// probabilities are in two parts, as in attend_few.  2048 tokens over 65536, 32 heads on 8 of 128 values, 19 blocks of 64
+// listed: four batches of 74 us, and 28 to join each one's parts.  Bound by latency and by writing the parts (647 MB in all;
+// without that 151 us for the whole): three workgroups to a CU 272 instead of 294 (32 keys are weighed at a time, in fewer registers), parts
+// written row by row through LDS the same, all heads at once 272 and 171 to join what is then no longer in the last cache.
 template <int kType, bool kFp8, bool kLarge, int D, bool kListed = false>
 __global__ __launch_bounds__(256, kListed && D == 128 ? 3 : many_waves(D, kFp8)) void attend_many(const Attend) {
   const Attend& a = arguments();

@@ -37,8 +37,10 @@ struct Summarise {
   int nworld, npage, width, kv_heads, page_shift, block_shift, tokens, count, per;   // per: blocks of a world's chunk at most
 };
 
-// A workgroup takes a block and a wave its heads in turn: lanes side by side along a key, as many keys as fit beside each other, sums in 64 bits
-// joined through LDS.  World w of ragged chunks has the items from start[w] / block_tokens + w on.
+// A workgroup takes a block and a wave its heads in turn (2048 tokens' 32 blocks, 8 heads of 128 values: 9.5 us; a step
+// in which few of 1024 worlds complete one: 4.7): lanes side by side along a key, as many keys as fit beside each
+// other, sums in 64 bits joined through LDS.  World w of ragged chunks has the items from start[w] / block_tokens + w
+// on.
 template <int kStore, int D>
 __global__ __launch_bounds__(256) void summarise_blocks(const Summarise a) {
   constexpr int kAcross = D / 8, kDown = 64 / kAcross, kPer = (D + 63) / 64;
@@ -165,10 +167,10 @@ __device__ inline unsigned sortable(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// 16 queries of a key head (rows beyond the group are zeros) in codes, as operands of products of 64 values, the last of them
-// zeros where D is no multiple of 64; and of the four rows that a lane has in a result the scales, and -infinity where there is no row.
-// (One product of 32 values in the place of the zeros: sums that went from a product of 64 into one of 32 were wrong now
-// and then in 96 values a head, in this loop and not by themselves.)
+// 16 queries of a key head (rows beyond the group are zeros) in codes, as operands of products of 64 values, the last
+// of them zeros where D is no multiple of 64; and of the four rows that a lane has in a result the scales, and
+// -infinity where there is no row. (One product of 32 values in the place of the zeros: sums that went from a product
+// of 64 into one of 32 were wrong now and then in 96 values a head, in this loop and not by themselves.)
 template <int D> struct Queries {
   i4 codes[(D + 63) / 64];
   float scale[4], none[4];
@@ -244,9 +246,9 @@ __device__ inline Seen seen_by(const Select& a, bool is, int position, int reach
   return s;
 }
 
-// One wave: of `rows` rows of 64 keys (0: none) the `want` largest, of equal ones the first, in their order.  The first `kept`
-// are those of blocks chosen before, whose numbers are in kept_block; the others' follow from `base`.  The key of the last
-// one chosen is found bit by bit, counting with ballots, until as many as are wanted are above.
+// One wave: of `rows` rows of 64 keys (0: none) the `want` largest, of equal ones the first, in their order.  The first
+// `kept` are those of blocks chosen before, whose numbers are in kept_block; the others' follow from `base`.  The key
+// of the last one chosen is found bit by bit, counting with ballots, until as many as are wanted are above.
 template <int kRows, class Put>
 __device__ inline void choose_rows(const unsigned* keys, int rows, int want, Put put) {
   const int lane = threadIdx.x & 63;
@@ -286,12 +288,15 @@ __device__ inline void choose_rows(const unsigned* keys, int rows, int want, Put
   }
 }
 
-// kTeam waves choose the blocks of up to kMostTile tokens of a world and a key head (1: four such units to a workgroup, of one token
-// each).  They score 64 blocks at a time for all of them, by products of 16 rows (tokens times query heads) with 16 summaries, into LDS; then a wave chooses for
-// each token.  More blocks than LDS has room for go in segments, the chosen ones of those before among the next.
+// kTeam waves choose the blocks of up to kMostTile tokens of a world and a key head (1: four such units to a workgroup,
+// of one token each).  They score 64 blocks at a time for all of them, by products of 16 rows (tokens times query
+// heads) with 16 summaries, into LDS; then a wave chooses for each token.  More blocks than LDS has room for go in
+// segments, the chosen ones of those before among the next.
 //
-// What bounds it: for a step's tokens a chain of loads that depend on each other (length, table, summaries), for prompts the
-// products and the counting.
+// What bounds it: for a step's tokens a chain of loads that depend on each other (length, table, summaries), for
+// prompts the instructions of scoring and counting (VALU 50 % busy).  1024 worlds' single tokens, 4 key heads of 64
+// values, up to 128 blocks: 14.6 us (the bytes 4); two worlds of 2048 blocks, 8 key heads of 128 values: 18.4; 2048
+// tokens over 1024 blocks: 98 (343 with a team to each token, whose waves counted together).
 template <int kType, int D, int kTeam>
 __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(const Select) {
   // read where they are used: as a parameter they would be in scalar registers throughout, and those of the loops spilled
@@ -360,21 +365,28 @@ __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(c
       const bool segment_before = segment > low;
       const int kept_rows = (kept + 63) >> 6, last = min(segment + 64 * (a.pieces - kept_rows), high);
       const int rows_new = (last - segment + 63) >> 6;
-      // few of many: each wave chooses from neighbouring rows of its own first, so that one wave is left with a share of all
-      // (32 of 2048 blocks 26 -> 19 us)
+      // few of many: each wave chooses from neighbouring rows of its own first, so that one wave is left with a share
+      // of all (32 of 2048 blocks 26 -> 19 us)
       const bool shared = kTeam == 16 && !segment_before && last == high && a.top <= kShare;
       const int each = (rows_new + kTeam - 1) / kTeam;
       // one piece at a time: with the next one's summaries under way a wave has half as many beside it (two pieces of 64
       // values 15.5 -> 22.5 us)
+      const int step = shared ? 1 : kTeam, rows_end = shared ? min((wave + 1) * each, rows_new) : rows_new;
+      int pages[4];                                // of the next piece's blocks
+      const auto look_up = [&](int row) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) pages[u] = table[min(segment + 64 * row + 16 * u + n16, last - 1) >> per_shift];
+      };
+      look_up(shared ? wave * each : wave);
 #pragma unroll 1
-      for (int row = shared ? wave * each : wave; row < (shared ? min((wave + 1) * each, rows_new) : rows_new); row += shared ? 1 : kTeam) {
+      for (int row = shared ? wave * each : wave; row < rows_end; row += step) {
         const int base = segment + 64 * row;
         i4 part[4][kParts];
         unsigned byte[4];
         bool there[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-          const int block = min(base + 16 * u + n16, last - 1), page = table[block >> per_shift];
+          const int block = min(base + 16 * u + n16, last - 1), page = pages[u];
           there[u] = (unsigned)page < (unsigned)a.npage;
           const int64_t entry = (((int64_t)(there[u] ? page : 0) * a.kv_heads + head) << per_shift) + (block & ((1 << per_shift) - 1));
           const int8_t* codes = a.codes + entry * D;
@@ -386,6 +398,7 @@ __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(c
           }
           byte[u] = a.exponent[entry];
         }
+        look_up(row + step);
         float best[4];                             // of the first token, where it has more rows than one product
 #pragma unroll
         for (int u = 0; u < 4; u++) best[u] = -INFINITY;
@@ -478,9 +491,9 @@ __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(c
 }
 
 // ---------------------------------------------------------------------------- rows gathered by their blocks
-// A workgroup takes 32 tokens of a world's chunk and a key head: the bits of all blocks that their lists name, collected in
-// LDS (so many blocks at a time), and written side by side: marks[world, key head][word][block].  Entries of whose keys
-// the row sees none get empty parts.
+// A workgroup takes 32 tokens of a world's chunk and a key head (2048 tokens' 19 blocks, 8 heads: 5 us; with atomics in
+// memory 28): the bits of all blocks that their lists name, collected in LDS (so many blocks at a time), and written
+// side by side: marks[world, key head][word][block].  Entries of whose keys the row sees none get empty parts.
 constexpr int kMarked = 8192;
 __global__ __launch_bounds__(256) void mark_rows(const Attend a) {
   __shared__ unsigned bits[kMarked];
@@ -512,8 +525,9 @@ __global__ __launch_bounds__(256) void mark_rows(const Attend a) {
   }
 }
 
-// A workgroup takes 16 blocks of a world's key head, a wave four of them in turn: how many tiles their tokens are, places for those in any
-// order among the others' of the batch, as each row's part is its own, and the tokens in their order.
+// A workgroup takes 16 blocks of a world's key head, a wave four of them in turn: how many tiles their tokens are,
+// places for those in any order among the others' of the batch, as each row's part is its own, and the tokens in their
+// order.
 constexpr int kCounted = 16;
 __global__ __launch_bounds__(256) void list_tiles(const Attend a) {
   __shared__ int sh_tokens[kCounted], sh_from[kCounted];

@@ -1,11 +1,13 @@
 // Room for tokens: the worlds' tables and lengths and the stack of free pages change on the GPU, and a chunk's rows learn
 // their worlds, positions and slots.
 //
-// Where a world's pages come off the stack follows from the needs of all worlds before it, and whether they do at all from
-// everyone's.  One workgroup does all for up to 1024 worlds with few pages.  For more there are two launches: there are few
-// numbers to a world, so each workgroup reads all of them again for its prefix and the totals instead of waiting for its
-// neighbours; lengths then change in the second launch, which also hands out the pages that the first has put on the stack.
-// Bound by launches and by a few dependent loads.
+// Where a world's pages come off the stack follows from the needs of all worlds before it, and whether they do at all
+// from everyone's.  One workgroup does all for up to 1024 worlds with few pages.  For more there are two launches:
+// there are few numbers to a world, so each workgroup reads all of them again for its prefix and the totals instead of
+// waiting for its neighbours; lengths then change in the second launch, which also hands out the pages that the first
+// has put on the stack. Bound by launches and by a few dependent loads: 67 worlds 3.6 us; 4096 worlds that all restart
+// 10 and 3 us, of which the reading of all worlds is most (with sums in 64 bits 13, with 1024 threads to a workgroup
+// 13).  The places of their 2.1 million rows (25 MB): 13 us, 9 where all worlds have the same number.
 #include "mx_episode_move.h"
 #include "mx_episode_launch.h"
 
@@ -20,8 +22,8 @@ struct Room {
   int nworld, width, npage, page_shift, tokens, each, rows, worlds_each;
 };
 
-// What a change does to a world: its tokens before (of which `base` stay at most) and after, its pages that stay, that it has,
-// and that it then has
+// What a change does to a world: its tokens before (of which `base` stay at most) and after, its pages that stay, that
+// it has, and that it then has
 struct Change {
   int base, after, kept, held, need, rows;
   bool refused;
@@ -168,9 +170,9 @@ __global__ __launch_bounds__(256) void update_count(const Room a) {
   __shared__ long long sums[4][2], sh[4][2], before[kMostWorlds];
   __shared__ int from[kMostWorlds], parts[4][6];
   const int first = blockIdx.x * a.worlds_each, worlds = min(a.nworld - first, a.worlds_each);
-  // sums over all worlds: pages needed and rows, in 64 bits as there may be any number of them; pages back (of emptied worlds alone,
-  // and all); and over those before this workgroup's: pages back, needed, and rows, which are right if the change is not
-  // refused
+  // sums over all worlds: pages needed and rows, in 64 bits as there may be any number of them; pages back (of emptied
+  // worlds alone, and all); and over those before this workgroup's: pages back, needed, and rows, which are right if
+  // the change is not refused
   long long wide[2] = {0, 0};
   int x[6] = {0, 0, 0, 0, 0, 0}, refused = 0;
   constexpr int kAhead = 8;                       // worlds of a thread whose numbers are under way together

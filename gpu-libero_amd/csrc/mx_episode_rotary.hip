@@ -1,9 +1,16 @@
 // Rotary positions: rows turned by given positions, and a chunk's queries and keys turned by their places in their
 // worlds, the keys on their way into the pages.
 //
-// A pair (x_a, x_b) of a row at position p turns by the angle p * turn: y_a = c x_a - s x_b, y_b = s x_a + c x_b.  Three
-// operations to a value that is read and written once: bound by memory, or, for a step's few rows, by the launch.  A
-// workgroup first computes cosines and sines of its tokens' pairs into LDS, once for all heads.
+// A pair (x_a, x_b) of a row at position p turns by the angle p * turn: y_a = c x_a - s x_b, y_b = s x_a + c x_b.
+// Three operations to a value that is read and written once: bound by memory, or, for a step's few rows, by the launch.
+// A workgroup first computes cosines and sines of its tokens' pairs into LDS, once for all heads; then a thread takes
+// 16 bytes of either half of a head (of a key its own 16 or 32 bytes, as the pages' scales want them, and reads the
+// others beside).
+//
+// Prompts of 4 x 4096 tokens, 32 and 8 heads of 128 values, bfloat16 (403 MB): 72 us, 5.6 TB/s.  67 prompts of up to
+// 501 tokens, float16 into 8-bit pages, half of each head turned (116 MB): 27 us, 4.3 TB/s.  4096 single tokens into
+// 8-bit pages (25 MB): 9.9 us.  16 x 1024 tokens of 16 heads of 64 values turned (67 MB, out of the last cache): 12.3
+// us.
 #include <type_traits>
 #include "mx_episode_move.h"
 #include "mx_episode_launch.h"
@@ -35,8 +42,8 @@ struct Enter {
 constexpr int kMostTokens = 64;                 // of a workgroup: their positions are kept in LDS
 constexpr int kMostAngles = 4096;               // of a workgroup, 8 bytes of LDS each
 
-// Cosine and sine of `position` times `turn` radians, to about 2^-23.  In revolutions and 64 bits the angle is brought within an
-// eighth of one, where seven terms of Taylor's series are off by less than 2^-30.
+// Cosine and sine of `position` times `turn` radians, to about 2^-23.  In revolutions and 64 bits the angle is brought
+// within an eighth of one, where seven terms of Taylor's series are off by less than 2^-30.
 __device__ inline f2 cos_sin(double position, double turn) {
   const double t = position * (turn * 0.15915494309189535);
   const double quarters = __builtin_rint(t * 4.0);
@@ -240,13 +247,13 @@ Turned turned_rows(const MxRotary* r, const MxRows* x, const MxRows* out, int he
   return t;
 }
 
-// Tokens of a workgroup, for `pieces` of a token that its threads take one at a time: 256 to 2048 pieces, the more the
-// less often the angles' latency is waited for, if there are so many workgroups of them (67 prompts of up to 501 tokens with 256, 512, 1024 and 2048
-// pieces 57, 33, 27 and 27 us, 4096 single tokens 10.0, 10.3, 15.0 and 14.7).
+// Tokens of a workgroup, for `pieces` of a token that its threads take one at a time: 256 to 1024 pieces, the more the
+// less often the angles' latency is waited for, if there are so many workgroups of them (67 prompts of up to 501 tokens
+// with 256, 512, 1024 and 2048 pieces 57, 33, 27 and 27 us, 4096 single tokens 10.0, 10.3, 15.0 and 14.7).
 int tokens_each(int64_t pieces, int half, int64_t tokens, int groups) {
   const int64_t angles = kMostAngles / half < kMostTokens ? kMostAngles / half : kMostTokens;
   int64_t most = tokens * pieces / groups;
-  most = most < 256 ? 256 : most > 2048 ? 2048 : most;
+  most = most < 256 ? 256 : most > 1024 ? 1024 : most;
   int64_t each = most / pieces;
   each = each < 1 ? 1 : each;
   if (tokens / each >= kMostGroups / 2) each = kMostTokens;
