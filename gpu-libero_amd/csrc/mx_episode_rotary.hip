@@ -22,9 +22,9 @@ struct Turned {
   const void* x;
   void* out;
   const double* turn;
+  double amplitude;
   int64_t x_token, x_head, o_token, o_head;
   int heads, head_dim, half, tokens, each;      // half: pairs; each: tokens of a workgroup
-  float amplitude;
   bool interleaved, back, pieces;               // pieces: of 16 bytes, that no pair's end cuts
 };
 struct Rotate {
@@ -42,17 +42,18 @@ struct Enter {
 constexpr int kMostTokens = 64;                 // of a workgroup: their positions are kept in LDS
 constexpr int kMostAngles = 4096;               // of a workgroup, 8 bytes of LDS each
 
-// Cosine and sine of `position` times `turn` radians, to about 2^-23.  In revolutions and 64 bits the angle is brought
-// within an eighth of one, where seven terms of Taylor's series are off by less than 2^-30.
-__device__ inline f2 cos_sin(double position, double turn) {
+// Cosine and sine of `position` times `turn` radians, times `amplitude`, each rounded once from 64 bits: it then has no part
+// in the error of what it turns.  In revolutions the angle is brought within an eighth of one, where six and seven terms of
+// Taylor's series are off by less than 2^-36.
+__device__ inline f2 cos_sin(double position, double turn, double amplitude) {
   const double t = position * (turn * 0.15915494309189535);
   const double quarters = __builtin_rint(t * 4.0);
-  const float x = (float)(__builtin_fma(quarters, -0.25, t) * 6.283185307179586);
-  const float y = x * x;
-  const float s = x * __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), 1.f);
-  const float c = __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+  const double x = __builtin_fma(quarters, -0.25, t) * 6.283185307179586, y = x * x;
+  const auto series = [&](double sum, double next) { return __builtin_fma(y, sum, next); };
+  const double s = x * series(series(series(series(series(-1. / 39916800., 1. / 362880.), -1. / 5040.), 1. / 120.), -1. / 6.), 1.);
+  const double c = series(series(series(series(series(series(1. / 479001600., -1. / 3628800.), 1. / 40320.), -1. / 720.), 1. / 24.), -0.5), 1.);
   const int quarter = (int)(quarters - 4.0 * __builtin_floor(quarters * 0.25)) & 3;
-  const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
+  const float a = (float)(amplitude * (quarter & 1 ? s : c)), b = (float)(amplitude * (quarter & 1 ? c : s));
   return f2{quarter == 1 || quarter == 2 ? -a : a, quarter & 2 ? -b : b};
 }
 
@@ -60,9 +61,9 @@ __device__ inline f2 cos_sin(double position, double turn) {
 __device__ inline void angles(const Turned& t, int tokens, const double* position, f2* cs) {
   for (int i = threadIdx.x; i < tokens * t.half; i += 256) {
     const int token = i / t.half, pair = i - token * t.half;
-    f2 x = cos_sin(position[token], t.turn[pair]) ;
+    f2 x = cos_sin(position[token], t.turn[pair], t.amplitude);
     if (t.back) x.y = -x.y;
-    cs[i] = x * t.amplitude;
+    cs[i] = x;
   }
 }
 

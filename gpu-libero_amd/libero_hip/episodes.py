@@ -70,7 +70,7 @@ class MxAttention(ct.Structure):
 
 
 class MxRotary(ct.Structure):
-    _fields_ = [('turn', ct.c_void_p), ('width', ct.c_int32), ('interleaved', ct.c_int32), ('amplitude', ct.c_float)]
+    _fields_ = [('turn', ct.c_void_p), ('width', ct.c_int32), ('interleaved', ct.c_int32), ('amplitude', ct.c_double)]
 
 
 class MxRoom(ct.Structure):

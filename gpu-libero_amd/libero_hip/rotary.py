@@ -135,7 +135,8 @@ class _Rotate(torch.autograd.Function):
 def rotate(rotary, x, positions, *, back=False, out=None, stream=None):
     """Rows turned by their positions: x (tokens, heads, head_dim) or (batch, tokens, heads, head_dim) in float32, bfloat16 or
     float16, any strides whose rows step evenly and whose head_dim is contiguous; ``positions`` int32 or int64, contiguous, one
-    to a row, or (tokens,) for all of a batch.  Computed in 32 bits, the angle's multiples in 64, and rounded once.
+    to a row, or (tokens,) for all of a batch.  Cosines and sines are computed in 64 bits and rounded to 32, the values turned in
+    32 and rounded once.
 
     ``back`` turns by the negative angles (with the same amplitude): that is the gradient, which autograd takes where x
     requires one; its own gradient is a rotation again.  ``out``, like x and apart from it, is written if given, where no

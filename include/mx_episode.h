@@ -118,7 +118,7 @@ size_t mx_episode_workspace(const MxPages* pages, const MxChunk* chunk, const Mx
 typedef struct MxRotary {
   const double* turn;
   int32_t width, interleaved;
-  float amplitude;
+  double amplitude;
 } MxRotary;
 
 size_t mx_rotary_bytes(void);                /* sizeof(MxRotary) */

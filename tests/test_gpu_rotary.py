@@ -1,8 +1,7 @@
 """Rotary positions on the GPU against their definition in 64 bits (tests/recall_reference.py).
 
-Tolerance, from the arithmetic: the angle is reduced in 64 bits and rounded to 32 within an eighth of a turn (2^-25 of at
-most 0.79), sine and cosine are series whose last steps round once each, so that each is within 2^-23; the amplitude, the
-product and the sum round once more each (2^-24).  With pairs (a, b): |error| <= amplitude (|a| + |b|) 2^-22 + u |y|, u the unit
+Tolerance, from the arithmetic: sine and cosine, times the amplitude, are rounded once to 32 bits (2^-24), a product and the sum
+round once more each (2^-24): three of the four that are allowed for.  With pairs (a, b): |error| <= amplitude (|a| + |b|) 2^-22 + u |y|, u the unit
 roundoff of the result, and for float16 half its smallest step, 2^-25.  Positions whose angle passes 2^24 add the angle's own rounding in 64 bits, three
 of 2^-53 each.
 """
@@ -345,3 +344,22 @@ def test_refusals(gpu_available):
         with pytest.raises(ValueError):
             call()
             print('not refused', i)
+
+
+@pytest.mark.parametrize('layout', ['half', 'interleaved'])
+def test_sines_are_rounded_once(gpu_available, layout):
+    """Turned units are the amplitude's cosines and sines: within half a step of 32 bits, whatever the amplitude, the angle in
+    64 bits to within 2^-36 of an eighth of a turn and three roundings of its own."""
+    import torch
+    print('case sines', layout, flush=True)
+    turn = torch.from_numpy(np.random.default_rng(5).uniform(0.0, 7.0, 64))
+    p = np.concatenate([np.arange(70), [1 << 12, -(1 << 12), 99999, 1 << 20]])
+    turning = rotary.Rotary(turn.cuda(), layout=layout, amplitude=0.1 * np.log(8.0) + 1.0)
+    x = torch.zeros((len(p), 1, 128), device='cuda')
+    x[..., :64] = 1.0
+    if layout == 'interleaved':
+        x = x.view(len(p), 1, 2, 64).transpose(2, 3).reshape(len(p), 1, 128).contiguous()
+    got = rotary.rotate(turning, x, torch.from_numpy(p).cuda()).double().cpu().numpy()
+    want = turned(x.double().cpu().numpy(), p, turn.numpy(), turning.amplitude, layout)
+    angle = np.abs(p).astype(np.float64)[:, None, None] * 7.0
+    assert np.all(np.abs(got - want) <= 2.0 ** -24 * np.abs(want) + turning.amplitude * (2.0 ** -36 + 4 * 2.0 ** -53 * (angle + 1)))
