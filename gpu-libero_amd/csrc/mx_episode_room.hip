@@ -108,7 +108,8 @@ __device__ inline void refuse(Change& c, bool over) {
 // Pieces of work, `many` of them, that belong to a workgroup's worlds from before[o] on: their table entries count on from
 // from[o], and are moved in turn
 template <int kThreads, class Move>
-__device__ inline void each_entry(const Room& a, int first, int worlds, const long long* before, const int* from, long long many, Move move) {
+__device__ inline void each_entry(const Room& a, int first, int worlds, const long long* before, const int* from, long long many,
+                                  Move move) {
   for (long long i = threadIdx.x; i < many; i += kThreads) {
     const int o = owner(before, worlds, i);
     const long long slot = from[o] + i - before[o];
@@ -436,7 +437,8 @@ int mx_room_places(const MxRoom* room, const MxChunk* c, int32_t* world, int32_t
   a.m.page_shift = __builtin_ctz(room->page_tokens); a.m.tokens = c->tokens; a.m.count = c->count;
   a.world = world; a.position = position; a.slot = slot;
   a.vector = !(((uintptr_t)world | (uintptr_t)position | (uintptr_t)slot) & 15);
-  hipLaunchKernelGGL(find_places, dim3((unsigned)((c->tokens + 256LL * kRowsEach - 1) / (256 * kRowsEach))), dim3(256), 0, (hipStream_t)stream, a);
+  const unsigned groups = (unsigned)((c->tokens + 256LL * kRowsEach - 1) / (256 * kRowsEach));
+  hipLaunchKernelGGL(find_places, dim3(groups), dim3(256), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 

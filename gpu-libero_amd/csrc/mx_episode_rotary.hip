@@ -49,9 +49,9 @@ __device__ inline f2 cos_sin(double position, double turn, double amplitude) {
   const double t = position * (turn * 0.15915494309189535);
   const double quarters = __builtin_rint(t * 4.0);
   const double x = __builtin_fma(quarters, -0.25, t) * 6.283185307179586, y = x * x;
-  const auto series = [&](double sum, double next) { return __builtin_fma(y, sum, next); };
-  const double s = x * series(series(series(series(series(-1. / 39916800., 1. / 362880.), -1. / 5040.), 1. / 120.), -1. / 6.), 1.);
-  const double c = series(series(series(series(series(series(1. / 479001600., -1. / 3628800.), 1. / 40320.), -1. / 720.), 1. / 24.), -0.5), 1.);
+  const auto to = [&](double sum, double next) { return __builtin_fma(y, sum, next); };
+  const double s = x * to(to(to(to(to(-1. / 39916800., 1. / 362880.), -1. / 5040.), 1. / 120.), -1. / 6.), 1.);
+  const double c = to(to(to(to(to(to(1. / 479001600., -1. / 3628800.), 1. / 40320.), -1. / 720.), 1. / 24.), -0.5), 1.);
   const int quarter = (int)(quarters - 4.0 * __builtin_floor(quarters * 0.25)) & 3;
   const float a = (float)(amplitude * (quarter & 1 ? s : c)), b = (float)(amplitude * (quarter & 1 ? c : s));
   return f2{quarter == 1 || quarter == 2 ? -a : a, quarter & 2 ? -b : b};
@@ -310,7 +310,8 @@ int mx_episode_enter(const MxPages* p, const MxChunk* c, const MxRotary* rotary,
   if ((int64_t)q->heads * p->head_dim > 1 << 24) return MX_ERR_DOMAIN;
   Enter a{};
   a.t = turned_rows(rotary, q, out, p->head_dim, c->tokens, false);
-  const int size = size_of(k->type), piece = piece_bytes(p->type == MX_TYPE_FP8, true, size) / size, q_piece = a.t.pieces ? 16 / size : 1;
+  const int size = size_of(k->type), piece = piece_bytes(p->type == MX_TYPE_FP8, true, size) / size;
+  const int q_piece = a.t.pieces ? 16 / size : 1;
   a.t.each = tokens_each(((int64_t)q->heads * p->head_dim + q_piece - 1) / q_piece, a.t.half, c->tokens, 2048);
   a.m.tokens_each = tokens_each((int64_t)p->kv_heads * p->head_dim / piece, a.t.half, c->tokens, 512);
   uint8_t *pages[2] = {(uint8_t*)p->k, (uint8_t*)p->v}, *scales[2] = {p->k_scale, p->v_scale};

@@ -603,9 +603,9 @@ class EpisodeCache(Layers):
 
     ``block_tokens``: blocks of so many tokens are summarised as they are written, for :meth:`recall`.
 
-    Each step, :meth:`extend` makes room for the new tokens; then, layer by layer, :meth:`write` (with positions: :meth:`enter`) stores their keys and
-    values and :meth:`attend` (over long episodes: :meth:`recall`) attends from their queries.  :meth:`reset` empties worlds, as
-    ``HipBatchEnv.reset(id)`` restarts them.  Tables and lengths live on the device (``table``, ``length``), with a
+    Each step, :meth:`extend` makes room for the new tokens; then, layer by layer, :meth:`write` (with positions:
+    :meth:`enter`) stores their keys and values and :meth:`attend` (over long episodes: :meth:`recall`) attends from their
+    queries.  :meth:`reset` empties worlds, as ``HipBatchEnv.reset(id)`` restarts them.  Tables and lengths live on the device (``table``, ``length``), with a
     copy on the host (``lengths``) that room is made by; pages are not cleared, their old contents are never read.
 
     :meth:`extend` and :meth:`reset` work on the current stream.  Calls on another one (``stream=``, or the current one then)

@@ -75,7 +75,8 @@ def summarise(summaries, start=None, *, count=None, tokens=None, stream=None):
     many, none = (count, tokens) if start is None else (tokens, count)
     _require(many is not None and none is None and many >= 0, 'give count (every world), or start and tokens')
     chunk = _chunk(pages, (pages.struct.nworld, count) if start is None else (tokens,), start)
-    rc = (episodes._LIB or episodes.load()).mx_episode_summarise(ct.byref(pages.struct), ct.byref(chunk), ct.byref(summaries.struct), _current(pages.index))
+    lib = episodes._LIB or episodes.load()
+    rc = lib.mx_episode_summarise(ct.byref(pages.struct), ct.byref(chunk), ct.byref(summaries.struct), _current(pages.index))
     if rc:
         _check(rc, 'mx_episode_summarise')
 
@@ -103,7 +104,8 @@ def select(summaries, q, start=None, *, top, near=1, first=0, causal=True, max_c
     _require(0 <= max_count < 2 ** 31 and 0 <= top <= MOST_TOP and near >= 1 and first >= 0,
              'max_count and first must not be negative, top at most %d and near at least 1', MOST_TOP)
     listed = first + near + top + (0 if causal else (max_count + summaries.block_tokens - 2) // summaries.block_tokens)
-    _require(listed <= MOST_LISTED, 'at most %d blocks can be listed, got %d: give max_count, the largest chunk of a world', MOST_LISTED, listed)
+    _require(listed <= MOST_LISTED, 'at most %d blocks can be listed, got %d: give max_count, the largest chunk of a world',
+             MOST_LISTED, listed)
     shape = shape[:-2] + (s.kv_heads, listed)
     if out is None:
         out = torch.empty(shape, dtype=torch.int32, device=q.device)
@@ -111,8 +113,9 @@ def select(summaries, q, start=None, *, top, near=1, first=0, causal=True, max_c
         _require(out.dtype == torch.int32 and out.shape == shape and out.is_contiguous() and out.get_device() == pages.index,
                  'out must be contiguous int32 of shape %s on the pages\' device', tuple(shape))
     m = MxSelection(out.data_ptr(), listed, top, near, first, max_count, 1 if causal else 0)
-    rc = (episodes._LIB or episodes.load()).mx_episode_select(ct.byref(s), ct.byref(chunk), ct.byref(summaries.struct), ct.byref(rows), ct.byref(m),
-                                           _current(pages.index))
+    lib = episodes._LIB or episodes.load()
+    rc = lib.mx_episode_select(ct.byref(s), ct.byref(chunk), ct.byref(summaries.struct), ct.byref(rows), ct.byref(m),
+                               _current(pages.index))
     if rc:
         _check(rc, 'mx_episode_select')
     return out
@@ -121,8 +124,10 @@ def select(summaries, q, start=None, *, top, near=1, first=0, causal=True, max_c
 def _queries(pages, q, rows):
     s = pages.struct
     if not (rows.type == s.type or s.type == 3 and rows.type) or rows.heads < 1 or rows.heads % s.kv_heads:
-        _require(rows.heads > 0 and rows.heads % s.kv_heads == 0, 'q has %d heads, not a multiple of the pages\' %d', rows.heads, s.kv_heads)
-        raise ValueError('q must be bfloat16 or float16, and of the pages\' type unless those are 8-bit: %s on %s' % (q.dtype, pages.k.dtype))
+        _require(rows.heads > 0 and rows.heads % s.kv_heads == 0, 'q has %d heads, not a multiple of the pages\' %d',
+                 rows.heads, s.kv_heads)
+        raise ValueError('q must be bfloat16 or float16, and of the pages\' type unless those are 8-bit: %s on %s'
+                         % (q.dtype, pages.k.dtype))
 
 
 def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal=True, scale=None, out=None, lse=None, stream=None):
@@ -161,7 +166,8 @@ def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal
                  and lse.get_device() == pages.index, 'lse must be contiguous float32 of q\'s shape without head_dim')
         a.lse = lse.data_ptr()
     m = MxSelection(blocks.data_ptr(), blocks.shape[-1])
-    lib, refs, raw = episodes._LIB or episodes.load(), (ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(m), block_tokens), _current(pages.index)
+    lib, raw = episodes._LIB or episodes.load(), _current(pages.index)
+    refs = ct.byref(s), ct.byref(chunk), ct.byref(a), ct.byref(m), block_tokens
     rc = lib.mx_episode_recall(*refs, raw)
     if rc == ERR_WORKSPACE:               # the keys are split: found before any launch
         need = lib.mx_recall_workspace(*refs)

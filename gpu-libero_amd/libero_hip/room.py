@@ -89,7 +89,8 @@ def make_room(room, count, over=None, *, rows=None, stream=None):
     change = MxRoomChange()
     if torch.is_tensor(count):
         _require(count.dtype == torch.int32 and count.shape == (s.nworld,) and count.is_contiguous()
-                 and count.get_device() == room.index, 'count must be a number, or contiguous int32 of shape (nworld,) on the room\'s device')
+                 and count.get_device() == room.index,
+                 'count must be a number, or contiguous int32 of shape (nworld,) on the room\'s device')
         change.count = count.data_ptr()
         rows = 2 ** 31 - 1 if rows is None else rows
     else:
@@ -137,7 +138,8 @@ def places(room, start=None, *, count=None, tokens=None, stream=None):
     step = rows if rows < 4096 else rows + -rows % 4          # many rows: each of the three is 16-byte aligned
     found = torch.empty((3, step), dtype=torch.int32, device=room.table.device)
     at = found.data_ptr()
-    rc = (episodes._LIB or episodes.load()).mx_room_places(ct.byref(s), ct.byref(chunk), at, at + 4 * step, at + 8 * step, _current(room.index))
+    lib = episodes._LIB or episodes.load()
+    rc = lib.mx_room_places(ct.byref(s), ct.byref(chunk), at, at + 4 * step, at + 8 * step, _current(room.index))
     if rc:
         _check(rc, 'mx_room_places')
     if step > rows:

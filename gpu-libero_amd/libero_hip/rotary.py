@@ -108,8 +108,9 @@ def _turn(rotary, x, positions, back, out):
     _require(tokens < 2 ** 31, 'fewer than 2^31 rows can be turned at once: %s', tokens)
     if not (tokens and rows.heads):
         return out
-    rc = (episodes._LIB or episodes.load()).mx_rotate(ct.byref(rotary.struct), ct.byref(rows), ct.byref(to), x.shape[-1], tokens, positions.data_ptr(),
-                                   positions.numel(), positions.dtype == torch.int64, back, _current(rotary.index))
+    lib = episodes._LIB or episodes.load()
+    rc = lib.mx_rotate(ct.byref(rotary.struct), ct.byref(rows), ct.byref(to), shape[-1], tokens, positions.data_ptr(),
+                       positions.numel(), positions.dtype == torch.int64, back, _current(rotary.index))
     if rc:
         _check(rc, 'mx_rotate')
     return out
@@ -196,8 +197,9 @@ def enter(pages, rotary, q, k, v, start=None, *, out=None, stream=None):
     else:
         _require(not (_overlap(out, q) or _overlap(out, k) or _overlap(out, v)), 'out must be apart from q, k and v')
         to = _rows(pages, _output(q, out), q.shape, 'out')
-    rc = (episodes._LIB or episodes.load()).mx_episode_enter(ct.byref(s), ct.byref(chunk), ct.byref(rotary.struct), ct.byref(a), ct.byref(to),
-                                          ct.byref(b), ct.byref(c), _current(pages.index))
+    lib = episodes._LIB or episodes.load()
+    rc = lib.mx_episode_enter(ct.byref(s), ct.byref(chunk), ct.byref(rotary.struct), ct.byref(a), ct.byref(to), ct.byref(b),
+                              ct.byref(c), _current(pages.index))
     if rc:
         _check(rc, 'mx_episode_enter')
     return out

@@ -114,7 +114,8 @@ size_t mx_episode_workspace(const MxPages* pages, const MxChunk* chunk, const Mx
  * multiplied by amplitude; the other values stay:
  *     y_a = amplitude * (x_a cos - x_b sin),  y_b = amplitude * (x_a sin + x_b cos)
  * Pair i is (i, i + width / 2), or with `interleaved` (2 i, 2 i + 1).  turn: width / 2 angles in radians, 64 bits, on the
- * device.  The angle is reduced in 64 bits (off by 2^-52 of itself at most), sine, cosine and products are in 32 bits. */
+ * device.  The angle is reduced in 64 bits (off by 2^-52 of itself at most); its sine and cosine, times amplitude, are
+ * rounded to 32 bits, and products are in 32. */
 typedef struct MxRotary {
   const double* turn;
   int32_t width, interleaved;
@@ -179,8 +180,9 @@ int mx_room_places(const MxRoom* room, const MxChunk* chunk, int32_t* world, int
  * blocks whose summaries match it best, the latest ones, and the first ones.
  *
  * The summary of a block that is full is the mean m of its keys (in 64 bits): codes c = rint(m / 2^e), |c| <= 127, with
- * the least e from -40 to 40 at which |m| is at most 127 * 2^e (codes beyond are cut off), and the byte e + 127; a block with a key that is
- * not finite has the byte 255.  codes [npage][kv_heads][page_tokens / block_tokens][head_dim], 16-byte aligned, exponent without head_dim. */
+ * the least e from -40 to 40 at which |m| is at most 127 * 2^e (codes beyond are cut off), and the byte e + 127; a block
+ * with a key that is not finite has the byte 255.  codes [npage][kv_heads][page_tokens / block_tokens][head_dim], 16-byte
+ * aligned, exponent without head_dim. */
 typedef struct MxSummaries {
   int8_t* codes;
   uint8_t* exponent;
@@ -193,9 +195,10 @@ typedef struct MxSummaries {
  *     max over the query heads h of the key head of  (sum_d q_hd c_d) 2^(e_h + e),
  * with q_h in codes of its own head by the rule above (a NaN counts as 0, an infinity as cut off): exact in 32 bits,
  * the same on any machine.  The byte 255 stands above all scores, a table entry that names no page below.
- * blocks: tokens x kv_heads x width, filled from the left in ascending order, then -1; all of it is written, -1 for rows that see nothing,
- * belong to no world, or lie beyond max_count in it.  width is at least first + near + top, and more by
- * (max_count + block_tokens - 2) / block_tokens where queries see tokens behind them (causal 0), and at most 4096; top at most 1024. */
+ * blocks: tokens x kv_heads x width, filled from the left in ascending order, then -1; all of it is written, -1 for rows
+ * that see nothing, belong to no world, or lie beyond max_count in it.  width is at least first + near + top, and more by
+ * (max_count + block_tokens - 2) / block_tokens where queries see tokens behind them (causal 0), and at most 4096; top at
+ * most 1024. */
 typedef struct MxSelection {
   int32_t* blocks;
   int32_t width, top, near, first, max_count, causal;
