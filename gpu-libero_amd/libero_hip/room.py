@@ -95,10 +95,9 @@ def make_room(room, count, over=None, *, rows=None, stream=None):
         rows = 2 ** 31 - 1 if rows is None else rows
     else:
         _require(-2 ** 31 < count < 2 ** 31, 'count must be a number of tokens, got %s', count)
-        change.each = int(count)
+        change.each = count
         rows = min(s.nworld * max(count, 0), 2 ** 31 - 1) if rows is None else rows
     _require(0 <= rows < 2 ** 31, 'rows must be a number of rows, got %s', rows)
-    rows = int(rows)
     if over is not None:
         _require(over.dtype in (torch.bool, torch.uint8) and over.shape == (s.nworld,) and over.is_contiguous()
                  and over.get_device() == room.index, 'over must be contiguous bool of shape (nworld,) on the room\'s device')

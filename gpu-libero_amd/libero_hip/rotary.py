@@ -140,8 +140,9 @@ def rotate(rotary, x, positions, *, back=False, out=None, stream=None):
     32 and rounded once.
 
     ``back`` turns by the negative angles (with the same amplitude): that is the gradient, which autograd takes where x
-    requires one; its own gradient is a rotation again.  ``out``, like x and apart from it, is written if given, where no
-    gradient is recorded.  Returns out."""
+    requires one; its own gradient is a rotation again.  A backward pass is captured as that of torch's own operations: where
+    an eager graph of the same leaves still lives, torch cannot (give the capture leaves of its own, ``x.detach()``, or drop
+    that graph first).  ``out``, like x and apart from it, is written if given, where no gradient is recorded.  Returns out."""
     shape = x.shape
     if not (x.get_device() == rotary.index and len(shape) in (3, 4) and rotary.struct.width <= shape[-1]
             and positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous()

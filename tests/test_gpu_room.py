@@ -337,6 +337,9 @@ def test_wrong_calls_change_nothing(gpu_available):
                  lambda: c.take_back(-1), lambda: c.reset(two), lambda: c.extend(1, two.bool()[:3]), lambda: c.extend(2 ** 31)):
         with pytest.raises(ValueError):
             call()
+    for call in (lambda: c.extend(2.5), lambda: c.extend(two, rows=8.5), lambda: c.take_back(0.5)):
+        with pytest.raises(TypeError):
+            call()
     c.take_back(-two)                                # counts that are not to be: refused on the device
     with pytest.raises(RuntimeError, match='more new rows'):
         c.check()
