@@ -129,6 +129,24 @@ def test_gradient(gpu_available, layout):
     first, = torch.autograd.grad(out, x, cotangent, create_graph=True)
     second, = torch.autograd.grad(first, cotangent, weight)
     compare(second, weight, p, turning, 'f32')
+    # positions that change in between are found
+    out = rotary.rotate(turning, x, positions)
+    positions.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(out, x, weight)
+    positions.sub_(1)
+    # no rows, a batch of one token, a cotangent of other strides
+    for shape in ((0, 2, 32), (3, 0, 2, 32)):
+        y = torch.empty(shape, device='cuda', requires_grad=True)
+        at = torch.zeros(shape[:-2], dtype=torch.int32, device='cuda')
+        grad, = torch.autograd.grad(rotary.rotate(turning, y, at), y, torch.empty(shape, device='cuda'))
+        assert grad.shape == shape
+    y, c = made((6, 1, 2, 32), 'f32').requires_grad_(), made((6, 2, 32, 1), 'f32', 3).permute(0, 3, 1, 2)
+    grad, = torch.autograd.grad(rotary.rotate(turning, y, positions.view(6, 1), back=True), y, c)
+    compare(grad[:, 0], c[:, 0], p, turning, 'f32')
+    c = made((2, 6, 32), 'f32', 4).transpose(0, 1)
+    grad, = torch.autograd.grad(rotary.rotate(turning, x, positions), x, c)
+    compare(grad, c, p, turning, 'f32', back=True)
     # an expanded cotangent, in 16 bits
     y = made((6, 2, 32), 'bf16').requires_grad_()
     rotary.rotate(turning, y, positions).sum().backward()
