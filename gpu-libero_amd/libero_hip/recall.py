@@ -156,7 +156,7 @@ def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal
     _require(0 <= max_count < 2 ** 31 and math.isfinite(scale), 'max_count must be a number of tokens and scale finite: %s, %s',
              max_count, scale)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
         to = MxRows(out.data_ptr(), rows.heads * s.head_dim, s.head_dim, rows.heads, rows.type)
     else:
         to = _rows(pages, _output(q, out), shape, 'out')

@@ -100,7 +100,7 @@ def _stepping(x, name):
 def _turn(rotary, x, positions, back, out):
     rows, shape = _stepping(x, 'x'), x.shape
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
         to = MxRows(out.data_ptr(), shape[-2] * shape[-1], shape[-1], shape[-2], rows.type)
     else:
         to = _stepping(out, 'out')
@@ -201,7 +201,7 @@ def enter(pages, rotary, q, k, v, start=None, *, out=None, stream=None):
     a, b, c = _rows(pages, q, q.shape, 'q'), _rows(pages, k, shape, 'k'), _rows(pages, v, shape, 'v')
     _require(a.heads > 0, 'q has no heads')
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
         to = MxRows(out.data_ptr(), a.heads * s.head_dim, s.head_dim, a.heads, a.type)
     else:
         _require(not (_overlap(out, q) or _overlap(out, k) or _overlap(out, v)), 'out must be apart from q, k and v')
