@@ -114,8 +114,9 @@ size_t mx_episode_workspace(const MxPages* pages, const MxChunk* chunk, const Mx
  * multiplied by amplitude; the other values stay:
  *     y_a = amplitude * (x_a cos - x_b sin),  y_b = amplitude * (x_a sin + x_b cos)
  * Pair i is (i, i + width / 2), or with `interleaved` (2 i, 2 i + 1).  turn: width / 2 angles in radians, 64 bits, on the
- * device.  The angle is reduced in 64 bits (off by 2^-52 of itself at most); its sine and cosine, times amplitude, are
- * rounded to 32 bits, and products are in 32. */
+ * device.  The angle is reduced in 64 bits (off by 3 * 2^-53 of itself at most; positions beyond 2^53 are rounded to 64-bit
+ * floating point first); its sine and cosine, times amplitude, are rounded to 32 bits, and so are each product and their
+ * sum, by themselves: none is fused. */
 typedef struct MxRotary {
   const double* turn;
   int32_t width, interleaved;
