@@ -496,9 +496,15 @@ class Layers:
         return ids
 
     @staticmethod
-    def _packed(chunk, x):
-        """Rows in the shape that the chunk's start wants."""
-        return x.flatten(0, 1) if chunk.start is not None and x.dim() == 4 else x
+    def _packed(chunk, x, behind=2):
+        """Rows in the shape that the chunk's start wants; ``behind``: the dimensions of a row.  Only a chunk of which every
+        world has the same number may come as (nworld, count, ...): of a ragged one such rows would be padded."""
+        if chunk.start is None or x.dim() == 1 + behind:
+            return x
+        _require(len(chunk.shape) == 2, 'rows of a ragged chunk must be packed: (tokens, heads, head_dim), got %s', tuple(x.shape))
+        _require(x.dim() == 2 + behind and x.shape[:2] == chunk.shape, 'rows must be packed, or of shape (%d, %d, heads, head_dim), got %s',
+                 *chunk.shape, tuple(x.shape))
+        return x.flatten(0, 1)
 
     @staticmethod
     def _bounds(chunk, stream, options, *names):
@@ -571,9 +577,9 @@ class Layers:
         if x is q:
             return call(q)
         given = options.get('out')
-        for name in ('out', 'lse'):
+        for name, behind in (('out', 2), ('lse', 1)):
             if options.get(name) is not None:
-                y = options[name].flatten(0, 1)
+                y = self._packed(chunk, options[name], behind)
                 _require(y.data_ptr() == options[name].data_ptr(), '%s: the rows of all worlds must step evenly', name)
                 options[name] = y
         out = call(x)
