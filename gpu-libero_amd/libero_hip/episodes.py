@@ -496,15 +496,22 @@ class Layers:
         return ids
 
     @staticmethod
-    def _packed(chunk, x, behind=2):
+    def _packed(chunk, x, behind=2, stream=None):
         """Rows in the shape that the chunk's start wants; ``behind``: the dimensions of a row.  Only a chunk of which every
-        world has the same number may come as (nworld, count, ...): of a ragged one such rows would be padded."""
+        world has the same number may come as (nworld, count, ...): of a ragged one such rows would be padded.  Rows that do
+        not step evenly are copied, on the stream of the call."""
         if chunk.start is None or x.dim() == 1 + behind:
             return x
         _require(len(chunk.shape) == 2, 'rows of a ragged chunk must be packed: (tokens, heads, head_dim), got %s', tuple(x.shape))
         _require(x.dim() == 2 + behind and x.shape[:2] == chunk.shape, 'rows must be packed, or of shape (%d, %d, heads, head_dim), got %s',
                  *chunk.shape, tuple(x.shape))
-        return x.flatten(0, 1)
+        if stream is None:
+            return x.flatten(0, 1)
+        with torch.cuda.stream(stream):
+            packed = x.flatten(0, 1)
+        if packed.data_ptr() != x.data_ptr():
+            x.record_stream(stream)
+        return packed
 
     @staticmethod
     def _bounds(chunk, stream, options, *names):
@@ -525,7 +532,8 @@ class Layers:
     def write(self, chunk, k, v, layer=0, *, stream=None):
         """:func:`write` of the chunk's keys and values to a layer, and the summaries of the blocks that they complete."""
         other = self._enter(stream, chunk.start)
-        write(self.layers[layer], self._packed(chunk, k), self._packed(chunk, v), chunk.start, stream=stream)
+        k, v = (self._packed(chunk, x, stream=stream) for x in (k, v))
+        write(self.layers[layer], k, v, chunk.start, stream=stream)
         self._summarise(chunk, layer, stream)
         self._leave(other)
 
@@ -535,11 +543,11 @@ class Layers:
         other = self._enter(stream, chunk.start)
         given = None if out is None else self._packed(chunk, out)
         _require(given is None or given.data_ptr() == out.data_ptr(), 'out: the rows of all worlds must step evenly')
-        turned = operators.enter(self.layers[layer], rotary, self._packed(chunk, q), self._packed(chunk, k), self._packed(chunk, v),
-                                 chunk.start, out=given, stream=stream)
+        shape, (q, k, v) = q.shape, (self._packed(chunk, x, stream=stream) for x in (q, k, v))
+        turned = operators.enter(self.layers[layer], rotary, q, k, v, chunk.start, out=given, stream=stream)
         self._summarise(chunk, layer, stream)
         self._leave(other)
-        return turned.view(q.shape) if out is None else out
+        return turned.view(shape) if out is None else out
 
     def attend(self, chunk, q, layer=0, **options):
         """:func:`attend` from the chunk's queries to a layer; options as there.  ``max_count`` and ``longest`` are the chunk's
@@ -573,7 +581,7 @@ class Layers:
 
     def _attended(self, chunk, q, options, call):
         """A call with queries, ``out`` and ``lse`` in the shape that the chunk's start wants, and its result in q's."""
-        x = self._packed(chunk, q)
+        x = self._packed(chunk, q, stream=options.get('stream'))
         if x is q:
             return call(q)
         given = options.get('out')
