@@ -218,7 +218,10 @@ class DeviceEpisodeCache(episodes.Layers):
 
     def places(self, chunk):
         """:func:`places` of the chunk's rows, in the chunk's shape."""
-        return tuple(x.view(chunk.shape) for x in places(self.room, chunk.start, tokens=chunk.tokens))
+        other = self._enter(None, chunk.start)
+        found = places(self.room, chunk.start, tokens=chunk.tokens)
+        self._leave(other)
+        return tuple(x.view(chunk.shape) for x in found)
 
     def _seen(self, x):
         """A tensor's values after the last change, on the host."""

@@ -37,3 +37,27 @@ def test_rows_that_step_unevenly_on_another_stream(gpu_available):
         assert torch.equal(a, b)
 
 
+
+
+@pytest.mark.parametrize('behind', ['changes', 'places'])
+def test_places_follow_the_last_change(gpu_available, behind):
+    """A chunk's places asked for on another stream than that of the changes before and after, whichever is behind."""
+    import torch
+    print('case places order', behind, flush=True)
+    cache = room.DeviceEpisodeCache(5, **OPTIONS)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(6):
+        if behind == 'changes':
+            torch.cuda._sleep(20_000_000)
+        chunk = cache.extend(3)
+        with torch.cuda.stream(side):
+            if behind == 'places':
+                torch.cuda._sleep(20_000_000)
+            world, position, slot = cache.places(chunk)
+        cache.extend(2)
+        torch.cuda.synchronize()
+        assert position.tolist() == [[5 * i, 5 * i + 1, 5 * i + 2]] * 5
+        assert world.tolist() == [[w] * 3 for w in range(5)]
+        pages = cache.table[:, [5 * i // 16, (5 * i + 1) // 16, (5 * i + 2) // 16]]
+        assert torch.equal(slot, pages * 16 + position % 16)
