@@ -90,7 +90,9 @@ def select(summaries, q, start=None, *, top, near=1, first=0, causal=True, max_c
     those between the ``top`` with the largest score, of equal ones the earlier.  The score is the largest, over the query heads
     of the key head, of the product of the query and the summary, both in 8-bit whole numbers with powers of two.
     ``max_count`` (with ``start``): the largest chunk of a world, if known; rows beyond it get no blocks.  ``listed`` is first +
-    near + top, and with ``causal=False`` as many more as ``max_count`` tokens may need.  ``out`` is written if given."""
+    near + top, and with ``causal=False`` as many more as the tokens behind a query may need: those of the chunk, or with ``start``
+    of ``max_count`` tokens.  Then, in a chunk that is longer all the same, no row's list has room for the last blocks of what it
+    sees: they are left out.  ``out`` is written if given."""
     pages = summaries.pages
     if _elsewhere(pages, stream):
         return _on(pages.device, stream, _held(pages, summaries.codes, summaries.exponent, q, start, out),
@@ -103,8 +105,10 @@ def select(summaries, q, start=None, *, top, near=1, first=0, causal=True, max_c
         max_count = chunk.tokens if start is not None else chunk.count
     _require(0 <= max_count < 2 ** 31 and 0 <= top <= MOST_TOP and near >= 1 and first >= 0,
              'max_count and first must not be negative, top at most %d and near at least 1', MOST_TOP)
-    listed = first + near + top + (0 if causal else (max_count + summaries.block_tokens - 2) // summaries.block_tokens)
-    _require(listed <= MOST_LISTED, 'at most %d blocks can be listed, got %d: give max_count, the largest chunk of a world',
+    listed = first + near + top
+    if not causal:                        # the blocks behind a query's own: of the whole chunk, whichever of its rows are left out
+        listed += ((max_count if start is not None else chunk.count) + summaries.block_tokens - 2) // summaries.block_tokens
+    _require(listed <= MOST_LISTED, 'at most %d blocks can be listed, got %d: give max_count, the largest chunk of a world, with start',
              MOST_LISTED, listed)
     shape = shape[:-2] + (s.kv_heads, listed)
     if out is None:

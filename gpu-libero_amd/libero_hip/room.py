@@ -183,7 +183,8 @@ class DeviceEpisodeCache(episodes.Layers):
         """Empty the worlds of ``over``, then make room for new tokens of every world, as :func:`make_room`, and return their
         chunk.  ``count``: a number, or int32 on the device, with ``rows`` (how many rows the step's tensors have; those beyond the
         counts' sum belong to no world, and what is computed from them is not defined) and ``most`` (the most of one world,
-        if known: rows of a world beyond it are not attended from)."""
+        if known: rows of a world beyond it are not attended from, and without causality :meth:`recall` has room for the last blocks
+        of ``most`` tokens only)."""
         if torch.is_tensor(count):
             _require(rows is not None, 'give rows with a tensor of counts')
             most = rows if most is None else most

@@ -197,9 +197,10 @@ typedef struct MxSummaries {
  * with q_h in codes of its own head by the rule above (a NaN counts as 0, an infinity as cut off): exact in 32 bits,
  * the same on any machine.  The byte 255 stands above all scores, a table entry that names no page below.
  * blocks: tokens x kv_heads x width, filled from the left in ascending order, then -1; all of it is written, -1 for rows
- * that see nothing, belong to no world, or lie beyond max_count in it.  width is at least first + near + top, and more by
- * (max_count + block_tokens - 2) / block_tokens where queries see tokens behind them (causal 0), and at most 4096; top at
- * most 1024. */
+ * that see nothing, belong to no world, or lie beyond max_count in it.  width is at least first + near + top, and at most
+ * 4096; top at most 1024.  Where queries see tokens behind them (causal 0) it has to be more by (n + block_tokens - 2) /
+ * block_tokens for chunks of n tokens, also where max_count is less: a list without that room leaves out its last
+ * blocks. */
 typedef struct MxSelection {
   int32_t* blocks;
   int32_t width, top, near, first, max_count, causal;
