@@ -284,16 +284,20 @@ constexpr int64_t kMostParts = 1 << 25, kMostBytes = 1 << 30, kBatchBytes = 192 
 bool choose_gathered(Attend& a, Launch& launch) {
   const int64_t blocks = (int64_t)a.width << (a.page_shift - a.block_shift), block = 1LL << a.block_shift;
   const int64_t tokens = a.start ? a.tokens : (int64_t)a.nworld * a.max_count, rows = tokens * a.heads;
-  if (a.lists < 2 || a.lists > kMostSplits || a.group > kManyRows || a.max_count > 32768 || rows > INT32_MAX) return false;
+  if (a.lists < 2 || a.lists > kMostSplits || a.group > kManyRows || rows > INT32_MAX) return false;
   const int many = kManyRows / a.group;
   const double share = (double)tokens * a.lists / ((double)a.nworld * blocks);      // tokens to a block
   const double kb = 2.0 * block * launch.head_dim * (launch.fp8 ? 1 : 2) / 1024, part_kb = 4.0 * a.group * launch.head_dim / 1024;
-  if (1.1 * (0.45 * part_kb + 10.0 * ceil(share / many) / share) > 0.3 + (launch.fp8 ? 0.095 : 0.075) * kb) return false;
+  // the marks, written and read once: 32 tokens of a world to a word, whatever is known of the chunks' sizes
+  const int64_t words = a.start ? tokens / 32 + a.nworld : a.nworld * ((a.max_count + 31LL) / 32);
+  const double marks_kb = 4.0 * words * blocks * a.kv_heads / 1024, marks = 2.0 * marks_kb / ((double)tokens * a.lists * a.kv_heads);
+  if (1.1 * (0.45 * part_kb + 10.0 * ceil(share / many) / share) + 0.25 * marks > 0.3 + (launch.fp8 ? 0.095 : 0.075) * kb) return false;
   const int64_t head_bytes = tokens * a.group * a.lists * launch.head_dim * 4;      // of a key head's sums
-  if (rows * a.lists > kMostParts || head_bytes > kMostBytes) return false;
-  // a tile for each full set of rows of a key head, and one that is not full for each block
-  const int64_t head_tiles = tokens * a.lists / many + a.nworld * blocks, tiles = head_tiles * a.kv_heads;
-  if (tiles > kMostGroups || (int64_t)a.nworld * a.kv_heads * ((a.max_count + 31) / 32) > kMostGroups) return false;
+  if (rows * a.lists > kMostParts || head_bytes > kMostBytes || marks_kb > kMostBytes / 1024) return false;
+  // a tile for each full set of rows of a key head, and one that is not full for each block that is listed
+  const int64_t entries = tokens * a.lists, world_blocks = a.nworld * blocks;
+  const int64_t head_tiles = entries / many + (world_blocks < entries ? world_blocks : entries), tiles = head_tiles * a.kv_heads;
+  if (tiles > kMostGroups || tiles * many > kMostBytes / 4 || words * a.kv_heads > kMostGroups || a.nworld * (blocks / 16 + 1) * a.kv_heads > kMostGroups) return false;
   launch.gathered = true;
   launch.rows = kManyRows;
   launch.tiles = (int)tiles;
@@ -303,6 +307,7 @@ bool choose_gathered(Attend& a, Launch& launch) {
   const int64_t batches = (head_bytes * a.kv_heads + kBatchBytes - 1) / kBatchBytes;
   a.batch_heads = batches >= a.kv_heads ? 1 : (int)((a.kv_heads + batches - 1) / batches);
   a.words = (a.max_count + 31) / 32;
+  a.words_all = (int)words;
   a.world_blocks = (int)blocks;
   a.tiles_most = (int)head_tiles * a.batch_heads;
   a.tiles = a.tiles_most;
@@ -363,7 +368,7 @@ int choose(Attend& a, Launch& launch) {
 int batches_of(const Attend& a) { return (a.kv_heads + a.batch_heads - 1) / a.batch_heads; }
 
 // The workspace: sums, (maximum, sum of weights) of each part, and for gathered rows the tiles' numbers, tiles, their
-// rows and marks
+// rows and marks.  Of a chunk whose sizes the host does not know it is as large as of one that it knows.
 struct Workspace {
   size_t ml, counts, tiles, rows, marks, bytes;
 };
@@ -382,7 +387,7 @@ Workspace workspace_for(const Attend& a, const Launch& launch) {
   w.tiles = after(w.counts, batches * sizeof(int));
   w.rows = after(w.tiles, tiles * sizeof(int4));
   w.marks = after(w.rows, tiles * (kManyRows / a.group) * sizeof(int));
-  w.bytes = after(w.marks, (size_t)a.nworld * a.kv_heads * a.world_blocks * a.words * sizeof(unsigned));
+  w.bytes = after(w.marks, (size_t)a.kv_heads * a.words_all * a.world_blocks * sizeof(unsigned));
   return w;
 }
 

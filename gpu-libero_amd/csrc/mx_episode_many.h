@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, kListed && D == 128 ? 3 : many_waves(D, kFp8))
     Fixed* tile = fixed((const int32_t*)(a.gathered + number));
     const int pair = tile[0], found = tile[2];
     block = tile[1];
-    if ((int)blockIdx.x >= listed) return;
+    if ((int)blockIdx.x >= listed || !found) return;
     if (threadIdx.x < kManyRows) {
       tokens[threadIdx.x] = threadIdx.x < found ? a.gathered_rows[number * many + threadIdx.x] : 0;
       places[threadIdx.x] = INT32_MAX;

@@ -495,20 +495,46 @@ __global__ __launch_bounds__(kTeam == 1 ? 256 : 64 * kTeam) void select_blocks(c
 }
 
 // ---------------------------------------------------------------------------- rows gathered by their blocks
+// The first word of a world's marks: ragged chunks of n tokens have n / 32 + 1 at most, so that the places of all follow from
+// `start` and their number from what the host knows, however large a chunk may be
+__device__ inline int first_word(const Attend& a, int world) {
+  return a.start ? (max(a.start[world], 0) >> 5) + world : world * a.words;
+}
+
+// Tokens of a world's chunk whose rows are computed, and its first packed one
+__device__ inline int marked_tokens(const Attend& a, int world, int& begin) {
+  begin = a.start ? a.start[world] : world * a.count;
+  const int stop = a.start ? min(a.start[world + 1], a.tokens) : begin + a.count;
+  return begin < 0 ? 0 : max(min(stop - begin, a.max_count), 0);
+}
+
 // A workgroup takes 32 tokens of a world's chunk and a key head (2048 tokens' 19 blocks, 8 heads: 5 us; with atomics in
 // memory 28): the bits of all blocks that their lists name, collected in LDS (so many blocks at a time), and written
-// side by side: marks[world, key head][word][block].  Entries of whose keys the row sees none get empty parts.
+// side by side: marks[key head][word][block].  Entries of whose keys the row sees none get empty parts.
 constexpr int kMarked = 8192;
 __global__ __launch_bounds__(256) void mark_rows(const Attend a) {
   __shared__ unsigned bits[kMarked];
-  const int word = blockIdx.x % a.words, pair = blockIdx.x / a.words, world = pair / a.kv_heads, head = pair - world * a.kv_heads;
+  const int item = blockIdx.x % a.words_all, head = blockIdx.x / a.words_all;
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i * a.batch_heads < a.kv_heads; i += 256) a.gathered_tiles[i] = 0;
-  const int begin = a.start ? a.start[world] : world * a.count, stop = a.start ? min(a.start[world + 1], a.tokens) : begin + a.count;
+  int world = 0;
+  if (a.start) {                                  // the last one whose words begin at or before this
+    for (int high = a.nworld; high - world > 1;) {
+      const int step = (high - world + 63) >> 6, probe = world + (threadIdx.x & 63) * step;
+      const int passed = max(1, (int)__popcll(__ballot(probe < high && first_word(a, probe) <= item)));
+      world += (passed - 1) * step;
+      high = min(high, world + step);
+    }
+    world = __builtin_amdgcn_readfirstlane(world);
+  } else {
+    world = item / a.words;
+  }
+  int begin;
+  const int word = item - first_word(a, world), tokens = min(marked_tokens(a, world, begin) - 32 * word, 32);
+  if (word < 0 || tokens <= 0) return;
   const int count = a.start ? a.start[world + 1] - begin : a.count, length = max(a.length[world], 0);
-  const int tokens = begin < 0 ? 0 : max(min(min(stop - begin, a.max_count) - 32 * word, 32), 0);
   const int reach = (int)min((long long)length, (long long)a.width << a.page_shift);
-  unsigned* marks = a.marks + ((int64_t)pair * a.words + word) * a.world_blocks;
+  unsigned* marks = a.marks + ((int64_t)head * a.words_all + item) * a.world_blocks;
   for (int first = 0; first < a.world_blocks; first += kMarked) {
     const int many = min(a.world_blocks - first, kMarked);
     for (int i = threadIdx.x; i < many; i += 256) bits[i] = 0;
@@ -537,14 +563,21 @@ __global__ __launch_bounds__(256) void list_tiles(const Attend a) {
   __shared__ int sh_tokens[kCounted], sh_from[kCounted];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, many = kManyRows / a.group;
   const int per = (a.world_blocks + kCounted - 1) / kCounted, pair = blockIdx.x / per, first = (blockIdx.x - pair * per) * kCounted;
-  const int batch = (pair % a.kv_heads) / a.batch_heads;
-  const unsigned* marks = a.marks + (int64_t)pair * a.words * a.world_blocks;
+  const int world = pair / a.kv_heads, head = pair - world * a.kv_heads, batch = head / a.batch_heads;
+  int begin;
+  const int in_all = marked_tokens(a, world, begin), words = (in_all + 31) >> 5;
+  const unsigned* marks = a.marks + ((int64_t)head * a.words_all + first_word(a, world)) * a.world_blocks;
+  // tokens that the chunk does not have are in no word, whatever is in the memory of one that no workgroup wrote
+  const auto word_of = [&](int w, int block) {
+    const int tokens = in_all - 32 * w;
+    return marks[(int64_t)w * a.world_blocks + block] & (tokens >= 32 ? ~0u : (1u << tokens) - 1);
+  };
   // the tokens of a block, by 16 threads
   {
     const int block = first + (threadIdx.x >> 4);
     int tokens = 0;
     if (block < a.world_blocks)
-      for (int w = threadIdx.x & 15; w < a.words; w += 16) tokens += __popc(marks[(int64_t)w * a.world_blocks + block]);
+      for (int w = threadIdx.x & 15; w < words; w += 16) tokens += __popc(word_of(w, block));
 #pragma unroll
     for (int by = 1; by < 16; by *= 2) tokens += __shfl_xor(tokens, by);
     if ((threadIdx.x & 15) == 0) sh_tokens[threadIdx.x >> 4] = tokens;
@@ -566,13 +599,17 @@ __global__ __launch_bounds__(256) void list_tiles(const Attend a) {
   __syncthreads();
   for (int i = wave; i < kCounted; i += 4) {
     const int tokens = sh_tokens[i], tiles = (tokens + many - 1) / many;
-    if (!tokens || sh_from[i] + tiles > a.tiles_most) continue;
+    if (!tokens) continue;
+    // (there is room for all where `start` is as it has to be; tiles of a block without are empty)
+    const bool fits = sh_from[i] + tiles <= a.tiles_most;
     const int64_t from = (int64_t)batch * a.tiles_most + sh_from[i];
-    for (int j = lane; j < tiles; j += 64) a.gathered[from + j] = int4{pair, first + i, min(tokens - j * many, many), 0};
+    for (int j = lane; j < min(tiles, a.tiles_most - sh_from[i]); j += 64)
+      a.gathered[from + j] = int4{pair, first + i, fits ? min(tokens - j * many, many) : 0, 0};
+    if (!fits) continue;
     int* rows = a.gathered_rows + from * many;
     int before = 0;                               // marked in the words before
-    for (int base = 0; base < a.words; base += 64) {
-      unsigned word = base + lane < a.words ? marks[(int64_t)(base + lane) * a.world_blocks + first + i] : 0;
+    for (int base = 0; base < words; base += 64) {
+      unsigned word = base + lane < words ? word_of(base + lane, first + i) : 0;
       int sum = __popc(word);
 #pragma unroll
       for (int by = 1; by < 64; by *= 2) {
@@ -589,7 +626,7 @@ __global__ __launch_bounds__(256) void list_tiles(const Attend a) {
 int gather_rows(Attend& a, const Launch& launch, void* stream) {
   const hipStream_t s = (hipStream_t)stream;
   const unsigned pairs = a.nworld * a.kv_heads, per = (a.world_blocks + kCounted - 1) / kCounted;
-  hipLaunchKernelGGL(mark_rows, dim3(pairs * a.words), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(mark_rows, dim3((unsigned)a.words_all * a.kv_heads), dim3(256), 0, s, a);
   hipLaunchKernelGGL(list_tiles, dim3(pairs * per), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }

@@ -126,13 +126,13 @@ struct Attend {
   bool q_vector, o_vector;           // q's rows are 16-byte aligned, out's 8-byte
   const int32_t* blocks;             // of attention to listed blocks: (token, key head, entry), `lists` entries
   int lists, block_shift;
-  // rows gathered by their blocks: the tokens of each (world and key head, block), a bit each in `words` words
-  // [pair][word][block]; tiles of (pair, block, number of tokens), how many of those there
+  // rows gathered by their blocks: the tokens of each (key head, world, block), a bit each in words [head][word][block],
+  // a world's from first_word() on; tiles of (world and key head, block, number of tokens), how many of those there
   // are, and their tokens, up to 128 / group of each tile
   unsigned* marks;
   int4* gathered;
   int *gathered_tiles, *gathered_rows;
-  int words, world_blocks;
+  int words, words_all, world_blocks;  // words: of a world, where all have as many
   int tiles_most, batch, batch_heads;  // tiles that the key heads of a batch have room for; which batch; its key heads
 };
 

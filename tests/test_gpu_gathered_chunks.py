@@ -1,0 +1,65 @@
+"""Rows gathered by their blocks from ragged chunks whose sizes the host does not know."""
+import numpy as np
+import pytest
+
+from libero_hip import recall
+from test_gpu_episodes import World, compare, queries
+from test_gpu_recall import gathers, listed_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('counts', [[33, 0, 0, 31, 1, 64, 65, 0, 95, 2, 127, 32], [0, 0, 300, 0], [1] * 30 + [200]],
+                         ids=['mixed', 'one', 'singles'])
+def test_unknown_sizes(gpu_available, counts):
+    """Chunks that begin anywhere in a word of marks, empty worlds among them; with the largest known, not known, and less."""
+    import torch
+    print('case gathered unknown', len(counts), flush=True)
+    world = World([min(c + 130, 420) for c in counts], 2, 64, 64, 'bf16', seed=len(counts))
+    q, start = queries(counts, 4, 64, 'bf16')
+    tokens = int(sum(counts))
+    assert gathers(world, counts, 4, 12, 64) and gathers(world, counts, 4, 12, 64, most=tokens)
+    blocks = np.random.default_rng(1).integers(-1, 7, (tokens, 2, 12)).astype(np.int32)
+    at, given = torch.from_numpy(start).cuda(), torch.from_numpy(blocks).cuda()
+    lse = torch.zeros((tokens, 4), device='cuda')
+    out = recall.recall(world.pages, q.cuda(), given, at, block_tokens=64, lse=lse)
+    compare(out, lse, listed_attention(world, q, start, blocks, 64, True), 'bf16')
+    assert torch.equal(out, recall.recall(world.pages, q.cuda(), given, at, block_tokens=64, max_count=max(counts)))
+    # rows behind the last world's, and those beyond max_count, stay as they were
+    more = torch.cat([q.cuda(), torch.ones((37, 4, 64), dtype=torch.bfloat16, device='cuda')])
+    lists = torch.cat([given, torch.zeros((37, 2, 12), dtype=torch.int32, device='cuda')])
+    target = torch.full_like(more, 7)
+    recall.recall(world.pages, more, lists, at, block_tokens=64, max_count=70, out=target)
+    kept = np.concatenate([np.arange(start[w], start[w] + min(c, 70)) for w, c in enumerate(counts)])
+    left = np.setdiff1d(np.arange(tokens + 37), kept)
+    assert bool((target[torch.from_numpy(left).cuda()] == 7).all())
+    if gathers(world, counts + [37], 4, 12, 64, most=70):
+        assert torch.equal(target[torch.from_numpy(kept).cuda()], out[torch.from_numpy(kept).cuda()])
+
+
+def test_many_worlds(gpu_available):
+    """A thousand worlds' ragged chunks over long tables: little more memory than the sums where the largest is not known."""
+    import torch
+    print('case gathered many worlds', flush=True)
+    n, kv, dim, width = 1024, 8, 128, 128
+    gen = torch.Generator('cuda').manual_seed(0)
+    k, v = (torch.randn((4096, kv, 64, dim), generator=gen, device='cuda').bfloat16() for _ in range(2))
+    from libero_hip import episodes
+    table = torch.randint(0, 4096, (n, width), generator=gen, dtype=torch.int32, device='cuda')
+    length = torch.randint(200, width * 64 + 1, (n,), generator=gen, dtype=torch.int32, device='cuda')
+    pages = episodes.Pages(k, v, table, length)
+    counts = torch.randint(0, 65, (n,), generator=gen, device='cuda')
+    start = torch.zeros(n + 1, dtype=torch.int32, device='cuda')
+    start[1:] = counts.cumsum(0)
+    tokens = 32768
+    q = torch.randn((tokens, kv, dim), generator=gen, device='cuda').bfloat16()
+    blocks = torch.randint(0, 128, (tokens, kv, 19), generator=gen, dtype=torch.int32, device='cuda')
+    made = []
+    for most in (64, None):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        made.append(recall.recall(pages, q, blocks, start, block_tokens=64, max_count=most, out=torch.zeros_like(q)))
+        torch.cuda.synchronize()
+        assert torch.cuda.max_memory_allocated() - before < 1.2 * 2 ** 30
+    assert torch.equal(*made) and bool(made[0][:int(start[-1])].any())
