@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256, kListed && D == 128 ? 3 : many_waves(D, kFp8))
     const int64_t tokens_all = a.part_rows / a.heads, row = part_row(a, t, token_in, query_head), token = row / a.heads;
     const int32_t* list = a.blocks + ((int64_t)(t.token + token_in) * a.kv_heads + head) * a.lists;
     int left = copies[which];
-    for (int e = places[which]; left; e++) {                 // as often as it is listed
+    for (int e = places[which]; left && e < a.lists; e++) {  // as often as it is listed (a list may have changed meanwhile)
       if (e > places[which] && list[e] != block) continue;
       left--;
       const int64_t at = (e * tokens_all + token) * a.part_heads + query_head - a.part_first;

@@ -1,4 +1,4 @@
-"""Rows gathered by their blocks from ragged chunks whose sizes the host does not know."""
+"""Rows gathered by their blocks: ragged chunks whose sizes the host does not know, and lists that change meanwhile."""
 import numpy as np
 import pytest
 
@@ -63,3 +63,27 @@ def test_many_worlds(gpu_available):
         torch.cuda.synchronize()
         assert torch.cuda.max_memory_allocated() - before < 1.2 * 2 ** 30
     assert torch.equal(*made) and bool(made[0][:int(start[-1])].any())
+
+
+def test_lists_that_change(gpu_available):
+    """Lists written from another stream while they are attended to: the call ends, and writes nothing but its results."""
+    import torch
+    print('case changing lists', flush=True)
+    world = World([500, 310], 2, 64, 64, 'bf16', seed=5)
+    q, start = queries([200, 130], 4, 64, 'bf16')
+    assert gathers(world, [200, 130], 4, 12, 64)
+    rng = np.random.default_rng(0)
+    lists = [torch.from_numpy(rng.integers(-1, 8, (330, 2, 12)).astype(np.int32)).cuda() for _ in range(2)]
+    given, at, side = lists[0].clone(), torch.from_numpy(start).cuda(), torch.cuda.Stream()
+    whole = torch.full((3, 330, 4, 64), 7.0, dtype=torch.bfloat16, device='cuda')
+    rows = q.cuda()
+    torch.cuda.synchronize()
+    for i in range(20):
+        with torch.cuda.stream(side):
+            for j in range(10):
+                given.copy_(lists[j % 2])
+        recall.recall(world.pages, rows, given, at, block_tokens=64, out=whole[1])
+    torch.cuda.synchronize()
+    assert bool((whole[0] == 7).all()) and bool((whole[2] == 7).all())
+    out = recall.recall(world.pages, rows, lists[1], at, block_tokens=64)
+    compare(out, None, listed_attention(world, q, start, lists[1].cpu().numpy(), 64, True), 'bf16')
