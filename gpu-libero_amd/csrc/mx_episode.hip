@@ -263,6 +263,7 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
   launch.head_dim = p->head_dim;
   launch.keys = (int64_t)p->width << a.page_shift;
   if (m->longest && m->longest < launch.keys) launch.keys = m->longest;
+  launch.held = launch.keys;
   if (s) {
     launch.listed = true;
     a.blocks = s->blocks; a.lists = s->width; a.block_shift = block_shift;
@@ -279,14 +280,16 @@ int plan(const MxPages* p, const MxChunk* c, const MxAttention* m, Attend& a, La
 // 65536, 32 heads on 8, 475 and 911 (8-bit pages 443 and 555), 512 tokens 171 and 234, 256 tokens 124 and 123; 4 x 1024
 // over 8192, 8 heads on 8, 265 and 1482, 32 on 4, 858 and 758, 32 on 8 of 256 values 1171 and 3808; 16 x 256 over 8192,
 // 16 on 4 of 64 values, 172 and 262 (163 and 201); 64 x 64 over 4096 205 and 240; 300 x 41 over 1024, 12 on 4 of 96
-// values, blocks of 32, 631 and 533.
+// values, blocks of 32, 631 and 533.  How many tokens share a block goes by the tokens that worlds have, as far as the caller
+// knows, not by what the table could hold: 4 x 1024 tokens over 8192, 8 heads on 8, in tables for 524288: 434 and 1518.
 constexpr int64_t kMostParts = 1 << 25, kMostBytes = 1 << 30, kBatchBytes = 192 << 20;
 bool choose_gathered(Attend& a, Launch& launch) {
   const int64_t blocks = (int64_t)a.width << (a.page_shift - a.block_shift), block = 1LL << a.block_shift;
   const int64_t tokens = a.start ? a.tokens : (int64_t)a.nworld * a.max_count, rows = tokens * a.heads;
   if (a.lists < 2 || a.lists > kMostSplits || a.group > kManyRows || rows > INT32_MAX) return false;
   const int many = kManyRows / a.group;
-  const double share = (double)tokens * a.lists / ((double)a.nworld * blocks);      // tokens to a block
+  const int64_t held = (launch.held + block - 1) >> a.block_shift;                  // blocks that a world has
+  const double share = (double)tokens * a.lists / ((double)a.nworld * held);        // tokens to a block
   const double kb = 2.0 * block * launch.head_dim * (launch.fp8 ? 1 : 2) / 1024, part_kb = 4.0 * a.group * launch.head_dim / 1024;
   // the marks, written and read once: 32 tokens of a world to a word, whatever is known of the chunks' sizes
   const int64_t words = a.start ? tokens / 32 + a.nworld : a.nworld * ((a.max_count + 31LL) / 32);

@@ -12,7 +12,7 @@ constexpr int64_t kMostGroups = (1 << 24) - 1;   // workgroups of 256 of a launc
 struct Launch {
   int type, head_dim, blocks, rows, tiles;    // blocks of 16 rows to a tile
   int team;                                   // waves of attend_few that share a tile
-  int64_t keys;                               // the most that a world has, as far as the host knows
+  int64_t keys, held;                         // the most that a row sees, and that a world has, as far as the host knows
   bool fp8, listed, gathered;                 // listed: attention to listed blocks; gathered: of rows that share one
   unsigned grid;
 };

@@ -508,9 +508,15 @@ __device__ inline int marked_tokens(const Attend& a, int world, int& begin) {
   return begin < 0 ? 0 : max(min(stop - begin, a.max_count), 0);
 }
 
+// Blocks of a world that have tokens: none behind them are marked
+__device__ inline int blocks_held(const Attend& a, int world) {
+  return min((int)((max(a.length[world], 0) + (1LL << a.block_shift) - 1) >> a.block_shift), a.world_blocks);
+}
+
 // A workgroup takes 32 tokens of a world's chunk and a key head (2048 tokens' 19 blocks, 8 heads: 5 us; with atomics in
 // memory 28): the bits of all blocks that their lists name, collected in LDS (so many blocks at a time), and written
-// side by side: marks[key head][word][block].  Entries of whose keys the row sees none get empty parts.
+// side by side: marks[key head][word][block], as far as the world has tokens.  Entries of whose keys the row sees none get
+// empty parts.
 constexpr int kMarked = 8192;
 __global__ __launch_bounds__(256) void mark_rows(const Attend a) {
   __shared__ unsigned bits[kMarked];
@@ -533,10 +539,10 @@ __global__ __launch_bounds__(256) void mark_rows(const Attend a) {
   const int word = item - first_word(a, world), tokens = min(marked_tokens(a, world, begin) - 32 * word, 32);
   if (word < 0 || tokens <= 0) return;
   const int count = a.start ? a.start[world + 1] - begin : a.count, length = max(a.length[world], 0);
-  const int reach = (int)min((long long)length, (long long)a.width << a.page_shift);
+  const int reach = (int)min((long long)length, (long long)a.width << a.page_shift), blocks = blocks_held(a, world);
   unsigned* marks = a.marks + ((int64_t)head * a.words_all + item) * a.world_blocks;
-  for (int first = 0; first < a.world_blocks; first += kMarked) {
-    const int many = min(a.world_blocks - first, kMarked);
+  for (int first = 0; first == 0 || first < blocks; first += kMarked) {
+    const int many = min(blocks - first, kMarked);
     for (int i = threadIdx.x; i < many; i += 256) bits[i] = 0;
     __syncthreads();
     for (int at = threadIdx.x; at < tokens * a.lists; at += 256) {
@@ -564,6 +570,8 @@ __global__ __launch_bounds__(256) void list_tiles(const Attend a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, many = kManyRows / a.group;
   const int per = (a.world_blocks + kCounted - 1) / kCounted, pair = blockIdx.x / per, first = (blockIdx.x - pair * per) * kCounted;
   const int world = pair / a.kv_heads, head = pair - world * a.kv_heads, batch = head / a.batch_heads;
+  const int blocks = blocks_held(a, world);
+  if (first >= blocks) return;
   int begin;
   const int in_all = marked_tokens(a, world, begin), words = (in_all + 31) >> 5;
   const unsigned* marks = a.marks + ((int64_t)head * a.words_all + first_word(a, world)) * a.world_blocks;
@@ -576,7 +584,7 @@ __global__ __launch_bounds__(256) void list_tiles(const Attend a) {
   {
     const int block = first + (threadIdx.x >> 4);
     int tokens = 0;
-    if (block < a.world_blocks)
+    if (block < blocks)
       for (int w = threadIdx.x & 15; w < words; w += 16) tokens += __popc(word_of(w, block));
 #pragma unroll
     for (int by = 1; by < 16; by *= 2) tokens += __shfl_xor(tokens, by);

@@ -561,14 +561,14 @@ class Layers:
 
     def recall(self, chunk, q, layer=0, *, top, near=1, first=0, **options):
         """:func:`libero_hip.recall.select` of blocks for the chunk's queries and :func:`libero_hip.recall.recall` of them: attention
-        whose cost does not grow with the episode.  The cache has to be made with ``block_tokens``.  ``max_count`` as in
-        :meth:`attend`; ``scale`` must not be negative, as the blocks of the largest scores are chosen."""
+        whose cost does not grow with the episode.  The cache has to be made with ``block_tokens``.  ``max_count`` and ``longest`` as
+        in :meth:`attend`; ``scale`` must not be negative, as the blocks of the largest scores are chosen."""
         from . import recall
         _require(self.summaries is not None, 'the cache has no summaries: make it with block_tokens')
         _require(options.get('scale') is None or options['scale'] >= 0, 'scale must not be negative, got %s', options.get('scale'))
         stream = options.get('stream')
         other = self._enter(stream, chunk.start)
-        self._bounds(chunk, stream, options)
+        self._bounds(chunk, stream, options, 'longest')
         both = {x: options[x] for x in ('causal', 'max_count', 'stream') if x in options}
 
         def call(x):

@@ -134,15 +134,17 @@ def _queries(pages, q, rows):
                          % (q.dtype, pages.k.dtype))
 
 
-def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal=True, scale=None, out=None, lse=None, stream=None):
+def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal=True, scale=None, out=None, lse=None, longest=0,
+           stream=None):
     """:func:`libero_hip.episodes.attend` over the keys of listed blocks: ``blocks`` (rows..., kv_heads, listed), contiguous
     int32, as :func:`select` returns or by the caller.  Block b holds the tokens from ``b * block_tokens`` on; of those the query sees
     what ``attend`` lets it see.  A block counts as often as it is listed, in any order; numbers that are no block of the
-    world's table are left out.  A query that sees nothing gives zeros (and ``lse`` -inf)."""
+    world's table are left out.  A query that sees nothing gives zeros (and ``lse`` -inf).  ``longest``, as for ``attend``, says how to
+    divide the work: without it the table's reach is taken for the worlds' tokens."""
     if _elsewhere(pages, stream):
         return _on(pages.device, stream, _held(pages, q, blocks, start, out, lse),
                    lambda: recall(pages, q, blocks, start, block_tokens=block_tokens, max_count=max_count, causal=causal, scale=scale,
-                                  out=out, lse=lse))
+                                  out=out, lse=lse, longest=longest))
     s, shape = pages.struct, q.shape
     chunk = _chunk(pages, shape[:-2], start)
     rows = _rows(pages, q, shape, 'q')
@@ -157,14 +159,14 @@ def recall(pages, q, blocks, start=None, *, block_tokens, max_count=None, causal
         scale = s.head_dim ** -0.5
     if max_count is None:
         max_count = chunk.tokens if start is not None else chunk.count
-    _require(0 <= max_count < 2 ** 31 and math.isfinite(scale), 'max_count must be a number of tokens and scale finite: %s, %s',
-             max_count, scale)
+    _require(0 <= max_count < 2 ** 31 and 0 <= longest < 2 ** 31 and math.isfinite(scale),
+             'max_count and longest must be numbers of tokens and scale finite: %s, %s, %s', max_count, longest, scale)
     if out is None:
         out = q.new_empty(shape)
         to = MxRows(out.data_ptr(), rows.heads * s.head_dim, s.head_dim, rows.heads, rows.type)
     else:
         to = _rows(pages, _output(q, out), shape, 'out')
-    a = MxAttention(rows, to, None, None, 0, max_count, 1 if causal else 0, 0, scale, 0)
+    a = MxAttention(rows, to, None, None, 0, max_count, 1 if causal else 0, 0, scale, longest)
     if lse is not None:
         _require(lse.dtype == torch.float32 and lse.shape == shape[:-1] and lse.is_contiguous()
                  and lse.get_device() == pages.index, 'lse must be contiguous float32 of q\'s shape without head_dim')

@@ -217,7 +217,8 @@ int mx_episode_select(const MxPages* pages, const MxChunk* chunk, const MxSummar
 
 /* mx_episode_attend over the keys of the listed blocks: s->blocks, s->width and block_tokens are read, the other numbers
  * of s are not.  A block counts as often as it is listed; numbers that are no block of the world's table are left out.
- * The probabilities are in two parts.  a->window must be 0. */
+ * The probabilities are in two parts.  a->longest says how to divide the work, as for mx_episode_attend.  a->window must
+ * be 0. */
 int mx_episode_recall(const MxPages* pages, const MxChunk* chunk, const MxAttention* a, const MxSelection* s,
                       int32_t block_tokens, void* stream);
 
