@@ -6,8 +6,9 @@
 // there are few numbers to a world, so each workgroup reads all of them again for its prefix and the totals instead of
 // waiting for its neighbours; lengths then change in the second launch, which also hands out the pages that the first
 // has put on the stack. Bound by launches and by a few dependent loads: 67 worlds 3.6 us; 4096 worlds that all restart
-// 10 and 3 us, of which the reading of all worlds is most (with sums in 64 bits 13, with 1024 threads to a workgroup
-// 13).  The places of their 2.1 million rows (25 MB): 13 us, 9 where all worlds have the same number.
+// 11 and 4 us, of which the reading of all worlds is most (with sums in 64 bits 13, with 1024 threads to a workgroup
+// 13); it grows with them, 31 us for a change of 16384 and 185 of 131072.  The places of the 4096 worlds' 2.1 million rows
+// (25 MB): 13 us, 9 where all worlds have the same number.
 #include "mx_episode_move.h"
 #include "mx_episode_launch.h"
 

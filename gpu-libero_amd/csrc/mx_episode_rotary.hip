@@ -7,9 +7,10 @@
 // 16 bytes of either half of a head (of a key its own 16 or 32 bytes, as the pages' scales want them, and reads the
 // others beside).
 //
-// Prompts of 4 x 4096 tokens, 32 and 8 heads of 128 values, bfloat16 (403 MB): 72 us, 5.6 TB/s.  67 prompts of up to
-// 501 tokens, float16 into 8-bit pages, half of each head turned (116 MB): 27 us, 4.3 TB/s.  4096 single tokens into
-// 8-bit pages (25 MB): 9.9 us.  16 x 1024 tokens of 16 heads of 64 values turned (67 MB, out of the last cache): 12.3
+// Prompts of 4 x 4096 tokens, 32 and 8 heads of 128 values, bfloat16 (403 MB): 72 us, 5.6 TB/s; float32 rows (738 MB): 132
+// for the call.  67 prompts of up to 501 tokens, float16 into 8-bit pages, half of each head turned (116 MB): 28.7 us,
+// 4.0 TB/s.  4096 single tokens into 8-bit pages (25 MB): 10.3 us, which is a chain: starts, lengths, table and angles come
+// before the first row is asked for.  16 x 1024 tokens of 16 heads of 64 values turned (67 MB, out of the last cache): 12.4
 // us.
 #include <type_traits>
 #include "mx_episode_move.h"

@@ -284,12 +284,10 @@ def _overlap(a, b):
     return first < second + reach[1] and second < first + reach[0]
 
 
-def _output(like, out, name='out'):
-    """``out`` for rows like ``like``: made here, or given and then checked."""
-    if out is None:
-        return torch.empty_like(like, memory_format=torch.contiguous_format)
-    _require(out.shape == like.shape and out.dtype == like.dtype, '%s must have the rows\' shape and type', name)
-    _require(all(step or n < 2 for n, step in zip(like.shape, out.stride())), '%s has elements that share memory', name)
+def _output(like, out):
+    """``out``, given for rows like ``like``, once it is checked."""
+    _require(out.shape == like.shape and out.dtype == like.dtype, 'out must have the rows\' shape and type')
+    _require(all(step or n < 2 for n, step in zip(like.shape, out.stride())), 'out has elements that share memory')
     return out
 
 
