@@ -107,7 +107,7 @@ def select(summaries, q, start=None, *, top, near=1, first=0, causal=True, max_c
              'max_count and first must not be negative, top at most %d and near at least 1', MOST_TOP)
     listed = first + near + top
     if not causal:                        # the blocks behind a query's own: of the whole chunk, whichever of its rows are left out
-        listed += ((max_count if start is not None else chunk.count) + summaries.block_tokens - 2) // summaries.block_tokens
+        listed += (max(max_count, chunk.count) + summaries.block_tokens - 2) // summaries.block_tokens
     _require(listed <= MOST_LISTED, 'at most %d blocks can be listed, got %d: give max_count, the largest chunk of a world, with start',
              MOST_LISTED, listed)
     shape = shape[:-2] + (s.kv_heads, listed)

@@ -8,7 +8,7 @@ from test_gpu_recall import expected_blocks, listed_attention, summarised
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize('most', [0, 1, 4, 39])
+@pytest.mark.parametrize('most', [0, 1, 4, 39, 100])
 def test_tokens_behind_max_count_are_seen(gpu_available, most):
     """Queries that see all of their world see its last blocks too, in chunks of one size that are longer than max_count."""
     import torch
@@ -19,6 +19,7 @@ def test_tokens_behind_max_count_are_seen(gpu_available, most):
     s = summarised(world, 16)
     x = q.cuda().view(3, 40, 4, 64)
     blocks = recall.select(s, x, top=1, near=1, causal=False, max_count=most)
+    assert blocks.shape[3] == 2 + (max(most, 40) + 14) // 16
     got = blocks.cpu().numpy().reshape(120, 2, -1)
     for r, row in enumerate(expected_blocks(world, q, start, 16, 1, 1, 0, False)):
         for h, want in enumerate(row if r % 40 < most else [[], []]):
