@@ -293,14 +293,19 @@ bool choose_gathered(Attend& a, Launch& launch) {
   const double kb = 2.0 * block * launch.head_dim * (launch.fp8 ? 1 : 2) / 1024, part_kb = 4.0 * a.group * launch.head_dim / 1024;
   // the marks, written and read once: 32 tokens of a world to a word, whatever is known of the chunks' sizes
   const int64_t words = a.start ? tokens / 32 + a.nworld : a.nworld * ((a.max_count + 31LL) / 32);
-  const double marks_kb = 4.0 * words * blocks * a.kv_heads / 1024, marks = 2.0 * marks_kb / ((double)tokens * a.lists * a.kv_heads);
-  if (1.1 * (0.45 * part_kb + 10.0 * ceil(share / many) / share) + 0.25 * marks > 0.3 + (launch.fp8 ? 0.095 : 0.075) * kb) return false;
+  const double marks_kb = 4.0 * words * blocks * a.kv_heads / 1024, marked_kb = 2.0 * marks_kb / ((double)tokens * a.lists * a.kv_heads);
+  // a tile for each full set of rows of a key head, and one that is not full for each block that is listed; as the table may
+  // hold more blocks than the worlds are known to have, there are workgroups for tiles that never are (0.7 ns each)
+  const int64_t entries = tokens * a.lists;
+  const auto tiles_of = [&](int64_t blocks) { return entries / many + (a.nworld * blocks < entries ? a.nworld * blocks : entries); };
+  const int64_t head_tiles = tiles_of(blocks), tiles = head_tiles * a.kv_heads;
+  const double gathered = 1.1 * (0.45 * part_kb + 10.0 * ceil(share / many) / share) + 0.25 * marked_kb
+                          + 0.7 * (head_tiles - tiles_of(held)) / entries;
+  if (gathered > 0.3 + (launch.fp8 ? 0.095 : 0.075) * kb) return false;
   const int64_t head_bytes = tokens * a.group * a.lists * launch.head_dim * 4;      // of a key head's sums
   if (rows * a.lists > kMostParts || head_bytes > kMostBytes || marks_kb > kMostBytes / 1024) return false;
-  // a tile for each full set of rows of a key head, and one that is not full for each block that is listed
-  const int64_t entries = tokens * a.lists, world_blocks = a.nworld * blocks;
-  const int64_t head_tiles = entries / many + (world_blocks < entries ? world_blocks : entries), tiles = head_tiles * a.kv_heads;
-  if (tiles > kMostGroups || tiles * many > kMostBytes / 4 || words * a.kv_heads > kMostGroups || a.nworld * (blocks / 16 + 1) * a.kv_heads > kMostGroups) return false;
+  if (tiles * many > kMostBytes / 4) return false;                                  // their tokens
+  if (tiles > kMostGroups || words * a.kv_heads > kMostGroups || a.nworld * (blocks / 16 + 1) * a.kv_heads > kMostGroups) return false;
   launch.gathered = true;
   launch.rows = kManyRows;
   launch.tiles = (int)tiles;
