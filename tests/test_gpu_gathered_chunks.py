@@ -87,3 +87,55 @@ def test_lists_that_change(gpu_available):
     assert bool((whole[0] == 7).all()) and bool((whole[2] == 7).all())
     out = recall.recall(world.pages, rows, lists[1], at, block_tokens=64)
     compare(out, None, listed_attention(world, q, start, lists[1].cpu().numpy(), 64, True), 'bf16')
+
+
+def test_replays_with_other_chunks(gpu_available):
+    """A captured call whose chunks and lengths change between replays: the same as the eager one."""
+    import torch
+    print('case gathered replays', flush=True)
+    world = World([420] * 9, 2, 64, 64, 'bf16', seed=8)
+    rng = np.random.default_rng(5)
+    tokens, at = 500, torch.zeros(10, dtype=torch.int32, device='cuda')
+    q = torch.randn((tokens, 4, 64), device='cuda').bfloat16()
+    lists = torch.from_numpy(rng.integers(-1, 7, (tokens, 2, 12)).astype(np.int32)).cuda()
+    out = torch.zeros_like(q)
+    assert gathers(world, [tokens] + [0] * 8, 4, 12, 64)
+
+    def call(to):
+        return recall.recall(world.pages, q, lists, at, block_tokens=64, out=to)
+
+    call(out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for i in range(8):
+        cuts = np.sort(rng.integers(0, tokens + 1, 8)) if i % 2 else np.repeat([0, 37, 400, tokens], 2)
+        start = np.concatenate([[0], cuts, [tokens if i < 6 else max(cuts[-1], 450)]])
+        at.copy_(torch.from_numpy(start.astype(np.int32)))
+        world.pages.length.copy_(torch.from_numpy(rng.integers(0, 421, 9).astype(np.int32)))
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call(torch.full_like(out, 7))
+        assert torch.equal(out, want), i
+        assert bool((out[int(start[-1]):] == 7).all())
+
+
+def test_chunks_without_rows(gpu_available):
+    import torch
+    from libero_hip import room
+    print('case no new tokens', flush=True)
+    cache = room.DeviceEpisodeCache(3, kv_heads=2, head_dim=32, tokens=64, storage='bf16', page_tokens=16, block_tokens=16)
+    cache.extend(5)
+    chunk = cache.extend(0)
+    q, k = (torch.zeros((3, 0, h, 32), dtype=torch.bfloat16, device='cuda') for h in (4, 2))
+    cache.write(chunk, k, k)
+    for causal in (True, False):
+        assert cache.recall(chunk, q, top=2, causal=causal).shape == q.shape and cache.attend(chunk, q, causal=causal).shape == q.shape
+    assert [x.shape for x in cache.places(chunk)] == [(3, 0)] * 3
+    none = cache.extend(torch.zeros(3, dtype=torch.int32, device='cuda'), rows=4)
+    rows = torch.ones((4, 4, 32), dtype=torch.bfloat16, device='cuda')
+    out = torch.full_like(rows, 7)
+    cache.write(none, rows[:, :2], rows[:, :2])
+    assert bool((cache.recall(none, rows, top=1, causal=False, out=out) == 7).all()) and cache.lengths.tolist() == [5] * 3
